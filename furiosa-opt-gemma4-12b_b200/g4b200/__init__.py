@@ -645,3 +645,10 @@ def decoder_feedforward_noalloc(residual, pre_ff_rms_weight, up_weight_packed, g
                5: f"intermediate size {n} is not 15360, 7680 or a multiple of 128 up to 3840",
                1: "a pointer is null or misaligned"}.get(code, "a CUDA call failed")
         raise G4Error("g4_decoder_feedforward_noalloc", code, why)
+
+
+from .paged import (PagedBatch, PagedCache, PagedCaches, PagePool, paged_attention, paged_compact,  # noqa: E402
+                    paged_copy, paged_store_qkv)
+
+__all__ += ["PagedBatch", "PagedCache", "PagedCaches", "PagePool", "paged_attention", "paged_compact", "paged_copy",
+            "paged_store_qkv"]

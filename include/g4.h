@@ -343,6 +343,122 @@ g4_status g4_attention_gqa(g4_ctx* ctx, const g4_bf16* q, const g4_bf16* k, cons
                            int n_rows, g4_bf16* out);
 
 /* ------------------------------------------------------------------------------ */
+/* Paged KV caches: many sequences, chunks of new tokens (no counterpart in the       */
+/* reference, whose host prefills one position per dispatch, src/host/generate.rs:194) */
+/* ------------------------------------------------------------------------------ */
+
+/* One layer's cache as pages of `page_rows` positions: element (page, row, head, dim) of
+ * K is k[page * k_page_stride + row * k_row_stride + head * k_head_stride + dim], V alike.
+ * Strides are in elements, multiples of 8, not negative; head_dim is 256 or 512 (the model's two attention
+ * kinds), page_rows a multiple of 8 up to 65536.  [n_pages, page_rows, n_kv_heads,
+ * head_dim] and [n_pages, n_kv_heads, page_rows, head_dim] are both such layouts, and so
+ * are the reference's 512-row pages laid back to back (g4_workspace_kv_cache). */
+typedef struct g4_paged_cache {
+  g4_bf16* k;
+  g4_bf16* v;
+  int64_t k_page_stride, k_row_stride, k_head_stride;
+  int64_t v_page_stride, v_row_stride, v_head_stride;
+  int32_t n_pages, page_rows, n_kv_heads, head_dim;
+} g4_paged_cache;
+
+/* The sequences of one call.  All arrays are DEVICE int32 arrays, read on the stream, so a
+ * captured call follows their contents:
+ *   q_start[n_seqs + 1]  sequence s has the new tokens q_start[s] .. q_start[s + 1] - 1;
+ *                        tokens from q_start[n_seqs] on belong to none and are left alone;
+ *   kv_len[n_seqs]       its rows in the cache INCLUDING the new tokens: new token i is at
+ *                        position kv_len[s] - (its number of new tokens) + i;
+ *   tables[n_seqs][table_stride]  page of positions [j * page_rows, (j + 1) * page_rows) at
+ *                        entry j < max_pages; entries no visible position falls into are
+ *                        never looked at (-1 past the end or below a window is usual).
+ * q_start outside 0..n_tokens or falling, kv_len outside 0..max_pages * page_rows, and page
+ * numbers outside 0..n_pages - 1 are cut off or skipped, never followed, and set a bit in
+ * the device status word (g4_ctx_poll_device_status). */
+#define G4_PAGED_MAX_SEQS 4096
+typedef struct g4_paged_batch {
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* q_start;
+  const int32_t* kv_len;
+  int32_t max_pages, n_seqs, n_tokens;
+} g4_paged_batch;
+
+/* Attention of new tokens over the pages of their sequences: q head h of the token at
+ * position p attends rows j <= p (and j > p - window if window > 0) of KV head
+ * h / (n_heads / n_kv_heads): out = sum_j softmax_j(scale * q . k_j) v_j.  A token no row is
+ * visible to (its position is negative: kv_len counts fewer rows than there are new tokens)
+ * gets zeros.  Rows outside the visible range of every new token of a sequence are not
+ * read, whatever they hold; within it K and V are expected to be finite.  Scores,
+ * softmax statistics and sums are f32; the weights of V are rounded to bf16 for the tensor
+ * cores.  q and out are [n_tokens, n_heads, head_dim] with the given strides in elements
+ * (multiples of 8).  The new tokens' own K and V rows must be in the cache already
+ * (g4_paged_store_qkv).  The first call of a context allocates its scratch
+ * (make it before a stream capture). */
+g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stride, int64_t q_head_stride,
+                             int n_heads, const g4_paged_cache* cache, const g4_paged_batch* batch, float scale,
+                             int window, g4_bf16* out, int64_t out_token_stride, int64_t out_head_stride);
+
+/* What g4_{sliding,full}_project_qkv do after their products, for every new token of a
+ * batch: q_out = rope(rmsnorm(q) * q_rms_weight); k = rope(rmsnorm(k) * k_rms_weight) and
+ * v = rmsnorm(v) into the token's cache row.  q [n_tokens, n_heads, head_dim], k and v
+ * [n_tokens, n_kv_heads, head_dim] are raw projection outputs in bf16 (the full layers have
+ * no V projection: pass k twice); cos/sin [n_positions, head_dim] as the decode entry points
+ * take them (sin of the low half negated).  Computed in f32 and rounded to bf16 once, where
+ * the single-token entry points round after each step.  q_out may be q.  A token at a
+ * negative position is not stored and gets a zero q_out; one at or past n_positions, or whose
+ * page is out of range, too, and sets a bit in the device status word. */
+g4_status g4_paged_store_qkv(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stride, int64_t q_head_stride,
+                             int n_heads, const g4_bf16* k, int64_t k_token_stride, int64_t k_head_stride,
+                             const g4_bf16* v, int64_t v_token_stride, int64_t v_head_stride,
+                             const g4_bf16* q_rms_weight, const g4_bf16* k_rms_weight, const g4_bf16* cos,
+                             const g4_bf16* sin, int n_positions, const g4_paged_cache* cache,
+                             const g4_paged_batch* batch, g4_bf16* q_out, int64_t out_token_stride,
+                             int64_t out_head_stride);
+
+/* Copies rows [0, rows[i]) of page src[i] to page dst[i], i < n, in K and V of every layer
+ * (`caches`: a HOST array; the layers share page_rows and n_pages, not head counts).  src,
+ * dst, rows: DEVICE int32 arrays.  No dst may be another dst or any src: the copies run at
+ * once.  Out-of-range pages and row counts are skipped or cut off, with a device status bit. */
+g4_status g4_paged_copy(g4_ctx* ctx, const g4_paged_cache* caches, int n_layers, const int32_t* src,
+                        const int32_t* dst, const int32_t* rows, int n);
+
+/* The same for whole pages, and every table entry e >= 0 becomes page_map[e]: tables
+ * [n_seqs][table_stride] with max_pages used entries per sequence, page_map[n_pages]
+ * (all DEVICE int32; page_map[p] = p for pages that stay). */
+g4_status g4_paged_compact(g4_ctx* ctx, const g4_paged_cache* caches, int n_layers, const int32_t* src,
+                           const int32_t* dst, int n, int32_t* tables, int64_t table_stride, int n_seqs,
+                           int max_pages, const int32_t* page_map);
+
+/* Which pages a cache's sequences hold: host bookkeeping, no GPU needed.  Pages are counted
+ * by their users; a fork shares every page of its parent, and the first of them to append
+ * into a shared last page gets its own copy of it. */
+typedef struct g4_page_pool g4_page_pool;
+g4_status g4_page_pool_create(int n_pages, int page_rows, g4_page_pool** out);
+g4_status g4_page_pool_destroy(g4_page_pool* pool);
+const char* g4_page_pool_last_error(const g4_page_pool* pool);
+/* A new empty sequence; its number (numbers of freed sequences are used again). */
+g4_status g4_page_pool_add(g4_page_pool* pool, int32_t* out_seq);
+/* Room for n_rows more rows: takes the free pages of the lowest numbers, and when the last
+ * page is partly filled and shared, a page for the sequence's own copy of it.  Not enough
+ * free pages: G4_ERR_TOO_LARGE, nothing changed. */
+g4_status g4_page_pool_extend(g4_page_pool* pool, int32_t seq, int n_rows);
+g4_status g4_page_pool_fork(g4_page_pool* pool, int32_t seq, int32_t* out_child);
+/* Gives back the pages that lie wholly below row first_row (below a sliding window); their
+ * table entries become -1. */
+g4_status g4_page_pool_trim(g4_page_pool* pool, int32_t seq, int first_row);
+g4_status g4_page_pool_free(g4_page_pool* pool, int32_t seq);
+/* Moves the pages in use to 0 .. n_used - 1: n moves src[i] -> dst[i] (arrays of n_pages) and
+ * page_map[n_pages] for g4_paged_compact, all in HOST memory.  Refused while copies wait. */
+g4_status g4_page_pool_compact(g4_page_pool* pool, int32_t* src, int32_t* dst, int32_t* page_map, int* out_n);
+/* The next page copies that extends asked for, in order, as host arrays for one
+ * g4_paged_copy; call until *out_n is 0.  A copy that must not run at once with an earlier one
+ * starts the next call's group. */
+g4_status g4_page_pool_take_copies(g4_page_pool* pool, int32_t* src, int32_t* dst, int32_t* rows, int cap,
+                                   int* out_n);
+/* Sequence seq's table into table[width] (-1 past its pages), its rows so far. */
+g4_status g4_page_pool_table(const g4_page_pool* pool, int32_t seq, int32_t* table, int width, int* out_rows);
+g4_status g4_page_pool_free_pages(const g4_page_pool* pool, int* out_n);
+
+/* ------------------------------------------------------------------------------ */
 /* Decode runtime (src/host/load.rs Model, src/host/runtime.rs Workspace / Decode)  */
 /* ------------------------------------------------------------------------------ */
 

@@ -325,6 +325,8 @@ g4_status g4_ctx_destroy(g4_ctx* ctx) {
   cudaFree(ctx->prefill.y);
   cudaFree(ctx->prefill.ginv);
   cudaFree(ctx->prefill.down_sf);
+  cudaFree(ctx->paged.part);
+  cudaFree(ctx->paged.tail);
   delete ctx;
   return G4_OK;
 }

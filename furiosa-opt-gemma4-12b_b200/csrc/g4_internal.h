@@ -87,6 +87,14 @@ struct PrefillBuffers {
                                // are not a multiple of 16 bytes: 8-way tensor parallel)
 };
 
+// Paged attention scratch, allocated at its first call and kept until the context is
+// destroyed: partial sums of items split between CTA pairs, and which items those are.
+struct PagedBuffers {
+  float* part = nullptr;
+  void* tail = nullptr;
+  int pairs[2] = {0, 0};  // CTA pairs the device runs at once (head_dim 256, 512)
+};
+
 }  // namespace g4
 
 struct g4_ctx {
@@ -110,6 +118,7 @@ struct g4_ctx {
   int mlp_kernel = 0;  // G4_MLP_AUTO / G4_MLP_STREAM / G4_MLP_TENSOR
   g4::PeerXch peers = {};  // TP exchange buffers mapped from every rank (world 0: NCCL path)
   g4::PrefillBuffers prefill;
+  g4::PagedBuffers paged;
   int prefill_pieces = 2;  // NVFP4 pieces per prefill activation (1..3)
 };
 

@@ -95,7 +95,7 @@ __device__ __forceinline__ uint4 ldg128(const uint16_t* p) { return *reinterpret
 __device__ __forceinline__ int seq_of_token(const PagedBatch& b, int t, int lane) {
   for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
     const int s = s0 + lane;
-    const bool mine = s < b.n_seqs && __ldg(b.q_start + s) <= t && t < __ldg(b.q_start + s + 1);
+    const bool mine = s < b.n_seqs && __ldcg(b.q_start + s) <= t && t < __ldcg(b.q_start + s + 1);
     const uint32_t hit = __ballot_sync(0xffffffffu, mine);
     if (hit != 0) return s0 + __ffs(hit) - 1;
   }
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreA
   if (pos >= a.n_positions) live = false, bad = true;
   int page = 0;
   if (live) {  // (pos < kv <= max_pages * page_rows)
-    page = __ldg(b.tables + s * b.table_stride + pos / b.page_rows);
+    page = __ldcg(b.tables + s * b.table_stride + pos / b.page_rows);
     if (page < 0 || page >= b.n_pages) live = false, bad = true;
   }
   if (bad && lane == 0) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);

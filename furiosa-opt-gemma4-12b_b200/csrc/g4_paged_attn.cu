@@ -1,7 +1,35 @@
-// Attention of a chunk of new tokens over the pages of their sequences.
+// Attention of a chunk of new tokens over the pages of their sequences, on tcgen05.
 //   o = sum_j softmax_j(scale q.k_j) v_j over the visible rows j of the token's sequence
-// One warp per (token, query head): lane l holds dims 8 l .. (and 256 + 8 l .. for D = 512),
-// one pass over the visible rows with the running maximum and sum of the softmax.
+//
+// Rows.  The query heads that share a KV head are rows of one matrix: row r of (sequence,
+// KV head) is token r / G, head r % G of the group (G = query heads per KV head).  A CTA
+// pair (cluster of 2, cta_group::2) works on a tile of 256 rows, 128 per CTA, over 128 cache
+// rows at a time: one item is (sequence, row tile, KV head), one unit of it a 128-row key tile.
+//   S[256][128] = Q K^T      each CTA stages its 128 Q rows and 64 of the 128 K rows
+//   O[256][256] += P V       each CTA stages 128 of the 256 V columns; P is read from tensor memory
+// so every K/V byte is fetched once per 256 rows (per SM pair), without multicast.  Tensor
+// memory holds O (256 columns) and two S tiles (128 each; P overwrites its S), all 512
+// columns: S of the next key tile runs while the softmax of this one does.  A head of 512 has
+// twice the O columns, so its two halves of V are two pairs' work: both compute S (1.5x the
+// products) and they run side by side, so the second fetch of K hits the L2.
+//
+// Softmax in f32 with the running maximum and sum, one thread per row.  O is rescaled only
+// when a row's maximum rises by more than 2^8 (the maximum that P is relative to may lag:
+// P <= 256 then, exact in range for f32 sums and for P's rounding to bf16).  P is rounded to
+// bf16 because kind::f16 wants both operands of the product of one 16-bit type; its error is
+// 2^-8 per weight, the size of the output's own rounding.
+//
+// Work split.  All units of the call, in order, are cut into as many equal ranges as there
+// are pairs (or half as many pairs of pairs for heads of 512), from the device-resident
+// lengths: a long cache with few rows is split along its keys, a batch of any raggedness is
+// balanced.  An item that crosses a range's end leaves partial sums (f32) that a second
+// kernel joins in range order.
+//
+// Roles of a CTA's 10 warps: 0-3 softmax and output, 4 TMA, 5 MMA (leader CTA) and tensor
+// memory, 6-9 Q rows and the V tiles at a sequence's ends (TMA cannot stop at its last row;
+// rows past it may hold NaN, and 0 * NaN is NaN, so these tiles are copied with zeros there).
+#include <cuda.h>
+
 #include <cmath>
 #include <string>
 
@@ -9,90 +37,840 @@
 
 namespace g4 {
 
+constexpr int kPaThreads = 320;
+constexpr int kPaRows = 256;      // rows per item (both CTAs)
+constexpr int kPaKeys = 128;      // cache rows per unit
+constexpr int kPaStage = 32768;   // bytes per ring stage: 64 K rows x 256 dims, or 128 V rows x 128 dims
+constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
+constexpr float kPaLag = 8.f;     // log2 of how far a row's maximum may rise before O is rescaled
+// kind::f16, D f32, A and B bf16, M = 256; S: N = 128, both K-major; O: N = 256, B (V) MN-major
+constexpr uint32_t kPaIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (16u << 17) | (16u << 24);
+constexpr uint32_t kPaIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (32u << 17) | (16u << 24);
+constexpr int kPaPartFloats = 128 * 256 + 2 * 128;  // a partial: O [128][256], then (m, l) [128][2]
+
 struct PaArgs {
   const uint16_t* q;
   long long q_ts, q_hs;
   uint16_t* out;
   long long o_ts, o_hs;
-  const uint16_t *kc, *vc;
-  long long kp, kr, kh, vp, vr, vh;
-  int n_heads, n_kv, window;
-  float scale;
+  const uint16_t* vc;
+  long long vp, vr, vh;
+  int group, n_kv, window;  // query heads per KV head, KV heads
+  float scale;              // times log2(e)
+  int k_box, v_box;         // cache rows per TMA box
+  int ranges;
+  float* part;              // [ranges][halves][2 CTAs][2][kPaPartFloats]
+  struct PaTail* tail;      // [ranges]
 };
-constexpr int kPaThreads = 256;
+// An item begun in a range and finished by later ones.
+struct PaTail {
+  int seq, tile, head, parts;  // seq -1: none
+};
 
-__device__ __forceinline__ void pa_unpack8(const uint4 w, float (&f)[8]) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+template <int D>
+struct __align__(1024) PaSmem {
+  static constexpr int kStages = D == 256 ? 5 : 3;
+  uint8_t q[D / 64][128 * 128];  // 64-dim blocks [128 rows][64], 128-byte swizzle
+  uint8_t ring[kStages][kPaStage];
+  uint64_t full[kStages], empty[kStages], s_full[2], p_full, pv_done, q_full, q_empty, edge_go, edge_done;
+  uint32_t tmem;
+  uint32_t abort;
+  long long units, first;  // of the call; of this range
+  int range_count;         // ranges in use
+  int seq, tile, head, unit;
+};
+
+// ---------------------------------------------------------------------------- PTX
+__device__ __forceinline__ uint32_t pa_map_to(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void pa_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ void pa_expect_cluster(uint32_t addr, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool pa_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait: after the budget, or once another role of the CTA gave up, false.
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort, uint64_t budget) {
+  for (int i = 0; i < 64; ++i)
+    if (pa_try(bar, parity)) return true;
+  const uint64_t end = global_ns() + budget;
+  while (!pa_try(bar, parity)) {
+    if (*abort != 0u) return false;
+    if (global_ns() > end) {
+      *abort = 1u;
+      return false;
+    }
+  }
+  return true;
+}
+// The same by a whole warp, with one answer.
+__device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort,
+                                             uint64_t budget) {
+  return __all_sync(0xffffffffu, pa_wait(bar, parity, abort, budget));
+}
+// And by the four copying warps.
+__device__ __forceinline__ bool pa_agree(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
+         (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (static_cast<uint64_t>(1u) << 46) |
+         (static_cast<uint64_t>(2u) << 61);
+}
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Arrives on the barrier at this address in both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void pa_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void pa_tma(uint32_t dst, uint64_t map, int x, int head, int row, int page,
+                                       uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(head), "r"(row), "r"(page), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pa_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(u[i] << 16);
-    f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void pa_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pa_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void pa_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pa_swizzle(int row, int c) {  // 16-byte chunk c of a 128-byte row
+  return static_cast<uint32_t>(row * 128 + (((c & 7) ^ (row & 7)) << 4));
+}
+
+// ---------------------------------------------------------------------------- work split
+// Key tiles of row tile `tile` of a sequence: [kt0, kt0 + n), n >= 1 (a tile nothing is
+// visible to still has its zeros to write).
+__device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, unsigned group, int window, int& kt0) {
+  const unsigned r0 = static_cast<unsigned>(tile) * kPaRows;
+  const int i0 = static_cast<int>(r0 / group);
+  const int i1 = min(s.n - 1, static_cast<int>((r0 + kPaRows - 1) / group));
+  const int first = s.kv - s.n;
+  const int hi = first + i1 + 1;
+  kt0 = 0;
+  if (hi <= 0) return 1;
+  if (window > 0) kt0 = max(0, first + i0 - window + 1) / kPaKeys;
+  return (hi + kPaKeys - 1) / kPaKeys - kt0;
+}
+__device__ __forceinline__ int pa_tiles(const PagedSeq& s, int group) {
+  return (s.n * group + kPaRows - 1) / kPaRows;  // (n * group < 2^30: checked by the host)
+}
+__device__ __forceinline__ long long pa_warp_sum(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ long long pa_warp_scan(long long v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+// Units of every sequence into w[]; the whole CTA.
+__device__ void pa_count(const PagedBatch& b, int group, int n_kv, int window, long long* w, Scratch* scr, bool report) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  for (int s0 = 0; s0 < b.n_seqs; s0 += kPaThreads) {
+    const int s = s0 + tid;
+    PagedSeq q = {0, 0, 0};
+    bool bad = false;
+    if (s < b.n_seqs) q = paged_seq(b, s, &bad);
+    if (report && s == 0 && b.n_seqs > 0 && __ldcg(b.q_start) < 0) bad = true;
+    if (report && bad) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
+    const int tiles = pa_tiles(q, group);
+    long long sum = 0;
+    int kt0;
+    if (tiles <= 2)
+      for (int t = 0; t < tiles; ++t) sum += pa_key_tiles(q, t, group, window, kt0);
+    for (uint32_t left = __ballot_sync(0xffffffffu, tiles > 2); left != 0; left &= left - 1) {
+      const int from = __ffs(left) - 1;
+      const PagedSeq o = {0, __shfl_sync(0xffffffffu, q.n, from), __shfl_sync(0xffffffffu, q.kv, from)};
+      long long x = 0;
+      for (int t = lane; t < pa_tiles(o, group); t += 32) x += pa_key_tiles(o, t, group, window, kt0);
+      x = pa_warp_sum(x);
+      if (lane == from) sum = x;
+    }
+    if (s < b.n_seqs) w[s] = sum * n_kv;
+  }
+}
+// Where unit number `want` (< the total) lies; one warp, every lane gets the answer.
+__device__ void pa_find(const PagedBatch& b, int group, int n_kv, int window, const long long* w, long long want,
+                        int lane, int& seq, int& tile, int& head, int& unit) {
+  long long base = 0;
+  seq = 0;
+  for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
+    const long long x = s0 + lane < b.n_seqs ? w[s0 + lane] : 0;
+    const long long incl = pa_warp_scan(x, lane);
+    const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
+    if (past != 0) {
+      const int at = __ffs(past) - 1;
+      seq = s0 + at;
+      base += __shfl_sync(0xffffffffu, incl - x, at);
+      break;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  bool bad;
+  const PagedSeq q = paged_seq(b, seq, &bad);
+  const int tiles = pa_tiles(q, group);
+  tile = 0;
+  int nk = 1, kt0;
+  for (int t0 = 0; t0 < tiles; t0 += 32) {
+    const int n = t0 + lane < tiles ? pa_key_tiles(q, t0 + lane, group, window, kt0) : 0;
+    const long long x = static_cast<long long>(n) * n_kv;
+    const long long incl = pa_warp_scan(x, lane);
+    const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
+    if (past != 0) {
+      const int at = __ffs(past) - 1;
+      tile = t0 + at;
+      nk = __shfl_sync(0xffffffffu, n, at);
+      base += __shfl_sync(0xffffffffu, incl - x, at);
+      break;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  head = static_cast<int>((want - base) / nk);
+  unit = static_cast<int>((want - base) % nk);
+}
+
+// The items of a range, in order; every role walks them alike.
+struct PaWalk {
+  const PagedBatch& b;
+  int group, n_kv, window;
+  long long left;  // units after the current item
+  int seq, tile, head;
+  PagedSeq s;
+  int kt0, nk, begin, end;  // key tiles of the current item: [begin, end) of its nk are this range's
+  int next_unit;
+  __device__ PaWalk(const PagedBatch& batch, const PaArgs& a, int seq_, int tile_, int head_, int unit_, long long n)
+      : b(batch), group(a.group), n_kv(a.n_kv), window(a.window), left(n), seq(seq_), tile(tile_), head(head_ - 1),
+        next_unit(unit_) {
+    bool bad;
+    s = left > 0 ? paged_seq(b, seq, &bad) : PagedSeq{0, 0, 0};
+  }
+  __device__ bool next() {
+    if (left <= 0) return false;
+    if (++head == n_kv) {
+      head = 0;
+      if (++tile >= pa_tiles(s, group)) {
+        bool bad;
+        tile = 0;
+        do {
+          s = paged_seq(b, ++seq, &bad);
+        } while (s.n == 0);
+      }
+    }
+    nk = pa_key_tiles(s, tile, group, window, kt0);
+    begin = next_unit;
+    next_unit = 0;
+    end = static_cast<int>(min(static_cast<long long>(nk), begin + left));
+    left -= end - begin;
+    return true;
+  }
+  // the first cache row any new token of the sequence sees
+  __device__ int low() const { return window > 0 ? max(0, s.kv - s.n - window + 1) : 0; }
+  // a V tile that reaches past the sequence's visible rows
+  __device__ bool edge(int kt) const { return (kt + 1) * kPaKeys > s.kv || kt * kPaKeys < low(); }
+};
+
+template <int D>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ PaArgs a, const __grid_constant__ PagedBatch b, Scratch* scr,
+                      uint64_t budget) {
+  using Smem = PaSmem<D>;
+  constexpr int kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 256;
+  extern __shared__ uint8_t pa_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(pa_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x & 1;  // rank in the pair
+  const int half = (blockIdx.x >> 1) % kHalves, range = (blockIdx.x >> 1) / kHalves;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 2);
+      mbar_init(&sm.empty[i], 1);
+    }
+    mbar_init(&sm.s_full[0], 1);
+    mbar_init(&sm.s_full[1], 1);
+    mbar_init(&sm.p_full, 8);
+    mbar_init(&sm.pv_done, 1);
+    mbar_init(&sm.q_full, 2);
+    mbar_init(&sm.q_empty, 1);
+    mbar_init(&sm.edge_go, 1);
+    mbar_init(&sm.edge_done, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  long long* w = reinterpret_cast<long long*>(&sm.ring[0][0]);  // (the ring is not in use yet)
+  static_assert(G4_PAGED_MAX_SEQS * 8 <= kStages * kPaStage, "unit counts fit the ring");
+  pa_count(b, a.group, a.n_kv, a.window, w, scr, blockIdx.x == 0);
+  pa_fence_before();
+  __syncthreads();
+  pa_fence_after();
+  if (warp == 0) {
+    long long u = 0;
+    for (int s = lane; s < b.n_seqs; s += 32) u += w[s];
+    u = pa_warp_sum(u);
+    const long long n = min(static_cast<long long>(a.ranges), u);  // ranges in use: each has a unit at least
+    int seq = 0, tile = 0, head = 0, unit = 0;
+    long long first = 0;
+    if (range < n) {
+      first = range * u / n;
+      pa_find(b, a.group, a.n_kv, a.window, w, first, lane, seq, tile, head, unit);
+    }
+    if (lane == 0) {
+      sm.units = u;
+      sm.first = first;
+      sm.range_count = static_cast<int>(n);
+      sm.seq = seq;
+      sm.tile = tile;
+      sm.head = head;
+      sm.unit = unit;
+    }
+    fence_proxy_async();  // the ring's next writers are TMA copies
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // both CTAs' barriers and memory are ready
+  const uint32_t tbase = sm.tmem;
+  const long long u_first = sm.first;
+  const long long u_end = range < sm.range_count ? (range + 1) * sm.units / sm.range_count : u_first;
+  volatile uint32_t* abort = &sm.abort;
+  PaWalk it(b, a, sm.seq, sm.tile, sm.head, sm.unit, u_end - u_first);
+
+  if (warp < 4) {
+    // -------------------------------------------------------------- softmax and output
+    const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
+    const uint32_t p_full = pa_map_to(smem_u32(&sm.p_full), 0);
+    uint32_t g = 0;  // unit of the range
+    PaTail tail = {-1, 0, 0, 0};
+    bool ok = true;
+    while (ok && it.next()) {
+      const unsigned rr = it.tile * kPaRows + cta * 128 + tid, group = a.group;
+      const int i = static_cast<int>(rr / group), hg = static_cast<int>(rr % group);
+      const bool valid = i < it.s.n;
+      const int pos = it.s.kv - it.s.n + i;
+      const int hi = valid ? pos + 1 : 0, lo = valid && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      float m = -CUDART_INF_F, l = 0.f;
+      for (int u = it.begin; u < it.end; ++u, ++g) {
+        const uint32_t st = tbase + kPaColS + (g & 1) * 128 + lanes;
+        ok = pa_wait_warp(&sm.s_full[g & 1], (g >> 1) & 1, abort, budget);
+        if (!ok) break;
+        pa_fence_after();
+        float s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) pa_ld32(st + 32 * c, s[c]);
+        pa_ld_wait();
+        const int base = (it.kt0 + u) * kPaKeys;
+        if (__any_sync(0xffffffffu, valid && (hi < base + kPaKeys || lo > base))) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int key = base + 32 * c + j;
+              s[c][j] = key >= lo && key < hi ? s[c][j] * a.scale : -CUDART_INF_F;
+            }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[c][j] *= a.scale;
+        }
+        float mx = -CUDART_INF_F;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, s[c][j]);
+        // the reference maximum: the first one seen, moved only when it lags too far
+        float factor = 1.f;
+        if (m == -CUDART_INF_F) {
+          m = mx;
+        } else if (mx > m + kPaLag) {
+          factor = pa_exp2(m - mx);
+          l *= factor;
+          m = mx;
+        }
+        const float ref = m == -CUDART_INF_F ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          uint32_t p[32];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float e0 = pa_exp2(s[c][j] - ref), e1 = pa_exp2(s[c][j + 1] - ref);
+            const float f0 = pa_exp2(s[c + 1][j] - ref), f1 = pa_exp2(s[c + 1][j + 1] - ref);
+            sum[0] += e0;
+            sum[1] += e1;
+            sum[2] += f0;
+            sum[3] += f1;
+            p[j / 2] = pack_bf16x2(e0, e1);
+            p[16 + j / 2] = pack_bf16x2(f0, f1);
+          }
+          pa_st32(st + 16 * c, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (u != it.begin) {  // the previous P V is done: O may be rescaled, and this unit's may follow
+          ok = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
+          if (!ok) break;
+          if (__any_sync(0xffffffffu, factor != 1.f)) {
+            pa_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 256; c += 32) {
+              float o[32];
+              uint32_t r[32];
+              pa_ld32(tbase + lanes + c, o);
+              pa_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(o[j] * factor);
+              pa_st32(tbase + lanes + c, r);
+            }
+          }
+        }
+        pa_st_wait();
+        pa_fence_before();
+        __syncwarp();
+        if (lane == 0) pa_arrive_cluster(p_full);
+      }
+      ok = ok && pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
+      if (!ok) break;
+      pa_fence_after();
+      const bool whole = it.begin == 0 && it.end == it.nk;
+      if (it.begin == 0 && it.end < it.nk) {
+        // the item's last unit is number u_end - it.end + it.nk - 1 of the call
+        const long long last = u_end - it.end + it.nk - 1;
+        const long long e = ((last + 1) * sm.range_count - 1) / sm.units;
+        tail = {it.seq, it.tile, it.head, static_cast<int>(e) - range + 1};
+      }
+      if (whole) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        uint16_t* dst = a.out + (it.s.t0 + i) * a.o_ts + (it.head * a.group + hg) * a.o_hs + 256 * half;
+#pragma unroll 1
+        for (int c = 0; c < 256; c += 32) {
+          float o[32];
+          pa_ld32(tbase + lanes + c, o);
+          pa_ld_wait();
+          if (valid) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              *reinterpret_cast<uint4*>(dst + c + j) =
+                  make_uint4(pack_bf16x2(o[j] * inv, o[j + 1] * inv), pack_bf16x2(o[j + 2] * inv, o[j + 3] * inv),
+                             pack_bf16x2(o[j + 4] * inv, o[j + 5] * inv), pack_bf16x2(o[j + 6] * inv, o[j + 7] * inv));
+          }
+        }
+      } else {
+        float* part = a.part + (((static_cast<size_t>(range) * kHalves + half) * 2 + cta) * 2 + (it.begin == 0 ? 1 : 0)) *
+                                   kPaPartFloats;
+#pragma unroll 1
+        for (int c = 0; c < 256; c += 32) {
+          float o[32];
+          pa_ld32(tbase + lanes + c, o);
+          pa_ld_wait();
+          if (valid) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<float4*>(part + tid * 256 + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        *reinterpret_cast<float2*>(part + 128 * 256 + 2 * tid) = make_float2(m, l);
+      }
+    }
+    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+    if (tid == 0 && cta == 0 && half == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
+  } else if (warp == 4) {
+    // -------------------------------------------------------------- TMA
+    uint32_t c = 0, edges = 0;  // stages filled, V tiles left to the copying warps
+    const uint64_t kmap_at = reinterpret_cast<uint64_t>(&kmap), vmap_at = reinterpret_cast<uint64_t>(&vmap);
+    const int k_boxes = 64 / a.k_box, v_boxes = kPaKeys / a.v_box;
+    bool ok = true, bad_page = false;
+    // one box per lane: K (chunk >= 0): 4 dim blocks x the CTA's 64 rows; V: 2 dim blocks x 128 rows
+    auto fill = [&](int kt, int chunk) {
+      const int stage = c % kStages;
+      if (c >= kStages) ok = pa_wait_warp(&sm.empty[stage], (c / kStages - 1) & 1, abort, budget);
+      ++c;
+      if (!ok) return;
+      if (chunk < 0 && it.edge(kt)) {
+        if (edges > 0) ok = pa_wait_warp(&sm.edge_done, (edges - 1) & 1, abort, budget);
+        if (ok && lane == 0) mbar_arrive(&sm.edge_go);
+        ++edges;
+        return;
+      }
+      const int slab = chunk >= 0 ? lane & 3 : lane & 1, rb = chunk >= 0 ? lane >> 2 : lane >> 1;
+      const int box = chunk >= 0 ? a.k_box : a.v_box;
+      const int in_tile = rb * box;
+      const int row = kt * kPaKeys + (chunk >= 0 ? 64 * cta : 0) + in_tile;
+      const bool mine = rb < (chunk >= 0 ? k_boxes : v_boxes) && row < it.s.kv && row + box > it.low();
+      int page = 0;
+      if (mine) {
+        page = __ldcg(b.tables + it.seq * b.table_stride + row / b.page_rows);
+        if (page < 0 || page >= b.n_pages) {
+          bad_page = true;
+          page = b.n_pages;  // out of the map's bounds: zeros
+        }
+      }
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine));
+      const uint32_t bar = pa_map_to(smem_u32(&sm.full[stage]), 0);
+      if (lane == 0) pa_expect_cluster(bar, n * box * 128u);
+      __syncwarp();
+      if (mine) {
+        const uint32_t dst = smem_u32(&sm.ring[stage][0]) + slab * (chunk >= 0 ? 8192u : 16384u) + in_tile * 128u;
+        const int x = chunk >= 0 ? 256 * chunk + 64 * slab : 256 * half + 128 * cta + 64 * slab;
+        pa_tma(dst, chunk >= 0 ? kmap_at : vmap_at, x, it.head, row % b.page_rows, page, bar);
+      }
+    };
+    while (ok && it.next()) {
+      for (int u = it.begin - 1; u < it.end && ok; ++u) {
+        if (u + 1 < it.end)
+          for (int ch = 0; ch < kChunks; ++ch) fill(it.kt0 + u + 1, ch);
+        if (u >= it.begin) fill(it.kt0 + u, -1);
+      }
+    }
+    // every stage is free again: no barrier of this CTA has an arrival outstanding when it exits
+    for (uint32_t x = c > kStages ? c - kStages : 0; x < c && ok; ++x)
+      ok = pa_wait_warp(&sm.empty[x % kStages], (x / kStages) & 1, abort, budget);
+    if (bad_page) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
+    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+  } else if (warp == 5) {
+    // -------------------------------------------------------------- MMA: one thread of the leader CTA
+    if (cta == 0 && lane == 0) {
+      uint32_t c = 0, g = 0, items = 0;
+      bool ok = true;
+      const uint32_t qb = smem_u32(&sm.q[0][0]);
+      auto scores = [&](uint32_t unit) {
+        for (int ch = 0; ch < kChunks && ok; ++ch, ++c) {
+          const int stage = c % kStages;
+          ok = pa_wait(&sm.full[stage], (c / kStages) & 1, abort, budget);
+          if (!ok) return;
+          pa_fence_after();
+          const uint32_t kb = smem_u32(&sm.ring[stage][0]);
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            pa_mma_ss(tbase + kPaColS + (unit & 1) * 128,
+                      pa_desc(qb + (4 * ch + (k >> 2)) * 16384 + 32 * (k & 3), 16, 1024),
+                      pa_desc(kb + (k >> 2) * 8192 + 32 * (k & 3), 16, 1024), kPaIdescS, (ch | k) ? 1u : 0u);
+          pa_commit(&sm.empty[stage]);
+        }
+        pa_commit(&sm.s_full[unit & 1]);
+      };
+      while (ok && it.next()) {
+        ok = pa_wait(&sm.q_full, items & 1, abort, budget);
+        ++items;
+        if (!ok) break;
+        for (int u = it.begin - 1; u < it.end && ok; ++u) {
+          if (u + 1 < it.end) {
+            scores(g + (u + 1 - it.begin));
+            if (!ok) break;
+            if (u + 2 == it.end) pa_commit(&sm.q_empty);
+          }
+          if (u < it.begin) continue;
+          const uint32_t unit = g + (u - it.begin);
+          const int stage = c % kStages;
+          ok = pa_wait(&sm.p_full, unit & 1, abort, budget) &&
+               pa_wait(&sm.full[stage], (c / kStages) & 1, abort, budget);
+          ++c;
+          if (!ok) break;
+          pa_fence_after();
+          const uint32_t vb = smem_u32(&sm.ring[stage][0]);
+#pragma unroll
+          for (int k = 0; k < kPaKeys / 16; ++k)
+            pa_mma_ts(tbase, tbase + kPaColS + (unit & 1) * 128 + 8 * k, pa_desc(vb + 2048 * k, 16384, 1024),
+                      kPaIdescO, (u > it.begin || k) ? 1u : 0u);
+          pa_commit(&sm.empty[stage]);
+          pa_commit(&sm.pv_done);
+        }
+        g += it.end - it.begin;
+      }
+      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+    }
+  } else {
+    // -------------------------------------------------------------- Q rows; V tiles at the ends
+    const int lt = tid - 192;
+    uint32_t c = 0, items = 0, edges = 0;
+    bool ok = true;
+    const uint32_t q_full = pa_map_to(smem_u32(&sm.q_full), 0);
+    while (ok && it.next()) {
+      if (items > 0) ok = pa_agree(pa_wait(&sm.q_empty, (items - 1) & 1, abort, budget));
+      ++items;
+      if (!ok) break;
+      {
+        const unsigned r0 = it.tile * kPaRows + cta * 128, group = a.group;
+        const uint32_t qb = smem_u32(&sm.q[0][0]);
+        constexpr int kRowChunks = D / 8;
+#pragma unroll 4
+        for (int x = lt; x < 128 * kRowChunks; x += 128) {
+          const int row = x / kRowChunks, ch = x % kRowChunks;
+          const int i = static_cast<int>((r0 + row) / group), hg = static_cast<int>((r0 + row) % group);
+          const bool in = i < it.s.n;
+          const uint16_t* src =
+              in ? a.q + (it.s.t0 + i) * a.q_ts + (it.head * a.group + hg) * a.q_hs + 8 * ch : a.q;
+          cp_async16(qb + (ch >> 3) * 16384 + pa_swizzle(row, ch), src, in ? 16u : 0u);
+        }
+      }
+      cp_async_wait_all();
+      asm volatile("fence.proxy.async;" ::: "memory");
+      named_bar_sync(2, 128);
+      if (lt == 0) pa_arrive_cluster(q_full);
+      for (int u = it.begin - 1; u < it.end && ok; ++u) {
+        if (u + 1 < it.end) c += kChunks;
+        if (u < it.begin) continue;
+        const int kt = it.kt0 + u, stage = c % kStages;
+        ++c;
+        if (!it.edge(kt)) continue;
+        ok = pa_agree(pa_wait(&sm.edge_go, edges & 1, abort, budget));
+        ++edges;
+        if (!ok) break;
+        const uint32_t vb = smem_u32(&sm.ring[stage][0]);
+#pragma unroll 4
+        for (int x = lt; x < kPaKeys * 16; x += 128) {
+          const int r = x >> 4, ch = x & 15, row = kt * kPaKeys + r;
+          bool in = row >= it.low() && row < it.s.kv;
+          const uint16_t* src = a.vc;
+          if (in) {
+            const int page = __ldcg(b.tables + it.seq * b.table_stride + row / b.page_rows);
+            if (page >= 0 && page < b.n_pages)
+              src = a.vc + page * a.vp + (row % b.page_rows) * a.vr + it.head * a.vh + 256 * half + 128 * cta + 8 * ch;
+            else
+              in = false;
+          }
+          cp_async16(vb + (ch >> 3) * 16384 + pa_swizzle(r, ch), src, in ? 16u : 0u);
+        }
+        cp_async_wait_all();
+        asm volatile("fence.proxy.async;" ::: "memory");
+        named_bar_sync(2, 128);
+        if (lt == 0) {
+          pa_arrive_cluster(pa_map_to(smem_u32(&sm.full[stage]), 0));
+          mbar_arrive(&sm.edge_done);
+        }
+      }
+    }
+    if (ok && items > 0) ok = pa_wait(&sm.q_empty, (items - 1) & 1, abort, budget);
+    if (!ok && lt == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+  }
+  __syncthreads();
+  if (sm.abort != 0) {  // gave up somewhere: let the copies in flight land (bounded)
+    const uint64_t end = global_ns() + 1000000;
+    while (global_ns() < end) __nanosleep(1000);
+  }
+  pa_fence_before();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  pa_fence_after();
+  if (warp == 5)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512u));
+}
+
+// Joins the parts of the items that cross range ends: with M the largest of the parts' reference
+// maxima, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in range order.  A block has two rows.
+constexpr int kPaJoinThreads = 128;
+template <int D>
+__global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid_constant__ PaArgs a,
+                                                                    const __grid_constant__ PagedBatch b) {
+  constexpr int kHalves = D / 256;
+  pdl_wait();
+  pdl_launch_dependents();
+  const PaTail t = a.tail[blockIdx.x];
+  if (t.seq < 0) return;
+  bool bad;
+  const PagedSeq s = paged_seq(b, t.seq, &bad);
+  const int col = (threadIdx.x & 63) * 4;
+  const int r = blockIdx.y * 2 + (threadIdx.x >> 6);
+  const unsigned rr = t.tile * kPaRows + r, group = a.group;
+  const int i = static_cast<int>(rr / group), hg = static_cast<int>(rr % group);
+  if (i >= s.n) return;
+  const int cta = r >> 7, row = r & 127;
+  auto part = [&](int k, int half) {  // the first part is its range's second slot, the others their first
+    return a.part + (((static_cast<size_t>(blockIdx.x + k) * kHalves + half) * 2 + cta) * 2 + (k == 0 ? 1 : 0)) *
+                        kPaPartFloats;
+  };
+  uint16_t* dst = a.out + (s.t0 + i) * a.o_ts + (t.head * a.group + hg) * a.o_hs + col;
+#pragma unroll
+  for (int half = 0; half < kHalves; ++half) {
+    float top = -CUDART_INF_F;
+#pragma unroll 8
+    for (int k = 0; k < t.parts; ++k) top = fmaxf(top, part(k, half)[128 * 256 + 2 * row]);
+    const float ref = top == -CUDART_INF_F ? 0.f : top;
+    float l = 0.f, o[4] = {};
+#pragma unroll 8
+    for (int k = 0; k < t.parts; ++k) {
+      const float2 ml = *reinterpret_cast<const float2*>(part(k, half) + 128 * 256 + 2 * row);
+      const float4 v = *reinterpret_cast<const float4*>(part(k, half) + row * 256 + col);
+      const float w = pa_exp2(ml.x - ref);
+      l = fmaf(w, ml.y, l);
+      o[0] = fmaf(w, v.x, o[0]);
+      o[1] = fmaf(w, v.y, o[1]);
+      o[2] = fmaf(w, v.z, o[2]);
+      o[3] = fmaf(w, v.w, o[3]);
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    *reinterpret_cast<uint2*>(dst + 256 * half) =
+        make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
   }
 }
 
+// ---------------------------------------------------------------------------- host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// The pages as a 4-D tensor (dims, heads, rows, pages), box 64 x 1 x rows x 1, 128-byte swizzle.
+static bool page_map(CUtensorMap* m, const uint16_t* base, const g4_paged_cache* c, int64_t page_stride,
+                     int64_t row_stride, int64_t head_stride, int rows) {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+               ? reinterpret_cast<EncodeFn>(p)
+               : nullptr;
+  }();
+  if (fn == nullptr) return false;
+  // the stride of a dimension of size one is never used, but has to be a legal one
+  auto bytes = [&](int64_t stride, int n) { return static_cast<cuuint64_t>(n > 1 ? stride : c->head_dim) * 2; };
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->head_dim), static_cast<cuuint64_t>(c->n_kv_heads),
+                              static_cast<cuuint64_t>(c->page_rows), static_cast<cuuint64_t>(c->n_pages)};
+  const cuuint64_t strides[3] = {bytes(head_stride, c->n_kv_heads), bytes(row_stride, c->page_rows),
+                                 bytes(page_stride, c->n_pages)};
+  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Scratch of the split items, allocated at the first call: room for every pair of CTAs.
+static g4_status attn_scratch(g4_ctx* ctx, int pairs) {
+  if (ctx->paged.part != nullptr) return G4_OK;
+  const size_t part = static_cast<size_t>(pairs) * 4 * kPaPartFloats * sizeof(float);
+  g4_status st = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice");
+  if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&ctx->paged.tail, pairs * sizeof(PaTail)), "cudaMalloc paged tails");
+  if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&ctx->paged.part, part), "cudaMalloc paged partials");
+  return st;
+}
+
 template <int D>
-__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a, const PagedBatch b, Scratch* scr) {
-  constexpr int C = D / 256;
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kPaThreads / 32) + (threadIdx.x >> 5);
-  const int t = static_cast<int>(unit / a.n_heads), h = static_cast<int>(unit % a.n_heads);
-  if (unit == 0) paged_check_batch(b, lane, scr);
-  if (t >= b.n_tokens) return;
-  int s = -1;
-  for (int s0 = 0; s0 < b.n_seqs && s < 0; s0 += 32) {
-    const int i = s0 + lane;
-    const bool mine = i < b.n_seqs && b.q_start[i] <= t && t < b.q_start[i + 1];
-    const uint32_t hit = __ballot_sync(0xffffffffu, mine);
-    if (hit != 0) s = s0 + __ffs(hit) - 1;
+static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_paged_cache* c) {
+  const void* fn = (const void*)paged_attn_kernel<D>;
+  const size_t smem = sizeof(PaSmem<D>) + 1024;
+  g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "paged attention");
+  if (st != G4_OK) return st;
+  int& pairs = ctx->paged.pairs[D == 256 ? 0 : 1];
+  if (pairs == 0) {  // CTA pairs the device runs at once: a range too many would run alone at the end
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctx->sm_count / 2 * 2);
+    cfg.blockDim = dim3(kPaThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    st = check_cuda(ctx, cudaOccupancyMaxActiveClusters(&n, fn, &cfg), "paged attention: active clusters");
+    if (st != G4_OK) return st;
+    n = n < ctx->sm_count / 2 ? n : ctx->sm_count / 2;
+    if (n < 2) return fail(ctx, G4_ERR_UNSUPPORTED, "paged attention: CTA pairs do not fit this device");
+    pairs = n;
   }
-  if (s < 0) return;
-  bool bad;
-  const PagedSeq sq = paged_seq(b, s, &bad);
-  const int pos = sq.kv - sq.n + (t - sq.t0);
-  const int hk = h / (a.n_heads / a.n_kv);
-  float q[C][8], o[C][8] = {}, m = -CUDART_INF_F, l = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-    pa_unpack8(*reinterpret_cast<const uint4*>(a.q + t * a.q_ts + h * a.q_hs + 256 * c + 8 * lane), q[c]);
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  for (int j = lo; j <= pos; ++j) {
-    const int page = b.tables[s * b.table_stride + j / b.page_rows];
-    if (page < 0 || page >= b.n_pages) {
-      bad = true;
-      continue;
-    }
-    const long long row = j % b.page_rows;
-    const uint16_t* kr = a.kc + page * a.kp + row * a.kr + hk * a.kh;
-    const uint16_t* vr = a.vc + page * a.vp + row * a.vr + hk * a.vh;
-    float dot = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float k[8];
-      pa_unpack8(*reinterpret_cast<const uint4*>(kr + 256 * c + 8 * lane), k);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dot = fmaf(q[c][i], k[i], dot);
-    }
-    dot = warp_sum(dot) * a.scale;
-    const float mn = fmaxf(m, dot);
-    const float corr = m == -CUDART_INF_F ? 0.f : __expf(m - mn), p = __expf(dot - mn);
-    l = l * corr + p;
-    m = mn;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float v[8];
-      pa_unpack8(*reinterpret_cast<const uint4*>(vr + 256 * c + 8 * lane), v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[c][i] = fmaf(p, v[i], o[c][i] * corr);
-    }
-  }
-  if (bad && lane == 0) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-    *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + 256 * c + 8 * lane) =
-        make_uint4(pack_bf16x2(o[c][0] * inv, o[c][1] * inv), pack_bf16x2(o[c][2] * inv, o[c][3] * inv),
-                   pack_bf16x2(o[c][4] * inv, o[c][5] * inv), pack_bf16x2(o[c][6] * inv, o[c][7] * inv));
+  if ((st = attn_scratch(ctx, ctx->sm_count / 2)) != G4_OK) return st;
+  a.part = ctx->paged.part;
+  a.tail = static_cast<PaTail*>(ctx->paged.tail);
+  // no more ranges than units there can be: row tiles x heads x key tiles
+  const long long rows = static_cast<long long>(b.n_tokens) * a.group;
+  const long long tiles = rows / kPaRows + (b.n_seqs < b.n_tokens ? b.n_seqs : b.n_tokens);
+  const long long keys = (static_cast<long long>(b.max_pages) * b.page_rows + kPaKeys - 1) / kPaKeys;
+  const long long most = tiles * a.n_kv * (keys < 1 ? 1 : keys);
+  a.ranges = pairs / (D / 256);
+  if (most < a.ranges) a.ranges = static_cast<int>(most);
+  const int low = b.page_rows & -b.page_rows;  // the largest power of two that divides a page's rows
+  a.k_box = low < 64 ? low : 64;
+  a.v_box = low < kPaKeys ? low : kPaKeys;
+  CUtensorMap km, vm;
+  if (!page_map(&km, c->k, c, c->k_page_stride, c->k_row_stride, c->k_head_stride, a.k_box) ||
+      !page_map(&vm, c->v, c, c->v_page_stride, c->v_row_stride, c->v_head_stride, a.v_box))
+    return fail(ctx, G4_ERR_UNSUPPORTED, "paged attention: the cache's layout has no TMA descriptor");
+  Scratch* scr = ctx->buf.scratch;
+  uint64_t budget = ctx->wait_budget_ns;
+  void* args[] = {(void*)&km, (void*)&vm, (void*)&a, (void*)&b, (void*)&scr, (void*)&budget};
+  st = launch_kernel(ctx, fn, dim3(a.ranges * (D / 256) * 2), dim3(kPaThreads), smem, args, false, "paged attention");
+  if (st != G4_OK) return st;
+  void* jargs[] = {(void*)&a, (void*)&b};
+  const int row_pairs = static_cast<int>(((rows < kPaRows ? rows : kPaRows) + 1) / 2);
+  return launch_kernel(ctx, (const void*)paged_join_kernel<D>, dim3(a.ranges, row_pairs), dim3(kPaJoinThreads), 0,
+                       jargs, false, "paged attention join");
 }
 
 }  // namespace g4
@@ -113,20 +891,29 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   if (window < 0) return fail(ctx, G4_ERR_BAD_ARG, "negative window");
   if (!std::isfinite(scale)) return fail(ctx, G4_ERR_BAD_ARG, "scale is not finite");
   if (batch->n_tokens == 0 || batch->n_seqs == 0) return G4_OK;
+  if (static_cast<long long>(batch->n_tokens) * (n_heads / cache->n_kv_heads) > (1 << 30))
+    return fail(ctx, G4_ERR_BAD_ARG, "too many tokens times query heads per KV head for one call");
   if ((st = check_rows(ctx, q, q_token_stride, q_head_stride, "q")) != G4_OK) return st;
   if ((st = check_out_rows(ctx, out, out_token_stride, out_head_stride, batch->n_tokens, n_heads, cache->head_dim,
                            "out")) != G4_OK)
     return st;
-  PaArgs a = {q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, cache->k, cache->v,
-              cache->k_page_stride, cache->k_row_stride, cache->k_head_stride, cache->v_page_stride,
-              cache->v_row_stride, cache->v_head_stride, n_heads, cache->n_kv_heads, window, scale};
-  PagedBatch b = paged_batch(batch, cache);
-  Scratch* scr = ctx->buf.scratch;
-  const long long warps = static_cast<long long>(batch->n_tokens) * n_heads;
-  void* args[] = {(void*)&a, (void*)&b, (void*)&scr};
-  const void* fn = cache->head_dim == DS ? (const void*)paged_attn_kernel<DS> : (const void*)paged_attn_kernel<DF>;
-  return launch_kernel(ctx, fn, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(kPaThreads), 0, args, false,
-                       "paged attention");
+  PaArgs a = {};
+  a.q = q;
+  a.q_ts = q_token_stride;
+  a.q_hs = q_head_stride;
+  a.out = out;
+  a.o_ts = out_token_stride;
+  a.o_hs = out_head_stride;
+  a.vc = cache->v;
+  a.vp = cache->v_page_stride;
+  a.vr = cache->v_row_stride;
+  a.vh = cache->v_head_stride;
+  a.group = n_heads / cache->n_kv_heads;
+  a.n_kv = cache->n_kv_heads;
+  a.window = window;
+  a.scale = scale * 1.4426950408889634f;
+  const PagedBatch b = paged_batch(batch, cache);
+  return cache->head_dim == DS ? launch_attention<DS>(ctx, a, b, cache) : launch_attention<DF>(ctx, a, b, cache);
 }
 
 }  // extern "C"

@@ -25,8 +25,8 @@
 // balanced.  An item that crosses a range's end leaves partial sums (f32) that a second
 // kernel joins in range order.
 //
-// Roles of a CTA's 10 warps: 0-3 softmax and output, 4 TMA, 5 MMA (leader CTA) and tensor
-// memory, 6-9 Q rows and the V tiles at a sequence's ends (TMA cannot stop at its last row;
+// Roles of a CTA's 8 warps: 0-3 softmax and output, 4 TMA, 5 MMA (leader CTA) and tensor
+// memory, 6-7 Q rows and the V tiles at a sequence's ends (TMA cannot stop at its last row;
 // rows past it may hold NaN, and 0 * NaN is NaN, so these tiles are copied with zeros there).
 #include <cuda.h>
 
@@ -37,16 +37,16 @@
 
 namespace g4 {
 
-constexpr int kPaThreads = 320;
+constexpr int kPaThreads = 256;
 constexpr int kPaRows = 256;      // rows per item (both CTAs)
 constexpr int kPaKeys = 128;      // cache rows per unit
-constexpr int kPaStage = 32768;   // bytes per ring stage: 64 K rows x 256 dims, or 128 V rows x 128 dims
+constexpr int kPaStage = 16384;   // bytes per ring stage: 64 K rows x 128 dims, or 64 V rows x 128 dims
 constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
 constexpr float kPaLag = 8.f;     // log2 of how far a row's maximum may rise before O is rescaled
 // kind::f16, D f32, A and B bf16, M = 256; S: N = 128, both K-major; O: N = 256, B (V) MN-major
 constexpr uint32_t kPaIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (16u << 17) | (16u << 24);
 constexpr uint32_t kPaIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (32u << 17) | (16u << 24);
-constexpr int kPaPartFloats = 128 * 256 + 2 * 128;  // a partial: O [128][256], then (m, l) [128][2]
+constexpr int kPaPartFloats = 128 * 256 + 2 * 128;  // a partial: O as [64 column quads][128 rows][4], then (m, l) [128][2]
 
 struct PaArgs {
   const uint16_t* q;
@@ -57,7 +57,7 @@ struct PaArgs {
   long long vp, vr, vh;
   int group, n_kv, window;  // query heads per KV head, KV heads
   float scale;              // times log2(e)
-  int k_box, v_box;         // cache rows per TMA box
+  int box;                  // cache rows per TMA box
   int ranges;
   float* part;              // [ranges][halves][2 CTAs][2][kPaPartFloats]
   struct PaTail* tail;      // [ranges]
@@ -69,7 +69,7 @@ struct PaTail {
 
 template <int D>
 struct __align__(1024) PaSmem {
-  static constexpr int kStages = D == 256 ? 5 : 3;
+  static constexpr int kStages = D == 256 ? 10 : 6;
   uint8_t q[D / 64][128 * 128];  // 64-dim blocks [128 rows][64], 128-byte swizzle
   uint8_t ring[kStages][kPaStage];
   uint64_t full[kStages], empty[kStages], s_full[2], p_full, pv_done, q_full, q_empty, edge_go, edge_done;
@@ -89,27 +89,44 @@ __device__ __forceinline__ uint32_t pa_map_to(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void pa_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
+// Relaxed: what they announce is ordered by the copies themselves (expect) or by the tensor
+// memory fences around them (P).  A release at cluster scope costs about 1000 cycles here.
 __device__ __forceinline__ void pa_expect_cluster(uint32_t addr, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes)
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes)
                : "memory");
 }
+__device__ __forceinline__ void pa_arrive_relaxed(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// kWide: the barrier also announces ordinary stores of the other CTA's threads.
+template <bool kWide>
 __device__ __forceinline__ bool pa_try(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
+  if (kWide)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
   return ok != 0;
 }
 // Bounded wait: after the budget, or once another role of the CTA gave up, false.
+template <bool kWide = false>
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort, uint64_t budget) {
   for (int i = 0; i < 64; ++i)
-    if (pa_try(bar, parity)) return true;
+    if (pa_try<kWide>(bar, parity)) return true;
   const uint64_t end = global_ns() + budget;
-  while (!pa_try(bar, parity)) {
+  while (!pa_try<kWide>(bar, parity)) {
     if (*abort != 0u) return false;
     if (global_ns() > end) {
       *abort = 1u;
@@ -123,12 +140,12 @@ __device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, vol
                                              uint64_t budget) {
   return __all_sync(0xffffffffu, pa_wait(bar, parity, abort, budget));
 }
-// And by the four copying warps.
+// And by the two copying warps.
 __device__ __forceinline__ bool pa_agree(bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "barrier.cta.red.and.pred q, 2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"(static_cast<uint32_t>(ok))
       : "memory");
@@ -200,6 +217,56 @@ __device__ __forceinline__ float pa_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pa_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void pa_unpair(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pa_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// The 16-byte chunks w[4 j .. 4 j + 3] (j < 4) of the four lanes of a quad, transposed: lane q
+// gets chunk q of the quad's lane j in place j.
+__device__ __forceinline__ void pa_quad_transpose(uint32_t (&w)[16], int lane) {
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1) {
+    const bool up = (lane & bit) != 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & bit) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t give = up ? w[4 * j + i] : w[4 * (j | bit) + i];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, bit);
+        if (up)
+          w[4 * j + i] = got;
+        else
+          w[4 * (j | bit) + i] = got;
+      }
+    }
+  }
 }
 __device__ __forceinline__ uint32_t pa_swizzle(int row, int c) {  // 16-byte chunk c of a 128-byte row
   return static_cast<uint32_t>(row * 128 + (((c & 7) ^ (row & 7)) << 4));
@@ -347,7 +414,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
                       const __grid_constant__ PaArgs a, const __grid_constant__ PagedBatch b, Scratch* scr,
                       uint64_t budget) {
   using Smem = PaSmem<D>;
-  constexpr int kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 256;
+  constexpr int kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 128;  // a K tile is kChunks stages
   extern __shared__ uint8_t pa_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(pa_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -416,6 +483,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // -------------------------------------------------------------- softmax and output
     const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
     const uint32_t p_full = pa_map_to(smem_u32(&sm.p_full), 0);
+    // scores are scaled within the exponent's FMA; a scale that is not positive goes first
+    const bool scale_first = !(a.scale > 0.f);
+    const float factor_s = scale_first ? 1.f : a.scale;
     uint32_t g = 0;  // unit of the range
     PaTail tail = {-1, 0, 0, 0};
     bool ok = true;
@@ -423,6 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const unsigned rr = it.tile * kPaRows + cta * 128 + tid, group = a.group;
       const int i = static_cast<int>(rr / group), hg = static_cast<int>(rr % group);
       const bool valid = i < it.s.n;
+      const bool any_row = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps step
       const int pos = it.s.kv - it.s.n + i;
       const int hi = valid ? pos + 1 : 0, lo = valid && a.window > 0 ? max(0, pos - a.window + 1) : 0;
       float m = -CUDART_INF_F, l = 0.f;
@@ -430,59 +501,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         const uint32_t st = tbase + kPaColS + (g & 1) * 128 + lanes;
         ok = pa_wait_warp(&sm.s_full[g & 1], (g >> 1) & 1, abort, budget);
         if (!ok) break;
-        pa_fence_after();
-        float s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) pa_ld32(st + 32 * c, s[c]);
-        pa_ld_wait();
-        const int base = (it.kt0 + u) * kPaKeys;
-        if (__any_sync(0xffffffffu, valid && (hi < base + kPaKeys || lo > base))) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int key = base + 32 * c + j;
-              s[c][j] = key >= lo && key < hi ? s[c][j] * a.scale : -CUDART_INF_F;
-            }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s[c][j] *= a.scale;
-        }
-        float mx = -CUDART_INF_F;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, s[c][j]);
-        // the reference maximum: the first one seen, moved only when it lags too far
         float factor = 1.f;
-        if (m == -CUDART_INF_F) {
-          m = mx;
-        } else if (mx > m + kPaLag) {
-          factor = pa_exp2(m - mx);
-          l *= factor;
-          m = mx;
-        }
-        const float ref = m == -CUDART_INF_F ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (any_row) {
+          pa_fence_after();
+          float s[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          uint32_t p[32];
+          for (int c = 0; c < 4; ++c) pa_ld32(st + 32 * c, s[c]);
+          pa_ld_wait();
+          if (scale_first) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float e0 = pa_exp2(s[c][j] - ref), e1 = pa_exp2(s[c][j + 1] - ref);
-            const float f0 = pa_exp2(s[c + 1][j] - ref), f1 = pa_exp2(s[c + 1][j + 1] - ref);
-            sum[0] += e0;
-            sum[1] += e1;
-            sum[2] += f0;
-            sum[3] += f1;
-            p[j / 2] = pack_bf16x2(e0, e1);
-            p[16 + j / 2] = pack_bf16x2(f0, f1);
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) s[c][j] *= a.scale;
           }
-          pa_st32(st + 16 * c, p);
+          const int base = (it.kt0 + u) * kPaKeys;
+          if (__any_sync(0xffffffffu, valid && (hi < base + kPaKeys || lo > base))) {
+            const int first = lo - base, count = hi - lo;  // visible: first <= column < first + count
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int x = 32 * c + j - first;
+                s[c][j] = x >= 0 && x < count ? s[c][j] : -CUDART_INF_F;
+              }
+          }
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            mx[c] = pa_max3(s[c][0], s[c][1], s[c][2]);
+#pragma unroll
+            for (int j = 3; j < 31; j += 2) mx[c] = pa_max3(mx[c], s[c][j], s[c][j + 1]);
+            mx[c] = fmaxf(mx[c], s[c][31]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * factor_s;
+          // the reference maximum: the first one seen, moved only when it lags too far
+          if (m == -CUDART_INF_F) {
+            m = top;
+          } else if (top > m + kPaLag) {
+            factor = pa_exp2(m - top);
+            l *= factor;
+            m = top;
+          }
+          const float ref = m == -CUDART_INF_F ? 0.f : -m;
+          const uint64_t f2 = pa_pair(factor_s, factor_s), r2 = pa_pair(ref, ref);
+          uint64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            uint32_t p[32];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float e0, e1, f0, f1;
+              pa_unpair(pa_fma2(pa_pair(s[c][j], s[c][j + 1]), f2, r2), e0, e1);
+              pa_unpair(pa_fma2(pa_pair(s[c + 1][j], s[c + 1][j + 1]), f2, r2), f0, f1);
+              e0 = pa_exp2(e0);
+              e1 = pa_exp2(e1);
+              f0 = pa_exp2(f0);
+              f1 = pa_exp2(f1);
+              sum[(j >> 1) & 1] = pa_add2(sum[(j >> 1) & 1], pa_pair(e0, e1));
+              sum[2 + ((j >> 1) & 1)] = pa_add2(sum[2 + ((j >> 1) & 1)], pa_pair(f0, f1));
+              p[j / 2] = pa_bf16x2(e0, e1);
+              p[16 + j / 2] = pa_bf16x2(f0, f1);
+            }
+            pa_st32(st + 16 * c, p);
+          }
+          float a0, a1;
+          pa_unpair(pa_add2(pa_add2(sum[0], sum[1]), pa_add2(sum[2], sum[3])), a0, a1);
+          l += a0 + a1;
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (u != it.begin) {  // the previous P V is done: O may be rescaled, and this unit's may follow
           ok = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
           if (!ok) break;
@@ -503,11 +588,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         pa_st_wait();
         pa_fence_before();
         __syncwarp();
-        if (lane == 0) pa_arrive_cluster(p_full);
+        if (lane == 0) pa_arrive_relaxed(p_full);
       }
       ok = ok && pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
       if (!ok) break;
-      pa_fence_after();
       const bool whole = it.begin == 0 && it.end == it.nk;
       if (it.begin == 0 && it.end < it.nk) {
         // the item's last unit is number u_end - it.end + it.nk - 1 of the call
@@ -515,26 +599,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         const long long e = ((last + 1) * sm.range_count - 1) / sm.units;
         tail = {it.seq, it.tile, it.head, static_cast<int>(e) - range + 1};
       }
+      if (!any_row) continue;
+      pa_fence_after();
       if (whole) {
+        // four lanes write 64 bytes of one row at a time: one row per lane would be 32 lines per store
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        uint16_t* dst = a.out + (it.s.t0 + i) * a.o_ts + (it.head * a.group + hg) * a.o_hs + 256 * half;
-#pragma unroll 1
+        uint16_t* row[4];
+        bool live[4];
+        const unsigned long long mine = reinterpret_cast<unsigned long long>(
+            a.out + (it.s.t0 + i) * a.o_ts + (it.head * a.group + hg) * a.o_hs + 256 * half);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          row[j] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, mine, (lane & 28) + j)) + 8 * (lane & 3);
+          live[j] = __shfl_sync(0xffffffffu, static_cast<int>(valid), (lane & 28) + j) != 0;
+        }
+#pragma unroll 2
         for (int c = 0; c < 256; c += 32) {
           float o[32];
+          uint32_t x[16];
           pa_ld32(tbase + lanes + c, o);
           pa_ld_wait();
-          if (valid) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              *reinterpret_cast<uint4*>(dst + c + j) =
-                  make_uint4(pack_bf16x2(o[j] * inv, o[j + 1] * inv), pack_bf16x2(o[j + 2] * inv, o[j + 3] * inv),
-                             pack_bf16x2(o[j + 4] * inv, o[j + 5] * inv), pack_bf16x2(o[j + 6] * inv, o[j + 7] * inv));
-          }
+          for (int j = 0; j < 16; ++j) x[j] = pa_bf16x2(o[2 * j] * inv, o[2 * j + 1] * inv);
+          pa_quad_transpose(x, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (live[j])
+              *reinterpret_cast<uint4*>(row[j] + c) = make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
         }
       } else {
         float* part = a.part + (((static_cast<size_t>(range) * kHalves + half) * 2 + cta) * 2 + (it.begin == 0 ? 1 : 0)) *
                                    kPaPartFloats;
-#pragma unroll 1
+#pragma unroll 2
         for (int c = 0; c < 256; c += 32) {
           float o[32];
           pa_ld32(tbase + lanes + c, o);
@@ -542,7 +638,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           if (valid) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(part + tid * 256 + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+              *reinterpret_cast<float4*>(part + ((c + j) / 4 * 128 + tid) * 4) =
+                  make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
         }
         *reinterpret_cast<float2*>(part + 128 * 256 + 2 * tid) = make_float2(m, l);
@@ -552,50 +649,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     if (tid == 0 && cta == 0 && half == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
   } else if (warp == 4) {
     // -------------------------------------------------------------- TMA
+    // One box per lane: lane & 1 is the 64-dim block, lane >> 1 the box of rows in the stage's 64.
     uint32_t c = 0, edges = 0;  // stages filled, V tiles left to the copying warps
     const uint64_t kmap_at = reinterpret_cast<uint64_t>(&kmap), vmap_at = reinterpret_cast<uint64_t>(&vmap);
-    const int k_boxes = 64 / a.k_box, v_boxes = kPaKeys / a.v_box;
+    const int slab = lane & 1, in_stage = (lane >> 1) * a.box;
     bool ok = true, bad_page = false;
-    // one box per lane: K (chunk >= 0): 4 dim blocks x the CTA's 64 rows; V: 2 dim blocks x 128 rows
-    auto fill = [&](int kt, int chunk) {
-      const int stage = c % kStages;
-      if (c >= kStages) ok = pa_wait_warp(&sm.empty[stage], (c / kStages - 1) & 1, abort, budget);
-      ++c;
-      if (!ok) return;
-      if (chunk < 0 && it.edge(kt)) {
-        if (edges > 0) ok = pa_wait_warp(&sm.edge_done, (edges - 1) & 1, abort, budget);
-        if (ok && lane == 0) mbar_arrive(&sm.edge_go);
-        ++edges;
-        return;
-      }
-      const int slab = chunk >= 0 ? lane & 3 : lane & 1, rb = chunk >= 0 ? lane >> 2 : lane >> 1;
-      const int box = chunk >= 0 ? a.k_box : a.v_box;
-      const int in_tile = rb * box;
-      const int row = kt * kPaKeys + (chunk >= 0 ? 64 * cta : 0) + in_tile;
-      const bool mine = rb < (chunk >= 0 ? k_boxes : v_boxes) && row < it.s.kv && row + box > it.low();
-      int page = 0;
-      if (mine) {
-        page = __ldcg(b.tables + it.seq * b.table_stride + row / b.page_rows);
-        if (page < 0 || page >= b.n_pages) {
-          bad_page = true;
-          page = b.n_pages;  // out of the map's bounds: zeros
-        }
-      }
-      const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine));
+    auto free_stage = [&]() {
+      if (c >= kStages) ok = ok && pa_wait_warp(&sm.empty[c % kStages], (c / kStages - 1) & 1, abort, budget);
+      return static_cast<int>(c++ % kStages);
+    };
+    // this lane's page of the 64 rows from `row0` on (-1: its box is not copied)
+    auto page_of = [&](int row0) {
+      const int row = row0 + in_stage;
+      if (in_stage >= 64 || row >= it.s.kv || row + a.box <= it.low()) return -1;
+      const int page = __ldcg(b.tables + it.seq * b.table_stride + row / b.page_rows);
+      if (page >= 0 && page < b.n_pages) return page;
+      bad_page = true;
+      return b.n_pages;  // out of the map's bounds: zeros
+    };
+    auto fill = [&](int stage, int row0, int page, uint64_t map, int x) {
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, page >= 0));
       const uint32_t bar = pa_map_to(smem_u32(&sm.full[stage]), 0);
-      if (lane == 0) pa_expect_cluster(bar, n * box * 128u);
+      if (lane == 0) pa_expect_cluster(bar, n * a.box * 128u);
       __syncwarp();
-      if (mine) {
-        const uint32_t dst = smem_u32(&sm.ring[stage][0]) + slab * (chunk >= 0 ? 8192u : 16384u) + in_tile * 128u;
-        const int x = chunk >= 0 ? 256 * chunk + 64 * slab : 256 * half + 128 * cta + 64 * slab;
-        pa_tma(dst, chunk >= 0 ? kmap_at : vmap_at, x, it.head, row % b.page_rows, page, bar);
-      }
+      if (page >= 0)
+        pa_tma(smem_u32(&sm.ring[stage][0]) + slab * 8192u + in_stage * 128u, map, x + 64 * slab, it.head,
+               (row0 + in_stage) % b.page_rows, page, bar);
     };
     while (ok && it.next()) {
+      auto k_row = [&](int u) { return (it.kt0 + u) * kPaKeys + 64 * cta; };
+      int pk = page_of(k_row(it.begin)), pv0 = 0, pv1 = 0;
       for (int u = it.begin - 1; u < it.end && ok; ++u) {
+        // the table entries of the next step are fetched while this one's stages become free
+        const int v_row = (it.kt0 + u) * kPaKeys;
+        const int k_now = pk, v0 = pv0, v1 = pv1;
+        if (u + 2 < it.end) pk = page_of(k_row(u + 2));
+        if (u + 1 < it.end) {
+          pv0 = page_of(v_row + kPaKeys);
+          pv1 = page_of(v_row + kPaKeys + 64);
+        }
         if (u + 1 < it.end)
-          for (int ch = 0; ch < kChunks; ++ch) fill(it.kt0 + u + 1, ch);
-        if (u >= it.begin) fill(it.kt0 + u, -1);
+          for (int ch = 0; ch < kChunks && ok; ++ch) {
+            const int stage = free_stage();
+            if (ok) fill(stage, k_row(u + 1), k_now, kmap_at, 128 * ch);
+          }
+        if (u < it.begin || !ok) continue;
+        const int s0 = free_stage();
+        const bool edge = it.edge(it.kt0 + u);
+        if (ok && !edge) fill(s0, v_row, v0, vmap_at, 256 * half + 128 * cta);
+        const int s1 = free_stage();
+        if (ok && !edge) fill(s1, v_row + 64, v1, vmap_at, 256 * half + 128 * cta);
+        if (ok && edge) {
+          if (edges > 0) ok = pa_wait_warp(&sm.edge_done, (edges - 1) & 1, abort, budget);
+          if (ok && lane == 0) mbar_arrive(&sm.edge_go);
+          ++edges;
+        }
       }
     }
     // every stage is free again: no barrier of this CTA has an arrival outstanding when it exits
@@ -609,26 +717,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       uint32_t c = 0, g = 0, items = 0;
       bool ok = true;
       const uint32_t qb = smem_u32(&sm.q[0][0]);
+      auto stage_full = [&](bool wide) {
+        uint64_t* bar = &sm.full[c % kStages];
+        const uint32_t parity = (c / kStages) & 1;
+        ok = ok && (wide ? pa_wait<true>(bar, parity, abort, budget) : pa_wait(bar, parity, abort, budget));
+        pa_fence_after();
+        return static_cast<int>(c++ % kStages);
+      };
       auto scores = [&](uint32_t unit) {
-        for (int ch = 0; ch < kChunks && ok; ++ch, ++c) {
-          const int stage = c % kStages;
-          ok = pa_wait(&sm.full[stage], (c / kStages) & 1, abort, budget);
+        for (int ch = 0; ch < kChunks; ++ch) {
+          const int stage = stage_full(false);
           if (!ok) return;
-          pa_fence_after();
           const uint32_t kb = smem_u32(&sm.ring[stage][0]);
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
+          for (int k = 0; k < 8; ++k)
             pa_mma_ss(tbase + kPaColS + (unit & 1) * 128,
-                      pa_desc(qb + (4 * ch + (k >> 2)) * 16384 + 32 * (k & 3), 16, 1024),
+                      pa_desc(qb + (2 * ch + (k >> 2)) * 16384 + 32 * (k & 3), 16, 1024),
                       pa_desc(kb + (k >> 2) * 8192 + 32 * (k & 3), 16, 1024), kPaIdescS, (ch | k) ? 1u : 0u);
           pa_commit(&sm.empty[stage]);
         }
         pa_commit(&sm.s_full[unit & 1]);
       };
       while (ok && it.next()) {
-        ok = pa_wait(&sm.q_full, items & 1, abort, budget);
+        ok = pa_wait<true>(&sm.q_full, items & 1, abort, budget);
         ++items;
-        if (!ok) break;
         for (int u = it.begin - 1; u < it.end && ok; ++u) {
           if (u + 1 < it.end) {
             scores(g + (u + 1 - it.begin));
@@ -637,19 +749,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           }
           if (u < it.begin) continue;
           const uint32_t unit = g + (u - it.begin);
-          const int stage = c % kStages;
-          ok = pa_wait(&sm.p_full, unit & 1, abort, budget) &&
-               pa_wait(&sm.full[stage], (c / kStages) & 1, abort, budget);
-          ++c;
-          if (!ok) break;
-          pa_fence_after();
-          const uint32_t vb = smem_u32(&sm.ring[stage][0]);
+          ok = pa_wait(&sm.p_full, unit & 1, abort, budget);
+          const bool edge = it.edge(it.kt0 + u);
+          for (int v = 0; v < 2 && ok; ++v) {
+            const int stage = stage_full(edge);
+            if (!ok) break;
+            const uint32_t vb = smem_u32(&sm.ring[stage][0]);
 #pragma unroll
-          for (int k = 0; k < kPaKeys / 16; ++k)
-            pa_mma_ts(tbase, tbase + kPaColS + (unit & 1) * 128 + 8 * k, pa_desc(vb + 2048 * k, 16384, 1024),
-                      kPaIdescO, (u > it.begin || k) ? 1u : 0u);
-          pa_commit(&sm.empty[stage]);
-          pa_commit(&sm.pv_done);
+            for (int k = 0; k < 4; ++k)
+              pa_mma_ts(tbase, tbase + kPaColS + (unit & 1) * 128 + 32 * v + 8 * k, pa_desc(vb + 2048 * k, 8192, 1024),
+                        kPaIdescO, (u > it.begin || v || k) ? 1u : 0u);
+            pa_commit(&sm.empty[stage]);
+          }
+          if (ok) pa_commit(&sm.pv_done);
         }
         g += it.end - it.begin;
       }
@@ -666,52 +778,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       ++items;
       if (!ok) break;
       {
-        const unsigned r0 = it.tile * kPaRows + cta * 128, group = a.group;
-        const uint32_t qb = smem_u32(&sm.q[0][0]);
-        constexpr int kRowChunks = D / 8;
-#pragma unroll 4
-        for (int x = lt; x < 128 * kRowChunks; x += 128) {
-          const int row = x / kRowChunks, ch = x % kRowChunks;
-          const int i = static_cast<int>((r0 + row) / group), hg = static_cast<int>((r0 + row) % group);
+        // a thread copies one 16-byte column of every kStep-th row
+        constexpr int kRowChunks = D / 8, kStep = 64 / kRowChunks;
+        const unsigned group = a.group, r0 = it.tile * kPaRows + cta * 128 + lt / kRowChunks;
+        const int ch = lt % kRowChunks, di = kStep / group, dh = kStep % group;
+        const uint32_t qb = smem_u32(&sm.q[0][0]) + (ch >> 3) * 16384;
+        const uint16_t* q = a.q + it.head * group * a.q_hs + it.s.t0 * a.q_ts + 8 * ch;
+        int i = static_cast<int>(r0 / group), hg = static_cast<int>(r0 % group);
+#pragma unroll 8
+        for (int row = lt / kRowChunks; row < 128; row += kStep) {
           const bool in = i < it.s.n;
-          const uint16_t* src =
-              in ? a.q + (it.s.t0 + i) * a.q_ts + (it.head * a.group + hg) * a.q_hs + 8 * ch : a.q;
-          cp_async16(qb + (ch >> 3) * 16384 + pa_swizzle(row, ch), src, in ? 16u : 0u);
+          cp_async16(qb + pa_swizzle(row, ch), in ? q + i * a.q_ts + hg * a.q_hs : a.q, in ? 16u : 0u);
+          i += di;
+          hg += dh;
+          if (hg >= static_cast<int>(group)) {
+            hg -= group;
+            ++i;
+          }
         }
       }
       cp_async_wait_all();
       asm volatile("fence.proxy.async;" ::: "memory");
-      named_bar_sync(2, 128);
+      named_bar_sync(2, 64);
       if (lt == 0) pa_arrive_cluster(q_full);
       for (int u = it.begin - 1; u < it.end && ok; ++u) {
         if (u + 1 < it.end) c += kChunks;
         if (u < it.begin) continue;
-        const int kt = it.kt0 + u, stage = c % kStages;
-        ++c;
-        if (!it.edge(kt)) continue;
+        const int row0 = (it.kt0 + u) * kPaKeys;
+        const int s0 = c % kStages, s1 = (c + 1) % kStages;
+        c += 2;
+        if (!it.edge(it.kt0 + u)) continue;
+        // lanes 0-15 hold the pages of the tile's 16 groups of 8 rows (-1: zeros)
+        int page = -1;
+        const int at = row0 + 8 * (lane & 15);
+        if (at < it.s.kv && at + 8 > it.low()) {
+          page = __ldcg(b.tables + it.seq * b.table_stride + at / b.page_rows);
+          if (page < 0 || page >= b.n_pages) page = -1;  // (reported by the TMA warp's K boxes)
+        }
         ok = pa_agree(pa_wait(&sm.edge_go, edges & 1, abort, budget));
         ++edges;
         if (!ok) break;
-        const uint32_t vb = smem_u32(&sm.ring[stage][0]);
-#pragma unroll 4
-        for (int x = lt; x < kPaKeys * 16; x += 128) {
-          const int r = x >> 4, ch = x & 15, row = kt * kPaKeys + r;
-          bool in = row >= it.low() && row < it.s.kv;
-          const uint16_t* src = a.vc;
-          if (in) {
-            const int page = __ldcg(b.tables + it.seq * b.table_stride + row / b.page_rows);
-            if (page >= 0 && page < b.n_pages)
-              src = a.vc + page * a.vp + (row % b.page_rows) * a.vr + it.head * a.vh + 256 * half + 128 * cta + 8 * ch;
-            else
-              in = false;
-          }
-          cp_async16(vb + (ch >> 3) * 16384 + pa_swizzle(r, ch), src, in ? 16u : 0u);
+        const int ch = lt & 15, low = it.low();
+        const uint16_t* v = a.vc + it.head * a.vh + 256 * half + 128 * cta + 8 * ch;
+        const uint32_t slab = (ch >> 3) * 8192;
+        const uint32_t vb0 = smem_u32(&sm.ring[s0][0]) + slab, vb1 = smem_u32(&sm.ring[s1][0]) + slab;
+#pragma unroll 8
+        for (int r = lt >> 4; r < kPaKeys; r += 4) {
+          const int pg = __shfl_sync(0xffffffffu, page, r >> 3), row = row0 + r;
+          const bool in = pg >= 0 && row >= low && row < it.s.kv;
+          const uint16_t* src = in ? v + pg * a.vp + (row % b.page_rows) * a.vr : a.vc;
+          cp_async16((r < 64 ? vb0 : vb1) + pa_swizzle(r & 63, ch), src, in ? 16u : 0u);
         }
         cp_async_wait_all();
         asm volatile("fence.proxy.async;" ::: "memory");
-        named_bar_sync(2, 128);
+        named_bar_sync(2, 64);
         if (lt == 0) {
-          pa_arrive_cluster(pa_map_to(smem_u32(&sm.full[stage]), 0));
+          pa_arrive_cluster(pa_map_to(smem_u32(&sm.full[s0]), 0));
+          pa_arrive_cluster(pa_map_to(smem_u32(&sm.full[s1]), 0));
           mbar_arrive(&sm.edge_done);
         }
       }
@@ -733,8 +856,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 }
 
 // Joins the parts of the items that cross range ends: with M the largest of the parts' reference
-// maxima, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in range order.  A block has two rows.
-constexpr int kPaJoinThreads = 128;
+// maxima, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in range order.  A block has
+// eight rows and 64 columns of one half.
+constexpr int kPaJoinThreads = 128, kPaJoinRows = 8;
 template <int D>
 __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid_constant__ PaArgs a,
                                                                     const __grid_constant__ PagedBatch b) {
@@ -745,39 +869,35 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid
   if (t.seq < 0) return;
   bool bad;
   const PagedSeq s = paged_seq(b, t.seq, &bad);
-  const int col = (threadIdx.x & 63) * 4;
-  const int r = blockIdx.y * 2 + (threadIdx.x >> 6);
+  const int half = blockIdx.z % kHalves, quad = (blockIdx.z / kHalves) * 16 + threadIdx.x / kPaJoinRows;
+  const int r = blockIdx.y * kPaJoinRows + threadIdx.x % kPaJoinRows;
   const unsigned rr = t.tile * kPaRows + r, group = a.group;
   const int i = static_cast<int>(rr / group), hg = static_cast<int>(rr % group);
   if (i >= s.n) return;
   const int cta = r >> 7, row = r & 127;
-  auto part = [&](int k, int half) {  // the first part is its range's second slot, the others their first
+  auto part = [&](int k) {  // the first part is its range's second slot, the others their first
     return a.part + (((static_cast<size_t>(blockIdx.x + k) * kHalves + half) * 2 + cta) * 2 + (k == 0 ? 1 : 0)) *
                         kPaPartFloats;
   };
-  uint16_t* dst = a.out + (s.t0 + i) * a.o_ts + (t.head * a.group + hg) * a.o_hs + col;
-#pragma unroll
-  for (int half = 0; half < kHalves; ++half) {
-    float top = -CUDART_INF_F;
+  float top = -CUDART_INF_F;
 #pragma unroll 8
-    for (int k = 0; k < t.parts; ++k) top = fmaxf(top, part(k, half)[128 * 256 + 2 * row]);
-    const float ref = top == -CUDART_INF_F ? 0.f : top;
-    float l = 0.f, o[4] = {};
+  for (int k = 0; k < t.parts; ++k) top = fmaxf(top, part(k)[128 * 256 + 2 * row]);
+  const float ref = top == -CUDART_INF_F ? 0.f : top;
+  float l = 0.f, o[4] = {};
 #pragma unroll 8
-    for (int k = 0; k < t.parts; ++k) {
-      const float2 ml = *reinterpret_cast<const float2*>(part(k, half) + 128 * 256 + 2 * row);
-      const float4 v = *reinterpret_cast<const float4*>(part(k, half) + row * 256 + col);
-      const float w = pa_exp2(ml.x - ref);
-      l = fmaf(w, ml.y, l);
-      o[0] = fmaf(w, v.x, o[0]);
-      o[1] = fmaf(w, v.y, o[1]);
-      o[2] = fmaf(w, v.z, o[2]);
-      o[3] = fmaf(w, v.w, o[3]);
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    *reinterpret_cast<uint2*>(dst + 256 * half) =
-        make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+  for (int k = 0; k < t.parts; ++k) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(k) + 128 * 256 + 2 * row);
+    const float4 v = *reinterpret_cast<const float4*>(part(k) + (quad * 128 + row) * 4);
+    const float w = pa_exp2(ml.x - ref);
+    l = fmaf(w, ml.y, l);
+    o[0] = fmaf(w, v.x, o[0]);
+    o[1] = fmaf(w, v.y, o[1]);
+    o[2] = fmaf(w, v.z, o[2]);
+    o[3] = fmaf(w, v.w, o[3]);
   }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  *reinterpret_cast<uint2*>(a.out + (s.t0 + i) * a.o_ts + (t.head * a.group + hg) * a.o_hs + 256 * half + 4 * quad) =
+      make_uint2(pa_bf16x2(o[0] * inv, o[1] * inv), pa_bf16x2(o[2] * inv, o[3] * inv));
 }
 
 // ---------------------------------------------------------------------------- host
@@ -856,11 +976,10 @@ static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_
   a.ranges = pairs / (D / 256);
   if (most < a.ranges) a.ranges = static_cast<int>(most);
   const int low = b.page_rows & -b.page_rows;  // the largest power of two that divides a page's rows
-  a.k_box = low < 64 ? low : 64;
-  a.v_box = low < kPaKeys ? low : kPaKeys;
+  a.box = low < 64 ? low : 64;
   CUtensorMap km, vm;
-  if (!page_map(&km, c->k, c, c->k_page_stride, c->k_row_stride, c->k_head_stride, a.k_box) ||
-      !page_map(&vm, c->v, c, c->v_page_stride, c->v_row_stride, c->v_head_stride, a.v_box))
+  if (!page_map(&km, c->k, c, c->k_page_stride, c->k_row_stride, c->k_head_stride, a.box) ||
+      !page_map(&vm, c->v, c, c->v_page_stride, c->v_row_stride, c->v_head_stride, a.box))
     return fail(ctx, G4_ERR_UNSUPPORTED, "paged attention: the cache's layout has no TMA descriptor");
   Scratch* scr = ctx->buf.scratch;
   uint64_t budget = ctx->wait_budget_ns;
@@ -868,9 +987,9 @@ static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_
   st = launch_kernel(ctx, fn, dim3(a.ranges * (D / 256) * 2), dim3(kPaThreads), smem, args, false, "paged attention");
   if (st != G4_OK) return st;
   void* jargs[] = {(void*)&a, (void*)&b};
-  const int row_pairs = static_cast<int>(((rows < kPaRows ? rows : kPaRows) + 1) / 2);
-  return launch_kernel(ctx, (const void*)paged_join_kernel<D>, dim3(a.ranges, row_pairs), dim3(kPaJoinThreads), 0,
-                       jargs, false, "paged attention join");
+  const int row_blocks = static_cast<int>(((rows < kPaRows ? rows : kPaRows) + kPaJoinRows - 1) / kPaJoinRows);
+  return launch_kernel(ctx, (const void*)paged_join_kernel<D>, dim3(a.ranges, row_blocks, 4 * (D / 256)),
+                       dim3(kPaJoinThreads), 0, jargs, false, "paged attention join");
 }
 
 }  // namespace g4

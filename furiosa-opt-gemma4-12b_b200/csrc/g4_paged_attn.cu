@@ -25,9 +25,9 @@
 // balanced.  An item that crosses a range's end leaves partial sums (f32) that a second
 // kernel joins in range order.
 //
-// Roles of a CTA's 8 warps: 0-3 softmax and output, 4 TMA, 5 MMA (leader CTA) and tensor
-// memory, 6-7 Q rows and the V tiles at a sequence's ends (TMA cannot stop at its last row;
-// rows past it may hold NaN, and 0 * NaN is NaN, so these tiles are copied with zeros there).
+// Roles of a CTA's 8 warps: 0-3 softmax and output, 4 K copies, 5 MMA (leader CTA) and tensor
+// memory, 6 V copies, 7 Q copies and the V tiles at a sequence's ends (TMA cannot stop at its
+// last row; rows past it may hold NaN, and 0 * NaN is NaN, so they are zeroed there).
 #include <cuda.h>
 
 #include <cmath>
@@ -48,6 +48,16 @@ constexpr uint32_t kPaIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (16u << 17) 
 constexpr uint32_t kPaIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (32u << 17) | (16u << 24);
 constexpr int kPaPartFloats = 128 * 256 + 2 * 128;  // a partial: O as [64 column quads][128 rows][4], then (m, l) [128][2]
 
+// Division by a number fixed for the call, by multiplication (round-up method; exact for
+// 0 <= n < 2^31): a hardware divide goes through the unit that the softmax's exponentials
+// keep busy, and took the copying warps over 1000 cycles.
+struct PaDiv {
+  uint32_t mul, shift;
+  __device__ __forceinline__ int div(int n) const {
+    const uint32_t u = static_cast<uint32_t>(n);
+    return static_cast<int>((__umulhi(u, mul) + u) >> shift);
+  }
+};
 struct PaArgs {
   const uint16_t* q;
   long long q_ts, q_hs;
@@ -56,8 +66,10 @@ struct PaArgs {
   const uint16_t* vc;
   long long vp, vr, vh;
   int group, n_kv, window;  // query heads per KV head, KV heads
+  PaDiv by_group, by_page;  // by group and by the rows of a page
   float scale;              // times log2(e)
   int box;                  // cache rows per TMA box
+  int q_tma;                // Q rows come by TMA (the group divides 128), else by the softmax warps
   int ranges;
   float* part;              // [ranges][halves][2 CTAs][2][kPaPartFloats]
   struct PaTail* tail;      // [ranges]
@@ -69,10 +81,12 @@ struct PaTail {
 
 template <int D>
 struct __align__(1024) PaSmem {
-  static constexpr int kStages = D == 256 ? 10 : 6;
+  // K and V each have a ring of their own: every ring has one filler, which meets the phases of
+  // its barriers one by one (a parity tells two neighbouring phases apart, not three)
+  static constexpr int kK = D == 256 ? 5 : 4, kV = D == 256 ? 5 : 2, kStages = kK + kV;
   uint8_t q[D / 64][128 * 128];  // 64-dim blocks [128 rows][64], 128-byte swizzle
-  uint8_t ring[kStages][kPaStage];
-  uint64_t full[kStages], empty[kStages], s_full[2], p_full, pv_done, q_full, q_empty, edge_go, edge_done;
+  uint8_t ring[kStages][kPaStage];  // K stages, then V stages
+  uint64_t full[kStages], empty[kStages], s_full[2], p_full, pv_done, q_full, q_empty, edge_full, edge_done;
   uint32_t tmem;
   uint32_t abort;
   long long units, first;  // of the call; of this range
@@ -140,17 +154,6 @@ __device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, vol
                                              uint64_t budget) {
   return __all_sync(0xffffffffu, pa_wait(bar, parity, abort, budget));
 }
-// And by the two copying warps.
-__device__ __forceinline__ bool pa_agree(bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(static_cast<uint32_t>(ok))
-      : "memory");
-  return r != 0;
-}
 __device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
   return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
          (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (static_cast<uint64_t>(1u) << 46) |
@@ -178,12 +181,11 @@ __device__ __forceinline__ void pa_commit(uint64_t* bar) {
       "h"(static_cast<uint16_t>(3))
       : "memory");
 }
-__device__ __forceinline__ void pa_tma(uint32_t dst, uint64_t map, int x, int head, int row, int page,
-                                       uint32_t bar) {
+__device__ __forceinline__ void pa_tma(uint32_t dst, uint64_t map, int c1, int c2, int c3, int c4, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(head), "r"(row), "r"(page), "r"(bar)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -275,15 +277,14 @@ __device__ __forceinline__ uint32_t pa_swizzle(int row, int c) {  // 16-byte chu
 // ---------------------------------------------------------------------------- work split
 // Key tiles of row tile `tile` of a sequence: [kt0, kt0 + n), n >= 1 (a tile nothing is
 // visible to still has its zeros to write).
-__device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, unsigned group, int window, int& kt0) {
-  const unsigned r0 = static_cast<unsigned>(tile) * kPaRows;
-  const int i0 = static_cast<int>(r0 / group);
-  const int i1 = min(s.n - 1, static_cast<int>((r0 + kPaRows - 1) / group));
+__device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, const PaArgs& a, int& kt0) {
+  const int r0 = tile * kPaRows;
+  const int i0 = a.by_group.div(r0), i1 = min(s.n - 1, a.by_group.div(r0 + kPaRows - 1));
   const int first = s.kv - s.n;
   const int hi = first + i1 + 1;
   kt0 = 0;
   if (hi <= 0) return 1;
-  if (window > 0) kt0 = max(0, first + i0 - window + 1) / kPaKeys;
+  if (a.window > 0) kt0 = max(0, first + i0 - a.window + 1) / kPaKeys;
   return (hi + kPaKeys - 1) / kPaKeys - kt0;
 }
 __device__ __forceinline__ int pa_tiles(const PagedSeq& s, int group) {
@@ -303,7 +304,7 @@ __device__ __forceinline__ long long pa_warp_scan(long long v, int lane) {  // i
   return v;
 }
 // Units of every sequence into w[]; the whole CTA.
-__device__ void pa_count(const PagedBatch& b, int group, int n_kv, int window, long long* w, Scratch* scr, bool report) {
+__device__ void pa_count(const PagedBatch& b, const PaArgs& a, long long* w, Scratch* scr, bool report) {
   const int tid = threadIdx.x, lane = tid & 31;
   for (int s0 = 0; s0 < b.n_seqs; s0 += kPaThreads) {
     const int s = s0 + tid;
@@ -312,25 +313,25 @@ __device__ void pa_count(const PagedBatch& b, int group, int n_kv, int window, l
     if (s < b.n_seqs) q = paged_seq(b, s, &bad);
     if (report && s == 0 && b.n_seqs > 0 && __ldcg(b.q_start) < 0) bad = true;
     if (report && bad) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
-    const int tiles = pa_tiles(q, group);
+    const int tiles = pa_tiles(q, a.group);
     long long sum = 0;
     int kt0;
     if (tiles <= 2)
-      for (int t = 0; t < tiles; ++t) sum += pa_key_tiles(q, t, group, window, kt0);
+      for (int t = 0; t < tiles; ++t) sum += pa_key_tiles(q, t, a, kt0);
     for (uint32_t left = __ballot_sync(0xffffffffu, tiles > 2); left != 0; left &= left - 1) {
       const int from = __ffs(left) - 1;
       const PagedSeq o = {0, __shfl_sync(0xffffffffu, q.n, from), __shfl_sync(0xffffffffu, q.kv, from)};
       long long x = 0;
-      for (int t = lane; t < pa_tiles(o, group); t += 32) x += pa_key_tiles(o, t, group, window, kt0);
+      for (int t = lane; t < pa_tiles(o, a.group); t += 32) x += pa_key_tiles(o, t, a, kt0);
       x = pa_warp_sum(x);
       if (lane == from) sum = x;
     }
-    if (s < b.n_seqs) w[s] = sum * n_kv;
+    if (s < b.n_seqs) w[s] = sum * a.n_kv;
   }
 }
 // Where unit number `want` (< the total) lies; one warp, every lane gets the answer.
-__device__ void pa_find(const PagedBatch& b, int group, int n_kv, int window, const long long* w, long long want,
-                        int lane, int& seq, int& tile, int& head, int& unit) {
+__device__ void pa_find(const PagedBatch& b, const PaArgs& a, const long long* w, long long want, int lane, int& seq,
+                        int& tile, int& head, int& unit) {
   long long base = 0;
   seq = 0;
   for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
@@ -347,12 +348,12 @@ __device__ void pa_find(const PagedBatch& b, int group, int n_kv, int window, co
   }
   bool bad;
   const PagedSeq q = paged_seq(b, seq, &bad);
-  const int tiles = pa_tiles(q, group);
+  const int tiles = pa_tiles(q, a.group);
   tile = 0;
   int nk = 1, kt0;
   for (int t0 = 0; t0 < tiles; t0 += 32) {
-    const int n = t0 + lane < tiles ? pa_key_tiles(q, t0 + lane, group, window, kt0) : 0;
-    const long long x = static_cast<long long>(n) * n_kv;
+    const int n = t0 + lane < tiles ? pa_key_tiles(q, t0 + lane, a, kt0) : 0;
+    const long long x = static_cast<long long>(n) * a.n_kv;
     const long long incl = pa_warp_scan(x, lane);
     const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
     if (past != 0) {
@@ -371,23 +372,22 @@ __device__ void pa_find(const PagedBatch& b, int group, int n_kv, int window, co
 // The items of a range, in order; every role walks them alike.
 struct PaWalk {
   const PagedBatch& b;
-  int group, n_kv, window;
+  const PaArgs& a;
   long long left;  // units after the current item
   int seq, tile, head;
   PagedSeq s;
   int kt0, nk, begin, end;  // key tiles of the current item: [begin, end) of its nk are this range's
   int next_unit;
-  __device__ PaWalk(const PagedBatch& batch, const PaArgs& a, int seq_, int tile_, int head_, int unit_, long long n)
-      : b(batch), group(a.group), n_kv(a.n_kv), window(a.window), left(n), seq(seq_), tile(tile_), head(head_ - 1),
-        next_unit(unit_) {
+  __device__ PaWalk(const PagedBatch& batch, const PaArgs& args, int seq_, int tile_, int head_, int unit_, long long n)
+      : b(batch), a(args), left(n), seq(seq_), tile(tile_), head(head_ - 1), next_unit(unit_) {
     bool bad;
     s = left > 0 ? paged_seq(b, seq, &bad) : PagedSeq{0, 0, 0};
   }
   __device__ bool next() {
     if (left <= 0) return false;
-    if (++head == n_kv) {
+    if (++head == a.n_kv) {
       head = 0;
-      if (++tile >= pa_tiles(s, group)) {
+      if (++tile >= pa_tiles(s, a.group)) {
         bool bad;
         tile = 0;
         do {
@@ -395,7 +395,7 @@ struct PaWalk {
         } while (s.n == 0);
       }
     }
-    nk = pa_key_tiles(s, tile, group, window, kt0);
+    nk = pa_key_tiles(s, tile, a, kt0);
     begin = next_unit;
     next_unit = 0;
     end = static_cast<int>(min(static_cast<long long>(nk), begin + left));
@@ -403,18 +403,39 @@ struct PaWalk {
     return true;
   }
   // the first cache row any new token of the sequence sees
-  __device__ int low() const { return window > 0 ? max(0, s.kv - s.n - window + 1) : 0; }
+  __device__ int low() const { return a.window > 0 ? max(0, s.kv - s.n - a.window + 1) : 0; }
   // a V tile that reaches past the sequence's visible rows
   __device__ bool edge(int kt) const { return (kt + 1) * kPaKeys > s.kv || kt * kPaKeys < low(); }
 };
 
+// A position in a ring of stages [first, first + n): the stage, the parity of the barrier phase
+// that its use ends, and the uses before it.
+struct PaRing {
+  const int first, n;
+  int stage;
+  uint32_t parity = 0, passed = 0;
+  __device__ __forceinline__ PaRing(int first_, int n_) : first(first_), n(n_), stage(first_) {}
+  __device__ __forceinline__ void next() {
+    ++passed;
+    if (++stage == first + n) {
+      stage = first;
+      parity ^= 1u;
+    }
+  }
+};
+__device__ __forceinline__ bool pa_elect() {  // one lane of a converged warp
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 template <int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                      const __grid_constant__ PaArgs a, const __grid_constant__ PagedBatch b, Scratch* scr,
-                      uint64_t budget) {
+                      const __grid_constant__ CUtensorMap qmap, const __grid_constant__ PaArgs a,
+                      const __grid_constant__ PagedBatch b, Scratch* scr, uint64_t budget) {
   using Smem = PaSmem<D>;
-  constexpr int kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 128;  // a K tile is kChunks stages
+  constexpr int kK = Smem::kK, kV = Smem::kV, kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 128;  // a K tile is kChunks stages
   extern __shared__ uint8_t pa_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(pa_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -429,9 +450,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     mbar_init(&sm.s_full[1], 1);
     mbar_init(&sm.p_full, 8);
     mbar_init(&sm.pv_done, 1);
-    mbar_init(&sm.q_full, 2);
+    mbar_init(&sm.q_full, a.q_tma ? 2 : 8);
     mbar_init(&sm.q_empty, 1);
-    mbar_init(&sm.edge_go, 1);
+    mbar_init(&sm.edge_full, 1);
     mbar_init(&sm.edge_done, 1);
     sm.abort = 0;
     fence_mbar_init();
@@ -445,7 +466,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   pdl_launch_dependents();
   long long* w = reinterpret_cast<long long*>(&sm.ring[0][0]);  // (the ring is not in use yet)
   static_assert(G4_PAGED_MAX_SEQS * 8 <= kStages * kPaStage, "unit counts fit the ring");
-  pa_count(b, a.group, a.n_kv, a.window, w, scr, blockIdx.x == 0);
+  pa_count(b, a, w, scr, blockIdx.x == 0);
   pa_fence_before();
   __syncthreads();
   pa_fence_after();
@@ -458,7 +479,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     long long first = 0;
     if (range < n) {
       first = range * u / n;
-      pa_find(b, a.group, a.n_kv, a.window, w, first, lane, seq, tile, head, unit);
+      pa_find(b, a, w, first, lane, seq, tile, head, unit);
     }
     if (lane == 0) {
       sm.units = u;
@@ -490,12 +511,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     PaTail tail = {-1, 0, 0, 0};
     bool ok = true;
     while (ok && it.next()) {
-      const unsigned rr = it.tile * kPaRows + cta * 128 + tid, group = a.group;
-      const int i = static_cast<int>(rr / group), hg = static_cast<int>(rr % group);
+      const int rr = it.tile * kPaRows + cta * 128 + tid;
+      const int i = a.by_group.div(rr), hg = rr - i * a.group;
       const bool valid = i < it.s.n;
       const bool any_row = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps step
       const int pos = it.s.kv - it.s.n + i;
       const int hi = valid ? pos + 1 : 0, lo = valid && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      if (!a.q_tma) {
+        // rows of any group size: a thread copies one 16-byte column of every kStep-th row (the
+        // previous item's scores are done: these warps have read them)
+        constexpr int kRowChunks = D / 8, kStep = 128 / kRowChunks;
+        const int ch = tid % kRowChunks;
+        const uint32_t qb = smem_u32(&sm.q[0][0]) + (ch >> 3) * 16384;
+        const uint16_t* q = a.q + it.head * a.group * a.q_hs + it.s.t0 * a.q_ts + 8 * ch;
+#pragma unroll 4
+        for (int row = tid / kRowChunks; row < 128; row += kStep) {
+          const int r = it.tile * kPaRows + cta * 128 + row, qi = a.by_group.div(r);
+          const bool in = qi < it.s.n;
+          cp_async16(qb + pa_swizzle(row, ch), in ? q + qi * a.q_ts + (r - qi * a.group) * a.q_hs : a.q, in ? 16u : 0u);
+        }
+        cp_async_wait_all();
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) pa_arrive_cluster(pa_map_to(smem_u32(&sm.q_full), 0));
+      }
       float m = -CUDART_INF_F, l = 0.f;
       for (int u = it.begin; u < it.end; ++u, ++g) {
         const uint32_t st = tbase + kPaColS + (g & 1) * 128 + lanes;
@@ -516,14 +555,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           }
           const int base = (it.kt0 + u) * kPaKeys;
           if (__any_sync(0xffffffffu, valid && (hi < base + kPaKeys || lo > base))) {
-            const int first = lo - base, count = hi - lo;  // visible: first <= column < first + count
+            const int from = lo - base, to = hi - base;  // visible: columns [from, to)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c) {
+              const int f = min(max(from - 32 * c, 0), 32), t = min(max(to - 32 * c, 0), 32);
+              const uint32_t see = static_cast<uint32_t>(((1ull << t) - 1ull) & ~((1ull << f) - 1ull));
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int x = 32 * c + j - first;
-                s[c][j] = x >= 0 && x < count ? s[c][j] : -CUDART_INF_F;
-              }
+              for (int j = 0; j < 32; ++j) s[c][j] = (see >> j) & 1u ? s[c][j] : -CUDART_INF_F;
+            }
           }
           float mx[4];
 #pragma unroll
@@ -613,7 +652,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           row[j] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, mine, (lane & 28) + j)) + 8 * (lane & 3);
           live[j] = __shfl_sync(0xffffffffu, static_cast<int>(valid), (lane & 28) + j) != 0;
         }
-#pragma unroll 2
+#pragma unroll 1
         for (int c = 0; c < 256; c += 32) {
           float o[32];
           uint32_t x[16];
@@ -630,7 +669,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       } else {
         float* part = a.part + (((static_cast<size_t>(range) * kHalves + half) * 2 + cta) * 2 + (it.begin == 0 ? 1 : 0)) *
                                    kPaPartFloats;
-#pragma unroll 2
+#pragma unroll 1
         for (int c = 0; c < 256; c += 32) {
           float o[32];
           pa_ld32(tbase + lanes + c, o);
@@ -647,200 +686,220 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     }
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     if (tid == 0 && cta == 0 && half == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
-  } else if (warp == 4) {
-    // -------------------------------------------------------------- TMA
-    // One box per lane: lane & 1 is the 64-dim block, lane >> 1 the box of rows in the stage's 64.
-    uint32_t c = 0, edges = 0;  // stages filled, V tiles left to the copying warps
-    const uint64_t kmap_at = reinterpret_cast<uint64_t>(&kmap), vmap_at = reinterpret_cast<uint64_t>(&vmap);
-    const int slab = lane & 1, in_stage = (lane >> 1) * a.box;
+  } else if (warp == 4 || warp == 6) {
+    // -------------------------------------------------------------- K copies (4), V copies (6)
+    // A stage is one box where a page holds its 64 rows, else one box per lane: lane & 1 is the
+    // 64-dim block, lane >> 1 the box of rows.
+    const bool is_k = warp == 4;
+    PaRing at(is_k ? 0 : kK, is_k ? kK : kV);
+    uint32_t edges = 0;  // V tiles that warp 7 finishes
+    const uint64_t map = reinterpret_cast<uint64_t>(is_k ? &kmap : &vmap);
+    const bool whole = a.box == 64;
+    const int slab = whole ? 0 : lane & 1, in_stage = (whole ? lane : lane >> 1) * a.box;
+    const uint32_t box_bytes = a.box * (whole ? 256u : 128u);
+    const uint32_t full0 = pa_map_to(smem_u32(&sm.full[0]), 0), edge_full = smem_u32(&sm.edge_full);
+    const uint32_t dst0 = smem_u32(&sm.ring[0][0]) + slab * 8192u + in_stage * 128u;
     bool ok = true, bad_page = false;
-    auto free_stage = [&]() {
-      if (c >= kStages) ok = ok && pa_wait_warp(&sm.empty[c % kStages], (c / kStages - 1) & 1, abort, budget);
-      return static_cast<int>(c++ % kStages);
+    auto free_stage = [&](const PaRing& r) {  // waits until the stage at `r` may be filled
+      if (ok && r.passed >= static_cast<uint32_t>(r.n))
+        ok = pa_wait_warp(&sm.empty[r.stage], r.parity ^ 1u, abort, budget);
+      return ok;
     };
-    // this lane's page of the 64 rows from `row0` on (-1: its box is not copied)
-    auto page_of = [&](int row0) {
+    // this lane's box of the 64 rows from `row0` on (row -1: not copied): its page, not looked
+    // at before the box is, and its row there
+    struct Box {
+      int page, row;
+    };
+    auto box_of = [&](int row0) {
       const int row = row0 + in_stage;
-      if (in_stage >= 64 || row >= it.s.kv || row + a.box <= it.low()) return -1;
-      const int page = __ldcg(b.tables + it.seq * b.table_stride + row / b.page_rows);
-      if (page >= 0 && page < b.n_pages) return page;
-      bad_page = true;
-      return b.n_pages;  // out of the map's bounds: zeros
+      Box x = {0, -1};
+      if (in_stage < 64 && row < it.s.kv && row + a.box > it.low()) {
+        const int j = a.by_page.div(row);
+        x.page = __ldcg(b.tables + it.seq * b.table_stride + j);
+        x.row = row - j * b.page_rows;
+      }
+      return x;
     };
-    auto fill = [&](int stage, int row0, int page, uint64_t map, int x) {
-      const uint32_t n = __popc(__ballot_sync(0xffffffffu, page >= 0));
-      const uint32_t bar = pa_map_to(smem_u32(&sm.full[stage]), 0);
-      if (lane == 0) pa_expect_cluster(bar, n * a.box * 128u);
+    auto fill = [&](Box& x, int dim_block, uint32_t bar, bool announce, uint32_t n) {
+      if (x.page < 0 || x.page >= b.n_pages) {
+        bad_page = true;
+        x.page = b.n_pages;  // out of the map's bounds: zeros
+      }
+      if (announce && lane == 0) pa_expect_cluster(bar, n);
+      if (x.row >= 0)
+        pa_tma(dst0 + at.stage * static_cast<uint32_t>(kPaStage), map, x.row, dim_block + slab, it.head, x.page, bar);
       __syncwarp();
-      if (page >= 0)
-        pa_tma(smem_u32(&sm.ring[stage][0]) + slab * 8192u + in_stage * 128u, map, x + 64 * slab, it.head,
-               (row0 + in_stage) % b.page_rows, page, bar);
+      at.next();
     };
-    while (ok && it.next()) {
-      auto k_row = [&](int u) { return (it.kt0 + u) * kPaKeys + 64 * cta; };
-      int pk = page_of(k_row(it.begin)), pv0 = 0, pv1 = 0;
-      for (int u = it.begin - 1; u < it.end && ok; ++u) {
-        // the table entries of the next step are fetched while this one's stages become free
-        const int v_row = (it.kt0 + u) * kPaKeys;
-        const int k_now = pk, v0 = pv0, v1 = pv1;
-        if (u + 2 < it.end) pk = page_of(k_row(u + 2));
-        if (u + 1 < it.end) {
-          pv0 = page_of(v_row + kPaKeys);
-          pv1 = page_of(v_row + kPaKeys + 64);
+    auto bytes = [&](const Box& x) { return __popc(__ballot_sync(0xffffffffu, x.row >= 0)) * box_bytes; };
+    if (is_k) {
+      while (ok && it.next()) {
+        auto k_row = [&](int u) { return (it.kt0 + u) * kPaKeys + 64 * cta; };
+        Box next = box_of(k_row(it.begin));
+        for (int u = it.begin; u < it.end && ok; ++u) {
+          Box now = next;  // the next tile's table entries are fetched while this one's stages become free
+          if (u + 1 < it.end) next = box_of(k_row(u + 1));
+          const uint32_t n = bytes(now);
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch)
+            if (free_stage(at)) fill(now, 2 * ch, full0 + 8u * at.stage, true, n);
         }
-        if (u + 1 < it.end)
-          for (int ch = 0; ch < kChunks && ok; ++ch) {
-            const int stage = free_stage();
-            if (ok) fill(stage, k_row(u + 1), k_now, kmap_at, 128 * ch);
+      }
+    } else {
+      const int v_block = 4 * half + 2 * cta;
+      while (ok && it.next()) {
+        Box next0 = box_of((it.kt0 + it.begin) * kPaKeys), next1 = box_of((it.kt0 + it.begin) * kPaKeys + 64);
+        for (int u = it.begin; u < it.end && ok; ++u) {
+          Box now0 = next0, now1 = next1;
+          const int row = (it.kt0 + u) * kPaKeys;
+          if (u + 1 < it.end) {
+            next0 = box_of(row + kPaKeys);
+            next1 = box_of(row + kPaKeys + 64);
           }
-        if (u < it.begin || !ok) continue;
-        const int s0 = free_stage();
-        const bool edge = it.edge(it.kt0 + u);
-        if (ok && !edge) fill(s0, v_row, v0, vmap_at, 256 * half + 128 * cta);
-        const int s1 = free_stage();
-        if (ok && !edge) fill(s1, v_row + 64, v1, vmap_at, 256 * half + 128 * cta);
-        if (ok && edge) {
-          if (edges > 0) ok = pa_wait_warp(&sm.edge_done, (edges - 1) & 1, abort, budget);
-          if (ok && lane == 0) mbar_arrive(&sm.edge_go);
+          const bool edge = it.edge(it.kt0 + u);
+          const uint32_t n0 = bytes(now0), n1 = bytes(now1);
+          if (!edge) {
+            if (free_stage(at)) fill(now0, v_block, full0 + 8u * at.stage, true, n0);
+            if (free_stage(at)) fill(now1, v_block, full0 + 8u * at.stage, true, n1);
+            continue;
+          }
+          // both stages report to warp 7, which zeroes rows of them (with no box to wait for, at
+          // once: so only when both are free) and reports to the leader
+          if (edges > 0) ok = ok && pa_wait_warp(&sm.edge_done, (edges - 1) & 1, abort, budget);
+          PaRing second = at;
+          second.next();
+          if (!free_stage(at) || !free_stage(second)) break;
+          if (lane == 0) mbar_arrive_expect_tx(&sm.edge_full, n0 + n1);
           ++edges;
+          fill(now0, v_block, edge_full, false, 0);
+          fill(now1, v_block, edge_full, false, 0);
         }
       }
     }
     // every stage is free again: no barrier of this CTA has an arrival outstanding when it exits
-    for (uint32_t x = c > kStages ? c - kStages : 0; x < c && ok; ++x)
-      ok = pa_wait_warp(&sm.empty[x % kStages], (x / kStages) & 1, abort, budget);
+    for (uint32_t n = at.n, x = at.passed > n ? at.passed - n : 0; x < at.passed && ok; ++x)
+      ok = pa_wait_warp(&sm.empty[at.first + x % n], (x / n) & 1, abort, budget);
     if (bad_page) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   } else if (warp == 5) {
-    // -------------------------------------------------------------- MMA: one thread of the leader CTA
-    if (cta == 0 && lane == 0) {
-      uint32_t c = 0, g = 0, items = 0;
+    // -------------------------------------------------------------- MMA: the leader CTA's
+    // The warp stays converged around the elected lane, so that descriptors live in uniform
+    // registers: N = 128 MMAs issued by a lone thread took 100-150 cycles instead of 64.
+    if (cta == 0) {
+      PaRing k_at(0, kK), v_at(kK, kV);
+      uint32_t g = 0, items = 0;
       bool ok = true;
-      const uint32_t qb = smem_u32(&sm.q[0][0]);
-      auto stage_full = [&](bool wide) {
-        uint64_t* bar = &sm.full[c % kStages];
-        const uint32_t parity = (c / kStages) & 1;
-        ok = ok && (wide ? pa_wait<true>(bar, parity, abort, budget) : pa_wait(bar, parity, abort, budget));
-        pa_fence_after();
-        return static_cast<int>(c++ % kStages);
-      };
+      const bool leader = pa_elect();
+      const uint64_t q_desc = pa_desc(smem_u32(&sm.q[0][0]), 16, 1024);
+      const uint64_t k_desc = pa_desc(smem_u32(&sm.ring[0][0]), 16, 1024);
+      const uint64_t v_desc = pa_desc(smem_u32(&sm.ring[0][0]), 8192, 1024);
       auto scores = [&](uint32_t unit) {
-        for (int ch = 0; ch < kChunks; ++ch) {
-          const int stage = stage_full(false);
-          if (!ok) return;
-          const uint32_t kb = smem_u32(&sm.ring[stage][0]);
+        const uint32_t d = tbase + kPaColS + (unit & 1) * 128;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            pa_mma_ss(tbase + kPaColS + (unit & 1) * 128,
-                      pa_desc(qb + (2 * ch + (k >> 2)) * 16384 + 32 * (k & 3), 16, 1024),
-                      pa_desc(kb + (k >> 2) * 8192 + 32 * (k & 3), 16, 1024), kPaIdescS, (ch | k) ? 1u : 0u);
-          pa_commit(&sm.empty[stage]);
+        for (int ch = 0; ch < kChunks; ++ch) {
+          ok = pa_wait_warp(&sm.full[k_at.stage], k_at.parity, abort, budget);
+          if (!ok) return;
+          pa_fence_after();
+          const uint64_t kd = k_desc + k_at.stage * static_cast<uint32_t>(kPaStage / 16);
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              pa_mma_ss(d, q_desc + ((2 * ch + (k >> 2)) * 16384 + 32 * (k & 3)) / 16,
+                        kd + ((k >> 2) * 8192 + 32 * (k & 3)) / 16, kPaIdescS, (ch | k) ? 1u : 0u);
+            pa_commit(&sm.empty[k_at.stage]);
+            if (ch == kChunks - 1) pa_commit(&sm.s_full[unit & 1]);
+          }
+          __syncwarp();
+          k_at.next();
         }
-        pa_commit(&sm.s_full[unit & 1]);
       };
       while (ok && it.next()) {
-        ok = pa_wait<true>(&sm.q_full, items & 1, abort, budget);
+        ok = __all_sync(0xffffffffu, pa_wait<true>(&sm.q_full, items & 1, abort, budget));
         ++items;
         for (int u = it.begin - 1; u < it.end && ok; ++u) {
           if (u + 1 < it.end) {
             scores(g + (u + 1 - it.begin));
             if (!ok) break;
-            if (u + 2 == it.end) pa_commit(&sm.q_empty);
+            if (u + 2 == it.end && leader) pa_commit(&sm.q_empty);
+            __syncwarp();
           }
           if (u < it.begin) continue;
           const uint32_t unit = g + (u - it.begin);
-          ok = pa_wait(&sm.p_full, unit & 1, abort, budget);
+          const uint32_t p = tbase + kPaColS + (unit & 1) * 128;
+          ok = pa_wait_warp(&sm.p_full, unit & 1, abort, budget);
           const bool edge = it.edge(it.kt0 + u);
-          for (int v = 0; v < 2 && ok; ++v) {
-            const int stage = stage_full(edge);
-            if (!ok) break;
-            const uint32_t vb = smem_u32(&sm.ring[stage][0]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              pa_mma_ts(tbase, tbase + kPaColS + (unit & 1) * 128 + 32 * v + 8 * k, pa_desc(vb + 2048 * k, 8192, 1024),
-                        kPaIdescO, (u > it.begin || v || k) ? 1u : 0u);
-            pa_commit(&sm.empty[stage]);
+          for (int v = 0; v < 2; ++v) {
+            if (ok)
+              ok = edge ? __all_sync(0xffffffffu, pa_wait<true>(&sm.full[v_at.stage], v_at.parity, abort, budget))
+                        : pa_wait_warp(&sm.full[v_at.stage], v_at.parity, abort, budget);
+            if (!ok) break;
+            pa_fence_after();
+            const uint64_t vd = v_desc + v_at.stage * static_cast<uint32_t>(kPaStage / 16);
+            const uint32_t more = u > it.begin ? 1u : 0u;
+            if (leader) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                pa_mma_ts(tbase, p + 32 * v + 8 * k, vd + 2048 * k / 16, kPaIdescO, (v | k) ? 1u : more);
+              pa_commit(&sm.empty[v_at.stage]);
+              if (v == 1) pa_commit(&sm.pv_done);
+            }
+            __syncwarp();
+            v_at.next();
           }
-          if (ok) pa_commit(&sm.pv_done);
         }
         g += it.end - it.begin;
       }
-      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+      if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     }
   } else {
-    // -------------------------------------------------------------- Q rows; V tiles at the ends
-    const int lt = tid - 192;
-    uint32_t c = 0, items = 0, edges = 0;
+    // -------------------------------------------------------------- Q copies; V tiles at the ends
+    PaRing at(kK, kV);
+    uint32_t items = 0, edges = 0;
     bool ok = true;
-    const uint32_t q_full = pa_map_to(smem_u32(&sm.q_full), 0);
+    const uint64_t map = reinterpret_cast<uint64_t>(&qmap);
+    const uint32_t q_full = pa_map_to(smem_u32(&sm.q_full), 0), full0 = pa_map_to(smem_u32(&sm.full[0]), 0);
     while (ok && it.next()) {
-      if (items > 0) ok = pa_agree(pa_wait(&sm.q_empty, (items - 1) & 1, abort, budget));
+      if (items > 0) ok = pa_wait_warp(&sm.q_empty, (items - 1) & 1, abort, budget);
       ++items;
       if (!ok) break;
-      {
-        // a thread copies one 16-byte column of every kStep-th row
-        constexpr int kRowChunks = D / 8, kStep = 64 / kRowChunks;
-        const unsigned group = a.group, r0 = it.tile * kPaRows + cta * 128 + lt / kRowChunks;
-        const int ch = lt % kRowChunks, di = kStep / group, dh = kStep % group;
-        const uint32_t qb = smem_u32(&sm.q[0][0]) + (ch >> 3) * 16384;
-        const uint16_t* q = a.q + it.head * group * a.q_hs + it.s.t0 * a.q_ts + 8 * ch;
-        int i = static_cast<int>(r0 / group), hg = static_cast<int>(r0 % group);
-#pragma unroll 8
-        for (int row = lt / kRowChunks; row < 128; row += kStep) {
-          const bool in = i < it.s.n;
-          cp_async16(qb + pa_swizzle(row, ch), in ? q + i * a.q_ts + hg * a.q_hs : a.q, in ? 16u : 0u);
-          i += di;
-          hg += dh;
-          if (hg >= static_cast<int>(group)) {
-            hg -= group;
-            ++i;
-          }
-        }
+      if (a.q_tma && lane == 0) {
+        pa_expect_cluster(q_full, 128 * D * 2);
+        const int token = it.s.t0 + a.by_group.div(it.tile * kPaRows + cta * 128);
+#pragma unroll
+        for (int blk = 0; blk < D / 64; blk += 4)
+          pa_tma(smem_u32(&sm.q[blk][0]), map, 0, token, blk, it.head, q_full);
       }
-      cp_async_wait_all();
-      asm volatile("fence.proxy.async;" ::: "memory");
-      named_bar_sync(2, 64);
-      if (lt == 0) pa_arrive_cluster(q_full);
-      for (int u = it.begin - 1; u < it.end && ok; ++u) {
-        if (u + 1 < it.end) c += kChunks;
-        if (u < it.begin) continue;
-        const int row0 = (it.kt0 + u) * kPaKeys;
-        const int s0 = c % kStages, s1 = (c + 1) % kStages;
-        c += 2;
+      __syncwarp();
+      for (int u = it.begin; u < it.end && ok; ++u) {
+        const int s0 = at.stage;
+        at.next();
+        const int s1 = at.stage;
+        at.next();
         if (!it.edge(it.kt0 + u)) continue;
-        // lanes 0-15 hold the pages of the tile's 16 groups of 8 rows (-1: zeros)
-        int page = -1;
-        const int at = row0 + 8 * (lane & 15);
-        if (at < it.s.kv && at + 8 > it.low()) {
-          page = __ldcg(b.tables + it.seq * b.table_stride + at / b.page_rows);
-          if (page < 0 || page >= b.n_pages) page = -1;  // (reported by the TMA warp's K boxes)
-        }
-        ok = pa_agree(pa_wait(&sm.edge_go, edges & 1, abort, budget));
+        ok = pa_wait_warp(&sm.edge_full, edges & 1, abort, budget);
         ++edges;
         if (!ok) break;
-        const int ch = lt & 15, low = it.low();
-        const uint16_t* v = a.vc + it.head * a.vh + 256 * half + 128 * cta + 8 * ch;
-        const uint32_t slab = (ch >> 3) * 8192;
-        const uint32_t vb0 = smem_u32(&sm.ring[s0][0]) + slab, vb1 = smem_u32(&sm.ring[s1][0]) + slab;
-#pragma unroll 8
-        for (int r = lt >> 4; r < kPaKeys; r += 4) {
-          const int pg = __shfl_sync(0xffffffffu, page, r >> 3), row = row0 + r;
-          const bool in = pg >= 0 && row >= low && row < it.s.kv;
-          const uint16_t* src = in ? v + pg * a.vp + (row % b.page_rows) * a.vr : a.vc;
-          cp_async16((r < 64 ? vb0 : vb1) + pa_swizzle(r & 63, ch), src, in ? 16u : 0u);
+        // rows outside [low, kv) of the tile's 128: this CTA's 128 columns are 16 chunks a row
+        const int row0 = (it.kt0 + u) * kPaKeys;
+        const int front = min(max(it.low() - row0, 0), kPaKeys), back = min(max(it.s.kv - row0, 0), kPaKeys);
+        const int n = front + kPaKeys - back;
+        for (int x = lane; x < 16 * n; x += 32) {
+          const int k = x >> 4, ch = x & 15, r = k < front ? k : back + k - front;
+          *reinterpret_cast<uint4*>(&sm.ring[r < 64 ? s0 : s1][(ch >> 3) * 8192 + pa_swizzle(r & 63, ch)]) =
+              make_uint4(0u, 0u, 0u, 0u);
         }
-        cp_async_wait_all();
         asm volatile("fence.proxy.async;" ::: "memory");
-        named_bar_sync(2, 64);
-        if (lt == 0) {
-          pa_arrive_cluster(pa_map_to(smem_u32(&sm.full[s0]), 0));
-          pa_arrive_cluster(pa_map_to(smem_u32(&sm.full[s1]), 0));
+        __syncwarp();
+        if (lane == 0) {
+          pa_arrive_cluster(full0 + 8u * s0);
+          pa_arrive_cluster(full0 + 8u * s1);
           mbar_arrive(&sm.edge_done);
         }
       }
     }
-    if (ok && items > 0) ok = pa_wait(&sm.q_empty, (items - 1) & 1, abort, budget);
-    if (!ok && lt == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+    if (ok && items > 0) ok = pa_wait_warp(&sm.q_empty, (items - 1) & 1, abort, budget);
+    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   }
   __syncthreads();
   if (sm.abort != 0) {  // gave up somewhere: let the copies in flight land (bounded)
@@ -871,8 +930,8 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid
   const PagedSeq s = paged_seq(b, t.seq, &bad);
   const int half = blockIdx.z % kHalves, quad = (blockIdx.z / kHalves) * 16 + threadIdx.x / kPaJoinRows;
   const int r = blockIdx.y * kPaJoinRows + threadIdx.x % kPaJoinRows;
-  const unsigned rr = t.tile * kPaRows + r, group = a.group;
-  const int i = static_cast<int>(rr / group), hg = static_cast<int>(rr % group);
+  const int rr = t.tile * kPaRows + r;
+  const int i = a.by_group.div(rr), hg = rr - i * a.group;
   if (i >= s.n) return;
   const int cta = r >> 7, row = r & 127;
   auto part = [&](int k) {  // the first part is its range's second slot, the others their first
@@ -901,12 +960,17 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid
 }
 
 // ---------------------------------------------------------------------------- host
+static PaDiv divisor(int d) {
+  uint32_t shift = 0;
+  while ((1ull << shift) < static_cast<uint64_t>(d)) ++shift;
+  return {static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
+}
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// The pages as a 4-D tensor (dims, heads, rows, pages), box 64 x 1 x rows x 1, 128-byte swizzle.
-static bool page_map(CUtensorMap* m, const uint16_t* base, const g4_paged_cache* c, int64_t page_stride,
-                     int64_t row_stride, int64_t head_stride, int rows) {
+// A 5-D tensor of 64-dim rows with the 128-byte swizzle; `stride` in elements.
+static bool tile_map(CUtensorMap* m, const uint16_t* base, const int (&n)[4], const int64_t (&stride)[4],
+                     const int (&box)[4]) {
   static EncodeFn fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -916,15 +980,16 @@ static bool page_map(CUtensorMap* m, const uint16_t* base, const g4_paged_cache*
                : nullptr;
   }();
   if (fn == nullptr) return false;
-  // the stride of a dimension of size one is never used, but has to be a legal one
-  auto bytes = [&](int64_t stride, int n) { return static_cast<cuuint64_t>(n > 1 ? stride : c->head_dim) * 2; };
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->head_dim), static_cast<cuuint64_t>(c->n_kv_heads),
-                              static_cast<cuuint64_t>(c->page_rows), static_cast<cuuint64_t>(c->n_pages)};
-  const cuuint64_t strides[3] = {bytes(head_stride, c->n_kv_heads), bytes(row_stride, c->page_rows),
-                                 bytes(page_stride, c->n_pages)};
-  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t*>(base), dims, strides, box, estr,
+  cuuint64_t dims[5] = {64}, strides[4];
+  cuuint32_t boxes[5] = {64};
+  for (int i = 0; i < 4; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(n[i]);
+    // the stride of a dimension of size one is never used, but has to be a legal one
+    strides[i] = static_cast<cuuint64_t>(n[i] > 1 ? stride[i] : 64) * 2;
+    boxes[i + 1] = static_cast<cuuint32_t>(box[i]);
+  }
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<uint16_t*>(base), dims, strides, boxes, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -977,13 +1042,26 @@ static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_
   if (most < a.ranges) a.ranges = static_cast<int>(most);
   const int low = b.page_rows & -b.page_rows;  // the largest power of two that divides a page's rows
   a.box = low < 64 ? low : 64;
-  CUtensorMap km, vm;
-  if (!page_map(&km, c->k, c, c->k_page_stride, c->k_row_stride, c->k_head_stride, a.box) ||
-      !page_map(&vm, c->v, c, c->v_page_stride, c->v_row_stride, c->v_head_stride, a.box))
+  // pages: rows, 64-dim blocks, heads, pages; a box is `box` rows of one block, or of two where
+  // that fills a stage
+  CUtensorMap km, vm, qm;
+  const int dims[4] = {c->page_rows, D / 64, c->n_kv_heads, c->n_pages};
+  const int box[4] = {a.box, a.box == 64 ? 2 : 1, 1, 1};
+  if (!tile_map(&km, c->k, dims, {c->k_row_stride, 64, c->k_head_stride, c->k_page_stride}, box) ||
+      !tile_map(&vm, c->v, dims, {c->v_row_stride, 64, c->v_head_stride, c->v_page_stride}, box))
     return fail(ctx, G4_ERR_UNSUPPORTED, "paged attention: the cache's layout has no TMA descriptor");
+  // Q: heads of a group, tokens, blocks, KV heads; a box is a CTA's 128 rows of four blocks
+  const int qdims[4] = {a.group, b.n_tokens, D / 64, a.n_kv};
+  const int64_t qstr[4] = {a.q_hs, a.q_ts, 64, a.q_hs * a.group};
+  a.q_tma = 0;
+  if (128 % a.group == 0 && (a.q_hs > 0 || a.group * a.n_kv == 1) && (a.q_ts > 0 || b.n_tokens == 1)) {
+    const int qbox[4] = {a.group, 128 / a.group, 4, 1};
+    a.q_tma = tile_map(&qm, a.q, qdims, qstr, qbox) ? 1 : 0;
+  }
+  if (!a.q_tma) qm = km;  // (not used)
   Scratch* scr = ctx->buf.scratch;
   uint64_t budget = ctx->wait_budget_ns;
-  void* args[] = {(void*)&km, (void*)&vm, (void*)&a, (void*)&b, (void*)&scr, (void*)&budget};
+  void* args[] = {(void*)&km, (void*)&vm, (void*)&qm, (void*)&a, (void*)&b, (void*)&scr, (void*)&budget};
   st = launch_kernel(ctx, fn, dim3(a.ranges * (D / 256) * 2), dim3(kPaThreads), smem, args, false, "paged attention");
   if (st != G4_OK) return st;
   void* jargs[] = {(void*)&a, (void*)&b};
@@ -1029,6 +1107,8 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   a.vh = cache->v_head_stride;
   a.group = n_heads / cache->n_kv_heads;
   a.n_kv = cache->n_kv_heads;
+  a.by_group = divisor(a.group);
+  a.by_page = divisor(cache->page_rows);
   a.window = window;
   a.scale = scale * 1.4426950408889634f;
   const PagedBatch b = paged_batch(batch, cache);

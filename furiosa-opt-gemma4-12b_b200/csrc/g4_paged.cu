@@ -62,9 +62,13 @@ PagedBatch paged_batch(const g4_paged_batch* b, const g4_paged_cache* c) {
 }
 
 // ---------------------------------------------------------------------------- norm, rotate, store
-// One warp per (token, head): the head's D values stay in its registers (8 per lane and
-// 16-byte chunk), so q, k and v are read once and written once.  Memory bound: 4 B per
-// element plus the token's cos/sin row, which its heads share through L1/L2.
+// A warp takes a token and kPer of its q, k and v heads; a head's D values stay in its
+// registers (8 per lane and 16-byte chunk), so q, k and v are read once and written once.
+// Memory bound: 4 B per element, and the token's cos/sin row, loaded once per warp.  The heads'
+// loads go out first, ahead of the chain token -> sequence -> page, whose two L2 round trips
+// they hide.  kPer = 4 where that still gives every SM 64 warps, else 1: a single token's heads
+// then go to as many warps.  4096 sliding tokens (138 MB): 33.6 us with 4, 34.7 with 8, 37.5 with
+// 2, 77 with 1; one token: 2.3 us with 1.
 struct StoreArgs {
   const uint16_t *q, *k, *v;
   long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
@@ -85,113 +89,131 @@ __device__ __forceinline__ void unpack8(const uint4 w, float (&f)[8]) {
     f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
   }
 }
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                    pack_bf16x2(f[6], f[7]));
+  return make_uint4(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]), bf16x2(f[4], f[5]), bf16x2(f[6], f[7]));
 }
 __device__ __forceinline__ uint4 ldg128(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// The sequence whose new tokens include token t (-1: none), found 32 boundaries at a time.
-__device__ __forceinline__ int seq_of_token(const PagedBatch& b, int t, int lane) {
+// The sequence whose new tokens include token t (-1: none), 32 sequences at a time, and its
+// position; bad: its numbers had to be cut off.
+__device__ __forceinline__ int seq_of_token(const PagedBatch& b, int t, int lane, int& pos, bool& bad) {
   for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-    const int s = s0 + lane;
-    const bool mine = s < b.n_seqs && __ldcg(b.q_start + s) <= t && t < __ldcg(b.q_start + s + 1);
-    const uint32_t hit = __ballot_sync(0xffffffffu, mine);
-    if (hit != 0) return s0 + __ffs(hit) - 1;
+    PagedSeq q = {0, 0, 0};
+    bool cut = false;
+    if (s0 + lane < b.n_seqs) q = paged_seq(b, s0 + lane, &cut);
+    const uint32_t hit = __ballot_sync(0xffffffffu, q.t0 <= t && t < q.t0 + q.n);
+    if (hit != 0) {
+      const int from = __ffs(hit) - 1;
+      pos = __shfl_sync(0xffffffffu, q.kv - q.n + (t - q.t0), from);
+      bad = __shfl_sync(0xffffffffu, static_cast<int>(cut), from) != 0;
+      return s0 + from;
+    }
   }
   return -1;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreArgs a, const PagedBatch b,
+template <int D, int kPer>
+__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const __grid_constant__ StoreArgs a,
+                                                                    const __grid_constant__ PagedBatch b,
                                                                     Scratch* scr) {
   constexpr int C = D / 256;  // 16-byte chunks per lane: chunk c holds dims 256 c + 8 lane ..
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int slots = a.n_heads + 2 * a.n_kv;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kStoreThreads / 32) + (threadIdx.x >> 5);
-  const int t = static_cast<int>(unit / slots), slot = static_cast<int>(unit % slots);
+  const int slots = a.n_heads + 2 * a.n_kv, groups = (slots + kPer - 1) / kPer;  // q heads, k heads, v heads
+  const int unit = blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5);
+  const int t = unit / groups, slot0 = unit % groups * kPer;
   if (unit == 0) paged_check_batch(b, lane, scr);
   if (t >= b.n_tokens) return;
-  const int s = seq_of_token(b, t, lane);
+  uint4 x[kPer][C];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int slot = slot0 + i, k = slot - a.n_heads, v = k - a.n_kv;
+    if (slot >= slots) continue;
+    const uint16_t* src = k < 0 ? a.q + t * a.q_ts + slot * a.q_hs
+                                : (v < 0 ? a.k + t * a.k_ts + k * a.k_hs : a.v + t * a.v_ts + v * a.v_hs);
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[i][c] = ldg128(src + 256 * c + 8 * lane);
+  }
+  int pos = -1;
+  bool bad = false;
+  const int s = seq_of_token(b, t, lane, pos, bad);
   if (s < 0) return;
-  bool bad;
-  const PagedSeq sq = paged_seq(b, s, &bad);
-  const int pos = sq.kv - sq.n + (t - sq.t0);
-  const bool is_q = slot < a.n_heads;
-  const bool is_v = slot >= a.n_heads + a.n_kv;
-  const int head = is_q ? slot : (is_v ? slot - a.n_heads - a.n_kv : slot - a.n_heads);
   bool live = pos >= 0;
   if (pos >= a.n_positions) live = false, bad = true;
-  int page = 0;
+  int page = 0, row = 0;
   if (live) {  // (pos < kv <= max_pages * page_rows)
-    page = __ldcg(b.tables + s * b.table_stride + pos / b.page_rows);
+    page = b.tables[s * b.table_stride + pos / b.page_rows];
+    row = pos % b.page_rows;
+  }
+  float cf[C][8], sf[C][8];
+  if (live) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      unpack8(ldg128(a.cos + static_cast<long long>(pos) * D + 256 * c + 8 * lane), cf[c]);
+      unpack8(ldg128(a.sin + static_cast<long long>(pos) * D + 256 * c + 8 * lane), sf[c]);
+    }
     if (page < 0 || page >= b.n_pages) live = false, bad = true;
   }
   if (bad && lane == 0) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
-  uint16_t* dst;
-  if (is_q) {
-    dst = a.out + t * a.o_ts + head * a.o_hs;
-  } else {
-    const int row = pos % b.page_rows;
-    dst = is_v ? a.vc + page * a.vp + row * a.vr + head * a.vh : a.kc + page * a.kp + row * a.kr + head * a.kh;
-  }
-  if (!live) {
-    if (is_q)
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int slot = slot0 + i, k = slot - a.n_heads, v = k - a.n_kv;
+    if (slot >= slots || (!live && k >= 0)) continue;
+    uint16_t* dst = k < 0 ? a.out + t * a.o_ts + slot * a.o_hs
+                          : (v < 0 ? a.kc + page * a.kp + row * a.kr + k * a.kh
+                                   : a.vc + page * a.vp + row * a.vr + v * a.vh);
+    if (!live) {
 #pragma unroll
       for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const uint16_t* src = is_q ? a.q + t * a.q_ts + head * a.q_hs
-                             : (is_v ? a.v + t * a.v_ts + head * a.v_hs : a.k + t * a.k_ts + head * a.k_hs);
-  const uint16_t* w = is_q ? a.qw : a.kw;
-  uint4 xr[C], wr[C], cr[C], sr[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) xr[c] = ldg128(src + 256 * c + 8 * lane);
-  if (!is_v) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      wr[c] = ldg128(w + 256 * c + 8 * lane);
-      cr[c] = ldg128(a.cos + static_cast<long long>(pos) * D + 256 * c + 8 * lane);
-      sr[c] = ldg128(a.sin + static_cast<long long>(pos) * D + 256 * c + 8 * lane);
+      continue;
     }
-  }
-  float x[C][8], ss = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    unpack8(xr[c], x[c]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[c][i], x[c][i], ss);
-  }
-  const float r = rms_factor(warp_sum(ss), D);
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    float wf[8];
-    if (!is_v) unpack8(wr[c], wf);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[c][i] = is_v ? x[c][i] * r : x[c][i] * r * wf[i];
-  }
-  if (!is_v) {
-    // out[d] = x[d] cos[d] + x[d +- D/2] sin[d]: the other half is chunk c ^ 1 of this lane
-    // (D = 512) or chunk 0 of lane ^ 16 (D = 256)
-    float y[C][8];
+    float f[C][8], ss = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float cf[8], sf[8];
-      unpack8(cr[c], cf);
-      unpack8(sr[c], sf);
+      unpack8(x[i][c], f[c]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = C == 2 ? x[(c ^ 1) & (C - 1)][i] : __shfl_xor_sync(0xffffffffu, x[c][i], 16);
-        y[c][i] = fmaf(x[c][i], cf[i], other * sf[i]);
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[c][j], f[c][j], ss);
+    }
+    const float r = rsqrtf(fmaf(warp_sum(ss), 1.f / D, EPS));  // (2 ulp: far below the one rounding to bf16)
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[c][j] *= r;
+    if (v < 0) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float wf[8];
+        unpack8(ldg128((k < 0 ? a.qw : a.kw) + 256 * c + 8 * lane), wf);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[c][j] *= wf[j];
       }
+      // out[d] = x[d] cos[d] + x[d +- D/2] sin[d]: the other half is chunk c ^ 1 of this lane
+      // (D = 512) or chunk 0 of lane ^ 16 (D = 256)
+      float y[C][8];
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float other = C == 2 ? f[(c ^ 1) & (C - 1)][j] : __shfl_xor_sync(0xffffffffu, f[c][j], 16);
+          y[c][j] = fmaf(f[c][j], cf[c][j], other * sf[c][j]);
+        }
+#pragma unroll
+      for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = pack8(y[c]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = pack8(f[c]);
     }
-#pragma unroll
-    for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = pack8(y[c]);
-  } else {
-#pragma unroll
-    for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = pack8(x[c]);
   }
+}
+constexpr int kStorePer = 4;
+template <int kPer>
+static const void* store_kernel(int head_dim) {
+  return head_dim == DS ? (const void*)paged_store_kernel<DS, kPer> : (const void*)paged_store_kernel<DF, kPer>;
 }
 
 // ---------------------------------------------------------------------------- page copies
@@ -339,11 +361,13 @@ g4_status g4_paged_store_qkv(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
                  cache->v_row_stride, cache->v_head_stride, q_out, out_token_stride, out_head_stride};
   PagedBatch b = paged_batch(batch, cache);
   Scratch* scr = ctx->buf.scratch;
-  const long long warps = static_cast<long long>(batch->n_tokens) * (n_heads + 2 * cache->n_kv_heads);
+  const int slots = n_heads + 2 * cache->n_kv_heads;
+  const int per = static_cast<long long>(batch->n_tokens) * slots >= 64ll * kStorePer * ctx->sm_count ? kStorePer : 1;
+  const long long warps = static_cast<long long>(batch->n_tokens) * ((slots + per - 1) / per);
   const long long blocks = (warps + kStoreThreads / 32 - 1) / (kStoreThreads / 32);
-  if (blocks > INT_MAX) return fail(ctx, G4_ERR_BAD_ARG, "too many tokens times heads for one call");
+  if (blocks > INT_MAX / (kStoreThreads / 32)) return fail(ctx, G4_ERR_BAD_ARG, "too many tokens times heads for one call");
   void* args[] = {(void*)&a, (void*)&b, (void*)&scr};
-  const void* fn = cache->head_dim == DS ? (const void*)paged_store_kernel<DS> : (const void*)paged_store_kernel<DF>;
+  const void* fn = per == 1 ? store_kernel<1>(cache->head_dim) : store_kernel<kStorePer>(cache->head_dim);
   return launch_kernel(ctx, fn, dim3(static_cast<unsigned>(blocks)), dim3(kStoreThreads), 0, args, false,
                        "paged store");
 }

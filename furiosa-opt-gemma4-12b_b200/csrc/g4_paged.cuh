@@ -22,7 +22,7 @@ struct PagedSeq {
   int t0, n, kv;
 };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s, bool* bad) {
-  const int a = __ldcg(b.q_start + s), e = __ldcg(b.q_start + s + 1), l = __ldcg(b.kv_len + s);
+  const int a = b.q_start[s], e = b.q_start[s + 1], l = b.kv_len[s];
   const long long room = min(static_cast<long long>(b.max_pages) * b.page_rows, 0x7fffff00ll);
   PagedSeq q;
   q.t0 = min(max(a, 0), b.n_tokens);
@@ -39,7 +39,7 @@ __device__ __forceinline__ void paged_check_batch(const PagedBatch& b, int lane,
     paged_seq(b, s, &bad);
     any |= bad;
   }
-  if (lane == 0 && b.n_seqs > 0 && __ldcg(b.q_start) < 0) any = true;
+  if (lane == 0 && b.n_seqs > 0 && b.q_start[0] < 0) any = true;
   if (any) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
 }
 

@@ -311,7 +311,7 @@ __device__ void pa_count(const PagedBatch& b, const PaArgs& a, long long* w, Scr
     PagedSeq q = {0, 0, 0};
     bool bad = false;
     if (s < b.n_seqs) q = paged_seq(b, s, &bad);
-    if (report && s == 0 && b.n_seqs > 0 && __ldcg(b.q_start) < 0) bad = true;
+    if (report && s == 0 && b.n_seqs > 0 && b.q_start[0] < 0) bad = true;
     if (report && bad) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
     const int tiles = pa_tiles(q, a.group);
     long long sum = 0;
@@ -715,7 +715,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       Box x = {0, -1};
       if (in_stage < 64 && row < it.s.kv && row + a.box > it.low()) {
         const int j = a.by_page.div(row);
-        x.page = __ldcg(b.tables + it.seq * b.table_stride + j);
+        x.page = b.tables[it.seq * b.table_stride + j];
         x.row = row - j * b.page_rows;
       }
       return x;

@@ -25,9 +25,10 @@
 // balanced.  An item that crosses a range's end leaves partial sums (f32) that a second
 // kernel joins in range order.
 //
-// Roles of a CTA's 8 warps: 0-3 softmax and output, 4 K copies, 5 MMA (leader CTA) and tensor
-// memory, 6 V copies, 7 Q copies and the V tiles at a sequence's ends (TMA cannot stop at its
-// last row; rows past it may hold NaN, and 0 * NaN is NaN, so they are zeroed there).
+// Roles of a CTA's 12 warps: 0-3 softmax, 4 K copies, 5 MMA (leader CTA) and tensor memory,
+// 6 V copies, 7 Q copies and the V tiles at a sequence's ends (TMA cannot stop at its last row;
+// rows past it may hold NaN, and 0 * NaN is NaN, so they are zeroed there), 8-11 output: O of
+// one item leaves while the scores and the softmax of the next are under way.
 #include <cuda.h>
 
 #include <cmath>
@@ -37,11 +38,12 @@
 
 namespace g4 {
 
-constexpr int kPaThreads = 256;
+constexpr int kPaThreads = 384;
 constexpr int kPaRows = 256;      // rows per item (both CTAs)
 constexpr int kPaKeys = 128;      // cache rows per unit
 constexpr int kPaStage = 16384;   // bytes per ring stage: 64 K rows x 128 dims, or 64 V rows x 128 dims
 constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
+constexpr int kPaItemCost = 2;     // an item's start and end, in units, for the work split
 constexpr float kPaLag = 8.f;     // log2 of how far a row's maximum may rise before O is rescaled
 // kind::f16, D f32, A and B bf16, M = 256; S: N = 128, both K-major; O: N = 256, B (V) MN-major
 constexpr uint32_t kPaIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (16u << 17) | (16u << 24);
@@ -87,11 +89,14 @@ struct __align__(1024) PaSmem {
   uint8_t q[D / 64][128 * 128];  // 64-dim blocks [128 rows][64], 128-byte swizzle
   uint8_t ring[kStages][kPaStage];  // K stages, then V stages
   uint64_t full[kStages], empty[kStages], s_full[2], p_full, pv_done, q_full, q_empty, edge_full, edge_done;
+  uint64_t o_full, o_free, ml_full, ml_free;
+  float2 ml[128];  // an item's reference maxima and sums, from the softmax warps to the output warps
   uint32_t tmem;
   uint32_t abort;
-  long long units, first;  // of the call; of this range
+  long long units, first;  // weight of the call; where this range starts
   int range_count;         // ranges in use
-  int seq, tile, head, unit;
+  int item_cost;
+  int seq, tile, head, offset;
 };
 
 // ---------------------------------------------------------------------------- PTX
@@ -303,8 +308,12 @@ __device__ __forceinline__ long long pa_warp_scan(long long v, int lane) {  // i
   }
   return v;
 }
-// Units of every sequence into w[]; the whole CTA.
-__device__ void pa_count(const PagedBatch& b, const PaArgs& a, long long* w, Scratch* scr, bool report) {
+// Units and items of every sequence into w[]; the whole CTA.
+struct PaCount {
+  long long units;
+  int items;
+};
+__device__ void pa_count(const PagedBatch& b, const PaArgs& a, PaCount* w, Scratch* scr, bool report) {
   const int tid = threadIdx.x, lane = tid & 31;
   for (int s0 = 0; s0 < b.n_seqs; s0 += kPaThreads) {
     const int s = s0 + tid;
@@ -326,16 +335,18 @@ __device__ void pa_count(const PagedBatch& b, const PaArgs& a, long long* w, Scr
       x = pa_warp_sum(x);
       if (lane == from) sum = x;
     }
-    if (s < b.n_seqs) w[s] = sum * a.n_kv;
+    if (s < b.n_seqs) w[s] = {sum * a.n_kv, tiles * a.n_kv};
   }
 }
-// Where unit number `want` (< the total) lies; one warp, every lane gets the answer.
-__device__ void pa_find(const PagedBatch& b, const PaArgs& a, const long long* w, long long want, int lane, int& seq,
-                        int& tile, int& head, int& unit) {
+// The item that position `want` (< the total) of the weighted order lies in, and how far into
+// it: an item weighs its units and `cost`.  One warp, every lane gets the answer.
+__device__ void pa_find(const PagedBatch& b, const PaArgs& a, const PaCount* w, int cost, long long want, int lane,
+                        int& seq, int& tile, int& head, int& offset) {
   long long base = 0;
   seq = 0;
   for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-    const long long x = s0 + lane < b.n_seqs ? w[s0 + lane] : 0;
+    long long x = 0;
+    if (s0 + lane < b.n_seqs) x = w[s0 + lane].units + static_cast<long long>(cost) * w[s0 + lane].items;
     const long long incl = pa_warp_scan(x, lane);
     const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
     if (past != 0) {
@@ -350,36 +361,38 @@ __device__ void pa_find(const PagedBatch& b, const PaArgs& a, const long long* w
   const PagedSeq q = paged_seq(b, seq, &bad);
   const int tiles = pa_tiles(q, a.group);
   tile = 0;
-  int nk = 1, kt0;
+  int weight = 1, kt0;
   for (int t0 = 0; t0 < tiles; t0 += 32) {
-    const int n = t0 + lane < tiles ? pa_key_tiles(q, t0 + lane, a, kt0) : 0;
+    const int n = t0 + lane < tiles ? pa_key_tiles(q, t0 + lane, a, kt0) + cost : 0;
     const long long x = static_cast<long long>(n) * a.n_kv;
     const long long incl = pa_warp_scan(x, lane);
     const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
     if (past != 0) {
       const int at = __ffs(past) - 1;
       tile = t0 + at;
-      nk = __shfl_sync(0xffffffffu, n, at);
+      weight = __shfl_sync(0xffffffffu, n, at);
       base += __shfl_sync(0xffffffffu, incl - x, at);
       break;
     }
     base += __shfl_sync(0xffffffffu, incl, 31);
   }
-  head = static_cast<int>((want - base) / nk);
-  unit = static_cast<int>((want - base) % nk);
+  head = static_cast<int>((want - base) / weight);
+  offset = static_cast<int>((want - base) % weight);
 }
 
 // The items of a range, in order; every role walks them alike.
 struct PaWalk {
   const PagedBatch& b;
   const PaArgs& a;
-  long long left;  // units after the current item
+  const int cost;
+  long long left;  // weight after the current item
   int seq, tile, head;
   PagedSeq s;
   int kt0, nk, begin, end;  // key tiles of the current item: [begin, end) of its nk are this range's
-  int next_unit;
-  __device__ PaWalk(const PagedBatch& batch, const PaArgs& args, int seq_, int tile_, int head_, int unit_, long long n)
-      : b(batch), a(args), left(n), seq(seq_), tile(tile_), head(head_ - 1), next_unit(unit_) {
+  int next_offset;
+  __device__ PaWalk(const PagedBatch& batch, const PaArgs& args, int cost_, int seq_, int tile_, int head_, int offset,
+                    long long weight)
+      : b(batch), a(args), cost(cost_), left(weight), seq(seq_), tile(tile_), head(head_ - 1), next_offset(offset) {
     bool bad;
     s = left > 0 ? paged_seq(b, seq, &bad) : PagedSeq{0, 0, 0};
   }
@@ -396,11 +409,14 @@ struct PaWalk {
       }
     }
     nk = pa_key_tiles(s, tile, a, kt0);
-    begin = next_unit;
-    next_unit = 0;
-    end = static_cast<int>(min(static_cast<long long>(nk), begin + left));
-    left -= end - begin;
-    return true;
+    // the item's first `cost` positions are its overhead, the others its units
+    const int offset = next_offset;
+    const int to = static_cast<int>(min(static_cast<long long>(nk + cost), offset + left));
+    next_offset = 0;
+    begin = max(0, offset - cost);
+    end = max(0, to - cost);
+    left -= to - offset;
+    return end > begin;  // (no unit: the range ends within the overhead)
   }
   // the first cache row any new token of the sequence sees
   __device__ int low() const { return a.window > 0 ? max(0, s.kv - s.n - a.window + 1) : 0; }
@@ -454,6 +470,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     mbar_init(&sm.q_empty, 1);
     mbar_init(&sm.edge_full, 1);
     mbar_init(&sm.edge_done, 1);
+    mbar_init(&sm.o_full, 1);
+    mbar_init(&sm.o_free, 8);
+    mbar_init(&sm.ml_full, 4);
+    mbar_init(&sm.ml_free, 4);
     sm.abort = 0;
     fence_mbar_init();
   }
@@ -464,31 +484,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   }
   pdl_wait();
   pdl_launch_dependents();
-  long long* w = reinterpret_cast<long long*>(&sm.ring[0][0]);  // (the ring is not in use yet)
-  static_assert(G4_PAGED_MAX_SEQS * 8 <= kStages * kPaStage, "unit counts fit the ring");
+  PaCount* w = reinterpret_cast<PaCount*>(&sm.ring[0][0]);  // (the ring is not in use yet)
+  static_assert(G4_PAGED_MAX_SEQS * sizeof(PaCount) <= kStages * kPaStage, "unit counts fit the ring");
   pa_count(b, a, w, scr, blockIdx.x == 0);
   pa_fence_before();
   __syncthreads();
   pa_fence_after();
   if (warp == 0) {
-    long long u = 0;
-    for (int s = lane; s < b.n_seqs; s += 32) u += w[s];
+    long long u = 0, items = 0;
+    for (int s = lane; s < b.n_seqs; s += 32) {
+      u += w[s].units;
+      items += w[s].items;
+    }
     u = pa_warp_sum(u);
-    const long long n = min(static_cast<long long>(a.ranges), u);  // ranges in use: each has a unit at least
-    int seq = 0, tile = 0, head = 0, unit = 0;
+    items = pa_warp_sum(items);
+    const int cost = u <= a.ranges ? 0 : kPaItemCost;  // with a pair for every unit, each gets one
+    u += cost * items;
+    const long long n = min(static_cast<long long>(a.ranges), u);  // ranges in use: none is empty
+    int seq = 0, tile = 0, head = 0, offset = 0;
     long long first = 0;
     if (range < n) {
       first = range * u / n;
-      pa_find(b, a, w, first, lane, seq, tile, head, unit);
+      pa_find(b, a, w, cost, first, lane, seq, tile, head, offset);
     }
     if (lane == 0) {
       sm.units = u;
       sm.first = first;
       sm.range_count = static_cast<int>(n);
+      sm.item_cost = cost;
       sm.seq = seq;
       sm.tile = tile;
       sm.head = head;
-      sm.unit = unit;
+      sm.offset = offset;
     }
     fence_proxy_async();  // the ring's next writers are TMA copies
   }
@@ -498,21 +525,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   const long long u_first = sm.first;
   const long long u_end = range < sm.range_count ? (range + 1) * sm.units / sm.range_count : u_first;
   volatile uint32_t* abort = &sm.abort;
-  PaWalk it(b, a, sm.seq, sm.tile, sm.head, sm.unit, u_end - u_first);
+  PaWalk it(b, a, sm.item_cost, sm.seq, sm.tile, sm.head, sm.offset, u_end - u_first);
 
+  // registers a thread: 168 at launch (384 x 168 in all), then 232, 96 and 168 (128 x 496 = 63488)
+  if (warp < 4)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+  else if (warp < 8)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   if (warp < 4) {
-    // -------------------------------------------------------------- softmax and output
+    // -------------------------------------------------------------- softmax
     const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
     const uint32_t p_full = pa_map_to(smem_u32(&sm.p_full), 0);
     // scores are scaled within the exponent's FMA; a scale that is not positive goes first
     const bool scale_first = !(a.scale > 0.f);
     const float factor_s = scale_first ? 1.f : a.scale;
-    uint32_t g = 0;  // unit of the range
-    PaTail tail = {-1, 0, 0, 0};
+    uint32_t g = 0, items = 0;  // units and items of the range
     bool ok = true;
     while (ok && it.next()) {
       const int rr = it.tile * kPaRows + cta * 128 + tid;
-      const int i = a.by_group.div(rr), hg = rr - i * a.group;
+      const int i = a.by_group.div(rr);
       const bool valid = i < it.s.n;
       const bool any_row = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps step
       const int pos = it.s.kv - it.s.n + i;
@@ -607,10 +638,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           pa_unpair(pa_add2(pa_add2(sum[0], sum[1]), pa_add2(sum[2], sum[3])), a0, a1);
           l += a0 + a1;
         }
-        if (u != it.begin) {  // the previous P V is done: O may be rescaled, and this unit's may follow
+        if (g != 0) {  // the previous P V is done: O may be rescaled, and this unit's may follow
           ok = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
           if (!ok) break;
-          if (__any_sync(0xffffffffu, factor != 1.f)) {
+          if (u != it.begin && __any_sync(0xffffffffu, factor != 1.f)) {
             pa_fence_after();
 #pragma unroll 1
             for (int c = 0; c < 256; c += 32) {
@@ -629,20 +660,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         __syncwarp();
         if (lane == 0) pa_arrive_relaxed(p_full);
       }
-      ok = ok && pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
+      if (ok && items > 0) ok = pa_wait_warp(&sm.ml_free, (items - 1) & 1, abort, budget);
       if (!ok) break;
+      ++items;
+      sm.ml[tid] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.ml_full);
+    }
+    if (ok && g > 0) ok = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
+    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+  } else if (warp >= 8) {
+    // -------------------------------------------------------------- output
+    const int r = tid - 256;  // row of the CTA's 128
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp - 8)) << 16;
+    const uint32_t o_free = pa_map_to(smem_u32(&sm.o_free), 0);
+    uint32_t items = 0;
+    PaTail tail = {-1, 0, 0, 0};
+    bool ok = true;
+    while (ok && it.next()) {
+      const int rr = it.tile * kPaRows + cta * 128 + r;
+      const int i = a.by_group.div(rr), hg = rr - i * a.group;
+      const bool valid = i < it.s.n;
+      ok = pa_wait_warp(&sm.ml_full, items & 1, abort, budget) && pa_wait_warp(&sm.o_full, items & 1, abort, budget);
+      if (!ok) break;
+      ++items;
+      const float2 ml = sm.ml[r];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.ml_free);
       const bool whole = it.begin == 0 && it.end == it.nk;
       if (it.begin == 0 && it.end < it.nk) {
-        // the item's last unit is number u_end - it.end + it.nk - 1 of the call
+        // the item's last unit is at position u_end - it.end + it.nk - 1 of the call
         const long long last = u_end - it.end + it.nk - 1;
         const long long e = ((last + 1) * sm.range_count - 1) / sm.units;
         tail = {it.seq, it.tile, it.head, static_cast<int>(e) - range + 1};
       }
-      if (!any_row) continue;
       pa_fence_after();
-      if (whole) {
+      if (!__any_sync(0xffffffffu, valid)) {
+        // no row of this warp's
+      } else if (whole) {
         // four lanes write 64 bytes of one row at a time: one row per lane would be 32 lines per store
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = ml.y > 0.f ? 1.f / ml.y : 0.f;
         uint16_t* row[4];
         bool live[4];
         const unsigned long long mine = reinterpret_cast<unsigned long long>(
@@ -653,39 +710,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           live[j] = __shfl_sync(0xffffffffu, static_cast<int>(valid), (lane & 28) + j) != 0;
         }
 #pragma unroll 1
-        for (int c = 0; c < 256; c += 32) {
-          float o[32];
-          uint32_t x[16];
-          pa_ld32(tbase + lanes + c, o);
+        for (int c = 0; c < 256; c += 64) {
+          float o[2][32];
+          pa_ld32(tbase + lanes + c, o[0]);
+          pa_ld32(tbase + lanes + c + 32, o[1]);
           pa_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] = pa_bf16x2(o[2 * j] * inv, o[2 * j + 1] * inv);
-          pa_quad_transpose(x, lane);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t x[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (live[j])
-              *reinterpret_cast<uint4*>(row[j] + c) = make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+            for (int j = 0; j < 16; ++j) x[j] = pa_bf16x2(o[h][2 * j] * inv, o[h][2 * j + 1] * inv);
+            pa_quad_transpose(x, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (live[j])
+                *reinterpret_cast<uint4*>(row[j] + c + 32 * h) =
+                    make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+          }
         }
       } else {
         float* part = a.part + (((static_cast<size_t>(range) * kHalves + half) * 2 + cta) * 2 + (it.begin == 0 ? 1 : 0)) *
                                    kPaPartFloats;
 #pragma unroll 1
-        for (int c = 0; c < 256; c += 32) {
-          float o[32];
-          pa_ld32(tbase + lanes + c, o);
+        for (int c = 0; c < 256; c += 64) {
+          float o[2][32];
+          pa_ld32(tbase + lanes + c, o[0]);
+          pa_ld32(tbase + lanes + c + 32, o[1]);
           pa_ld_wait();
           if (valid) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(part + ((c + j) / 4 * 128 + tid) * 4) =
-                  make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<float4*>(part + ((c + 32 * h + j) / 4 * 128 + r) * 4) =
+                    make_float4(o[h][j], o[h][j + 1], o[h][j + 2], o[h][j + 3]);
           }
         }
-        *reinterpret_cast<float2*>(part + 128 * 256 + 2 * tid) = make_float2(m, l);
+        *reinterpret_cast<float2*>(part + 128 * 256 + 2 * r) = ml;
       }
+      pa_fence_before();
+      __syncwarp();
+      if (lane == 0) pa_arrive_relaxed(o_free);
     }
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
-    if (tid == 0 && cta == 0 && half == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
+    if (r == 0 && cta == 0 && half == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
   } else if (warp == 4 || warp == 6) {
     // -------------------------------------------------------------- K copies (4), V copies (6)
     // A stage is one box where a page holds its 64 rows, else one box per lane: lane & 1 is the
@@ -827,6 +895,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           const uint32_t unit = g + (u - it.begin);
           const uint32_t p = tbase + kPaColS + (unit & 1) * 128;
           ok = pa_wait_warp(&sm.p_full, unit & 1, abort, budget);
+          if (ok && u == it.begin && items > 1) ok = pa_wait_warp(&sm.o_free, (items - 2) & 1, abort, budget);
           const bool edge = it.edge(it.kt0 + u);
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
@@ -843,6 +912,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
                 pa_mma_ts(tbase, p + 32 * v + 8 * k, vd + 2048 * k / 16, kPaIdescO, (v | k) ? 1u : more);
               pa_commit(&sm.empty[v_at.stage]);
               if (v == 1) pa_commit(&sm.pv_done);
+              if (v == 1 && u + 1 == it.end) pa_commit(&sm.o_full);
             }
             __syncwarp();
             v_at.next();

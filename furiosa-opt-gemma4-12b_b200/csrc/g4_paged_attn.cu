@@ -41,7 +41,7 @@ namespace g4 {
 constexpr int kPaThreads = 384;
 constexpr int kPaRows = 256;      // rows per item (both CTAs)
 constexpr int kPaKeys = 128;      // cache rows per unit
-constexpr int kPaStage = 16384;   // bytes per ring stage: 64 K rows x 128 dims, or 64 V rows x 128 dims
+constexpr int kPaStage = 32768;   // bytes per ring stage: 64 K rows x 256 dims, or 128 V rows x 128 dims
 constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
 constexpr int kPaItemCost = 2;     // an item's start and end, in units, for the work split
 constexpr float kPaLag = 8.f;     // log2 of how far a row's maximum may rise before O is rescaled
@@ -70,7 +70,7 @@ struct PaArgs {
   int group, n_kv, window;  // query heads per KV head, KV heads
   PaDiv by_group, by_page;  // by group and by the rows of a page
   float scale;              // times log2(e)
-  int box;                  // cache rows per TMA box
+  int log_box;              // log2 of the cache rows per TMA box
   int q_tma;                // Q rows come by TMA (the group divides 128), else by the softmax warps
   int ranges;
   float* part;              // [ranges][halves][2 CTAs][2][kPaPartFloats]
@@ -85,7 +85,7 @@ template <int D>
 struct __align__(1024) PaSmem {
   // K and V each have a ring of their own: every ring has one filler, which meets the phases of
   // its barriers one by one (a parity tells two neighbouring phases apart, not three)
-  static constexpr int kK = D == 256 ? 5 : 4, kV = D == 256 ? 5 : 2, kStages = kK + kV;
+  static constexpr int kK = D == 256 ? 3 : 2, kV = D == 256 ? 2 : 1, kStages = kK + kV;
   uint8_t q[D / 64][128 * 128];  // 64-dim blocks [128 rows][64], 128-byte swizzle
   uint8_t ring[kStages][kPaStage];  // K stages, then V stages
   uint64_t full[kStages], empty[kStages], s_full[2], p_full, pv_done, q_full, q_empty, edge_full, edge_done;
@@ -451,7 +451,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
                       const __grid_constant__ CUtensorMap qmap, const __grid_constant__ PaArgs a,
                       const __grid_constant__ PagedBatch b, Scratch* scr, uint64_t budget) {
   using Smem = PaSmem<D>;
-  constexpr int kK = Smem::kK, kV = Smem::kV, kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 128;  // a K tile is kChunks stages
+  constexpr int kK = Smem::kK, kV = Smem::kV, kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 256;  // a K tile is kChunks stages
   extern __shared__ uint8_t pa_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(pa_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -756,99 +756,92 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     if (r == 0 && cta == 0 && half == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
   } else if (warp == 4 || warp == 6) {
     // -------------------------------------------------------------- K copies (4), V copies (6)
-    // A stage is one box where a page holds its 64 rows, else one box per lane: lane & 1 is the
-    // 64-dim block, lane >> 1 the box of rows.
+    // A K stage is 4 blocks of 64 dims x 64 rows, a V stage 2 halves of 64 rows x 2 blocks.  Where
+    // a page holds 64 rows in one piece, a box is all of a K stage or of a half; else a box is
+    // 2^log_box rows of one block.  A lane copies one box; the lanes run on their own.
     const bool is_k = warp == 4;
     PaRing at(is_k ? 0 : kK, is_k ? kK : kV);
     uint32_t edges = 0;  // V tiles that warp 7 finishes
     const uint64_t map = reinterpret_cast<uint64_t>(is_k ? &kmap : &vmap);
-    const bool whole = a.box == 64;
-    const int slab = whole ? 0 : lane & 1, in_stage = (whole ? lane : lane >> 1) * a.box;
-    const uint32_t box_bytes = a.box * (whole ? 256u : 128u);
+    const int box = 1 << a.log_box, rows = is_k ? 64 : kPaKeys;
+    const int blocks = a.log_box == 6 ? 1 : (is_k ? 4 : 2);  // boxes side by side
+    const int slab = lane & (blocks - 1), in_stage = lane / blocks * box;
+    const uint32_t rows_bytes = (is_k ? 512u : 256u) * box;  // of a box of rows over all blocks
     const uint32_t full0 = pa_map_to(smem_u32(&sm.full[0]), 0), edge_full = smem_u32(&sm.edge_full);
-    const uint32_t dst0 = smem_u32(&sm.ring[0][0]) + slab * 8192u + in_stage * 128u;
+    const uint32_t dst0 = smem_u32(&sm.ring[0][0]) + slab * 8192u +
+                          (is_k ? in_stage * 128u : (in_stage >> 6) * 16384u + (in_stage & 63) * 128u);
     bool ok = true, bad_page = false;
-    auto free_stage = [&](const PaRing& r) {  // waits until the stage at `r` may be filled
-      if (ok && r.passed >= static_cast<uint32_t>(r.n))
-        ok = pa_wait_warp(&sm.empty[r.stage], r.parity ^ 1u, abort, budget);
-      return ok;
-    };
-    // this lane's box of the 64 rows from `row0` on (row -1: not copied): its page, not looked
-    // at before the box is, and its row there
+    // the stage's `rows` rows from row0 on: this lane's box (row -1: not copied), its page, not
+    // looked at before the box is copied, and the bytes of all boxes
     struct Box {
       int page, row;
+      uint32_t bytes;
     };
     auto box_of = [&](int row0) {
-      const int row = row0 + in_stage;
-      Box x = {0, -1};
-      if (in_stage < 64 && row < it.s.kv && row + a.box > it.low()) {
+      const int low = it.low(), row = row0 + in_stage;
+      Box x = {0, -1, 0};
+      const int from = max(low - row0, 0) >> a.log_box, to = (min(it.s.kv - row0, rows) + box - 1) >> a.log_box;
+      x.bytes = max(to - from, 0) * rows_bytes;
+      if (in_stage < rows && row < it.s.kv && row + box > low) {
         const int j = a.by_page.div(row);
         x.page = b.tables[it.seq * b.table_stride + j];
         x.row = row - j * b.page_rows;
       }
       return x;
     };
-    auto fill = [&](Box& x, int dim_block, uint32_t bar, bool announce, uint32_t n) {
-      if (x.page < 0 || x.page >= b.n_pages) {
-        bad_page = true;
-        x.page = b.n_pages;  // out of the map's bounds: zeros
-      }
-      if (announce && lane == 0) pa_expect_cluster(bar, n);
-      if (x.row >= 0)
+    auto free_stage = [&]() {  // waits until the stage at `at` may be filled
+      if (ok && at.passed >= static_cast<uint32_t>(at.n))
+        ok = pa_wait(&sm.empty[at.stage], at.parity ^ 1u, abort, budget);
+      return ok;
+    };
+    auto fill = [&](Box& x, int dim_block, uint32_t bar) {
+      if (x.row >= 0) {
+        if (x.page < 0 || x.page >= b.n_pages) {
+          bad_page = true;
+          x.page = b.n_pages;  // out of the map's bounds: zeros
+        }
         pa_tma(dst0 + at.stage * static_cast<uint32_t>(kPaStage), map, x.row, dim_block + slab, it.head, x.page, bar);
-      __syncwarp();
+      }
       at.next();
     };
-    auto bytes = [&](const Box& x) { return __popc(__ballot_sync(0xffffffffu, x.row >= 0)) * box_bytes; };
-    if (is_k) {
-      while (ok && it.next()) {
-        auto k_row = [&](int u) { return (it.kt0 + u) * kPaKeys + 64 * cta; };
-        Box next = box_of(k_row(it.begin));
-        for (int u = it.begin; u < it.end && ok; ++u) {
-          Box now = next;  // the next tile's table entries are fetched while this one's stages become free
-          if (u + 1 < it.end) next = box_of(k_row(u + 1));
-          const uint32_t n = bytes(now);
+    const int v_block = 4 * half + 2 * cta;
+    while (ok && it.next()) {
+      auto first_row = [&](int u) { return (it.kt0 + u) * kPaKeys + (is_k ? 64 * cta : 0); };
+      Box next = box_of(first_row(it.begin));
+      for (int u = it.begin; u < it.end && ok; ++u) {
+        Box now = next;  // the next tile's table entries are fetched while this one's stages become free
+        if (u + 1 < it.end) next = box_of(first_row(u + 1));
+        if (is_k) {
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            if (free_stage(at)) fill(now, 2 * ch, full0 + 8u * at.stage, true, n);
-        }
-      }
-    } else {
-      const int v_block = 4 * half + 2 * cta;
-      while (ok && it.next()) {
-        Box next0 = box_of((it.kt0 + it.begin) * kPaKeys), next1 = box_of((it.kt0 + it.begin) * kPaKeys + 64);
-        for (int u = it.begin; u < it.end && ok; ++u) {
-          Box now0 = next0, now1 = next1;
-          const int row = (it.kt0 + u) * kPaKeys;
-          if (u + 1 < it.end) {
-            next0 = box_of(row + kPaKeys);
-            next1 = box_of(row + kPaKeys + 64);
+            if (free_stage()) {
+              const uint32_t bar = full0 + 8u * at.stage;
+              if (lane == 0) pa_expect_cluster(bar, now.bytes);
+              fill(now, 4 * ch, bar);
+            }
+        } else if (!it.edge(it.kt0 + u)) {
+          if (free_stage()) {
+            const uint32_t bar = full0 + 8u * at.stage;
+            if (lane == 0) pa_expect_cluster(bar, now.bytes);
+            fill(now, v_block, bar);
           }
-          const bool edge = it.edge(it.kt0 + u);
-          const uint32_t n0 = bytes(now0), n1 = bytes(now1);
-          if (!edge) {
-            if (free_stage(at)) fill(now0, v_block, full0 + 8u * at.stage, true, n0);
-            if (free_stage(at)) fill(now1, v_block, full0 + 8u * at.stage, true, n1);
-            continue;
-          }
-          // both stages report to warp 7, which zeroes rows of them (with no box to wait for, at
-          // once: so only when both are free) and reports to the leader
-          if (edges > 0) ok = ok && pa_wait_warp(&sm.edge_done, (edges - 1) & 1, abort, budget);
-          PaRing second = at;
-          second.next();
-          if (!free_stage(at) || !free_stage(second)) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sm.edge_full, n0 + n1);
+        } else {
+          // the stage reports to warp 7, which zeroes rows of it (with no box to wait for, at
+          // once: so only when it is free) and reports to the leader
+          if (edges > 0) ok = pa_wait(&sm.edge_done, (edges - 1) & 1, abort, budget);
           ++edges;
-          fill(now0, v_block, edge_full, false, 0);
-          fill(now1, v_block, edge_full, false, 0);
+          if (free_stage()) {
+            if (lane == 0) mbar_arrive_expect_tx(&sm.edge_full, now.bytes);
+            fill(now, v_block, edge_full);
+          }
         }
       }
     }
     // every stage is free again: no barrier of this CTA has an arrival outstanding when it exits
     for (uint32_t n = at.n, x = at.passed > n ? at.passed - n : 0; x < at.passed && ok; ++x)
-      ok = pa_wait_warp(&sm.empty[at.first + x % n], (x / n) & 1, abort, budget);
+      ok = pa_wait(&sm.empty[at.first + x % n], (x / n) & 1, abort, budget);
     if (bad_page) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
-    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+    if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   } else if (warp == 5) {
     // -------------------------------------------------------------- MMA: the leader CTA's
     // The warp stays converged around the elected lane, so that descriptors live in uniform
@@ -871,8 +864,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           const uint64_t kd = k_desc + k_at.stage * static_cast<uint32_t>(kPaStage / 16);
           if (leader) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              pa_mma_ss(d, q_desc + ((2 * ch + (k >> 2)) * 16384 + 32 * (k & 3)) / 16,
+            for (int k = 0; k < 16; ++k)
+              pa_mma_ss(d, q_desc + ((4 * ch + (k >> 2)) * 16384 + 32 * (k & 3)) / 16,
                         kd + ((k >> 2) * 8192 + 32 * (k & 3)) / 16, kPaIdescS, (ch | k) ? 1u : 0u);
             pa_commit(&sm.empty[k_at.stage]);
             if (ch == kChunks - 1) pa_commit(&sm.s_full[unit & 1]);
@@ -897,26 +890,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           ok = pa_wait_warp(&sm.p_full, unit & 1, abort, budget);
           if (ok && u == it.begin && items > 1) ok = pa_wait_warp(&sm.o_free, (items - 2) & 1, abort, budget);
           const bool edge = it.edge(it.kt0 + u);
+          if (ok)
+            ok = edge ? __all_sync(0xffffffffu, pa_wait<true>(&sm.full[v_at.stage], v_at.parity, abort, budget))
+                      : pa_wait_warp(&sm.full[v_at.stage], v_at.parity, abort, budget);
+          if (!ok) break;
+          pa_fence_after();
+          const uint64_t vd = v_desc + v_at.stage * static_cast<uint32_t>(kPaStage / 16);
+          const uint32_t more = u > it.begin ? 1u : 0u;
+          if (leader) {
 #pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            if (ok)
-              ok = edge ? __all_sync(0xffffffffu, pa_wait<true>(&sm.full[v_at.stage], v_at.parity, abort, budget))
-                        : pa_wait_warp(&sm.full[v_at.stage], v_at.parity, abort, budget);
-            if (!ok) break;
-            pa_fence_after();
-            const uint64_t vd = v_desc + v_at.stage * static_cast<uint32_t>(kPaStage / 16);
-            const uint32_t more = u > it.begin ? 1u : 0u;
-            if (leader) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                pa_mma_ts(tbase, p + 32 * v + 8 * k, vd + 2048 * k / 16, kPaIdescO, (v | k) ? 1u : more);
-              pa_commit(&sm.empty[v_at.stage]);
-              if (v == 1) pa_commit(&sm.pv_done);
-              if (v == 1 && u + 1 == it.end) pa_commit(&sm.o_full);
-            }
-            __syncwarp();
-            v_at.next();
+            for (int k = 0; k < 8; ++k)
+              pa_mma_ts(tbase, p + 8 * k, vd + ((k >> 2) * 16384 + 2048 * (k & 3)) / 16, kPaIdescO, k ? 1u : more);
+            pa_commit(&sm.empty[v_at.stage]);
+            pa_commit(&sm.pv_done);
+            if (u + 1 == it.end) pa_commit(&sm.o_full);
           }
+          __syncwarp();
+          v_at.next();
         }
         g += it.end - it.begin;
       }
@@ -942,9 +932,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       }
       __syncwarp();
       for (int u = it.begin; u < it.end && ok; ++u) {
-        const int s0 = at.stage;
-        at.next();
-        const int s1 = at.stage;
+        const int stage = at.stage;
         at.next();
         if (!it.edge(it.kt0 + u)) continue;
         ok = pa_wait_warp(&sm.edge_full, edges & 1, abort, budget);
@@ -956,14 +944,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         const int n = front + kPaKeys - back;
         for (int x = lane; x < 16 * n; x += 32) {
           const int k = x >> 4, ch = x & 15, r = k < front ? k : back + k - front;
-          *reinterpret_cast<uint4*>(&sm.ring[r < 64 ? s0 : s1][(ch >> 3) * 8192 + pa_swizzle(r & 63, ch)]) =
+          *reinterpret_cast<uint4*>(&sm.ring[stage][(r >> 6) * 16384 + (ch >> 3) * 8192 + pa_swizzle(r & 63, ch)]) =
               make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-          pa_arrive_cluster(full0 + 8u * s0);
-          pa_arrive_cluster(full0 + 8u * s1);
+          pa_arrive_cluster(full0 + 8u * stage);
           mbar_arrive(&sm.edge_done);
         }
       }
@@ -1111,14 +1098,16 @@ static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_
   a.ranges = pairs / (D / 256);
   if (most < a.ranges) a.ranges = static_cast<int>(most);
   const int low = b.page_rows & -b.page_rows;  // the largest power of two that divides a page's rows
-  a.box = low < 64 ? low : 64;
-  // pages: rows, 64-dim blocks, heads, pages; a box is `box` rows of one block, or of two where
-  // that fills a stage
+  a.log_box = 0;
+  while ((1 << a.log_box) < low && a.log_box < 6) ++a.log_box;
+  // pages: rows, 64-dim blocks, heads, pages; a box is 2^log_box rows of one block, or 64 rows of
+  // a K stage's four or a V stage's two
   CUtensorMap km, vm, qm;
   const int dims[4] = {c->page_rows, D / 64, c->n_kv_heads, c->n_pages};
-  const int box[4] = {a.box, a.box == 64 ? 2 : 1, 1, 1};
-  if (!tile_map(&km, c->k, dims, {c->k_row_stride, 64, c->k_head_stride, c->k_page_stride}, box) ||
-      !tile_map(&vm, c->v, dims, {c->v_row_stride, 64, c->v_head_stride, c->v_page_stride}, box))
+  const int whole = a.log_box == 6;
+  const int kbox[4] = {1 << a.log_box, whole ? 4 : 1, 1, 1}, vbox[4] = {1 << a.log_box, whole ? 2 : 1, 1, 1};
+  if (!tile_map(&km, c->k, dims, {c->k_row_stride, 64, c->k_head_stride, c->k_page_stride}, kbox) ||
+      !tile_map(&vm, c->v, dims, {c->v_row_stride, 64, c->v_head_stride, c->v_page_stride}, vbox))
     return fail(ctx, G4_ERR_UNSUPPORTED, "paged attention: the cache's layout has no TMA descriptor");
   // Q: heads of a group, tokens, blocks, KV heads; a box is a CTA's 128 rows of four blocks
   const int qdims[4] = {a.group, b.n_tokens, D / 64, a.n_kv};

@@ -972,48 +972,78 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 }
 
 // Joins the parts of the items that cross range ends: with M the largest of the parts' reference
-// maxima, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in range order.  A block has
-// eight rows and 64 columns of one half.
-constexpr int kPaJoinThreads = 128, kPaJoinRows = 8;
+// maxima, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in range order.  A block has 32 rows
+// (lanes: the parts hold a column quad's rows side by side) and 64 columns of one half; each of
+// its 8 warps takes 8 columns, and the results leave through shared memory, 128 bytes a row.
+constexpr int kPaJoinThreads = 256, kPaJoinRows = 32;
 template <int D>
 __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid_constant__ PaArgs a,
                                                                     const __grid_constant__ PagedBatch b) {
   constexpr int kHalves = D / 256;
+  __shared__ uint4 tile[kPaJoinRows][9];  // (9: the rows of a 16-byte column fall into different banks)
   pdl_wait();
   pdl_launch_dependents();
   const PaTail t = a.tail[blockIdx.x];
   if (t.seq < 0) return;
   bool bad;
   const PagedSeq s = paged_seq(b, t.seq, &bad);
-  const int half = blockIdx.z % kHalves, quad = (blockIdx.z / kHalves) * 16 + threadIdx.x / kPaJoinRows;
-  const int r = blockIdx.y * kPaJoinRows + threadIdx.x % kPaJoinRows;
-  const int rr = t.tile * kPaRows + r;
-  const int i = a.by_group.div(rr), hg = rr - i * a.group;
-  if (i >= s.n) return;
-  const int cta = r >> 7, row = r & 127;
-  auto part = [&](int k) {  // the first part is its range's second slot, the others their first
-    return a.part + (((static_cast<size_t>(blockIdx.x + k) * kHalves + half) * 2 + cta) * 2 + (k == 0 ? 1 : 0)) *
-                        kPaPartFloats;
-  };
-  float top = -CUDART_INF_F;
-#pragma unroll 8
-  for (int k = 0; k < t.parts; ++k) top = fmaxf(top, part(k)[128 * 256 + 2 * row]);
-  const float ref = top == -CUDART_INF_F ? 0.f : top;
-  float l = 0.f, o[4] = {};
-#pragma unroll 8
-  for (int k = 0; k < t.parts; ++k) {
-    const float2 ml = *reinterpret_cast<const float2*>(part(k) + 128 * 256 + 2 * row);
-    const float4 v = *reinterpret_cast<const float4*>(part(k) + (quad * 128 + row) * 4);
-    const float w = pa_exp2(ml.x - ref);
-    l = fmaf(w, ml.y, l);
-    o[0] = fmaf(w, v.x, o[0]);
-    o[1] = fmaf(w, v.y, o[1]);
-    o[2] = fmaf(w, v.z, o[2]);
-    o[3] = fmaf(w, v.w, o[3]);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int half = blockIdx.z % kHalves, col0 = blockIdx.z / kHalves * 64;
+  const int row0 = blockIdx.y * kPaJoinRows, cta = row0 >> 7, row = (row0 & 127) + lane;
+  if (a.by_group.div(t.tile * kPaRows + row0) >= s.n) return;  // (of all rows)
+  // the first part is its range's second slot, the others their first
+  const float* first = a.part + (((static_cast<size_t>(blockIdx.x) * kHalves + half) * 2 + cta) * 2 + 1) * kPaPartFloats;
+  const size_t step = static_cast<size_t>(kHalves) * 4 * kPaPartFloats;
+  constexpr int kBatch = 4;
+  float top = -CUDART_INF_F, l = 0.f, o[2][4] = {};
+  for (int k0 = 0; k0 < t.parts; k0 += kBatch) {
+    float2 ml[kBatch];
+    float4 v[kBatch][2];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      ml[k] = make_float2(-CUDART_INF_F, 0.f);
+      v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + k < t.parts) {
+        const float* p = k0 + k == 0 ? first : first - kPaPartFloats + (k0 + k) * step;
+        ml[k] = *reinterpret_cast<const float2*>(p + 128 * 256 + 2 * row);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          v[k][h] = *reinterpret_cast<const float4*>(p + ((col0 / 4 + 2 * warp + h) * 128 + row) * 4);
+      }
+    }
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) now = fmaxf(now, ml[k].x);
+    const float ref = now == -CUDART_INF_F ? 0.f : now, w0 = pa_exp2(top - ref);
+    top = now;
+    l *= w0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[h][j] *= w0;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float w = pa_exp2(ml[k].x - ref);
+      l = fmaf(w, ml[k].y, l);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        o[h][0] = fmaf(w, v[k][h].x, o[h][0]);
+        o[h][1] = fmaf(w, v[k][h].y, o[h][1]);
+        o[h][2] = fmaf(w, v[k][h].z, o[h][2]);
+        o[h][3] = fmaf(w, v[k][h].w, o[h][3]);
+      }
+    }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  *reinterpret_cast<uint2*>(a.out + (s.t0 + i) * a.o_ts + (t.head * a.group + hg) * a.o_hs + 256 * half + 4 * quad) =
-      make_uint2(pa_bf16x2(o[0] * inv, o[1] * inv), pa_bf16x2(o[2] * inv, o[3] * inv));
+  tile[lane][warp] = make_uint4(pa_bf16x2(o[0][0] * inv, o[0][1] * inv), pa_bf16x2(o[0][2] * inv, o[0][3] * inv),
+                                pa_bf16x2(o[1][0] * inv, o[1][1] * inv), pa_bf16x2(o[1][2] * inv, o[1][3] * inv));
+  __syncthreads();
+  const int r = threadIdx.x / 8, c = threadIdx.x % 8;
+  const int rr = t.tile * kPaRows + row0 + r;
+  const int i = a.by_group.div(rr), hg = rr - i * a.group;
+  if (i >= s.n) return;
+  *reinterpret_cast<uint4*>(a.out + (s.t0 + i) * a.o_ts + (t.head * a.group + hg) * a.o_hs + 256 * half + col0 + 8 * c) =
+      tile[r][c];
 }
 
 // ---------------------------------------------------------------------------- host

@@ -93,7 +93,7 @@ struct __align__(1024) PaSmem {
   float2 ml[128];  // an item's reference maxima and sums, from the softmax warps to the output warps
   uint32_t tmem;
   uint32_t abort;
-  long long units, first;  // weight of the call; where this range starts
+  int units, first;        // weight of the call; where this range starts
   int range_count;         // ranges in use
   int item_cost;
   int seq, tile, head, offset;
@@ -295,23 +295,23 @@ __device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, const P
 __device__ __forceinline__ int pa_tiles(const PagedSeq& s, int group) {
   return (s.n * group + kPaRows - 1) / kPaRows;  // (n * group < 2^30: checked by the host)
 }
-__device__ __forceinline__ long long pa_warp_sum(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ long long pa_warp_scan(long long v, int lane) {  // inclusive
+__device__ __forceinline__ int pa_warp_scan(int v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, v, o);
+    const int x = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += x;
   }
   return v;
 }
-// Units and items of every sequence into w[]; the whole CTA.
+// Where range r of n starts: r * u / n.
+__device__ __forceinline__ int pa_share(int r, int u, int n) {
+  return u < (1 << 22) ? static_cast<int>(static_cast<uint32_t>(r) * static_cast<uint32_t>(u) / static_cast<uint32_t>(n))
+                       : static_cast<int>(static_cast<long long>(r) * u / n);
+}
+// Units and items of every sequence into w[]; the whole CTA.  (The call's sum is below 2^30:
+// checked by the host.)
 struct PaCount {
-  long long units;
-  int items;
+  int units, items;
 };
 __device__ void pa_count(const PagedBatch& b, const PaArgs& a, PaCount* w, Scratch* scr, bool report) {
   const int tid = threadIdx.x, lane = tid & 31;
@@ -323,16 +323,15 @@ __device__ void pa_count(const PagedBatch& b, const PaArgs& a, PaCount* w, Scrat
     if (report && s == 0 && b.n_seqs > 0 && b.q_start[0] < 0) bad = true;
     if (report && bad) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
     const int tiles = pa_tiles(q, a.group);
-    long long sum = 0;
-    int kt0;
+    int sum = 0, kt0;
     if (tiles <= 2)
       for (int t = 0; t < tiles; ++t) sum += pa_key_tiles(q, t, a, kt0);
     for (uint32_t left = __ballot_sync(0xffffffffu, tiles > 2); left != 0; left &= left - 1) {
       const int from = __ffs(left) - 1;
       const PagedSeq o = {0, __shfl_sync(0xffffffffu, q.n, from), __shfl_sync(0xffffffffu, q.kv, from)};
-      long long x = 0;
+      int x = 0;
       for (int t = lane; t < pa_tiles(o, a.group); t += 32) x += pa_key_tiles(o, t, a, kt0);
-      x = pa_warp_sum(x);
+      x = __reduce_add_sync(0xffffffffu, x);
       if (lane == from) sum = x;
     }
     if (s < b.n_seqs) w[s] = {sum * a.n_kv, tiles * a.n_kv};
@@ -340,14 +339,13 @@ __device__ void pa_count(const PagedBatch& b, const PaArgs& a, PaCount* w, Scrat
 }
 // The item that position `want` (< the total) of the weighted order lies in, and how far into
 // it: an item weighs its units and `cost`.  One warp, every lane gets the answer.
-__device__ void pa_find(const PagedBatch& b, const PaArgs& a, const PaCount* w, int cost, long long want, int lane,
-                        int& seq, int& tile, int& head, int& offset) {
-  long long base = 0;
+__device__ void pa_find(const PagedBatch& b, const PaArgs& a, const PaCount* w, int cost, int want, int lane, int& seq,
+                        int& tile, int& head, int& offset) {
+  int base = 0;
   seq = 0;
   for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-    long long x = 0;
-    if (s0 + lane < b.n_seqs) x = w[s0 + lane].units + static_cast<long long>(cost) * w[s0 + lane].items;
-    const long long incl = pa_warp_scan(x, lane);
+    const int x = s0 + lane < b.n_seqs ? w[s0 + lane].units + cost * w[s0 + lane].items : 0;
+    const int incl = pa_warp_scan(x, lane);
     const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
     if (past != 0) {
       const int at = __ffs(past) - 1;
@@ -364,8 +362,8 @@ __device__ void pa_find(const PagedBatch& b, const PaArgs& a, const PaCount* w, 
   int weight = 1, kt0;
   for (int t0 = 0; t0 < tiles; t0 += 32) {
     const int n = t0 + lane < tiles ? pa_key_tiles(q, t0 + lane, a, kt0) + cost : 0;
-    const long long x = static_cast<long long>(n) * a.n_kv;
-    const long long incl = pa_warp_scan(x, lane);
+    const int x = n * a.n_kv;
+    const int incl = pa_warp_scan(x, lane);
     const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
     if (past != 0) {
       const int at = __ffs(past) - 1;
@@ -376,8 +374,8 @@ __device__ void pa_find(const PagedBatch& b, const PaArgs& a, const PaCount* w, 
     }
     base += __shfl_sync(0xffffffffu, incl, 31);
   }
-  head = static_cast<int>((want - base) / weight);
-  offset = static_cast<int>((want - base) % weight);
+  head = (want - base) / weight;
+  offset = want - base - head * weight;
 }
 
 // The items of a range, in order; every role walks them alike.
@@ -385,13 +383,13 @@ struct PaWalk {
   const PagedBatch& b;
   const PaArgs& a;
   const int cost;
-  long long left;  // weight after the current item
+  int left;  // weight after the current item
   int seq, tile, head;
   PagedSeq s;
   int kt0, nk, begin, end;  // key tiles of the current item: [begin, end) of its nk are this range's
   int next_offset;
   __device__ PaWalk(const PagedBatch& batch, const PaArgs& args, int cost_, int seq_, int tile_, int head_, int offset,
-                    long long weight)
+                    int weight)
       : b(batch), a(args), cost(cost_), left(weight), seq(seq_), tile(tile_), head(head_ - 1), next_offset(offset) {
     bool bad;
     s = left > 0 ? paged_seq(b, seq, &bad) : PagedSeq{0, 0, 0};
@@ -411,7 +409,7 @@ struct PaWalk {
     nk = pa_key_tiles(s, tile, a, kt0);
     // the item's first `cost` positions are its overhead, the others its units
     const int offset = next_offset;
-    const int to = static_cast<int>(min(static_cast<long long>(nk + cost), offset + left));
+    const int to = min(nk + cost, offset + left);
     next_offset = 0;
     begin = max(0, offset - cost);
     end = max(0, to - cost);
@@ -491,26 +489,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   __syncthreads();
   pa_fence_after();
   if (warp == 0) {
-    long long u = 0, items = 0;
+    int u = 0, items = 0;
     for (int s = lane; s < b.n_seqs; s += 32) {
       u += w[s].units;
       items += w[s].items;
     }
-    u = pa_warp_sum(u);
-    items = pa_warp_sum(items);
+    u = __reduce_add_sync(0xffffffffu, u);
+    items = __reduce_add_sync(0xffffffffu, items);
     const int cost = u <= a.ranges ? 0 : kPaItemCost;  // with a pair for every unit, each gets one
     u += cost * items;
-    const long long n = min(static_cast<long long>(a.ranges), u);  // ranges in use: none is empty
+    const int n = min(a.ranges, u);  // ranges in use: none is empty
     int seq = 0, tile = 0, head = 0, offset = 0;
-    long long first = 0;
+    int first = 0;
     if (range < n) {
-      first = range * u / n;
+      first = pa_share(range, u, n);
       pa_find(b, a, w, cost, first, lane, seq, tile, head, offset);
     }
     if (lane == 0) {
       sm.units = u;
       sm.first = first;
-      sm.range_count = static_cast<int>(n);
+      sm.range_count = n;
       sm.item_cost = cost;
       sm.seq = seq;
       sm.tile = tile;
@@ -522,8 +520,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // both CTAs' barriers and memory are ready
   const uint32_t tbase = sm.tmem;
-  const long long u_first = sm.first;
-  const long long u_end = range < sm.range_count ? (range + 1) * sm.units / sm.range_count : u_first;
+  const int u_first = sm.first;
+  const int u_end = range < sm.range_count ? pa_share(range + 1, sm.units, sm.range_count) : u_first;
   volatile uint32_t* abort = &sm.abort;
   PaWalk it(b, a, sm.item_cost, sm.seq, sm.tile, sm.head, sm.offset, u_end - u_first);
 
@@ -690,8 +688,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const bool whole = it.begin == 0 && it.end == it.nk;
       if (it.begin == 0 && it.end < it.nk) {
         // the item's last unit is at position u_end - it.end + it.nk - 1 of the call
-        const long long last = u_end - it.end + it.nk - 1;
-        const long long e = ((last + 1) * sm.range_count - 1) / sm.units;
+        const int last = u_end - it.end + it.nk - 1;
+        const long long e = ((last + 1ll) * sm.range_count - 1) / sm.units;
         tail = {it.seq, it.tile, it.head, static_cast<int>(e) - range + 1};
       }
       pa_fence_after();
@@ -910,6 +908,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         }
         g += it.end - it.begin;
       }
+      if (ok && items > 0) ok = pa_wait_warp(&sm.o_free, (items - 1) & 1, abort, budget);
       if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     }
   } else {
@@ -963,9 +962,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const uint64_t end = global_ns() + 1000000;
     while (global_ns() < end) __nanosleep(1000);
   }
+  // Both CTAs are done with both tensor memories.  Every arrival from the other CTA has been
+  // waited for, so nothing but this order is asked of the barrier: a release would wait for
+  // the output stores in flight.
   pa_fence_before();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   pa_fence_after();
   if (warp == 5)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512u));
@@ -1125,6 +1127,8 @@ static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_
   const long long tiles = rows / kPaRows + (b.n_seqs < b.n_tokens ? b.n_seqs : b.n_tokens);
   const long long keys = (static_cast<long long>(b.max_pages) * b.page_rows + kPaKeys - 1) / kPaKeys;
   const long long most = tiles * a.n_kv * (keys < 1 ? 1 : keys);
+  if ((tiles * a.n_kv) * ((keys < 1 ? 1 : keys) + kPaItemCost) >= (1ll << 30))
+    return fail(ctx, G4_ERR_TOO_LARGE, "paged attention: more than 2^30 tiles in one call");
   a.ranges = pairs / (D / 256);
   if (most < a.ranges) a.ranges = static_cast<int>(most);
   const int low = b.page_rows & -b.page_rows;  // the largest power of two that divides a page's rows

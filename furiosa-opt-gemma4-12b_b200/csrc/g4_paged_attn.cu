@@ -29,57 +29,23 @@
 // 6 V copies, 7 Q copies and the V tiles at a sequence's ends (TMA cannot stop at its last row;
 // rows past it may hold NaN, and 0 * NaN is NaN, so they are zeroed there), 8-11 output: O of
 // one item leaves while the scores and the softmax of the next are under way.
-#include <cuda.h>
-
 #include <cmath>
 #include <string>
 
-#include "g4_paged.cuh"
+#include "g4_paged_split.cuh"
 
 namespace g4 {
 
 constexpr int kPaThreads = 384;
 constexpr int kPaRows = 256;      // rows per item (both CTAs)
-constexpr int kPaKeys = 128;      // cache rows per unit
 constexpr int kPaStage = 32768;   // bytes per ring stage: 64 K rows x 256 dims, or 128 V rows x 128 dims
 constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
 constexpr int kPaItemCost = 2;     // an item's start and end, in units, for the work split
-constexpr float kPaLag = 8.f;     // log2 of how far a row's maximum may rise before O is rescaled
+constexpr int kPaFewPerSeq = 64;   // tokens per sequence up to which single tokens are looked for
 // kind::f16, D f32, A and B bf16, M = 256; S: N = 128, both K-major; O: N = 256, B (V) MN-major
 constexpr uint32_t kPaIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (16u << 17) | (16u << 24);
 constexpr uint32_t kPaIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (32u << 17) | (16u << 24);
 constexpr int kPaPartFloats = 128 * 256 + 2 * 128;  // a partial: O as [64 column quads][128 rows][4], then (m, l) [128][2]
-
-// Division by a number fixed for the call, by multiplication (round-up method; exact for
-// 0 <= n < 2^31): a hardware divide goes through the unit that the softmax's exponentials
-// keep busy, and took the copying warps over 1000 cycles.
-struct PaDiv {
-  uint32_t mul, shift;
-  __device__ __forceinline__ int div(int n) const {
-    const uint32_t u = static_cast<uint32_t>(n);
-    return static_cast<int>((__umulhi(u, mul) + u) >> shift);
-  }
-};
-struct PaArgs {
-  const uint16_t* q;
-  long long q_ts, q_hs;
-  uint16_t* out;
-  long long o_ts, o_hs;
-  const uint16_t* vc;
-  long long vp, vr, vh;
-  int group, n_kv, window;  // query heads per KV head, KV heads
-  PaDiv by_group, by_page;  // by group and by the rows of a page
-  float scale;              // times log2(e)
-  int log_box;              // log2 of the cache rows per TMA box
-  int q_tma;                // Q rows come by TMA (the group divides 128), else by the softmax warps
-  int ranges;
-  float* part;              // [ranges][halves][2 CTAs][2][kPaPartFloats]
-  struct PaTail* tail;      // [ranges]
-};
-// An item begun in a range and finished by later ones.
-struct PaTail {
-  int seq, tile, head, parts;  // seq -1: none
-};
 
 template <int D>
 struct __align__(1024) PaSmem {
@@ -117,53 +83,6 @@ __device__ __forceinline__ void pa_expect_cluster(uint32_t addr, uint32_t bytes)
 __device__ __forceinline__ void pa_arrive_relaxed(uint32_t addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// kWide: the barrier also announces ordinary stores of the other CTA's threads.
-template <bool kWide>
-__device__ __forceinline__ bool pa_try(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  if (kWide)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-  return ok != 0;
-}
-// Bounded wait: after the budget, or once another role of the CTA gave up, false.
-template <bool kWide = false>
-__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort, uint64_t budget) {
-  for (int i = 0; i < 64; ++i)
-    if (pa_try<kWide>(bar, parity)) return true;
-  const uint64_t end = global_ns() + budget;
-  while (!pa_try<kWide>(bar, parity)) {
-    if (*abort != 0u) return false;
-    if (global_ns() > end) {
-      *abort = 1u;
-      return false;
-    }
-  }
-  return true;
-}
-// The same by a whole warp, with one answer.
-__device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort,
-                                             uint64_t budget) {
-  return __all_sync(0xffffffffu, pa_wait(bar, parity, abort, budget));
-}
-__device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
-         (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (static_cast<uint64_t>(1u) << 46) |
-         (static_cast<uint64_t>(2u) << 61);
-}
 __device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -193,67 +112,6 @@ __device__ __forceinline__ void pa_tma(uint32_t dst, uint64_t map, int c1, int c
       "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void pa_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void pa_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pa_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void pa_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float pa_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float pa_max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-// Two f32 at a time.
-__device__ __forceinline__ uint64_t pa_pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void pa_unpair(uint64_t r, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t pa_bf16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 // The 16-byte chunks w[4 j .. 4 j + 3] (j < 4) of the four lanes of a quad, transposed: lane q
 // gets chunk q of the quad's lane j in place j.
 __device__ __forceinline__ void pa_quad_transpose(uint32_t (&w)[16], int lane) {
@@ -275,174 +133,6 @@ __device__ __forceinline__ void pa_quad_transpose(uint32_t (&w)[16], int lane) {
     }
   }
 }
-__device__ __forceinline__ uint32_t pa_swizzle(int row, int c) {  // 16-byte chunk c of a 128-byte row
-  return static_cast<uint32_t>(row * 128 + (((c & 7) ^ (row & 7)) << 4));
-}
-
-// ---------------------------------------------------------------------------- work split
-// Key tiles of row tile `tile` of a sequence: [kt0, kt0 + n), n >= 1 (a tile nothing is
-// visible to still has its zeros to write).
-__device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, const PaArgs& a, int& kt0) {
-  const int r0 = tile * kPaRows;
-  const int i0 = a.by_group.div(r0), i1 = min(s.n - 1, a.by_group.div(r0 + kPaRows - 1));
-  const int first = s.kv - s.n;
-  const int hi = first + i1 + 1;
-  kt0 = 0;
-  if (hi <= 0) return 1;
-  if (a.window > 0) kt0 = max(0, first + i0 - a.window + 1) / kPaKeys;
-  return (hi + kPaKeys - 1) / kPaKeys - kt0;
-}
-__device__ __forceinline__ int pa_tiles(const PagedSeq& s, int group) {
-  return (s.n * group + kPaRows - 1) / kPaRows;  // (n * group < 2^30: checked by the host)
-}
-__device__ __forceinline__ int pa_warp_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
-// Where range r of n starts: r * u / n.
-__device__ __forceinline__ int pa_share(int r, int u, int n) {
-  return u < (1 << 22) ? static_cast<int>(static_cast<uint32_t>(r) * static_cast<uint32_t>(u) / static_cast<uint32_t>(n))
-                       : static_cast<int>(static_cast<long long>(r) * u / n);
-}
-// Units and items of every sequence into w[]; the whole CTA.  (The call's sum is below 2^30:
-// checked by the host.)
-struct PaCount {
-  int units, items;
-};
-__device__ void pa_count(const PagedBatch& b, const PaArgs& a, PaCount* w, Scratch* scr, bool report) {
-  const int tid = threadIdx.x, lane = tid & 31;
-  for (int s0 = 0; s0 < b.n_seqs; s0 += kPaThreads) {
-    const int s = s0 + tid;
-    PagedSeq q = {0, 0, 0};
-    bool bad = false;
-    if (s < b.n_seqs) q = paged_seq(b, s, &bad);
-    if (report && s == 0 && b.n_seqs > 0 && b.q_start[0] < 0) bad = true;
-    if (report && bad) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
-    const int tiles = pa_tiles(q, a.group);
-    int sum = 0, kt0;
-    if (tiles <= 2)
-      for (int t = 0; t < tiles; ++t) sum += pa_key_tiles(q, t, a, kt0);
-    for (uint32_t left = __ballot_sync(0xffffffffu, tiles > 2); left != 0; left &= left - 1) {
-      const int from = __ffs(left) - 1;
-      const PagedSeq o = {0, __shfl_sync(0xffffffffu, q.n, from), __shfl_sync(0xffffffffu, q.kv, from)};
-      int x = 0;
-      for (int t = lane; t < pa_tiles(o, a.group); t += 32) x += pa_key_tiles(o, t, a, kt0);
-      x = __reduce_add_sync(0xffffffffu, x);
-      if (lane == from) sum = x;
-    }
-    if (s < b.n_seqs) w[s] = {sum * a.n_kv, tiles * a.n_kv};
-  }
-}
-// The item that position `want` (< the total) of the weighted order lies in, and how far into
-// it: an item weighs its units and `cost`.  One warp, every lane gets the answer.
-__device__ void pa_find(const PagedBatch& b, const PaArgs& a, const PaCount* w, int cost, int want, int lane, int& seq,
-                        int& tile, int& head, int& offset) {
-  int base = 0;
-  seq = 0;
-  for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-    const int x = s0 + lane < b.n_seqs ? w[s0 + lane].units + cost * w[s0 + lane].items : 0;
-    const int incl = pa_warp_scan(x, lane);
-    const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
-    if (past != 0) {
-      const int at = __ffs(past) - 1;
-      seq = s0 + at;
-      base += __shfl_sync(0xffffffffu, incl - x, at);
-      break;
-    }
-    base += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  bool bad;
-  const PagedSeq q = paged_seq(b, seq, &bad);
-  const int tiles = pa_tiles(q, a.group);
-  tile = 0;
-  int weight = 1, kt0;
-  for (int t0 = 0; t0 < tiles; t0 += 32) {
-    const int n = t0 + lane < tiles ? pa_key_tiles(q, t0 + lane, a, kt0) + cost : 0;
-    const int x = n * a.n_kv;
-    const int incl = pa_warp_scan(x, lane);
-    const uint32_t past = __ballot_sync(0xffffffffu, base + incl > want);
-    if (past != 0) {
-      const int at = __ffs(past) - 1;
-      tile = t0 + at;
-      weight = __shfl_sync(0xffffffffu, n, at);
-      base += __shfl_sync(0xffffffffu, incl - x, at);
-      break;
-    }
-    base += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  head = (want - base) / weight;
-  offset = want - base - head * weight;
-}
-
-// The items of a range, in order; every role walks them alike.
-struct PaWalk {
-  const PagedBatch& b;
-  const PaArgs& a;
-  const int cost;
-  int left;  // weight after the current item
-  int seq, tile, head;
-  PagedSeq s;
-  int kt0, nk, begin, end;  // key tiles of the current item: [begin, end) of its nk are this range's
-  int next_offset;
-  __device__ PaWalk(const PagedBatch& batch, const PaArgs& args, int cost_, int seq_, int tile_, int head_, int offset,
-                    int weight)
-      : b(batch), a(args), cost(cost_), left(weight), seq(seq_), tile(tile_), head(head_ - 1), next_offset(offset) {
-    bool bad;
-    s = left > 0 ? paged_seq(b, seq, &bad) : PagedSeq{0, 0, 0};
-  }
-  __device__ bool next() {
-    if (left <= 0) return false;
-    if (++head == a.n_kv) {
-      head = 0;
-      if (++tile >= pa_tiles(s, a.group)) {
-        bool bad;
-        tile = 0;
-        do {
-          s = paged_seq(b, ++seq, &bad);
-        } while (s.n == 0);
-      }
-    }
-    nk = pa_key_tiles(s, tile, a, kt0);
-    // the item's first `cost` positions are its overhead, the others its units
-    const int offset = next_offset;
-    const int to = min(nk + cost, offset + left);
-    next_offset = 0;
-    begin = max(0, offset - cost);
-    end = max(0, to - cost);
-    left -= to - offset;
-    return end > begin;  // (no unit: the range ends within the overhead)
-  }
-  // the first cache row any new token of the sequence sees
-  __device__ int low() const { return a.window > 0 ? max(0, s.kv - s.n - a.window + 1) : 0; }
-  // a V tile that reaches past the sequence's visible rows
-  __device__ bool edge(int kt) const { return (kt + 1) * kPaKeys > s.kv || kt * kPaKeys < low(); }
-};
-
-// A position in a ring of stages [first, first + n): the stage, the parity of the barrier phase
-// that its use ends, and the uses before it.
-struct PaRing {
-  const int first, n;
-  int stage;
-  uint32_t parity = 0, passed = 0;
-  __device__ __forceinline__ PaRing(int first_, int n_) : first(first_), n(n_), stage(first_) {}
-  __device__ __forceinline__ void next() {
-    ++passed;
-    if (++stage == first + n) {
-      stage = first;
-      parity ^= 1u;
-    }
-  }
-};
-__device__ __forceinline__ bool pa_elect() {  // one lane of a converged warp
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
-
 template <int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -496,7 +186,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     }
     u = __reduce_add_sync(0xffffffffu, u);
     items = __reduce_add_sync(0xffffffffu, items);
-    const int cost = u <= a.ranges ? 0 : kPaItemCost;  // with a pair for every unit, each gets one
+    const int cost = u <= a.ranges ? 0 : a.item_cost;  // with a pair for every unit, each gets one
     u += cost * items;
     const int n = min(a.ranges, u);  // ranges in use: none is empty
     int seq = 0, tile = 0, head = 0, offset = 0;
@@ -1049,48 +739,19 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid
 }
 
 // ---------------------------------------------------------------------------- host
-static PaDiv divisor(int d) {
-  uint32_t shift = 0;
-  while ((1ull << shift) < static_cast<uint64_t>(d)) ++shift;
-  return {static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
-}
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// A 5-D tensor of 64-dim rows with the 128-byte swizzle; `stride` in elements.
-static bool tile_map(CUtensorMap* m, const uint16_t* base, const int (&n)[4], const int64_t (&stride)[4],
-                     const int (&box)[4]) {
-  static EncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    return (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-               ? reinterpret_cast<EncodeFn>(p)
-               : nullptr;
-  }();
-  if (fn == nullptr) return false;
-  cuuint64_t dims[5] = {64}, strides[4];
-  cuuint32_t boxes[5] = {64};
-  for (int i = 0; i < 4; ++i) {
-    dims[i + 1] = static_cast<cuuint64_t>(n[i]);
-    // the stride of a dimension of size one is never used, but has to be a legal one
-    strides[i] = static_cast<cuuint64_t>(n[i] > 1 ? stride[i] : 64) * 2;
-    boxes[i + 1] = static_cast<cuuint32_t>(box[i]);
+g4_status paged_scratch(g4_ctx* ctx, PaArgs& a) {
+  if (ctx->paged.part == nullptr) {
+    // a pair's four partials outweigh what two CTAs of the other kernel leave
+    const size_t part = static_cast<size_t>(ctx->sm_count / 2) * 4 * kPaPartFloats * sizeof(float);
+    g4_status st = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice");
+    if (st == G4_OK && ctx->paged.tail == nullptr)
+      st = check_cuda(ctx, cudaMalloc(&ctx->paged.tail, ctx->sm_count * sizeof(PaTail)), "cudaMalloc paged tails");
+    if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&ctx->paged.part, part), "cudaMalloc paged partials");
+    if (st != G4_OK) return st;
   }
-  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<uint16_t*>(base), dims, strides, boxes, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Scratch of the split items, allocated at the first call: room for every pair of CTAs.
-static g4_status attn_scratch(g4_ctx* ctx, int pairs) {
-  if (ctx->paged.part != nullptr) return G4_OK;
-  const size_t part = static_cast<size_t>(pairs) * 4 * kPaPartFloats * sizeof(float);
-  g4_status st = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice");
-  if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&ctx->paged.tail, pairs * sizeof(PaTail)), "cudaMalloc paged tails");
-  if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&ctx->paged.part, part), "cudaMalloc paged partials");
-  return st;
+  a.part = ctx->paged.part;
+  a.tail = static_cast<PaTail*>(ctx->paged.tail);
+  return G4_OK;
 }
 
 template <int D>
@@ -1119,18 +780,14 @@ static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_
     if (n < 2) return fail(ctx, G4_ERR_UNSUPPORTED, "paged attention: CTA pairs do not fit this device");
     pairs = n;
   }
-  if ((st = attn_scratch(ctx, ctx->sm_count / 2)) != G4_OK) return st;
-  a.part = ctx->paged.part;
-  a.tail = static_cast<PaTail*>(ctx->paged.tail);
-  // no more ranges than units there can be: row tiles x heads x key tiles
-  const long long rows = static_cast<long long>(b.n_tokens) * a.group;
-  const long long tiles = rows / kPaRows + (b.n_seqs < b.n_tokens ? b.n_seqs : b.n_tokens);
-  const long long keys = (static_cast<long long>(b.max_pages) * b.page_rows + kPaKeys - 1) / kPaKeys;
-  const long long most = tiles * a.n_kv * (keys < 1 ? 1 : keys);
-  if ((tiles * a.n_kv) * ((keys < 1 ? 1 : keys) + kPaItemCost) >= (1ll << 30))
+  a.tile_rows = kPaRows;
+  a.item_cost = kPaItemCost;
+  long long items, keys;
+  paged_bounds(b, a, items, keys);
+  if (items * (keys + kPaItemCost) >= (1ll << 30))
     return fail(ctx, G4_ERR_TOO_LARGE, "paged attention: more than 2^30 tiles in one call");
   a.ranges = pairs / (D / 256);
-  if (most < a.ranges) a.ranges = static_cast<int>(most);
+  if (items * keys < a.ranges) a.ranges = static_cast<int>(items * keys);  // no more than there can be units
   const int low = b.page_rows & -b.page_rows;  // the largest power of two that divides a page's rows
   a.log_box = 0;
   while ((1 << a.log_box) < low && a.log_box < 6) ++a.log_box;
@@ -1158,6 +815,7 @@ static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_
   st = launch_kernel(ctx, fn, dim3(a.ranges * (D / 256) * 2), dim3(kPaThreads), smem, args, false, "paged attention");
   if (st != G4_OK) return st;
   void* jargs[] = {(void*)&a, (void*)&b};
+  const long long rows = static_cast<long long>(b.n_tokens) * a.group;
   const int row_blocks = static_cast<int>(((rows < kPaRows ? rows : kPaRows) + kPaJoinRows - 1) / kPaJoinRows);
   return launch_kernel(ctx, (const void*)paged_join_kernel<D>, dim3(a.ranges, row_blocks, 4 * (D / 256)),
                        dim3(kPaJoinThreads), 0, jargs, false, "paged attention join");
@@ -1205,6 +863,17 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   a.window = window;
   a.scale = scale * 1.4426950408889634f;
   const PagedBatch b = paged_batch(batch, cache);
+  if ((st = paged_scratch(ctx, a)) != G4_OK) return st;
+  // Sequences of few rows go to the other kernel.  Which ones is known on the device alone, so
+  // both kernels are launched and each takes its own, unless no sequence can be on one side or
+  // the tokens per sequence are so many that a kernel for the rest would hardly pay.
+  const long long rows = static_cast<long long>(b.n_tokens) * a.group;
+  const bool all_few = rows <= kPaFewRows;
+  const bool some_few = a.group <= kPaFewRows && b.n_seqs > 1 && b.n_tokens <= kPaFewPerSeq * b.n_seqs;
+  a.pick = all_few ? PA_ALL : PA_FEW;
+  if ((all_few || some_few) && (st = launch_paged_few(ctx, a, b, cache)) != G4_OK) return st;
+  if (all_few) return G4_OK;
+  a.pick = some_few ? PA_MANY : PA_ALL;
   return cache->head_dim == DS ? launch_attention<DS>(ctx, a, b, cache) : launch_attention<DF>(ctx, a, b, cache);
 }
 

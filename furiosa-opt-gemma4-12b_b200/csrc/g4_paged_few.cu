@@ -9,6 +9,8 @@
 // A thread has one key of the tile: maxima over the keys go through shuffles (16 columns at a
 // time: 16 exchanges instead of 80) and shared memory, P as bf16 (the one type of both operands)
 // into the shared tile the second product reads, sums stay with the thread until the item ends.
+// Up to four rows (one token of two heads) take a quarter of that work.  The scores of the next
+// tile are computed before the values of this one, so that K keeps arriving meanwhile.
 //
 // Work split, partial sums and the join are as there, with one CTA per range.  Warps: 0-3
 // softmax, Q and output, 4 copies, 5 MMA and tensor memory, 6 zeroes V rows past a sequence's ends.
@@ -20,7 +22,8 @@ namespace g4 {
 
 constexpr int kFewThreads = 224;
 constexpr int kFewStage = 32768, kFewStages = 6;
-constexpr uint32_t kFewCols = 128;  // tensor memory: S [0, 16), O block j [16 + 16 j, 32 + 16 j)
+constexpr uint32_t kFewCols = 128;  // tensor memory: S [0, 16) and [16, 32), O block j [32 + 16 j, 48 + 16 j)
+constexpr uint32_t kFewColO = 32;
 constexpr uint32_t kFewIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (2u << 17) | (8u << 24);
 constexpr uint32_t kFewIdescO = kFewIdescS | (1u << 15);  // A (V) dims-contiguous
 
@@ -29,10 +32,10 @@ struct __align__(1024) FewSmem {
   uint8_t ring[kFewStages][kFewStage];  // 2 blocks of 64 dims x [128 rows][64], 128-byte swizzle
   uint8_t q[D / 64][16 * 128];
   uint8_t p[2][16 * 128];               // P: blocks of 64 keys x [16 rows][64]
-  float top[2][4][16];                  // the warps' column maxima of a tile (two tiles' worth)
-  float sum[4][16];
+  float4 top[2][4][4];                  // the warps' maxima of a tile's 16 columns (two tiles' worth)
+  float4 sum[4][4];
   uint64_t full[kFewStages], empty[kFewStages], raw[kFewStages];  // raw: copied, rows not zeroed yet
-  uint64_t s_full, p_full, pv_done, q_full;
+  uint64_t s_full[2], p_full, pv_done, q_full;
   uint32_t tmem, abort;
   int units, first, range_count, item_cost;
   int seq, tile, head, offset;
@@ -87,15 +90,15 @@ __device__ __forceinline__ bool few_agree(bool ok) {
       : "memory");
   return r != 0;
 }
-// Column maxima or sums over the warp's 32 lanes: each exchange halves the columns a lane still
-// carries; lane l ends up with column (l >> 1) & 15.
-template <bool kMax>
+// Maxima or sums of N (4 or 16) columns over the warp's 32 lanes: while a lane carries more than
+// one column, each exchange halves them; lane l ends up with column l / (32 / N).
+template <bool kMax, int N>
 __device__ __forceinline__ float few_reduce(const float (&v)[16], int lane) {
-  float x[16];
+  float x[N];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = v[i];
+  for (int i = 0; i < N; ++i) x[i] = v[i];
 #pragma unroll
-  for (int n = 8, bit = 16; n >= 1; n >>= 1, bit >>= 1) {
+  for (int n = N / 2, bit = 16; n >= 1; n >>= 1, bit >>= 1) {
     const bool up = (lane & bit) != 0;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
@@ -104,8 +107,86 @@ __device__ __forceinline__ float few_reduce(const float (&v)[16], int lane) {
       x[i] = kMax ? fmaxf(keep, got) : keep + got;
     }
   }
-  const float got = __shfl_xor_sync(0xffffffffu, x[0], 1);
-  return kMax ? fmaxf(x[0], got) : x[0] + got;
+#pragma unroll
+  for (int bit = 16 / N; bit >= 1; bit >>= 1) {
+    const float got = __shfl_xor_sync(0xffffffffu, x[0], bit);
+    x[0] = kMax ? fmaxf(x[0], got) : x[0] + got;
+  }
+  return x[0];
+}
+// The softmax of one tile, for one key (thread) and N columns: P into the shared tile, m and l
+// updated.  False when a wait gave up.
+template <int D, int N>
+__device__ __forceinline__ bool few_tile(FewSmem<D>& sm, const PaArgs& a, const PaWalk& it, int u, uint32_t g, bool good,
+                                         uint32_t tbase, float factor_s, bool scale_first, float (&m)[16],
+                                         float (&l)[16], uint64_t budget) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
+  float s[16];
+  pa_fence_after();
+  few_ld16(tbase + 16 * (g & 1) + lanes, s);
+  if (scale_first) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) s[c] *= a.scale;
+  }
+  // the tile's keys are [key0, key0 + 128); the item's tokens are at positions [first, last]
+  const int key0 = (it.kt0 + u) * kPaKeys, base = it.s.kv - it.s.n, r0 = it.tile * 16;
+  const int first = base + a.by_group.div(r0), last = base + min(it.s.n - 1, a.by_group.div(r0 + 15));
+  if (key0 + kPaKeys - 1 > first || (a.window > 0 && key0 <= last - a.window)) {
+    const int key = key0 + tid;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {  // (columns past the rows: whatever they hold stays theirs)
+      const int pos = base + a.by_group.div(r0 + c);
+      if (key > pos || (a.window > 0 && key <= pos - a.window)) s[c] = -CUDART_INF_F;
+    }
+  }
+  const float mine = few_reduce<true, N>(s, lane) * factor_s;
+  if (lane % (32 / N) == 0) reinterpret_cast<float*>(&sm.top[g & 1][warp][0])[lane / (32 / N)] = mine;
+  good = good && (g == 0 || pa_wait_warp(&sm.pv_done, (g - 1) & 1, &sm.abort, budget));
+  if (!few_agree(good)) return false;
+  bool moved = false;
+  float f[16];
+#pragma unroll
+  for (int q = 0; q < N / 4; ++q) {
+    const float4 t0 = sm.top[g & 1][0][q], t1 = sm.top[g & 1][1][q], t2 = sm.top[g & 1][2][q], t3 = sm.top[g & 1][3][q];
+    const float top[4] = {fmaxf(fmaxf(t0.x, t1.x), fmaxf(t2.x, t3.x)), fmaxf(fmaxf(t0.y, t1.y), fmaxf(t2.y, t3.y)),
+                          fmaxf(fmaxf(t0.z, t1.z), fmaxf(t2.z, t3.z)), fmaxf(fmaxf(t0.w, t1.w), fmaxf(t2.w, t3.w))};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 4 * q + j;
+      f[c] = 1.f;
+      if (m[c] == -CUDART_INF_F) {
+        m[c] = top[j];
+      } else if (top[j] > m[c] + kPaLag) {
+        f[c] = pa_exp2(m[c] - top[j]);
+        l[c] *= f[c];
+        m[c] = top[j];
+        moved = true;  // (the same in every thread)
+      }
+    }
+  }
+  if (moved && u != it.begin) {
+#pragma unroll
+    for (int c = N; c < 16; ++c) f[c] = 1.f;
+#pragma unroll 1
+    for (int blk = 0; blk < D / 128; ++blk) {
+      float o[16];
+      few_ld16(tbase + lanes + kFewColO + 16 * blk, o);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) o[c] *= f[c];
+      few_st16(tbase + lanes + kFewColO + 16 * blk, o);
+    }
+    pa_st_wait();
+  }
+  uint8_t* p = &sm.p[tid >> 6][0];
+  const int ch = (tid & 63) >> 3, eb = (tid & 7) * 2;
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const float e = pa_exp2(fmaf(s[c], factor_s, m[c] == -CUDART_INF_F ? 0.f : -m[c]));
+    l[c] += e;
+    *reinterpret_cast<uint16_t*>(p + pa_swizzle(c, ch) + eb) = f32_to_bf16(e);
+  }
+  return true;
 }
 
 template <int D>
@@ -124,7 +205,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       mbar_init(&sm.empty[i], 1);
       mbar_init(&sm.raw[i], 1);
     }
-    mbar_init(&sm.s_full, 1);
+    mbar_init(&sm.s_full[0], 1);
+    mbar_init(&sm.s_full[1], 1);
     mbar_init(&sm.p_full, 4);
     mbar_init(&sm.pv_done, 1);
     mbar_init(&sm.q_full, 4);
@@ -206,58 +288,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
       for (int c = 0; c < 16; ++c) m[c] = -CUDART_INF_F, l[c] = 0.f;
       for (int u = it.begin; u < it.end; ++u, ++g) {
-        bool good = pa_wait_warp(&sm.s_full, g & 1, abort, budget);
-        float s[16];
-        pa_fence_after();
-        few_ld16(tbase + lanes, s);
-        // visible columns of this key: rows of tokens at or after it, and before it leaves the window
-        const int key = (it.kt0 + u) * kPaKeys + tid, first = it.s.kv - it.s.n;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const int pos = first + a.by_group.div(it.tile * 16 + c);
-          const bool see = c < rows && key <= pos && (a.window <= 0 || key > pos - a.window);
-          s[c] = see ? (scale_first ? s[c] * a.scale : s[c]) : -CUDART_INF_F;
-        }
-        const float mine = few_reduce<true>(s, lane) * factor_s;
-        if ((lane & 1) == 0) sm.top[g & 1][warp][lane >> 1] = mine;
-        good = good && (g == 0 || pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget));
-        ok = few_agree(good);
+        const bool good = pa_wait_warp(&sm.s_full[g & 1], (g >> 1) & 1, abort, budget);
+        ok = rows <= 4 ? few_tile<D, 4>(sm, a, it, u, g, good, tbase, factor_s, scale_first, m, l, budget)
+                       : few_tile<D, 16>(sm, a, it, u, g, good, tbase, factor_s, scale_first, m, l, budget);
         if (!ok) break;
-        bool moved = false;
-        float f[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float (*t)[16] = sm.top[g & 1];
-          const float top = fmaxf(fmaxf(t[0][c], t[1][c]), fmaxf(t[2][c], t[3][c]));
-          f[c] = 1.f;
-          if (m[c] == -CUDART_INF_F) {
-            m[c] = top;
-          } else if (top > m[c] + kPaLag) {
-            f[c] = pa_exp2(m[c] - top);
-            l[c] *= f[c];
-            m[c] = top;
-            moved = true;  // (the same in every thread)
-          }
-        }
-        if (moved && u != it.begin) {
-#pragma unroll 1
-          for (int blk = 0; blk < kBlocks; ++blk) {
-            float o[16];
-            few_ld16(tbase + lanes + 16 + 16 * blk, o);
-#pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] *= f[c];
-            few_st16(tbase + lanes + 16 + 16 * blk, o);
-          }
-          pa_st_wait();
-        }
-        uint8_t* p = &sm.p[tid >> 6][0];
-        const int ch = (tid & 63) >> 3, eb = (tid & 7) * 2;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float e = pa_exp2(fmaf(s[c], factor_s, m[c] == -CUDART_INF_F ? 0.f : -m[c]));
-          l[c] += e;
-          *reinterpret_cast<uint16_t*>(p + pa_swizzle(c, ch) + eb) = f32_to_bf16(e);
-        }
         fence_proxy_async();
         pa_fence_before();
         __syncwarp();
@@ -265,13 +299,19 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       }
       if (!ok) break;
       bool good = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
-      const float part_sum = few_reduce<false>(l, lane);
-      if ((lane & 1) == 0) sm.sum[warp][lane >> 1] = part_sum;
+      const float part_sum = few_reduce<false, 16>(l, lane);
+      if ((lane & 1) == 0) reinterpret_cast<float*>(&sm.sum[warp][0])[lane >> 1] = part_sum;
       ok = few_agree(good);
       if (!ok) break;
       pa_fence_after();
 #pragma unroll
-      for (int c = 0; c < 16; ++c) l[c] = (sm.sum[0][c] + sm.sum[1][c]) + (sm.sum[2][c] + sm.sum[3][c]);
+      for (int q = 0; q < 4; ++q) {
+        const float4 t0 = sm.sum[0][q], t1 = sm.sum[1][q], t2 = sm.sum[2][q], t3 = sm.sum[3][q];
+        l[4 * q] = (t0.x + t1.x) + (t2.x + t3.x);
+        l[4 * q + 1] = (t0.y + t1.y) + (t2.y + t3.y);
+        l[4 * q + 2] = (t0.z + t1.z) + (t2.z + t3.z);
+        l[4 * q + 3] = (t0.w + t1.w) + (t2.w + t3.w);
+      }
       const bool whole = it.begin == 0 && it.end == it.nk;
       if (it.begin == 0 && it.end < it.nk) {
         const int last = u_end - it.end + it.nk - 1;  // the item's last unit, as a position of the call
@@ -282,23 +322,29 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll 1
       for (int blk = 0; blk < kBlocks; ++blk) {
         float o[16];
-        few_ld16(tbase + lanes + 16 + 16 * blk, o);
+        few_ld16(tbase + lanes + kFewColO + 16 * blk, o);
+        if (whole) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          if (c >= rows) continue;
-          if (whole) {
+          for (int c = 0; c < 16; ++c) {
+            if (c >= rows) continue;
             const int rr = it.tile * 16 + c, i = a.by_group.div(rr);
             a.out[(it.s.t0 + i) * a.o_ts + (it.head * a.group + rr - i * a.group) * a.o_hs + 128 * blk + tid] =
-                f32_to_bf16(l[c] > 0.f ? o[c] / l[c] : 0.f);
-          } else {
-            part[c * D + 128 * blk + tid] = o[c];
+                f32_to_bf16(l[c] > 0.f ? __fdividef(o[c], l[c]) : 0.f);
           }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c)
+            if (c < rows) part[c * D + 128 * blk + tid] = o[c];
         }
       }
-      if (!whole) {
+      if (!whole && tid < 16) {
+        float mc = m[0], lc = l[0];
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-          if (tid == c) *reinterpret_cast<float2*>(part + 16 * D + 2 * c) = make_float2(m[c], l[c]);
+        for (int c = 1; c < 16; ++c) {
+          mc = tid == c ? m[c] : mc;
+          lc = tid == c ? l[c] : lc;
+        }
+        *reinterpret_cast<float2*>(part + 16 * D + 2 * tid) = make_float2(mc, lc);
       }
       // (sum is written again only past the next tile's agreement; O only after its P)
     }
@@ -330,29 +376,32 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       }
       return x;
     };
-    while (ok && it.next()) {
-      Box next = box_of((it.kt0 + it.begin) * kPaKeys);
-      for (int u = it.begin; u < it.end && ok; ++u) {
-        Box now = next;
-        if (u + 1 < it.end) next = box_of((it.kt0 + u + 1) * kPaKeys);
-        const bool edge = it.edge(it.kt0 + u);
-        for (int x = 0; x < 2 * kBlocks && ok; ++x) {  // K's stages, then V's
-          if (at.passed >= kFewStages) ok = pa_wait(&sm.empty[at.stage], at.parity ^ 1u, abort, budget);
-          if (!ok) break;
-          const bool is_v = x >= kBlocks;
-          uint64_t* bar = is_v && edge ? &sm.raw[at.stage] : &sm.full[at.stage];
-          if (lane == 0) mbar_arrive_expect_tx(bar, now.bytes);
-          if (now.row >= 0) {
-            int page = now.page;
-            if (page < 0 || page >= b.n_pages) {
-              bad_page = true;
-              page = b.n_pages;  // out of the map's bounds: zeros
-            }
-            few_tma(dst0 + at.stage * static_cast<uint32_t>(kFewStage), maps[is_v ? 1 : 0], now.row,
-                    2 * (is_v ? x - kBlocks : x) + slab, it.head, page, smem_u32(bar));
+    auto copy = [&](const Box& x, bool is_v, bool edge) {  // a tile's kBlocks stages
+      for (int blk = 0; blk < kBlocks && ok; ++blk) {
+        if (at.passed >= kFewStages) ok = pa_wait(&sm.empty[at.stage], at.parity ^ 1u, abort, budget);
+        if (!ok) break;
+        uint64_t* bar = edge ? &sm.raw[at.stage] : &sm.full[at.stage];
+        if (lane == 0) mbar_arrive_expect_tx(bar, x.bytes);
+        if (x.row >= 0) {
+          int page = x.page;
+          if (page < 0 || page >= b.n_pages) {
+            bad_page = true;
+            page = b.n_pages;  // out of the map's bounds: zeros
           }
-          at.next();
+          few_tma(dst0 + at.stage * static_cast<uint32_t>(kFewStage), maps[is_v ? 1 : 0], x.row, 2 * blk + slab,
+                  it.head, page, smem_u32(bar));
         }
+        at.next();
+      }
+    };
+    while (ok && it.next()) {
+      Box next = box_of((it.kt0 + it.begin) * kPaKeys), now = next;
+      for (int u = it.begin - 1; u < it.end && ok; ++u) {  // K of u + 1, then V of u
+        const Box v = now;
+        now = next;
+        if (u + 2 < it.end) next = box_of((it.kt0 + u + 2) * kPaKeys);
+        if (u + 1 < it.end) copy(now, false, false);
+        if (u >= it.begin) copy(v, true, it.edge(it.kt0 + u));
       }
     }
     // every stage is free again: no copy or arrival is outstanding when the CTA exits
@@ -372,25 +421,29 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     while (ok && it.next()) {
       ok = pa_wait_warp(&sm.q_full, items & 1, abort, budget);
       ++items;
-      for (int u = it.begin; u < it.end && ok; ++u, ++g) {
+      for (int u = it.begin - 1; u < it.end && ok; ++u) {
+        if (u + 1 < it.end) {
+          const uint32_t unit = g + (u + 1 - it.begin);
 #pragma unroll
-        for (int x = 0; x < kBlocks; ++x) {
-          ok = ok && pa_wait_warp(&sm.full[at.stage], at.parity, abort, budget);
-          if (!ok) break;
-          pa_fence_after();
-          const uint64_t kd = k_desc + at.stage * static_cast<uint32_t>(kFewStage / 16);
-          if (leader) {
+          for (int x = 0; x < kBlocks; ++x) {
+            ok = ok && pa_wait_warp(&sm.full[at.stage], at.parity, abort, budget);
+            if (!ok) break;
+            pa_fence_after();
+            const uint64_t kd = k_desc + at.stage * static_cast<uint32_t>(kFewStage / 16);
+            if (leader) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              few_mma(tbase, kd + ((k >> 2) * 16384 + 32 * (k & 3)) / 16,
-                      q_desc + ((2 * x + (k >> 2)) * 2048 + 32 * (k & 3)) / 16, kFewIdescS, (x | k) ? 1u : 0u);
-            few_commit(&sm.empty[at.stage]);
-            if (x == kBlocks - 1) few_commit(&sm.s_full);
+              for (int k = 0; k < 8; ++k)
+                few_mma(tbase + 16 * (unit & 1), kd + ((k >> 2) * 16384 + 32 * (k & 3)) / 16,
+                        q_desc + ((2 * x + (k >> 2)) * 2048 + 32 * (k & 3)) / 16, kFewIdescS, (x | k) ? 1u : 0u);
+              few_commit(&sm.empty[at.stage]);
+              if (x == kBlocks - 1) few_commit(&sm.s_full[unit & 1]);
+            }
+            __syncwarp();
+            at.next();
           }
-          __syncwarp();
-          at.next();
         }
-        ok = ok && pa_wait_warp(&sm.p_full, g & 1, abort, budget);
+        if (u < it.begin) continue;
+        ok = ok && pa_wait_warp(&sm.p_full, (g + (u - it.begin)) & 1, abort, budget);
         const uint32_t more = u > it.begin ? 1u : 0u;
 #pragma unroll
         for (int x = 0; x < kBlocks; ++x) {
@@ -401,7 +454,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           if (leader) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              few_mma(tbase + 16 + 16 * x, vd + 2048 * k / 16, p_desc + ((k >> 2) * 2048 + 32 * (k & 3)) / 16,
+              few_mma(tbase + kFewColO + 16 * x, vd + 2048 * k / 16, p_desc + ((k >> 2) * 2048 + 32 * (k & 3)) / 16,
                       kFewIdescO, k ? 1u : more);
             few_commit(&sm.empty[at.stage]);
             if (x == kBlocks - 1) few_commit(&sm.pv_done);
@@ -410,6 +463,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           at.next();
         }
       }
+      g += it.end - it.begin;
     }
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   } else {
@@ -418,8 +472,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     uint32_t parity = 0;  // of each stage's `raw`
     bool ok = true;
     while (ok && it.next()) {
+      for (int x = 0; x < kBlocks; ++x) at.next();  // K of the first tile
       for (int u = it.begin; u < it.end && ok; ++u) {
-        for (int x = 0; x < kBlocks; ++x) at.next();
+        if (u + 1 < it.end)
+          for (int x = 0; x < kBlocks; ++x) at.next();
         const int row0 = (it.kt0 + u) * kPaKeys;
         const int front = min(max(it.low() - row0, 0), kPaKeys), back = min(max(it.s.kv - row0, 0), kPaKeys);
         const int n = front + kPaKeys - back;  // rows outside [low, kv)

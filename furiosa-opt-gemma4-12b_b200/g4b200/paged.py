@@ -19,6 +19,8 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 from . import LIB, Context, G4Error, _i32, _i64, _vp
 
 _f32 = ctypes.c_float
@@ -57,8 +59,6 @@ LIB.g4_page_pool_free_pages.argtypes = [_vp, _p_i32]
 
 
 def _cuda(name: str, t, dtype, dims: int):
-    import torch
-
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch tensor")
     if not t.is_cuda:
@@ -72,19 +72,22 @@ def _cuda(name: str, t, dtype, dims: int):
 
 def _same_device(ctx: Context, **named) -> None:
     for name, t in named.items():
-        if t.device.index != ctx.device:
+        if t.get_device() != ctx.device:
             raise ValueError(f"{name}: on {t.device}, the context is on cuda:{ctx.device}")
 
 
-def _rows(name: str, t, tokens: int, heads: int | None, dim: int):
-    """A [tokens, heads, dim] bf16 operand; returns its pointer and strides in elements."""
-    import torch
-
+def _rows(ctx: Context, name: str, t, tokens: int, heads: int, dim: int) -> tuple:
+    """A [tokens, heads, dim] bf16 operand on the context's device; returns its pointer and its
+    token and head strides in elements (0 along a dimension of size one)."""
     _cuda(name, t, torch.bfloat16, 3)
-    n, h, d = t.shape
-    if n != tokens or d != dim or (heads is not None and h != heads):
-        raise ValueError(f"{name}: shape {list(t.shape)}, expected [{tokens}, {heads or 'heads'}, {dim}]")
-    return (t.data_ptr(),) + _row_strides(name, t, (0, 1))
+    if t.shape != (tokens, heads, dim):
+        raise ValueError(f"{name}: shape {list(t.shape)}, expected [{tokens}, {heads}, {dim}]")
+    if t.get_device() != ctx.device:
+        raise ValueError(f"{name}: on {t.device}, the context is on cuda:{ctx.device}")
+    token_stride, head_stride, last = t.stride()
+    if last != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return t.data_ptr(), token_stride if tokens > 1 else 0, head_stride if heads > 1 else 0
 
 
 def _row_strides(name: str, t, dims) -> tuple:
@@ -95,6 +98,14 @@ def _row_strides(name: str, t, dims) -> tuple:
     return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in dims)
 
 
+def _tokens_heads(name: str, t) -> tuple:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch tensor")
+    if t.dim() != 3:
+        raise ValueError(f"{name}: {t.dim()} dimensions, expected 3")
+    return t.shape[0], t.shape[1]
+
+
 class PagedCache:
     """One layer's K and V pages (g4_paged_cache): bf16 CUDA tensors of shape
     [n_pages, page_rows, n_kv_heads, head_dim] with any strides of multiples of 8 over a
@@ -102,8 +113,6 @@ class PagedCache:
     passed as its transpose(1, 2)."""
 
     def __init__(self, k, v):
-        import torch
-
         for name, t in (("k", k), ("v", v)):
             _cuda(name, t, torch.bfloat16, 4)
         if k.shape != v.shape:
@@ -112,6 +121,7 @@ class PagedCache:
             raise ValueError("k and v are on different devices")
         self.k, self.v = k, v
         self.n_pages, self.page_rows, self.n_kv_heads, self.head_dim = k.shape
+        self.device = k.get_device()
         self.desc = _CacheDesc(k.data_ptr(), v.data_ptr(), *_row_strides("k", k, (0, 1, 2)),
                                *_row_strides("v", v, (0, 1, 2)), *k.shape)
 
@@ -135,8 +145,6 @@ class PagedBatch:
     call, so they may be updated in place between calls."""
 
     def __init__(self, tables, q_start, kv_len):
-        import torch
-
         _cuda("tables", tables, torch.int32, 2)
         for name, t in (("q_start", q_start), ("kv_len", kv_len)):
             _cuda(name, t, torch.int32, 1)
@@ -155,10 +163,12 @@ class PagedBatch:
         self.stride = max(tables.stride(0), width) if n > 1 else width
         if n > 1 and tables.stride(0) < width:
             raise ValueError("tables: rows overlap")
+        self.device = kv_len.get_device()
+        self._desc = _BatchDesc(tables.data_ptr(), self.stride, q_start.data_ptr(), kv_len.data_ptr(), width, n, 0)
 
     def desc(self, n_tokens: int) -> _BatchDesc:
-        return _BatchDesc(self.tables.data_ptr(), self.stride, self.q_start.data_ptr(), self.kv_len.data_ptr(),
-                          self.tables.shape[1], self.n_seqs, n_tokens)
+        self._desc.n_tokens = n_tokens  # (the library copies the descriptor within the call)
+        return self._desc
 
 
 def paged_attention(ctx: Context, q, cache: PagedCache, batch: PagedBatch, out, *, scale: float = 1.0,
@@ -166,16 +176,17 @@ def paged_attention(ctx: Context, q, cache: PagedCache, batch: PagedBatch, out, 
     """Attention of every new token of the batch over its sequence's pages, causal, within the
     last `window` positions if window > 0 (g4_paged_attention).  q, out: bf16
     [n_tokens, n_heads, head_dim]; the model's scale is 1."""
-    n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else None
-    qa = _rows("q", q, n, heads, cache.head_dim)
-    oa = _rows("out", out, n, heads, cache.head_dim)
-    _same_device(ctx, q=q, out=out, cache=cache.k, batch=batch.kv_len)
+    n, heads = _tokens_heads("q", q)
+    qa = _rows(ctx, "q", q, n, heads, cache.head_dim)
+    oa = _rows(ctx, "out", out, n, heads, cache.head_dim)
+    if cache.device != ctx.device or batch.device != ctx.device:
+        raise ValueError(f"cache or batch: not on the context's device cuda:{ctx.device}")
     if heads % cache.n_kv_heads:
         raise ValueError(f"q: {heads} heads is not a multiple of the cache's {cache.n_kv_heads}")
     if n == 0:
         return
     ctx._check("g4_paged_attention", LIB.g4_paged_attention(
-        ctx.handle, *qa, heads, ctypes.byref(cache.desc), ctypes.byref(batch.desc(n)), float(scale), int(window), *oa))
+        ctx.handle, *qa, heads, cache.desc, batch.desc(n), float(scale), int(window), *oa))
 
 
 def paged_store_qkv(ctx: Context, q, k, v, q_rms_weight, k_rms_weight, cos, sin, cache: PagedCache,
@@ -184,32 +195,27 @@ def paged_store_qkv(ctx: Context, q, k, v, q_rms_weight, k_rms_weight, cos, sin,
     of the new tokens (g4_paged_store_qkv).  q, q_out: bf16 [n_tokens, n_heads, head_dim]; k, v:
     [n_tokens, n_kv_heads, head_dim] (slices of a fused projection are fine; full layers
     pass k as v); cos, sin: [n_positions, head_dim] with sin's low half negated."""
-    import torch
-
-    n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else None
+    n, heads = _tokens_heads("q", q)
     d, hkv = cache.head_dim, cache.n_kv_heads
-    qa = _rows("q", q, n, heads, d)
-    ka, va = _rows("k", k, n, hkv, d), _rows("v", v, n, hkv, d)
-    oa = _rows("q_out", q_out, n, heads, d)
+    qa, oa = _rows(ctx, "q", q, n, heads, d), _rows(ctx, "q_out", q_out, n, heads, d)
+    ka, va = _rows(ctx, "k", k, n, hkv, d), _rows(ctx, "v", v, n, hkv, d)
+    if cache.device != ctx.device or batch.device != ctx.device:
+        raise ValueError(f"cache or batch: not on the context's device cuda:{ctx.device}")
     for name, t, dims in (("q_rms_weight", q_rms_weight, 1), ("k_rms_weight", k_rms_weight, 1), ("cos", cos, 2),
                           ("sin", sin, 2)):
         _cuda(name, t, torch.bfloat16, dims)
-        if t.shape[-1] != d or not t.is_contiguous():
-            raise ValueError(f"{name}: must be contiguous with {d} columns")
-    _same_device(ctx, q=q, k=k, v=v, q_out=q_out, cos=cos, sin=sin, q_rms_weight=q_rms_weight,
-                 k_rms_weight=k_rms_weight, cache=cache.k, batch=batch.kv_len)
+        if t.shape[-1] != d or not t.is_contiguous() or t.get_device() != ctx.device:
+            raise ValueError(f"{name}: must be contiguous with {d} columns, on cuda:{ctx.device}")
     if cos.shape != sin.shape:
         raise ValueError("cos and sin differ in shape")
     if n == 0:
         return
     ctx._check("g4_paged_store_qkv", LIB.g4_paged_store_qkv(
         ctx.handle, *qa, heads, *ka, *va, q_rms_weight.data_ptr(), k_rms_weight.data_ptr(), cos.data_ptr(),
-        sin.data_ptr(), cos.shape[0], ctypes.byref(cache.desc), ctypes.byref(batch.desc(n)), *oa))
+        sin.data_ptr(), cos.shape[0], cache.desc, batch.desc(n), *oa))
 
 
 def _words(name: str, t, n: int | None = None):
-    import torch
-
     _cuda(name, t, torch.int32, 1)
     if not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
@@ -231,8 +237,6 @@ def paged_copy(ctx: Context, caches: PagedCaches, src, dst, rows) -> None:
 def paged_compact(ctx: Context, caches: PagedCaches, src, dst, tables, page_map) -> None:
     """Whole pages src[i] into dst[i] in every layer, and tables = page_map[tables] where an
     entry is not negative (g4_paged_compact), in one launch per 56 layers."""
-    import torch
-
     n = src.numel()
     a = _words("src", src), _words("dst", dst, n)
     _cuda("tables", tables, torch.int32, 2)
@@ -360,8 +364,6 @@ class PagePool:
 def _upload(ctx: Context, values):
     """An int32 CUDA tensor written on the context's stream (so the calls that read it, and
     the reuse of its memory, are in stream order)."""
-    import torch
-
     with torch.cuda.stream(ctx.stream):
         return torch.tensor(values, dtype=torch.int32, device=f"cuda:{ctx.device}")
 

@@ -13,7 +13,9 @@
 // twice the O columns, so its two halves of V are two pairs' work: both compute S (1.5x the
 // products) and they run side by side, so the second fetch of K hits the L2.
 //
-// Softmax in f32 with the running maximum and sum, one thread per row.  O is rescaled only
+// Softmax in f32 with the running maximum and sum, two threads per row (64 of the tile's 128
+// columns each; the maxima meet in shared memory): the time from S to P is what the tensor
+// cores wait for when a head is 256 wide.  O is rescaled only
 // when a row's maximum rises by more than 2^8 (the maximum that P is relative to may lag:
 // P <= 256 then, exact in range for f32 sums and for P's rounding to bf16).  P is rounded to
 // bf16 because kind::f16 wants both operands of the product of one 16-bit type; its error is
@@ -25,9 +27,9 @@
 // balanced.  An item that crosses a range's end leaves partial sums (f32) that a second
 // kernel joins in range order.
 //
-// Roles of a CTA's 12 warps: 0-3 softmax, 4 K copies, 5 MMA (leader CTA) and tensor memory,
-// 6 V copies, 7 Q copies and the V tiles at a sequence's ends (TMA cannot stop at its last row;
-// rows past it may hold NaN, and 0 * NaN is NaN, so they are zeroed there), 8-11 output: O of
+// Roles of a CTA's 16 warps: 0-7 softmax, 8 K copies, 9 MMA (leader CTA) and tensor memory,
+// 10 V copies, 11 Q copies and the V tiles at a sequence's ends (TMA cannot stop at its last row;
+// rows past it may hold NaN, and 0 * NaN is NaN, so they are zeroed there), 12-15 output: O of
 // one item leaves while the scores and the softmax of the next are under way.
 #include <cmath>
 #include <string>
@@ -36,7 +38,7 @@
 
 namespace g4 {
 
-constexpr int kPaThreads = 384;
+constexpr int kPaThreads = 512;
 constexpr int kPaRows = 256;      // rows per item (both CTAs)
 constexpr int kPaStage = 32768;   // bytes per ring stage: 64 K rows x 256 dims, or 128 V rows x 128 dims
 constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
@@ -56,7 +58,8 @@ struct __align__(1024) PaSmem {
   uint8_t ring[kStages][kPaStage];  // K stages, then V stages
   uint64_t full[kStages], empty[kStages], s_full[2], p_full, pv_done, q_full, q_empty, edge_full, edge_done;
   uint64_t o_full, o_free, ml_full, ml_free;
-  float2 ml[128];  // an item's reference maxima and sums, from the softmax warps to the output warps
+  float m[128], l[2][128];  // an item's reference maxima and column halves' sums, for the output warps
+  float top[2][128];        // the rows' maxima over each half of a tile's columns
   uint32_t tmem;
   uint32_t abort;
   int units, first;        // weight of the call; where this range starts
@@ -112,6 +115,17 @@ __device__ __forceinline__ void pa_tma(uint32_t dst, uint64_t map, int c1, int c
       "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
+// The eight softmax warps agree on whether all of their waits held.
+__device__ __forceinline__ bool pa_agree(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
+}
 // The 16-byte chunks w[4 j .. 4 j + 3] (j < 4) of the four lanes of a quad, transposed: lane q
 // gets chunk q of the quad's lane j in place j.
 __device__ __forceinline__ void pa_quad_transpose(uint32_t (&w)[16], int lane) {
@@ -140,8 +154,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
                       const __grid_constant__ PagedBatch b, Scratch* scr, uint64_t budget) {
   using Smem = PaSmem<D>;
   constexpr int kK = Smem::kK, kV = Smem::kV, kStages = Smem::kStages, kHalves = D / 256, kChunks = D / 256;  // a K tile is kChunks stages
-  extern __shared__ uint8_t pa_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(pa_raw) + 1023) & ~uintptr_t(1023));
+  // (all of an SM's shared memory: there is no room to align it by hand)
+  static_assert(sizeof(Smem) <= 232448, "an SM's shared memory");
+  extern __shared__ __align__(1024) uint8_t pa_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(pa_raw);
+  if ((smem_u32(pa_raw) & 1023u) != 0) {  // the swizzle counts on it
+    if (threadIdx.x == 0) {
+      atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
+      a.tail[(blockIdx.x >> 1) / kHalves] = PaTail{-1, 0, 0, 0};
+    }
+    return;
+  }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x & 1;  // rank in the pair
   const int half = (blockIdx.x >> 1) % kHalves, range = (blockIdx.x >> 1) / kHalves;
@@ -152,20 +175,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     }
     mbar_init(&sm.s_full[0], 1);
     mbar_init(&sm.s_full[1], 1);
-    mbar_init(&sm.p_full, 8);
+    mbar_init(&sm.p_full, 16);
     mbar_init(&sm.pv_done, 1);
-    mbar_init(&sm.q_full, a.q_tma ? 2 : 8);
+    mbar_init(&sm.q_full, a.q_tma ? 2 : 16);
     mbar_init(&sm.q_empty, 1);
     mbar_init(&sm.edge_full, 1);
     mbar_init(&sm.edge_done, 1);
     mbar_init(&sm.o_full, 1);
     mbar_init(&sm.o_free, 8);
-    mbar_init(&sm.ml_full, 4);
+    mbar_init(&sm.ml_full, 8);
     mbar_init(&sm.ml_free, 4);
     sm.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 5) {
+  if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
                  "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
@@ -215,22 +238,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   volatile uint32_t* abort = &sm.abort;
   PaWalk it(b, a, sm.item_cost, sm.seq, sm.tile, sm.head, sm.offset, u_end - u_first);
 
-  // registers a thread: 168 at launch (384 x 168 in all), then 232, 96 and 168 (128 x 496 = 63488)
-  if (warp < 4)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-  else if (warp < 8)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-  if (warp < 4) {
+  // registers a thread: 128 at launch (512 x 128 in all), then 152 for the softmax, 80 for the
+  // copies and 128 for the output (128 x (2 x 152 + 80 + 128) = 65536)
+  if (warp < 8)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+  else if (warp < 12)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  if (warp < 8) {
     // -------------------------------------------------------------- softmax
-    const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
+    const int side = warp >> 2, r = tid & 127;  // half of the columns; row of the CTA's 128
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t p_full = pa_map_to(smem_u32(&sm.p_full), 0);
     // scores are scaled within the exponent's FMA; a scale that is not positive goes first
     const bool scale_first = !(a.scale > 0.f);
     const float factor_s = scale_first ? 1.f : a.scale;
     uint32_t g = 0, items = 0;  // units and items of the range
-    bool ok = true;
+    // good: this warp's waits held; ok: every softmax warp's did, as of the last tile they met at
+    // (they leave together: the others would wait at the barrier for a warp that left alone)
+    bool good = true, ok = true;
     while (ok && it.next()) {
-      const int rr = it.tile * kPaRows + cta * 128 + tid;
+      const int rr = it.tile * kPaRows + cta * 128 + r;
       const int i = a.by_group.div(rr);
       const bool valid = i < it.s.n;
       const bool any_row = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps step
@@ -238,16 +265,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const int hi = valid ? pos + 1 : 0, lo = valid && a.window > 0 ? max(0, pos - a.window + 1) : 0;
       if (!a.q_tma) {
         // rows of any group size: a thread copies one 16-byte column of every kStep-th row (the
-        // previous item's scores are done: these warps have read them)
-        constexpr int kRowChunks = D / 8, kStep = 128 / kRowChunks;
+        // previous item's scores are done: all these warps have read them and met since)
+        constexpr int kRowChunks = D / 8, kStep = 256 / kRowChunks;
         const int ch = tid % kRowChunks;
         const uint32_t qb = smem_u32(&sm.q[0][0]) + (ch >> 3) * 16384;
         const uint16_t* q = a.q + it.head * a.group * a.q_hs + it.s.t0 * a.q_ts + 8 * ch;
 #pragma unroll 4
         for (int row = tid / kRowChunks; row < 128; row += kStep) {
-          const int r = it.tile * kPaRows + cta * 128 + row, qi = a.by_group.div(r);
+          const int x = it.tile * kPaRows + cta * 128 + row, qi = a.by_group.div(x);
           const bool in = qi < it.s.n;
-          cp_async16(qb + pa_swizzle(row, ch), in ? q + qi * a.q_ts + (r - qi * a.group) * a.q_hs : a.q, in ? 16u : 0u);
+          cp_async16(qb + pa_swizzle(row, ch), in ? q + qi * a.q_ts + (x - qi * a.group) * a.q_hs : a.q, in ? 16u : 0u);
         }
         cp_async_wait_all();
         asm volatile("fence.proxy.async;" ::: "memory");
@@ -257,26 +284,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       float m = -CUDART_INF_F, l = 0.f;
       for (int u = it.begin; u < it.end; ++u, ++g) {
         const uint32_t st = tbase + kPaColS + (g & 1) * 128 + lanes;
-        ok = pa_wait_warp(&sm.s_full[g & 1], (g >> 1) & 1, abort, budget);
-        if (!ok) break;
-        float factor = 1.f;
+        good = good && pa_wait_warp(&sm.s_full[g & 1], (g >> 1) & 1, abort, budget);
+        float s[2][32];
+        float mine = -CUDART_INF_F;
         if (any_row) {
           pa_fence_after();
-          float s[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) pa_ld32(st + 32 * c, s[c]);
+          pa_ld32(st + 64 * side, s[0]);
+          pa_ld32(st + 64 * side + 32, s[1]);
           pa_ld_wait();
           if (scale_first) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
               for (int j = 0; j < 32; ++j) s[c][j] *= a.scale;
           }
           const int base = (it.kt0 + u) * kPaKeys;
           if (__any_sync(0xffffffffu, valid && (hi < base + kPaKeys || lo > base))) {
-            const int from = lo - base, to = hi - base;  // visible: columns [from, to)
+            const int from = lo - base - 64 * side, to = hi - base - 64 * side;  // visible: columns [from, to)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
               const int f = min(max(from - 32 * c, 0), 32), t = min(max(to - 32 * c, 0), 32);
               const uint32_t see = static_cast<uint32_t>(((1ull << t) - 1ull) & ~((1ull << f) - 1ull));
 #pragma unroll
@@ -286,12 +312,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           float mx[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            mx[c] = pa_max3(s[c][0], s[c][1], s[c][2]);
+            const float* x = &s[c >> 1][16 * (c & 1)];
+            mx[c] = pa_max3(x[0], x[1], x[2]);
 #pragma unroll
-            for (int j = 3; j < 31; j += 2) mx[c] = pa_max3(mx[c], s[c][j], s[c][j + 1]);
-            mx[c] = fmaxf(mx[c], s[c][31]);
+            for (int j = 3; j < 15; j += 2) mx[c] = pa_max3(mx[c], x[j], x[j + 1]);
+            mx[c] = fmaxf(mx[c], x[15]);
           }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * factor_s;
+          mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * factor_s;
+        }
+        named_bar_sync(3, 256);  // the previous tile's maxima have been read
+        sm.top[side][r] = mine;
+        ok = pa_agree(good);
+        if (!ok) break;
+        float factor = 1.f;
+        if (any_row) {
+          const float top = fmaxf(sm.top[0][r], sm.top[1][r]);
           // the reference maximum: the first one seen, moved only when it lags too far
           if (m == -CUDART_INF_F) {
             m = top;
@@ -303,64 +338,62 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           const float ref = m == -CUDART_INF_F ? 0.f : -m;
           const uint64_t f2 = pa_pair(factor_s, factor_s), r2 = pa_pair(ref, ref);
           uint64_t sum[4] = {0, 0, 0, 0};
+          uint32_t p[32];
 #pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            uint32_t p[32];
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float e0, e1, f0, f1;
-              pa_unpair(pa_fma2(pa_pair(s[c][j], s[c][j + 1]), f2, r2), e0, e1);
-              pa_unpair(pa_fma2(pa_pair(s[c + 1][j], s[c + 1][j + 1]), f2, r2), f0, f1);
-              e0 = pa_exp2(e0);
-              e1 = pa_exp2(e1);
-              f0 = pa_exp2(f0);
-              f1 = pa_exp2(f1);
-              sum[(j >> 1) & 1] = pa_add2(sum[(j >> 1) & 1], pa_pair(e0, e1));
-              sum[2 + ((j >> 1) & 1)] = pa_add2(sum[2 + ((j >> 1) & 1)], pa_pair(f0, f1));
-              p[j / 2] = pa_bf16x2(e0, e1);
-              p[16 + j / 2] = pa_bf16x2(f0, f1);
-            }
-            pa_st32(st + 16 * c, p);
+          for (int j = 0; j < 32; j += 2) {
+            float e0, e1, f0, f1;
+            pa_unpair(pa_fma2(pa_pair(s[0][j], s[0][j + 1]), f2, r2), e0, e1);
+            pa_unpair(pa_fma2(pa_pair(s[1][j], s[1][j + 1]), f2, r2), f0, f1);
+            e0 = pa_exp2(e0);
+            e1 = pa_exp2(e1);
+            f0 = pa_exp2(f0);
+            f1 = pa_exp2(f1);
+            sum[(j >> 1) & 1] = pa_add2(sum[(j >> 1) & 1], pa_pair(e0, e1));
+            sum[2 + ((j >> 1) & 1)] = pa_add2(sum[2 + ((j >> 1) & 1)], pa_pair(f0, f1));
+            p[j / 2] = pa_bf16x2(e0, e1);
+            p[16 + j / 2] = pa_bf16x2(f0, f1);
           }
+          pa_st32(st + 32 * side, p);  // (both sides' scores have been read: the warps have met)
           float a0, a1;
           pa_unpair(pa_add2(pa_add2(sum[0], sum[1]), pa_add2(sum[2], sum[3])), a0, a1);
           l += a0 + a1;
         }
-        if (g != 0) {  // the previous P V is done: O may be rescaled, and this unit's may follow
-          ok = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
-          if (!ok) break;
-          if (u != it.begin && __any_sync(0xffffffffu, factor != 1.f)) {
+        // the previous P V is done: O may be rescaled, and this unit's may follow
+        if (g != 0) {
+          good = good && pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
+          if (good && u != it.begin && __any_sync(0xffffffffu, factor != 1.f)) {
             pa_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < 256; c += 32) {
+            for (int c = 128 * side; c < 128 * side + 128; c += 32) {
               float o[32];
-              uint32_t r[32];
+              uint32_t x[32];
               pa_ld32(tbase + lanes + c, o);
               pa_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(o[j] * factor);
-              pa_st32(tbase + lanes + c, r);
+              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(o[j] * factor);
+              pa_st32(tbase + lanes + c, x);
             }
           }
         }
         pa_st_wait();
         pa_fence_before();
         __syncwarp();
-        if (lane == 0) pa_arrive_relaxed(p_full);
+        if (lane == 0 && good) pa_arrive_relaxed(p_full);
       }
-      if (ok && items > 0) ok = pa_wait_warp(&sm.ml_free, (items - 1) & 1, abort, budget);
       if (!ok) break;
+      if (items > 0) good = good && pa_wait_warp(&sm.ml_free, (items - 1) & 1, abort, budget);
       ++items;
-      sm.ml[tid] = make_float2(m, l);
+      if (side == 0) sm.m[r] = m;
+      sm.l[side][r] = l;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.ml_full);
+      if (lane == 0 && good) mbar_arrive(&sm.ml_full);
     }
-    if (ok && g > 0) ok = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
-    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
-  } else if (warp >= 8) {
+    if (ok && good && g > 0) good = pa_wait_warp(&sm.pv_done, (g - 1) & 1, abort, budget);
+    if (!(ok && good) && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+  } else if (warp >= 12) {
     // -------------------------------------------------------------- output
-    const int r = tid - 256;  // row of the CTA's 128
-    const uint32_t lanes = static_cast<uint32_t>(32 * (warp - 8)) << 16;
+    const int r = tid - 384;  // row of the CTA's 128
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp - 12)) << 16;
     const uint32_t o_free = pa_map_to(smem_u32(&sm.o_free), 0);
     uint32_t items = 0;
     PaTail tail = {-1, 0, 0, 0};
@@ -372,7 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       ok = pa_wait_warp(&sm.ml_full, items & 1, abort, budget) && pa_wait_warp(&sm.o_full, items & 1, abort, budget);
       if (!ok) break;
       ++items;
-      const float2 ml = sm.ml[r];
+      const float2 ml = make_float2(sm.m[r], sm.l[0][r] + sm.l[1][r]);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.ml_free);
       const bool whole = it.begin == 0 && it.end == it.nk;
@@ -442,14 +475,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     }
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     if (r == 0 && cta == 0 && half == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
-  } else if (warp == 4 || warp == 6) {
-    // -------------------------------------------------------------- K copies (4), V copies (6)
+  } else if (warp == 8 || warp == 10) {
+    // -------------------------------------------------------------- K copies (8), V copies (10)
     // A K stage is 4 blocks of 64 dims x 64 rows, a V stage 2 halves of 64 rows x 2 blocks.  Where
     // a page holds 64 rows in one piece, a box is all of a K stage or of a half; else a box is
     // 2^log_box rows of one block.  A lane copies one box; the lanes run on their own.
-    const bool is_k = warp == 4;
+    const bool is_k = warp == 8;
     PaRing at(is_k ? 0 : kK, is_k ? kK : kV);
-    uint32_t edges = 0;  // V tiles that warp 7 finishes
+    uint32_t edges = 0;  // V tiles that warp 11 finishes
     const uint64_t map = reinterpret_cast<uint64_t>(is_k ? &kmap : &vmap);
     const int box = 1 << a.log_box, rows = is_k ? 64 : kPaKeys;
     const int blocks = a.log_box == 6 ? 1 : (is_k ? 4 : 2);  // boxes side by side
@@ -514,7 +547,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
             fill(now, v_block, bar);
           }
         } else {
-          // the stage reports to warp 7, which zeroes rows of it (with no box to wait for, at
+          // the stage reports to warp 11, which zeroes rows of it (with no box to wait for, at
           // once: so only when it is free) and reports to the leader
           if (edges > 0) ok = pa_wait(&sm.edge_done, (edges - 1) & 1, abort, budget);
           ++edges;
@@ -530,7 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       ok = pa_wait(&sm.empty[at.first + x % n], (x / n) & 1, abort, budget);
     if (bad_page) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
     if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // -------------------------------------------------------------- MMA: the leader CTA's
     // The warp stays converged around the elected lane, so that descriptors live in uniform
     // registers: N = 128 MMAs issued by a lone thread took 100-150 cycles instead of 64.
@@ -659,7 +692,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   pa_fence_after();
-  if (warp == 5)
+  if (warp == 9)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512u));
 }
 
@@ -757,7 +790,7 @@ g4_status paged_scratch(g4_ctx* ctx, PaArgs& a) {
 template <int D>
 static g4_status launch_attention(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_paged_cache* c) {
   const void* fn = (const void*)paged_attn_kernel<D>;
-  const size_t smem = sizeof(PaSmem<D>) + 1024;
+  const size_t smem = sizeof(PaSmem<D>);
   g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "paged attention");
   if (st != G4_OK) return st;
   int& pairs = ctx->paged.pairs[D == 256 ? 0 : 1];

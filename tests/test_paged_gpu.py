@@ -531,3 +531,81 @@ def test_pool_on_the_gpu(gpu_ctx):
     v[64 - pool.free_pages:] = float("nan")
     check([e, b, c], [2, 1, 1], batch)
     append([c, b, e], [2, 2, 2])
+
+
+def test_serving_example():
+    """The example's users, served from shared, copied and compacted pages, get what they get
+    alone: both sides round each weight and each output to bf16 once, in different tilings
+    (2^-8 apiece in relative norm at most)."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    import paged_serving
+
+    r = paged_serving.main()
+    assert r["pages moved"] > 0 and r["relative difference"] <= 4 * U
+
+
+# sequences that the few-row kernel gets in several tiles, on its own or beside the other's
+SPLIT = [
+    ([(33, 33), (0, 5), (0, 0)] + [(0, 7)] * 30, SLIDING, 16, 0),  # as many tokens as sequences
+    ([(20, 900), (0, 5), (1, 300), (0, 0)] + [(0, 7)] * 17, FULL, 24, 0),
+    ([(1, 700)] * 9 + [(200, 1500)] + [(8, 400), (9, 400), (7, 7)], SLIDING, 8, 100),
+    ([(1, 700)] * 9 + [(200, 1500)] + [(2, 400), (3, 400), (0, 9)], FULL, 64, 0),
+    ([(1, 300), (1, 1), (5, 260), (6, 131)], (15, 5, 256), 16, 40),
+    ([(1, 300), (1, 1), (2, 260), (3, 131)], (7, 1, 512), 16, 0),
+    ([(1, 300), (2, 1), (3, 0), (90, 40)], (17, 1, 256), 16, 0),  # no group of 17 is few
+    ([(1, 300), (40, 200)], (200, 1, 256), 16, 0),
+    ([(1, 12), (4, 4)], (4, 4, 512), 512, 0),
+    ([(1, 1 + i % 90) for i in range(1500)], SLIDING, 8, 0),
+    ([(i % 3, 1 + i % 90) for i in range(400)], FULL, 16, 33),
+    ([(1, 30000), (1, 12345)], SLIDING, 512, 0),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SPLIT)))
+def test_attention_split_between_kernels(gpu_ctx, case):
+    lens, heads, page_rows, window = SPLIT[case]
+    q, cache, batch, tables = _setup(lens, heads, page_rows, window, seed=100 + case)
+    out = _attend(gpu_ctx, q, cache, batch, window=window)
+    _check_attention(out, q, cache, tables, lens, window=window)
+    assert torch.equal(out, _attend(gpu_ctx, q, cache, batch, window=window))
+
+
+def test_attention_of_one_token_repeated_by_a_zero_stride(gpu_ctx):
+    lens = [(40, 100)]
+    q, cache, batch, tables = _setup(lens, SLIDING)
+    same = q[:1, :1].expand(40, 16, 256)
+    out = torch.empty_like(q)
+    g4.paged_attention(gpu_ctx, same, cache, batch, out)
+    torch.cuda.synchronize()
+    assert gpu_ctx.poll() == 0
+    _check_attention(out, same.contiguous(), cache, tables, lens)
+
+
+def test_attention_on_another_stream():
+    """The call runs on its context's stream, whatever torch's current stream is."""
+    stream = torch.cuda.Stream()
+    ctx = g4.Context(0, stream)
+    lens = [(50, 300), (1, 77)]
+    q, cache, batch, tables = _setup(lens, FULL)
+    out = torch.full_like(q, float("nan"))
+    stream.wait_stream(torch.cuda.current_stream())
+    g4.paged_attention(ctx, q, cache, batch, out)
+    torch.cuda.current_stream().wait_stream(stream)
+    _check_attention(out, q, cache, tables, lens)
+    assert ctx.poll() == 0
+    ctx.close()
+
+
+def test_attention_refuses_more_tiles_than_it_counts(gpu_ctx):
+    rows = 65536
+    k = torch.zeros(1, rows, 1, 256, dtype=torch.bfloat16, device="cuda")
+    tables = torch.zeros(1, 2 ** 21, dtype=torch.int32, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = g4.PagedBatch(tables, i32([0, 2000]), i32([2000]))
+    q = torch.zeros(2000, 16, 256, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(g4.G4Error) as e:
+        g4.paged_attention(gpu_ctx, q, g4.PagedCache(k, k), batch, q.clone())
+    assert e.value.code == 6

@@ -43,7 +43,6 @@ constexpr int kPaRows = 256;      // rows per item (both CTAs)
 constexpr int kPaStage = 32768;   // bytes per ring stage: 64 K rows x 256 dims, or 128 V rows x 128 dims
 constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
 constexpr int kPaItemCost = 2;     // an item's start and end, in units, for the work split
-constexpr int kPaFewPerSeq = 64;   // tokens per sequence up to which single tokens are looked for
 // kind::f16, D f32, A and B bf16, M = 256; S: N = 128, both K-major; O: N = 256, B (V) MN-major
 constexpr uint32_t kPaIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (16u << 17) | (16u << 24);
 constexpr uint32_t kPaIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (32u << 17) | (16u << 24);
@@ -898,19 +897,14 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   a.scale = scale * 1.4426950408889634f;
   const PagedBatch b = paged_batch(batch, cache);
   if ((st = paged_scratch(ctx, a)) != G4_OK) return st;
-  // Sequences of few rows go to the other kernel.  Which ones is known on the device alone, so
-  // both kernels are launched and each takes its own; except that as many tokens as sequences is
-  // taken for a decode step, all the other kernel's (it is right for longer ones too, a tile of 16
-  // rows at a time), and that with many tokens per sequence, or rows that cannot be few, all are
-  // this one's.  32 single tokens over up to 8192 rows: 64 us with one kernel, 78 us with both.
-  const long long rows = static_cast<long long>(b.n_tokens) * a.group;
-  const bool groups_fit = a.group <= kPaFewRows;
-  const bool all_few = rows <= kPaFewRows || (groups_fit && b.n_tokens == b.n_seqs);
-  const bool some_few = groups_fit && b.n_seqs > 1 && b.n_tokens <= static_cast<long long>(kPaFewPerSeq) * b.n_seqs;
-  a.pick = all_few ? PA_ALL : PA_FEW;
-  if ((all_few || some_few) && (st = launch_paged_few(ctx, a, b, cache)) != G4_OK) return st;
-  if (all_few) return G4_OK;
-  a.pick = some_few ? PA_MANY : PA_ALL;
+  // Decode steps go to the kernel for few rows: at most 16 rows in all, or as many tokens as
+  // sequences, which is taken for one token each (the lengths themselves are on the device; other
+  // lengths are right there too, 16 rows at a time).  32 single tokens of full layers over up to
+  // 8192 rows: 56.5 us there, 80 us here.  With a chunk among them one launch of this kernel beats
+  // one of each (31 tokens beside 509 new ones, sliding: 78 us against 89).
+  const bool few = static_cast<long long>(b.n_tokens) * a.group <= kPaFewRows ||
+                   (a.group <= kPaFewRows && b.n_tokens == b.n_seqs);
+  if (few) return launch_paged_few(ctx, a, b, cache);
   return cache->head_dim == DS ? launch_attention<DS>(ctx, a, b, cache) : launch_attention<DF>(ctx, a, b, cache);
 }
 

@@ -1,6 +1,5 @@
-// Attention of sequences with few rows (new tokens x query heads per KV head <= 16: a decode
-// step, a few speculative tokens) over their pages, on tcgen05 with the roles of the operands
-// exchanged: the cache rows are the 128 rows of the MMA, the query rows its N = 16 columns.
+// Attention of sequences with few rows (new tokens x query heads per KV head: a decode step) over
+// their pages, on tcgen05 with the roles of the operands exchanged: the cache rows are the 128 rows of the MMA, the query rows its N = 16 columns.
 //   S^T[128 keys][16] = K Q^T           O^T[128 dims][16] += V^T P^T   (per 128 dims of the head)
 // so a tile of 128 cache rows costs 32 (head of 256) or 64 (512) small MMAs instead of the
 // 256-row products of g4_paged_attn.cu, and every K/V byte is fetched once.  Bound by HBM: 192 KB
@@ -509,11 +508,12 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 
 // Joins an item's parts as paged_join_kernel does; a block has one row: D / 4 threads a part,
 // kGroups parts at a time, joined in range order within a group and the groups in order.
-constexpr int kFewJoinThreads = 512;
-template <int D>
-__global__ void __launch_bounds__(kFewJoinThreads) paged_few_join_kernel(const __grid_constant__ PaArgs a,
+// kThreads: 512 where one item may be in all CTAs' hands (one token over 8192 rows of a full layer:
+// 18.0 us in all, 20.1 with 256), 256 where most have two parts (32 tokens: 56.5 us, 58.5 with 512).
+template <int D, int kThreads>
+__global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const __grid_constant__ PaArgs a,
                                                                          const __grid_constant__ PagedBatch b) {
-  constexpr int kGroups = kFewJoinThreads / (D / 4), kBatch = 4;
+  constexpr int kGroups = kThreads / (D / 4), kBatch = 4;
   __shared__ float4 acc[kGroups][D / 4];
   __shared__ float2 stat[kGroups];
   pdl_wait();
@@ -590,7 +590,7 @@ static g4_status launch_few(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_paged_
   const size_t smem = sizeof(FewSmem<D>) + 1024;
   g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "paged attention (few rows)");
   if (st != G4_OK) return st;
-  a.tile_rows = 16;
+  a.tile_rows = kPaFewRows;
   a.item_cost = 1;  // (32 single tokens: 59 us with 1, 64 us with 0)
   long long items, keys;
   paged_bounds(b, a, items, keys);
@@ -614,8 +614,10 @@ static g4_status launch_few(g4_ctx* ctx, PaArgs a, PagedBatch b, const g4_paged_
   if (st != G4_OK) return st;
   const long long rows = static_cast<long long>(b.n_tokens) * a.group;
   void* jargs[] = {(void*)&a, (void*)&b};
-  return launch_kernel(ctx, (const void*)paged_few_join_kernel<D>, dim3(a.ranges, rows < 16 ? static_cast<int>(rows) : 16),
-                       dim3(kFewJoinThreads), 0, jargs, false, "paged attention join (few rows)");
+  const bool many_parts = 4 * items <= a.ranges;
+  const void* join = many_parts ? (const void*)paged_few_join_kernel<D, 512> : (const void*)paged_few_join_kernel<D, 256>;
+  return launch_kernel(ctx, join, dim3(a.ranges, rows < kPaFewRows ? static_cast<int>(rows) : kPaFewRows),
+                       dim3(many_parts ? 512 : 256), 0, jargs, false, "paged attention join (few rows)");
 }
 
 g4_status launch_paged_few(g4_ctx* ctx, PaArgs a, const PagedBatch& b, const g4_paged_cache* c) {

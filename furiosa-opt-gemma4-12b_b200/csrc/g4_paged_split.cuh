@@ -19,8 +19,7 @@ struct PaDiv {
     return static_cast<int>((__umulhi(u, mul) + u) >> shift);
   }
 };
-enum { PA_ALL = 0, PA_FEW = 1, PA_MANY = 2 };
-constexpr int kPaFewRows = 16;  // new tokens x group of a sequence that g4_paged_few.cu takes
+constexpr int kPaFewRows = 16;  // rows of an item of g4_paged_few.cu
 constexpr int kPaKeys = 128;    // cache rows per unit
 constexpr float kPaLag = 8.f;   // log2 of how far a row's maximum may rise before O is rescaled
 struct PaArgs {
@@ -33,7 +32,6 @@ struct PaArgs {
   int group, n_kv, window;  // query heads per KV head, KV heads
   int tile_rows;            // rows of an item
   int item_cost;            // what an item's start and end cost, in units, for the work split
-  int pick;                 // PA_ALL sequences, those of at most kPaFewRows rows, or the others
   PaDiv by_group, by_page;  // by group and by the rows of a page
   float scale;              // times log2(e)
   int log_box;              // log2 of the cache rows per TMA box
@@ -176,12 +174,6 @@ __device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, const P
 __device__ __forceinline__ int pa_tiles(const PagedSeq& s, const PaArgs& a) {
   return (s.n * a.group + a.tile_rows - 1) / a.tile_rows;  // (n * group < 2^30: checked by the host)
 }
-// A sequence of the batch; without tokens when it is the other kernel's.
-__device__ __forceinline__ PagedSeq pa_seq(const PagedBatch& b, const PaArgs& a, int s, bool* bad) {
-  PagedSeq q = paged_seq(b, s, bad);
-  if (a.pick != PA_ALL && (q.n * a.group <= kPaFewRows) != (a.pick == PA_FEW)) q.n = 0;
-  return q;
-}
 __device__ __forceinline__ int pa_warp_scan(int v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -206,7 +198,7 @@ __device__ __forceinline__ void pa_count(const PagedBatch& b, const PaArgs& a, P
     const int s = s0 + tid;
     PagedSeq q = {0, 0, 0};
     bool bad = false;
-    if (s < b.n_seqs) q = pa_seq(b, a, s, &bad);
+    if (s < b.n_seqs) q = paged_seq(b, s, &bad);
     if (report && s == 0 && b.n_seqs > 0 && b.q_start[0] < 0) bad = true;
     if (report && bad) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
     const int tiles = pa_tiles(q, a);
@@ -243,7 +235,7 @@ __device__ __forceinline__ void pa_find(const PagedBatch& b, const PaArgs& a, co
     base += __shfl_sync(0xffffffffu, incl, 31);
   }
   bool bad;
-  const PagedSeq q = pa_seq(b, a, seq, &bad);
+  const PagedSeq q = paged_seq(b, seq, &bad);
   const int tiles = pa_tiles(q, a);
   tile = 0;
   int weight = 1, kt0;
@@ -279,7 +271,7 @@ struct PaWalk {
                     int weight)
       : b(batch), a(args), cost(cost_), left(weight), seq(seq_), tile(tile_), head(head_ - 1), next_offset(offset) {
     bool bad;
-    s = left > 0 ? pa_seq(b, a, seq, &bad) : PagedSeq{0, 0, 0};
+    s = left > 0 ? paged_seq(b, seq, &bad) : PagedSeq{0, 0, 0};
   }
   __device__ bool next() {
     if (left <= 0) return false;
@@ -289,7 +281,7 @@ struct PaWalk {
         bool bad;
         tile = 0;
         do {
-          s = pa_seq(b, a, ++seq, &bad);
+          s = paged_seq(b, ++seq, &bad);
         } while (s.n == 0);
       }
     }
@@ -369,7 +361,7 @@ inline bool tile_map(CUtensorMap* m, const uint16_t* base, const int (&n)[4], co
 // Scratch of split items for `ranges` tails and `floats` of partial sums, allocated at the first
 // call; both kernels use it, one after the other on the context's stream.
 g4_status paged_scratch(g4_ctx* ctx, PaArgs& a);
-// Rows of at most kPaFewRows per sequence (g4_paged_few.cu).
+// The kernel of g4_paged_few.cu.
 g4_status launch_paged_few(g4_ctx* ctx, PaArgs a, const PagedBatch& b, const g4_paged_cache* c);
 // No more items than this, and 128-row key tiles of the longest cache there can be.
 inline void paged_bounds(const PagedBatch& b, const PaArgs& a, long long& items, long long& keys) {

@@ -547,7 +547,7 @@ def test_serving_example():
     assert r["pages moved"] > 0 and r["relative difference"] <= 4 * U
 
 
-# sequences that the few-row kernel gets in several tiles, on its own or beside the other's
+# batches near the line between the two kernels (as many tokens as sequences), skewed ones too
 SPLIT = [
     ([(33, 33), (0, 5), (0, 0)] + [(0, 7)] * 30, SLIDING, 16, 0),  # as many tokens as sequences
     ([(20, 900), (0, 5), (1, 300), (0, 0)] + [(0, 7)] * 17, FULL, 24, 0),

@@ -62,13 +62,13 @@ PagedBatch paged_batch(const g4_paged_batch* b, const g4_paged_cache* c) {
 }
 
 // ---------------------------------------------------------------------------- norm, rotate, store
-// A warp takes a token and kPer of its q, k and v heads; a head's D values stay in its
-// registers (8 per lane and 16-byte chunk), so q, k and v are read once and written once.
-// Memory bound: 4 B per element, and the token's cos/sin row, loaded once per warp.  The heads'
-// loads go out first, ahead of the chain token -> sequence -> page, whose two L2 round trips
-// they hide.  kPer = 4 where that still gives every SM 64 warps, else 1: a single token's heads
-// then go to as many warps.  4096 sliding tokens (138 MB): 33.6 us with 4, 34.7 with 8, 37.5 with
-// 2, 77 with 1; one token: 2.3 us with 1.
+// out[d] = n[d] cos[d] + n[d +- D/2] sin[d], n = x rsqrt(mean x^2 + eps) w.  D / 16 lanes have a
+// head: a lane its dims 8 l .. 8 l + 7 and D / 2 + 8 l .. , so the pairs that turn into each
+// other meet in one lane, and a warp has two heads of 256 or one of 512 at a time.  A warp takes
+// kIter such steps of one token's q, k or v heads: q, k and v are read once and written once,
+// the token's cos/sin row and the norm weights once per warp.  The heads' loads go out first,
+// ahead of the chain token -> sequence -> page, whose two round trips they hide.  Memory bound by
+// its bytes (4 per element), by instructions before the arithmetic went two f32 at a time.
 struct StoreArgs {
   const uint16_t *q, *k, *v;
   long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
@@ -79,25 +79,25 @@ struct StoreArgs {
   uint16_t* out;
   long long o_ts, o_hs;
 };
-constexpr int kStoreThreads = 256;
+constexpr int kStoreThreads = 128;
 
-__device__ __forceinline__ void unpack8(const uint4 w, float (&f)[8]) {
+__device__ __forceinline__ uint4 ldg128(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+// Eight bf16 as four pairs of f32, and back.
+__device__ __forceinline__ void unpack8(const uint4 w, uint64_t (&f)[4]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = pa_pair(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint4 pack8(const uint64_t (&f)[4]) {
+  uint32_t u[4];
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(u[i] << 16);
-    f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    float a, b;
+    pa_unpair(f[i], a, b);
+    u[i] = pa_bf16x2(a, b);
   }
+  return make_uint4(u[0], u[1], u[2], u[3]);
 }
-__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]), bf16x2(f[4], f[5]), bf16x2(f[6], f[7]));
-}
-__device__ __forceinline__ uint4 ldg128(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // The sequence whose new tokens include token t (-1: none), 32 sequences at a time, and its
 // position; bad: its numbers had to be cut off.
@@ -117,27 +117,36 @@ __device__ __forceinline__ int seq_of_token(const PagedBatch& b, int t, int lane
   return -1;
 }
 
-template <int D, int kPer>
+template <int D, int kIter>
 __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const __grid_constant__ StoreArgs a,
                                                                     const __grid_constant__ PagedBatch b,
                                                                     Scratch* scr) {
-  constexpr int C = D / 256;  // 16-byte chunks per lane: chunk c holds dims 256 c + 8 lane ..
+  constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes, kPer = kIter * kAtOnce;  // lanes a head; heads a step, a warp
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int slots = a.n_heads + 2 * a.n_kv, groups = (slots + kPer - 1) / kPer;  // q heads, k heads, v heads
+  const int lane = threadIdx.x & 31, hl = lane % kLanes, sub = lane / kLanes;
+  const int q_groups = (a.n_heads + kPer - 1) / kPer, kv_groups = (a.n_kv + kPer - 1) / kPer;
+  const int groups = q_groups + 2 * kv_groups;  // of q heads, of k heads, of v heads
   const int unit = blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5);
-  const int t = unit / groups, slot0 = unit % groups * kPer;
+  const int t = unit / groups, group = unit - t * groups;
   if (unit == 0) paged_check_batch(b, lane, scr);
   if (t >= b.n_tokens) return;
-  uint4 x[kPer][C];
+  const bool is_q = group < q_groups, is_v = group >= q_groups + kv_groups;
+  const int head0 = (is_q ? group : (group - q_groups) % kv_groups) * kPer + sub, heads = is_q ? a.n_heads : a.n_kv;
+  const uint16_t* src = is_q ? a.q + t * a.q_ts : (is_v ? a.v + t * a.v_ts : a.k + t * a.k_ts);
+  const long long src_hs = is_q ? a.q_hs : (is_v ? a.v_hs : a.k_hs);
+  uint4 x[kIter][2];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int slot = slot0 + i, k = slot - a.n_heads, v = k - a.n_kv;
-    if (slot >= slots) continue;
-    const uint16_t* src = k < 0 ? a.q + t * a.q_ts + slot * a.q_hs
-                                : (v < 0 ? a.k + t * a.k_ts + k * a.k_hs : a.v + t * a.v_ts + v * a.v_hs);
-#pragma unroll
-    for (int c = 0; c < C; ++c) x[i][c] = ldg128(src + 256 * c + 8 * lane);
+  for (int i = 0; i < kIter; ++i) {
+    const int head = head0 + i * kAtOnce;
+    if (head >= heads) continue;
+    x[i][0] = ldg128(src + head * src_hs + 8 * hl);
+    x[i][1] = ldg128(src + head * src_hs + D / 2 + 8 * hl);
+  }
+  uint64_t w[2][4];
+  if (!is_v) {
+    const uint16_t* weight = is_q ? a.qw : a.kw;
+    unpack8(ldg128(weight + 8 * hl), w[0]);
+    unpack8(ldg128(weight + D / 2 + 8 * hl), w[1]);
   }
   int pos = -1;
   bool bad = false;
@@ -147,73 +156,76 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const __grid
   if (pos >= a.n_positions) live = false, bad = true;
   int page = 0, row = 0;
   if (live) {  // (pos < kv <= max_pages * page_rows)
-    page = b.tables[s * b.table_stride + pos / b.page_rows];
-    row = pos % b.page_rows;
+    const int j = pos / b.page_rows;
+    page = b.tables[s * b.table_stride + j];
+    row = pos - j * b.page_rows;
   }
-  float cf[C][8], sf[C][8];
+  uint64_t cs[2][4], sn[2][4];
   if (live) {
+    if (!is_v) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      unpack8(ldg128(a.cos + static_cast<long long>(pos) * D + 256 * c + 8 * lane), cf[c]);
-      unpack8(ldg128(a.sin + static_cast<long long>(pos) * D + 256 * c + 8 * lane), sf[c]);
+      for (int c = 0; c < 2; ++c) {
+        unpack8(ldg128(a.cos + static_cast<long long>(pos) * D + c * (D / 2) + 8 * hl), cs[c]);
+        unpack8(ldg128(a.sin + static_cast<long long>(pos) * D + c * (D / 2) + 8 * hl), sn[c]);
+      }
     }
     if (page < 0 || page >= b.n_pages) live = false, bad = true;
   }
   if (bad && lane == 0) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
+  if (!live && !is_q) return;
+  uint16_t* dst = is_q ? a.out + t * a.o_ts : (is_v ? a.vc + page * a.vp + row * a.vr : a.kc + page * a.kp + row * a.kr);
+  const long long dst_hs = is_q ? a.o_hs : (is_v ? a.vh : a.kh);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int slot = slot0 + i, k = slot - a.n_heads, v = k - a.n_kv;
-    if (slot >= slots || (!live && k >= 0)) continue;
-    uint16_t* dst = k < 0 ? a.out + t * a.o_ts + slot * a.o_hs
-                          : (v < 0 ? a.kc + page * a.kp + row * a.kr + k * a.kh
-                                   : a.vc + page * a.vp + row * a.vr + v * a.vh);
-    if (!live) {
+  for (int i = 0; i < kIter; ++i) {
+    const int head = head0 + i * kAtOnce;
+    const bool mine = head < heads;
+    uint64_t f[2][4], ss = 0;
 #pragma unroll
-      for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = make_uint4(0, 0, 0, 0);
-      continue;
+    for (int c = 0; c < 2; ++c) {
+      unpack8(mine ? x[i][c] : make_uint4(0, 0, 0, 0), f[c]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss = pa_fma2(f[c][j], f[c][j], ss);
     }
-    float f[C][8], ss = 0.f;
+    float s0, s1;
+    pa_unpair(ss, s0, s1);
+    s0 += s1;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      unpack8(x[i][c], f[c]);
+    for (int o = kLanes / 2; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    const float r = rsqrtf(fmaf(s0, 1.f / D, EPS));  // (2 ulp: far below the one rounding to bf16)
+    const uint64_t rr = pa_pair(r, r);
+    uint4 y0, y1;
+    if (is_v) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(f[c][j], f[c][j], ss);
-    }
-    const float r = rsqrtf(fmaf(warp_sum(ss), 1.f / D, EPS));  // (2 ulp: far below the one rounding to bf16)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[c][j] *= r;
-    if (v < 0) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float wf[8];
-        unpack8(ldg128((k < 0 ? a.qw : a.kw) + 256 * c + 8 * lane), wf);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[c][j] *= wf[j];
-      }
-      // out[d] = x[d] cos[d] + x[d +- D/2] sin[d]: the other half is chunk c ^ 1 of this lane
-      // (D = 512) or chunk 0 of lane ^ 16 (D = 256)
-      float y[C][8];
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float other = C == 2 ? f[(c ^ 1) & (C - 1)][j] : __shfl_xor_sync(0xffffffffu, f[c][j], 16);
-          y[c][j] = fmaf(f[c][j], cf[c][j], other * sf[c][j]);
-        }
-#pragma unroll
-      for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = pack8(y[c]);
+        for (int j = 0; j < 4; ++j) f[c][j] = pa_mul2(f[c][j], rr);
+      y0 = pack8(f[0]);
+      y1 = pack8(f[1]);
     } else {
+      uint64_t y[2][4];
 #pragma unroll
-      for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + 256 * c + 8 * lane) = pack8(f[c]);
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[c][j] = pa_mul2(pa_mul2(f[c][j], rr), w[c][j]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[c][j] = pa_fma2(f[c][j], cs[c][j], pa_mul2(f[c ^ 1][j], sn[c][j]));
+      y0 = live ? pack8(y[0]) : make_uint4(0, 0, 0, 0);
+      y1 = live ? pack8(y[1]) : make_uint4(0, 0, 0, 0);
+    }
+    if (mine) {
+      *reinterpret_cast<uint4*>(dst + head * dst_hs + 8 * hl) = y0;
+      *reinterpret_cast<uint4*>(dst + head * dst_hs + D / 2 + 8 * hl) = y1;
     }
   }
 }
-constexpr int kStorePer = 4;
-template <int kPer>
-static const void* store_kernel(int head_dim) {
-  return head_dim == DS ? (const void*)paged_store_kernel<DS, kPer> : (const void*)paged_store_kernel<DF, kPer>;
+// Steps a warp: kStoreIter where that still gives every SM 32 warps, else one.  4096 sliding tokens
+// (138 MB): 29.6 us with 4, 33.6 with 2, 36.5 with 8; one token 2.5 us with 1.
+constexpr int kStoreIter = 4;
+template <int D>
+static const void* store_kernel(bool many) {
+  return many ? (const void*)paged_store_kernel<D, kStoreIter> : (const void*)paged_store_kernel<D, 1>;
 }
 
 // ---------------------------------------------------------------------------- page copies
@@ -361,13 +373,16 @@ g4_status g4_paged_store_qkv(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
                  cache->v_row_stride, cache->v_head_stride, q_out, out_token_stride, out_head_stride};
   PagedBatch b = paged_batch(batch, cache);
   Scratch* scr = ctx->buf.scratch;
-  const int slots = n_heads + 2 * cache->n_kv_heads;
-  const int per = static_cast<long long>(batch->n_tokens) * slots >= 64ll * kStorePer * ctx->sm_count ? kStorePer : 1;
-  const long long warps = static_cast<long long>(batch->n_tokens) * ((slots + per - 1) / per);
+  const int at_once = 512 / cache->head_dim;
+  const long long all = static_cast<long long>(batch->n_tokens) * (n_heads + 2 * cache->n_kv_heads);
+  const bool many = all >= 32ll * kStoreIter * at_once * ctx->sm_count;
+  const int per = (many ? kStoreIter : 1) * at_once;
+  const void* fn = cache->head_dim == DS ? store_kernel<DS>(many) : store_kernel<DF>(many);
+  const int groups = (n_heads + per - 1) / per + 2 * ((cache->n_kv_heads + per - 1) / per);
+  const long long warps = static_cast<long long>(batch->n_tokens) * groups;
   const long long blocks = (warps + kStoreThreads / 32 - 1) / (kStoreThreads / 32);
   if (blocks > INT_MAX / (kStoreThreads / 32)) return fail(ctx, G4_ERR_BAD_ARG, "too many tokens times heads for one call");
   void* args[] = {(void*)&a, (void*)&b, (void*)&scr};
-  const void* fn = per == 1 ? store_kernel<1>(cache->head_dim) : store_kernel<kStorePer>(cache->head_dim);
   return launch_kernel(ctx, fn, dim3(static_cast<unsigned>(blocks)), dim3(kStoreThreads), 0, args, false,
                        "paged store");
 }

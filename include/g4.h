@@ -63,7 +63,7 @@ typedef enum g4_status {
   G4_ERR_NCCL = 3,        /* an NCCL call failed                                */
   G4_ERR_TIMEOUT = 4,     /* a bounded device-side wait gave up                 */
   G4_ERR_UNSUPPORTED = 5, /* configuration not built into this library          */
-  G4_ERR_TOO_LARGE = 6    /* a size exceeds a fixed limit (no-alloc entry point) */
+  G4_ERR_TOO_LARGE = 6    /* a size exceeds a fixed limit, or a page pool's pages  */
 } g4_status;
 
 /* Model constants (src/lib.rs:19-22, src/axes.rs:4-29). */
@@ -391,8 +391,10 @@ typedef struct g4_paged_batch {
  * softmax statistics and sums are f32; the weights of V are rounded to bf16 for the tensor
  * cores.  q and out are [n_tokens, n_heads, head_dim] with the given strides in elements
  * (multiples of 8).  The new tokens' own K and V rows must be in the cache already
- * (g4_paged_store_qkv).  The first call of a context allocates its scratch
- * (make it before a stream capture). */
+ * (g4_paged_store_qkv).  The first call of a context allocates its scratch (39 MB; make it
+ * before a stream capture).  Up to 2^22 new tokens, 2^30 rows (tokens x query heads per KV
+ * head: else G4_ERR_BAD_ARG) and 2^30 tiles of 128 cache rows that max_pages and n_tokens
+ * leave room for (else G4_ERR_TOO_LARGE). */
 g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stride, int64_t q_head_stride,
                              int n_heads, const g4_paged_cache* cache, const g4_paged_batch* batch, float scale,
                              int window, g4_bf16* out, int64_t out_token_stride, int64_t out_head_stride);

@@ -75,7 +75,7 @@ extern "C" {
 g4_status g4_page_pool_create(int n_pages, int page_rows, g4_page_pool** out) {
   if (out == nullptr) return G4_ERR_BAD_ARG;
   *out = nullptr;
-  if (n_pages < 1 || page_rows < 8 || page_rows > 65536 || page_rows % 8 != 0) return G4_ERR_BAD_ARG;
+  if (n_pages < 1 || n_pages > (1 << 24) || page_rows < 8 || page_rows > 65536 || page_rows % 8 != 0) return G4_ERR_BAD_ARG;
   g4_page_pool* pool = new (std::nothrow) g4_page_pool();
   const g4_status st = guarded(pool, [&] {
     pool->n_pages = n_pages;

@@ -257,7 +257,12 @@ struct PaWalk {
         bool bad;
         tile = 0;
         do {
-          s = paged_seq(b, ++seq, &bad);
+          // (never past the last one, as long as nobody writes the batch during the call)
+          if (++seq >= b.n_seqs) {
+            left = 0;
+            return false;
+          }
+          s = paged_seq(b, seq, &bad);
         } while (s.n == 0);
       }
     }

@@ -224,6 +224,14 @@ def _words(name: str, t, n: int | None = None):
     return t.data_ptr()
 
 
+def _check_tables(tables) -> None:
+    _cuda("tables", tables, torch.int32, 2)
+    if tables.shape[1] > 1 and tables.stride(1) != 1:
+        raise ValueError("tables: rows must be contiguous")
+    if tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]:
+        raise ValueError("tables: rows overlap")
+
+
 def paged_copy(ctx: Context, caches: PagedCaches, src, dst, rows) -> None:
     """Rows [0, rows[i]) of page src[i] into page dst[i] in K and V of every layer
     (g4_paged_copy; int32 CUDA tensors).  No dst may be another dst or any src."""
@@ -239,12 +247,8 @@ def paged_compact(ctx: Context, caches: PagedCaches, src, dst, tables, page_map)
     entry is not negative (g4_paged_compact), in one launch per 56 layers."""
     n = src.numel()
     a = _words("src", src), _words("dst", dst, n)
-    _cuda("tables", tables, torch.int32, 2)
-    if tables.shape[1] > 1 and tables.stride(1) != 1:
-        raise ValueError("tables: rows must be contiguous")
+    _check_tables(tables)
     seqs, width = tables.shape
-    if seqs > 1 and tables.stride(0) < width:
-        raise ValueError("tables: rows overlap")
     m = _words("page_map", page_map, caches.layers[0].n_pages)
     _same_device(ctx, src=src, dst=dst, tables=tables, page_map=page_map, caches=caches.layers[0].k)
     ctx._check("g4_paged_compact", LIB.g4_paged_compact(
@@ -308,6 +312,12 @@ class PagePool:
         self._check("g4_page_pool_table", code)
         return list(out[:(rows.value + self.page_rows - 1) // self.page_rows]), rows.value
 
+    def _check_caches(self, ctx: Context, caches: PagedCaches) -> None:
+        for c in caches.layers:
+            if (c.n_pages, c.page_rows) != (self.n_pages, self.page_rows) or c.device != ctx.device:
+                raise ValueError(f"caches: a layer of {c.n_pages} pages of {c.page_rows} rows on cuda:{c.device}, the pool "
+                                 f"has {self.n_pages} of {self.page_rows}, the context is on cuda:{ctx.device}")
+
     def take_copies(self) -> list[tuple[list[int], list[int], list[int]]]:
         """The waiting page copies as (src, dst, rows) groups, to be run one after another."""
         groups = []
@@ -322,12 +332,16 @@ class PagePool:
 
     def run_copies(self, ctx: Context, caches: PagedCaches) -> None:
         """Runs the waiting copies on the context's stream."""
+        self._check_caches(ctx, caches)
         for group in self.take_copies():
             paged_copy(ctx, caches, *[_upload(ctx, x) for x in group])
 
     def compact(self, ctx: Context, caches: PagedCaches, tables) -> int:
         """Moves the pages in use to the front of every layer's cache and rewrites `tables`
         (int32 CUDA [n_seqs, max_pages], as `batch` makes them); returns the pages moved."""
+        self._check_caches(ctx, caches)  # before the pool forgets where the pages were
+        _check_tables(tables)
+        _same_device(ctx, tables=tables)
         src, dst, page_map = ((_i32 * self.n_pages)() for _ in range(3))
         n = _i32()
         self._check("g4_page_pool_compact",

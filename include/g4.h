@@ -432,7 +432,8 @@ g4_status g4_paged_compact(g4_ctx* ctx, const g4_paged_cache* caches, int n_laye
 
 /* Which pages a cache's sequences hold: host bookkeeping, no GPU needed.  Pages are counted
  * by their users; a fork shares every page of its parent, and the first of them to append
- * into a shared last page gets its own copy of it. */
+ * into a shared last page gets its own copy of it.  Up to 2^24 pages of page_rows rows (a
+ * multiple of 8 up to 65536). */
 typedef struct g4_page_pool g4_page_pool;
 g4_status g4_page_pool_create(int n_pages, int page_rows, g4_page_pool** out);
 g4_status g4_page_pool_destroy(g4_page_pool* pool);

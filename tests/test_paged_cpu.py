@@ -120,7 +120,7 @@ def test_pool_fork_of_whole_pages_copies_nothing():
 
 
 def test_pool_refusals():
-    for args in ((0, 8), (4, 0), (4, 12), (4, -8), (4, 65544), (-1, 8)):
+    for args in ((0, 8), (4, 0), (4, 12), (4, -8), (4, 65544), (-1, 8), (2 ** 24 + 1, 8), (2 ** 31 - 1, 8)):
         with pytest.raises(g4.G4Error):
             g4.PagePool(*args)
     pool = g4.PagePool(4, 8)

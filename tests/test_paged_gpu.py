@@ -322,6 +322,14 @@ def test_refusals(gpu_ctx):
             with_cache(k)
         assert e.value.code == code, (k.shape, k.stride())
     small = g4.PagedCache(cache.k[:1], cache.v[:1])
+    pool = g4.PagePool(cache.n_pages + 1, cache.page_rows)  # not this cache's pool: nothing changes
+    s = pool.add()
+    pool.extend(s, 30)
+    for call in (lambda: pool.compact(gpu_ctx, g4.PagedCaches([cache]), batch.tables),
+                 lambda: pool.run_copies(gpu_ctx, g4.PagedCaches([cache]))):
+        with pytest.raises(ValueError, match="pool"):
+            call()
+    assert pool.table(s)[1] == 30
     with pytest.raises(g4.G4Error):
         g4.paged_copy(gpu_ctx, g4.PagedCaches([cache, small]), batch.kv_len, batch.kv_len, batch.kv_len)
     assert gpu_ctx.poll() == 0

@@ -1,13 +1,18 @@
 // Attention of sequences with few rows (new tokens x query heads per KV head: a decode step) over
-// their pages, on tcgen05 with the roles of the operands exchanged: the cache rows are the 128 rows of the MMA, the query rows its N = 16 columns.
-//   S^T[128 keys][16] = K Q^T           O^T[128 dims][16] += V^T P^T   (per 128 dims of the head)
+// their pages, on tcgen05 with the roles of the operands exchanged: the cache rows are the 128 rows
+// of the MMA, the query rows its columns (N = 16 for S, 32 for O).
+//   S^T[128 keys][16] = K Q^T           O^T[128 dims][32] += V^T P^T   (per 128 dims of the head)
 // so a tile of 128 cache rows costs 32 (head of 256) or 64 (512) small MMAs instead of the
 // 256-row products of g4_paged_attn.cu, and every K/V byte is fetched once.  Bound by HBM: 192 KB
 // of K and V per SM are in flight, in stages of 128 rows x 128 dims (32 KB).
 //
 // A thread has one key of the tile: maxima over the keys go through shuffles (16 columns at a
-// time: 16 exchanges instead of 80) and shared memory, P as bf16 (the one type of both operands)
-// into the shared tile the second product reads, sums stay with the thread until the item ends.
+// time: 16 exchanges instead of 80) and shared memory, P into the shared tile the second product
+// reads, sums stay with the thread until the item ends.  Both operands of a kind::f16 MMA have one
+// type, V's bf16, so P goes in as two bf16: its rounding in rows 0-15 of the tile, what that left
+// over in rows 16-31, N = 32 columns of O that are added at the end.  A weight is off by 2^-16 of
+// itself at most; the tensor cores have the time (32 single tokens of full layers over up to 8192
+// rows 56.4 us, 55.6 with P rounded once; one sliding token 10.9 us, 10.7).
 // Up to four rows (one token of two heads) take a quarter of that work.  The scores of the next
 // tile are computed before the values of this one, so that K keeps arriving meanwhile.
 //
@@ -21,16 +26,18 @@ namespace g4 {
 
 constexpr int kFewThreads = 224;
 constexpr int kFewStage = 32768, kFewStages = 6;
-constexpr uint32_t kFewCols = 128;  // tensor memory: S [0, 16) and [16, 32), O block j [32 + 16 j, 48 + 16 j)
-constexpr uint32_t kFewColO = 32;
+constexpr uint32_t kFewCols = 256;  // tensor memory: S [0, 16) and [16, 32), O block j [32 + 32 j, 64 + 32 j)
+constexpr uint32_t kFewColO = 32;   // (of P's rounded part in 16 columns, of its remainder in 16)
 constexpr uint32_t kFewIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (2u << 17) | (8u << 24);
-constexpr uint32_t kFewIdescO = kFewIdescS | (1u << 15);  // A (V) dims-contiguous
+constexpr uint32_t kFewIdescO =  // N = 32; A (V) dims-contiguous
+    (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (4u << 17) | (8u << 24);
+constexpr int kFewPBlock = 32 * 128;  // bytes of P over 64 keys
 
 template <int D>
 struct __align__(1024) FewSmem {
   uint8_t ring[kFewStages][kFewStage];  // 2 blocks of 64 dims x [128 rows][64], 128-byte swizzle
   uint8_t q[D / 64][16 * 128];
-  uint8_t p[2][16 * 128];               // P: blocks of 64 keys x [16 rows][64]
+  uint8_t p[2][kFewPBlock];             // P: blocks of 64 keys x [16 rows, their remainders][64]
   float4 top[2][4][4];                  // the warps' maxima of a tile's 16 columns (two tiles' worth)
   float4 sum[4][4];
   uint64_t full[kFewStages], empty[kFewStages], raw[kFewStages];  // raw: copied, rows not zeroed yet
@@ -168,12 +175,12 @@ __device__ __forceinline__ bool few_tile(FewSmem<D>& sm, const PaArgs& a, const 
 #pragma unroll
     for (int c = N; c < 16; ++c) f[c] = 1.f;
 #pragma unroll 1
-    for (int blk = 0; blk < D / 128; ++blk) {
+    for (int x = 0; x < D / 128 * 2; ++x) {  // a block's 16 columns, or those of their remainders
       float o[16];
-      few_ld16(tbase + lanes + kFewColO + 16 * blk, o);
+      few_ld16(tbase + lanes + kFewColO + 16 * x, o);
 #pragma unroll
       for (int c = 0; c < 16; ++c) o[c] *= f[c];
-      few_st16(tbase + lanes + kFewColO + 16 * blk, o);
+      few_st16(tbase + lanes + kFewColO + 16 * x, o);
     }
     pa_st_wait();
   }
@@ -183,7 +190,10 @@ __device__ __forceinline__ bool few_tile(FewSmem<D>& sm, const PaArgs& a, const 
   for (int c = 0; c < N; ++c) {
     const float e = pa_exp2(fmaf(s[c], factor_s, m[c] == -CUDART_INF_F ? 0.f : -m[c]));
     l[c] += e;
-    *reinterpret_cast<uint16_t*>(p + pa_swizzle(c, ch) + eb) = f32_to_bf16(e);
+    const uint16_t hi = f32_to_bf16(e);
+    uint16_t* at = reinterpret_cast<uint16_t*>(p + pa_swizzle(c, ch) + eb);
+    at[0] = hi;
+    at[16 * 64] = f32_to_bf16(e - bf16_to_f32(hi));  // (16 rows on: the same place in the swizzle)
   }
   return true;
 }
@@ -320,8 +330,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       float* part = a.part + (static_cast<size_t>(range) * 2 + (it.begin == 0 ? 1 : 0)) * few_part_floats(D);
 #pragma unroll 1
       for (int blk = 0; blk < kBlocks; ++blk) {
-        float o[16];
-        few_ld16(tbase + lanes + kFewColO + 16 * blk, o);
+        float o[16], o_rest[16];
+        few_ld16(tbase + lanes + kFewColO + 32 * blk, o);
+        few_ld16(tbase + lanes + kFewColO + 32 * blk + 16, o_rest);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] += o_rest[c];
         if (whole) {
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
@@ -453,8 +466,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           if (leader) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              few_mma(tbase + kFewColO + 16 * x, vd + 2048 * k / 16, p_desc + ((k >> 2) * 2048 + 32 * (k & 3)) / 16,
-                      kFewIdescO, k ? 1u : more);
+              few_mma(tbase + kFewColO + 32 * x, vd + 2048 * k / 16,
+                      p_desc + ((k >> 2) * kFewPBlock + 32 * (k & 3)) / 16, kFewIdescO, k ? 1u : more);
             few_commit(&sm.empty[at.stage]);
             if (x == kBlocks - 1) few_commit(&sm.pv_done);
           }

@@ -388,8 +388,9 @@ typedef struct g4_paged_batch {
  * visible to (its position is negative: kv_len counts fewer rows than there are new tokens)
  * gets zeros.  Rows outside the visible range of every new token of a sequence are not
  * read, whatever they hold; within it K and V are expected to be finite.  Scores,
- * softmax statistics and sums are f32; the weights of V are rounded to bf16 for the tensor
- * cores.  q and out are [n_tokens, n_heads, head_dim] with the given strides in elements
+ * softmax statistics and sums are f32; the weights of V go to the tensor cores as two bf16
+ * (16 bits) in calls of as many tokens as sequences or of at most 16 rows (tokens x query heads
+ * per KV head), rounded to one bf16 (8 bits) in others.  q and out are [n_tokens, n_heads, head_dim] with the given strides in elements
  * (multiples of 8).  The new tokens' own K and V rows must be in the cache already
  * (g4_paged_store_qkv).  The first call of a context allocates its scratch (39 MB; make it
  * before a stream capture).  Up to 2^22 new tokens, 2^30 rows (tokens x query heads per KV

@@ -1,0 +1,38 @@
+"""Paged caches on the GPU: the corners of the paged operators that tests/test_paged_gpu.py does not
+reach, against the same float64 oracle (u = 2^-8, half a unit in the last place of bf16)."""
+
+import pytest
+import torch
+
+import g4b200 as g4
+from oracle import paged as op
+from test_paged_gpu import FULL, SLIDING, U, _attend, _check_attention, _setup
+
+pytestmark = pytest.mark.gpu
+
+# calls of few rows (as many tokens as sequences, or 16 rows at most)
+FEW = [
+    ([(1, 1000)], SLIDING, 64, 1024),
+    ([(1, 8192)], FULL, 512, 0),
+    ([(1, n) for n in (1, 2, 127, 130, 700, 1023)], SLIDING, 16, 0),
+    ([(1, n) for n in (1, 2, 127, 130, 700, 1023)], FULL, 24, 0),
+    ([(1, 40 * i + 300) for i in range(40)], FULL, 40, 0),
+    ([(3, 900), (0, 5), (0, 7)], SLIDING, 16, 100),
+    ([(8, 500)], SLIDING, 8, 0),
+    ([(1, 400)], (5, 1, 256), 16, 0),
+    ([(1, 400), (1, 3000)], (9, 1, 512), 16, 0),
+]
+
+
+@pytest.mark.parametrize("case", range(len(FEW)))
+def test_few_rows_keep_the_weights_of_v(gpu_ctx, case):
+    """The kernel for few rows carries a weight as two bf16: off by u^2 = 2^-16 of itself at most.
+    Scores, softmax and sums in f32 are off by less than 2^-15 of sum p |v| (scores of std 2.5: their
+    sums of |q k| are below 40, in f32 by a tensor core 2^-22 of that), so 2^-13 covers both with
+    room; the output is rounded once."""
+    lens, heads, page_rows, window = FEW[case]
+    q, cache, batch, tables = _setup(lens, heads, page_rows, window, seed=40 + case)
+    out = _attend(gpu_ctx, q, cache, batch, window=window)
+    want, weight = op.attention(q, cache.k, cache.v, tables, lens, 1.0, window)
+    err = (out.double() - want).abs() - (U * want.abs() + 2.0 ** -13 * weight)
+    assert err.max().item() <= 0

@@ -265,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const bool valid = i < it.s.n;
       const bool any_row = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps step
       const int pos = it.s.kv - it.s.n + i;
-      const int hi = valid ? pos + 1 : 0, lo = valid && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      const int hi = valid ? pos + 1 : 0, lo = valid ? pa_low(pos, a.window) : 0;
       if (!a.q_tma) {
         // rows of any group size: a thread copies one 16-byte column of every kStep-th row (the
         // previous item's scores are done: all these warps have read them and met since)

@@ -138,12 +138,12 @@ __device__ __forceinline__ bool few_tile(FewSmem<D>& sm, const PaArgs& a, const 
   // the tile's keys are [key0, key0 + 128); the item's tokens are at positions [first, last]
   const int key0 = (it.kt0 + u) * kPaKeys, base = it.s.kv - it.s.n, r0 = it.tile * 16;
   const int first = base + a.by_group.div(r0), last = base + min(it.s.n - 1, a.by_group.div(r0 + 15));
-  if (key0 + kPaKeys - 1 > first || (a.window > 0 && key0 <= last - a.window)) {
+  if (key0 + kPaKeys - 1 > first || (a.window > 0 && last - key0 >= a.window)) {
     const int key = key0 + tid;
 #pragma unroll
     for (int c = 0; c < N; ++c) {  // (columns past the rows: whatever they hold stays theirs)
       const int pos = base + a.by_group.div(r0 + c);
-      if (key > pos || (a.window > 0 && key <= pos - a.window)) s[c] = -CUDART_INF_F;
+      if (key > pos || (a.window > 0 && pos - key >= a.window)) s[c] = -CUDART_INF_F;
     }
   }
   const float mine = few_reduce<true, N>(s, lane) * factor_s;

@@ -135,6 +135,11 @@ __device__ __forceinline__ uint32_t pa_swizzle(int row, int c) {  // 16-byte chu
 }
 
 // ---------------------------------------------------------------------------- work split
+// The first row that a token at `pos` sees.  (A position may be negative and a window as large as
+// an int holds: nothing is subtracted that could wrap.)
+__device__ __forceinline__ int pa_low(int pos, int window) {
+  return window > 0 && pos >= window ? pos - window + 1 : 0;
+}
 // Key tiles of row tile `tile` of a sequence: [kt0, kt0 + n), n >= 1 (a tile nothing is
 // visible to still has its zeros to write).
 __device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, const PaArgs& a, int& kt0) {
@@ -144,7 +149,7 @@ __device__ __forceinline__ int pa_key_tiles(const PagedSeq& s, int tile, const P
   const int hi = first + i1 + 1;
   kt0 = 0;
   if (hi <= 0) return 1;
-  if (a.window > 0) kt0 = max(0, first + i0 - a.window + 1) / kPaKeys;
+  kt0 = pa_low(first + i0, a.window) / kPaKeys;
   return (hi + kPaKeys - 1) / kPaKeys - kt0;
 }
 __device__ __forceinline__ int pa_tiles(const PagedSeq& s, const PaArgs& a) {
@@ -277,7 +282,7 @@ struct PaWalk {
     return end > begin;  // (no unit: the range ends within the overhead)
   }
   // the first cache row any new token of the sequence sees
-  __device__ int low() const { return a.window > 0 ? max(0, s.kv - s.n - a.window + 1) : 0; }
+  __device__ int low() const { return pa_low(s.kv - s.n, a.window); }
   // a V tile that reaches past the sequence's visible rows
   __device__ bool edge(int kt) const { return (kt + 1) * kPaKeys > s.kv || kt * kPaKeys < low(); }
 };

@@ -36,3 +36,22 @@ def test_few_rows_keep_the_weights_of_v(gpu_ctx, case):
     want, weight = op.attention(q, cache.k, cache.v, tables, lens, 1.0, window)
     err = (out.double() - want).abs() - (U * want.abs() + 2.0 ** -13 * weight)
     assert err.max().item() <= 0
+
+
+WIDE = [
+    [(5, 2)],
+    [(10, 5), (1, 300), (64, 64)],
+    [(10, 5), (1, 300)] + [(0, 3)] * 9,  # as many tokens as sequences: few rows
+    [(3, 0), (1, 200), (2, 700)] + [(0, 0)] * 3,
+]
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, 1])
+@pytest.mark.parametrize("heads", [SLIDING, FULL])
+@pytest.mark.parametrize("case", range(len(WIDE)))
+def test_attention_windows_beyond_every_position(gpu_ctx, case, heads, window):
+    """The largest windows an int holds mask nothing, also beside tokens at negative positions (a
+    sequence of more new tokens than rows), which see nothing."""
+    lens = WIDE[case]
+    q, cache, batch, tables = _setup(lens, heads, 16, window, seed=60 + case)
+    _check_attention(_attend(gpu_ctx, q, cache, batch, window=window), q, cache, tables, lens, window=window)

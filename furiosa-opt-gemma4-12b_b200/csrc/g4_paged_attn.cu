@@ -64,10 +64,7 @@ struct __align__(1024) PaSmem {
   float top[2][128];        // the rows' maxima over each half of a tile's columns
   uint32_t tmem;
   uint32_t abort;
-  int units, first;        // weight of the call; where this range starts
-  int range_count;         // ranges in use
-  int item_cost;
-  int seq, tile, head, offset;
+  PaRange range;
 };
 
 // ---------------------------------------------------------------------------- PTX
@@ -204,41 +201,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   __syncthreads();
   pa_fence_after();
   if (warp == 0) {
-    int u = 0, items = 0;
-    for (int s = lane; s < b.n_seqs; s += 32) {
-      u += w[s].units;
-      items += w[s].items;
-    }
-    u = __reduce_add_sync(0xffffffffu, u);
-    items = __reduce_add_sync(0xffffffffu, items);
-    const int cost = u <= a.ranges ? 0 : a.item_cost;  // with a pair for every unit, each gets one
-    u += cost * items;
-    const int n = min(a.ranges, u);  // ranges in use: none is empty
-    int seq = 0, tile = 0, head = 0, offset = 0;
-    int first = 0;
-    if (range < n) {
-      first = pa_share(range, u, n);
-      pa_find(b, a, w, cost, first, lane, seq, tile, head, offset);
-    }
-    if (lane == 0) {
-      sm.units = u;
-      sm.first = first;
-      sm.range_count = n;
-      sm.item_cost = cost;
-      sm.seq = seq;
-      sm.tile = tile;
-      sm.head = head;
-      sm.offset = offset;
-    }
+    const PaRange found = pa_range(b, a, w, range, lane, scr);
+    if (lane == 0) sm.range = found;
     fence_proxy_async();  // the ring's next writers are TMA copies
   }
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // both CTAs' barriers and memory are ready
   const uint32_t tbase = sm.tmem;
-  const int u_first = sm.first;
-  const int u_end = range < sm.range_count ? pa_share(range + 1, sm.units, sm.range_count) : u_first;
+  const int u_first = sm.range.first;
+  const int u_end = range < sm.range.count ? pa_share(range + 1, sm.range.units, sm.range.count) : u_first;
   volatile uint32_t* abort = &sm.abort;
-  PaWalk it(b, a, sm.item_cost, sm.seq, sm.tile, sm.head, sm.offset, u_end - u_first);
+  PaWalk it(b, a, sm.range, u_end - u_first);
 
   // registers a thread: 128 at launch (512 x 128 in all), 8 of the output's for each softmax warp
   // group: 128 x (2 x 136 + 128 + 112) = 65536.  (Sliding 4096-token prompt: 69.4 us; 76.2 us
@@ -415,7 +388,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       if (it.begin == 0 && it.end < it.nk) {
         // the item's last unit is at position u_end - it.end + it.nk - 1 of the call
         const int last = u_end - it.end + it.nk - 1;
-        const long long e = ((last + 1ll) * sm.range_count - 1) / sm.units;
+        const long long e = ((last + 1ll) * sm.range.count - 1) / sm.range.units;
         tail = {it.seq, it.tile, it.head, static_cast<int>(e) - range + 1};
       }
       pa_fence_after();

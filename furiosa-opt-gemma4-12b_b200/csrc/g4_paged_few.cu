@@ -43,8 +43,7 @@ struct __align__(1024) FewSmem {
   uint64_t full[kFewStages], empty[kFewStages], raw[kFewStages];  // raw: copied, rows not zeroed yet
   uint64_t s_full[2], p_full, pv_done, q_full;
   uint32_t tmem, abort;
-  int units, first, range_count, item_cost;
-  int seq, tile, head, offset;
+  PaRange range;
 };
 constexpr int few_part_floats(int d) { return 16 * d + 32; }  // O [16][D], then (m, l) [16][2]
 
@@ -234,41 +233,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   pa_count(b, a, w, scr, blockIdx.x == 0);
   __syncthreads();
   if (warp == 0) {
-    int u = 0, items = 0;
-    for (int s = lane; s < b.n_seqs; s += 32) {
-      u += w[s].units;
-      items += w[s].items;
-    }
-    u = __reduce_add_sync(0xffffffffu, u);
-    items = __reduce_add_sync(0xffffffffu, items);
-    const int cost = u <= a.ranges ? 0 : a.item_cost;  // with a CTA for every unit, each gets one
-    u += cost * items;
-    const int n = min(a.ranges, u);
-    int seq = 0, tile = 0, head = 0, offset = 0, first = 0;
-    if (range < n) {
-      first = pa_share(range, u, n);
-      pa_find(b, a, w, cost, first, lane, seq, tile, head, offset);
-    }
-    if (lane == 0) {
-      sm.units = u;
-      sm.first = first;
-      sm.range_count = n;
-      sm.item_cost = cost;
-      sm.seq = seq;
-      sm.tile = tile;
-      sm.head = head;
-      sm.offset = offset;
-    }
+    const PaRange found = pa_range(b, a, w, range, lane, scr);
+    if (lane == 0) sm.range = found;
     fence_proxy_async();  // the ring's next writers are TMA copies
   }
   pa_fence_before();
   __syncthreads();
   pa_fence_after();
   const uint32_t tbase = sm.tmem;
-  const int u_first = sm.first;
-  const int u_end = range < sm.range_count ? pa_share(range + 1, sm.units, sm.range_count) : u_first;
+  const int u_first = sm.range.first;
+  const int u_end = range < sm.range.count ? pa_share(range + 1, sm.range.units, sm.range.count) : u_first;
   volatile uint32_t* abort = &sm.abort;
-  PaWalk it(b, a, sm.item_cost, sm.seq, sm.tile, sm.head, sm.offset, u_end - u_first);
+  PaWalk it(b, a, sm.range, u_end - u_first);
 
   if (warp < 4) {
     // -------------------------------------------------------------- Q, softmax, output
@@ -324,7 +300,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const bool whole = it.begin == 0 && it.end == it.nk;
       if (it.begin == 0 && it.end < it.nk) {
         const int last = u_end - it.end + it.nk - 1;  // the item's last unit, as a position of the call
-        const long long e = ((last + 1ll) * sm.range_count - 1) / sm.units;
+        const long long e = ((last + 1ll) * sm.range.count - 1) / sm.range.units;
         tail = {it.seq, it.tile, it.head, static_cast<int>(e) - range + 1};
       }
       float* part = a.part + (static_cast<size_t>(range) * 2 + (it.begin == 0 ? 1 : 0)) * few_part_floats(D);

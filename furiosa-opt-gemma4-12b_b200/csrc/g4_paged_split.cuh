@@ -238,6 +238,43 @@ __device__ __forceinline__ void pa_find(const PagedBatch& b, const PaArgs& a, co
   offset = want - base - head * weight;
 }
 
+// A CTA's (or pair's) share of the call: the weight of all items, where the range starts in it, the
+// ranges in use, an item's cost in units, and the item that the range starts in.
+struct PaRange {
+  int units, first, count, cost;
+  int seq, tile, head, offset;
+};
+// Range `range` of the call, from the counts; one warp.  What the host lets through weighs less
+// than 2^30, as long as q_start does not fall: where it does, sequences may share tokens, and a call
+// that weighs more by that is not done at all (reported once).
+__device__ __forceinline__ PaRange pa_range(const PagedBatch& b, const PaArgs& a, const PaCount* w, int range, int lane,
+                                            Scratch* scr) {
+  constexpr uint32_t kMost = 1u << 30;  // (a sequence alone stays below it; sums stop there)
+  uint32_t units = 0, items = 0;
+#pragma unroll 1
+  for (int s = lane; s < b.n_seqs; s += 32) {
+    units = min(units + w[s].units, kMost);
+    items = min(items + w[s].items, kMost);
+  }
+  // in 32nds, so that the lanes' sum fits: below kMost / 32 what follows is off by no wrap
+  const bool most = __reduce_add_sync(0xffffffffu, (units + a.item_cost * items) / 32) >= kMost / 32;
+  units = __reduce_add_sync(0xffffffffu, units);
+  items = __reduce_add_sync(0xffffffffu, items);
+  PaRange r = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (most) {
+    if (range == 0 && lane == 0) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
+    return r;
+  }
+  r.cost = static_cast<int>(units) <= a.ranges ? 0 : a.item_cost;  // with a CTA (pair) for every unit, each gets one
+  r.units = static_cast<int>(units + r.cost * items);
+  r.count = min(a.ranges, r.units);  // none is empty
+  if (range < r.count) {
+    r.first = pa_share(range, r.units, r.count);
+    pa_find(b, a, w, r.cost, r.first, lane, r.seq, r.tile, r.head, r.offset);
+  }
+  return r;
+}
+
 // The items of a range, in order; every role walks them alike.
 struct PaWalk {
   const PagedBatch& b;
@@ -248,9 +285,8 @@ struct PaWalk {
   PagedSeq s;
   int kt0, nk, begin, end;  // key tiles of the current item: [begin, end) of its nk are this range's
   int next_offset;
-  __device__ PaWalk(const PagedBatch& batch, const PaArgs& args, int cost_, int seq_, int tile_, int head_, int offset,
-                    int weight)
-      : b(batch), a(args), cost(cost_), left(weight), seq(seq_), tile(tile_), head(head_ - 1), next_offset(offset) {
+  __device__ PaWalk(const PagedBatch& batch, const PaArgs& args, const PaRange& r, int weight)
+      : b(batch), a(args), cost(r.cost), left(weight), seq(r.seq), tile(r.tile), head(r.head - 1), next_offset(r.offset) {
     bool bad;
     s = left > 0 ? paged_seq(b, seq, &bad) : PagedSeq{0, 0, 0};
   }

@@ -372,7 +372,8 @@ typedef struct g4_paged_cache {
  *                        never looked at (-1 past the end or below a window is usual).
  * q_start outside 0..n_tokens or falling, kv_len outside 0..max_pages * page_rows, and page
  * numbers outside 0..n_pages - 1 are cut off or skipped, never followed, and set a bit in
- * the device status word (g4_ctx_poll_device_status). */
+ * the device status word (g4_ctx_poll_device_status).  (Where q_start falls, sequences may share
+ * tokens; a g4_paged_attention that would have 2^30 tiles or more by that does nothing else.) */
 #define G4_PAGED_MAX_SEQS 4096
 typedef struct g4_paged_batch {
   const int32_t* tables;

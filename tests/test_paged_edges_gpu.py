@@ -55,3 +55,23 @@ def test_attention_windows_beyond_every_position(gpu_ctx, case, heads, window):
     lens = WIDE[case]
     q, cache, batch, tables = _setup(lens, heads, 16, window, seed=60 + case)
     _check_attention(_attend(gpu_ctx, q, cache, batch, window=window), q, cache, tables, lens, window=window)
+
+
+@pytest.mark.parametrize("tokens", [4096, 4097])  # as many tokens as sequences, and not
+def test_attention_of_a_batch_that_counts_its_tokens_over_and_over(gpu_ctx, tokens):
+    """q_start goes up and down, so that half of the sequences have the same 4096 tokens: 8.6e9 tiles
+    of 256 rows (or 1.4e11 of 16), past what an int counts.  The host lets 2^30 through and takes it
+    that a token is of one sequence.  Nothing is done, and the status word says so."""
+    pages, seqs = 256, 4096  # every table entry is the one page: 2^24 rows a sequence
+    k = torch.zeros(1, 65536, 1, 256, dtype=torch.bfloat16, device="cuda")
+    cache = g4.PagedCache(k, k)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    starts = torch.zeros(seqs + 1, **i32)
+    starts[1::2] = 4096
+    batch = g4.PagedBatch(torch.zeros(seqs, pages, **i32), starts, torch.full((seqs,), pages * 65536, **i32))
+    q = torch.zeros(tokens, 2, 256, dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, 5.0)
+    g4.paged_attention(gpu_ctx, q, cache, batch, out)
+    with pytest.raises(g4.G4Error):
+        gpu_ctx.poll()
+    assert gpu_ctx.poll() == 0 and (out == 5).all()

@@ -171,6 +171,7 @@ __device__ __forceinline__ bool few_tile(FewSmem<D>& sm, const PaArgs& a, const 
     }
   }
   if (moved && u != it.begin) {
+    pa_fence_after();  // O is read behind the products that pv_done stood for
 #pragma unroll
     for (int c = N; c < 16; ++c) f[c] = 1.f;
 #pragma unroll 1

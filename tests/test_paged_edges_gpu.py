@@ -75,3 +75,34 @@ def test_attention_of_a_batch_that_counts_its_tokens_over_and_over(gpu_ctx, toke
     with pytest.raises(g4.G4Error):
         gpu_ctx.poll()
     assert gpu_ctx.poll() == 0 and (out == 5).all()
+
+
+# batches of single tokens over so many tiles that a CTA has several of one item; <= 4 and > 4 rows
+TOKENS = [([(1, 9000), (1, 8300), (1, 8999)], SLIDING), ([(1, 16000)] * 4, FULL), ([(1, 16000)] * 4, (5, 1, 256)),
+          ([(1, 12000)] * 3, (6, 2, 512))]
+
+
+@pytest.mark.parametrize("case", range(len(TOKENS)))
+def test_few_rows_rising_scores(gpu_ctx, case):
+    """Scores that rise by 30 every 100 rows, in a CTA's many tiles of an item: O is scaled again at
+    each of them."""
+    lens, heads = TOKENS[case]
+    q, cache, batch, tables = _setup(lens, heads, 64, 0, seed=80 + case)
+    q.zero_()
+    q[:, :, 0] = 1.0
+    for s, (n, kv) in enumerate(lens):
+        for p in range(-(-kv // 64)):
+            rows = torch.arange(64 * p, 64 * p + 64, device="cuda")
+            cache.k[tables[s][p], :, :, 0] = torch.where(rows < kv, 0.3 * rows, float("nan"))[:, None].bfloat16()
+    out = _attend(gpu_ctx, q, cache, batch)
+    _check_attention(out, q, cache, tables, lens)
+    assert torch.equal(out, _attend(gpu_ctx, q, cache, batch))
+
+
+@pytest.mark.parametrize("scale,std", [(0.0, 1.0), (0.0625, 20.0), (-1.0, 2.0), (1.0, 40.0), (1e-3, 1.0)])
+@pytest.mark.parametrize("case", range(len(TOKENS)))
+def test_few_rows_scales(gpu_ctx, case, scale, std):
+    """The scales and score sizes of test_attention_scales, where they meet the kernel for few rows."""
+    lens, heads = TOKENS[case]
+    q, cache, batch, tables = _setup(lens, heads, 32, 0, seed=90 + case, std=std)
+    _check_attention(_attend(gpu_ctx, q, cache, batch, scale=scale), q, cache, tables, lens, scale=scale)

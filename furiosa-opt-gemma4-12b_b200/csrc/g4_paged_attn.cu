@@ -455,7 +455,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // -------------------------------------------------------------- K copies (8), V copies (10)
     // A K stage is 4 blocks of 64 dims x 64 rows, a V stage 2 halves of 64 rows x 2 blocks.  Where
     // a page holds 64 rows in one piece, a box is all of a K stage or of a half; else a box is
-    // 2^log_box rows of one block.  A lane copies one box; the lanes run on their own.
+    // 2^log_box rows of one block.  A lane copies one box.  The lanes meet at every wait: those that
+    // have no box hold no stage back, and a parity tells only two neighbouring phases apart, so that
+    // a lane which lags or runs ahead by one more would wait for the wrong one.
     const bool is_k = warp == 8;
     PaRing at(is_k ? 0 : kK, is_k ? kK : kV);
     uint32_t edges = 0;  // V tiles that warp 11 finishes
@@ -488,7 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     };
     auto free_stage = [&]() {  // waits until the stage at `at` may be filled
       if (ok && at.passed >= static_cast<uint32_t>(at.n))
-        ok = pa_wait(&sm.empty[at.stage], at.parity ^ 1u, abort, budget);
+        ok = pa_wait_warp(&sm.empty[at.stage], at.parity ^ 1u, abort, budget);
       return ok;
     };
     auto fill = [&](Box& x, int dim_block, uint32_t bar) {
@@ -525,7 +527,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         } else {
           // the stage reports to warp 11, which zeroes rows of it (with no box to wait for, at
           // once: so only when it is free) and reports to the leader
-          if (edges > 0) ok = pa_wait(&sm.edge_done, (edges - 1) & 1, abort, budget);
+          if (edges > 0) ok = pa_wait_warp(&sm.edge_done, (edges - 1) & 1, abort, budget);
           ++edges;
           if (free_stage()) {
             if (lane == 0) mbar_arrive_expect_tx(&sm.edge_full, now.bytes);
@@ -536,7 +538,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     }
     // every stage is free again: no barrier of this CTA has an arrival outstanding when it exits
     for (uint32_t n = at.n, x = at.passed > n ? at.passed - n : 0; x < at.passed && ok; ++x)
-      ok = pa_wait(&sm.empty[at.first + x % n], (x / n) & 1, abort, budget);
+      ok = pa_wait_warp(&sm.empty[at.first + x % n], (x / n) & 1, abort, budget);
     if (bad_page) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
     if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   } else if (warp == 9) {

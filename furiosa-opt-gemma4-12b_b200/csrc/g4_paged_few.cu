@@ -342,7 +342,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     if (tid == 0) a.tail[range] = ok ? tail : PaTail{-1, 0, 0, 0};
   } else if (warp == 4) {
     // -------------------------------------------------------------- copies
-    // A box is 2^log_box rows of one 64-dim block, or all of a stage; a lane copies one.
+    // A box is 2^log_box rows of one 64-dim block, or all of a stage; a lane copies one.  The lanes
+    // meet at every wait: one without a box would hold no stage back, and could lag behind, or run
+    // ahead of, the two phases that a parity tells apart.
     PaRing at(0, kFewStages);
     const uint64_t maps[2] = {reinterpret_cast<uint64_t>(&kmap), reinterpret_cast<uint64_t>(&vmap)};
     const int box = 1 << a.log_box, blocks = a.log_box == 7 ? 1 : 2;
@@ -366,8 +368,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       return x;
     };
     auto copy = [&](const Box& x, bool is_v, bool edge) {  // a tile's kBlocks stages
+#pragma unroll 1
       for (int blk = 0; blk < kBlocks && ok; ++blk) {
-        if (at.passed >= kFewStages) ok = pa_wait(&sm.empty[at.stage], at.parity ^ 1u, abort, budget);
+        if (at.passed >= kFewStages) ok = pa_wait_warp(&sm.empty[at.stage], at.parity ^ 1u, abort, budget);
         if (!ok) break;
         uint64_t* bar = edge ? &sm.raw[at.stage] : &sm.full[at.stage];
         if (lane == 0) mbar_arrive_expect_tx(bar, x.bytes);
@@ -395,7 +398,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     }
     // every stage is free again: no copy or arrival is outstanding when the CTA exits
     for (uint32_t x = at.passed > kFewStages ? at.passed - kFewStages : 0; x < at.passed && ok; ++x)
-      ok = pa_wait(&sm.empty[x % kFewStages], (x / kFewStages) & 1, abort, budget);
+      ok = pa_wait_warp(&sm.empty[x % kFewStages], (x / kFewStages) & 1, abort, budget);
     if (bad_page) atomicOr(&scr->status, DEV_ERR_BAD_OFFSET);
     if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   } else if (warp == 5) {

@@ -106,3 +106,15 @@ def test_few_rows_scales(gpu_ctx, case, scale, std):
     lens, heads = TOKENS[case]
     q, cache, batch, tables = _setup(lens, heads, 32, 0, seed=90 + case, std=std)
     _check_attention(_attend(gpu_ctx, q, cache, batch, scale=scale), q, cache, tables, lens, scale=scale)
+
+
+@pytest.mark.parametrize("heads,page_rows,window", [((60, 20, 256), 128, 64), ((60, 20, 256), 8, 64),
+                                                    ((12, 4, 512), 64, 40), (SLIDING, 64, 200), ((32, 16, 256), 24, 8)])
+def test_attention_of_many_short_items(gpu_ctx, heads, page_rows, window):
+    """Small windows over a long chunk: every CTA pair has many items of few tiles, hardly any of them
+    at a sequence's ends; query groups that TMA can copy and ones that it cannot."""
+    lens = [(1800, 2500), (700, 700), (1, 40)]
+    q, cache, batch, tables = _setup(lens, heads, page_rows, window, seed=7)
+    out = _attend(gpu_ctx, q, cache, batch, window=window)
+    _check_attention(out, q, cache, tables, lens, window=window)
+    assert torch.equal(out, _attend(gpu_ctx, q, cache, batch, window=window))

@@ -580,7 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           if (u + 1 < it.end) {
             scores(g + (u + 1 - it.begin));
             if (!ok) break;
-            if (u + 2 == it.end && leader) pa_commit(&sm.q_empty);
+            if (a.q_tma && u + 2 == it.end && leader) pa_commit(&sm.q_empty);
             __syncwarp();
           }
           if (u < it.begin) continue;
@@ -620,7 +620,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const uint64_t map = reinterpret_cast<uint64_t>(&qmap);
     const uint32_t q_full = pa_map_to(smem_u32(&sm.q_full), 0), full0 = pa_map_to(smem_u32(&sm.full[0]), 0);
     while (ok && it.next()) {
-      if (items > 0) ok = pa_wait_warp(&sm.q_empty, (items - 1) & 1, abort, budget);
+      // (the softmax warps copy Q behind their own waits, and nothing would then keep this one within
+      // a phase of q_empty)
+      if (a.q_tma && items > 0) ok = pa_wait_warp(&sm.q_empty, (items - 1) & 1, abort, budget);
       ++items;
       if (!ok) break;
       if (a.q_tma && lane == 0) {
@@ -655,7 +657,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         }
       }
     }
-    if (ok && items > 0) ok = pa_wait_warp(&sm.q_empty, (items - 1) & 1, abort, budget);
+    if (ok && a.q_tma && items > 0) ok = pa_wait_warp(&sm.q_empty, (items - 1) & 1, abort, budget);
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   }
   __syncthreads();

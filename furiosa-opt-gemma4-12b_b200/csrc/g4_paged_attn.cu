@@ -396,7 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         // no row of this warp's
       } else if (whole) {
         // four lanes write 64 bytes of one row at a time: one row per lane would be 32 lines per store
-        const float inv = ml.y > 0.f ? 1.f / ml.y : 0.f;
+        const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;  // (a NaN sum is not zero: it goes out)
         uint16_t* row[4];
         bool live[4];
         const unsigned long long mine = reinterpret_cast<unsigned long long>(
@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const __grid
       }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   tile[lane][warp] = make_uint4(pa_bf16x2(o[0][0] * inv, o[0][1] * inv), pa_bf16x2(o[0][2] * inv, o[0][3] * inv),
                                 pa_bf16x2(o[1][0] * inv, o[1][1] * inv), pa_bf16x2(o[1][2] * inv, o[1][3] * inv));
   __syncthreads();

@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             if (c >= rows) continue;
             const int rr = it.tile * 16 + c, i = a.by_group.div(rr);
             a.out[(it.s.t0 + i) * a.o_ts + (it.head * a.group + rr - i * a.group) * a.o_hs + 128 * blk + tid] =
-                f32_to_bf16(l[c] > 0.f ? __fdividef(o[c], l[c]) : 0.f);
+                f32_to_bf16(l[c] == 0.f ? 0.f : __fdividef(o[c], l[c]));  // (a NaN sum is not zero: it goes out)
           }
         } else {
 #pragma unroll
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const __grid_c
     r[2] = fmaf(w, v.z, r[2]);
     r[3] = fmaf(w, v.w, r[3]);
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *reinterpret_cast<uint2*>(a.out + (s.t0 + i) * a.o_ts + (t.head * a.group + hg) * a.o_hs + 4 * quad) =
       make_uint2(pa_bf16x2(r[0] * inv, r[1] * inv), pa_bf16x2(r[2] * inv, r[3] * inv));
 }

@@ -387,7 +387,8 @@ typedef struct g4_paged_batch {
  * position p attends rows j <= p (and j > p - window if window > 0) of KV head
  * h / (n_heads / n_kv_heads): out = sum_j softmax_j(scale * q . k_j) v_j.  A token no row is
  * visible to (its position is negative: kv_len counts fewer rows than there are new tokens)
- * gets zeros.  Rows outside the visible range of every new token of a sequence are not
+ * gets zeros.  A NaN in a query head's row, or a score that overflows f32 to +inf, makes that
+ * head's output NaN (one that overflows to -inf weighs nothing).  Rows outside the visible range of every new token of a sequence are not
  * read, whatever they hold; within it K and V are expected to be finite.  Scores,
  * softmax statistics and sums are f32; the weights of V go to the tensor cores as two bf16
  * (16 bits) in calls of as many tokens as sequences or of at most 16 rows (tokens x query heads

@@ -1,6 +1,8 @@
 """Paged caches on the GPU: the corners of the paged operators that tests/test_paged_gpu.py does not
 reach, against the same float64 oracle (u = 2^-8, half a unit in the last place of bf16)."""
 
+import math
+
 import pytest
 import torch
 
@@ -118,3 +120,44 @@ def test_attention_of_many_short_items(gpu_ctx, heads, page_rows, window):
     out = _attend(gpu_ctx, q, cache, batch, window=window)
     _check_attention(out, q, cache, tables, lens, window=window)
     assert torch.equal(out, _attend(gpu_ctx, q, cache, batch, window=window))
+
+
+NOT_FINITE = [
+    [(1, 100)],  # within one CTA, no join
+    [(1, 8192)],  # in many CTAs' hands
+    [(1, 40), (1, 700), (1, 1000), (1, 2)],
+    [(130, 300), (1, 40)],  # not the kernel for few rows
+    [(3, 2), (1, 300), (0, 4), (0, 4)],  # some rows see nothing
+]
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, 3e38])
+@pytest.mark.parametrize("heads", [SLIDING, FULL])
+@pytest.mark.parametrize("case", range(len(NOT_FINITE)))
+def test_attention_rows_that_are_not_finite(gpu_ctx, case, heads, value):
+    """A query head with a NaN, an infinity, or scores past f32's range has no softmax: its output is
+    NaN (if it sees anything), in one CTA's hands as in many, and the rows beside it are right.  (Two
+    dimensions of q and k are +-value and positive, so that a score is +inf and not only -inf.)"""
+    lens = NOT_FINITE[case]
+    q, cache, batch, tables = _setup(lens, heads, 16, 0, seed=20 + case)
+    tokens, hq, _ = q.shape
+    cache.k[..., 1] = torch.where(torch.isnan(cache.k[..., 1]), cache.k[..., 1], 10.0)
+    hit = torch.zeros(tokens, hq, dtype=torch.bool, device="cuda")
+    hit[::3, ::5] = True
+    clean = q.clone()
+    q[..., 1][hit] = value
+    out = _prefilled(gpu_ctx, q, cache, batch)
+    sees = torch.tensor([kv - n + i >= 0 for n, kv in lens for i in range(n)], device="cuda")[:, None].expand(tokens, hq)
+    assert torch.isnan(out[hit & sees]).all()
+    assert (out[~sees] == 0).all()
+    want, weight = op.attention(clean, cache.k, cache.v, tables, lens)
+    err = (out.double() - want).abs() - (2 * U + 2.0 ** -11) * weight
+    assert err[~hit].max().item() <= 0
+
+
+def _prefilled(ctx, q, cache, batch):
+    out = torch.full_like(q, 7.0)
+    g4.paged_attention(ctx, q, cache, batch, out)
+    torch.cuda.synchronize()
+    assert ctx.poll() == 0
+    return out

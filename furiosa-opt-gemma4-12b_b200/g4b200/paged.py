@@ -164,11 +164,11 @@ class PagedBatch:
         if n > 1 and tables.stride(0) < width:
             raise ValueError("tables: rows overlap")
         self.device = kv_len.get_device()
-        self._desc = _BatchDesc(tables.data_ptr(), self.stride, q_start.data_ptr(), kv_len.data_ptr(), width, n, 0)
+        self._fields = tables.data_ptr(), self.stride, q_start.data_ptr(), kv_len.data_ptr(), width, n
 
     def desc(self, n_tokens: int) -> _BatchDesc:
-        self._desc.n_tokens = n_tokens  # (the library copies the descriptor within the call)
-        return self._desc
+        """A descriptor of the call's own: calls of other threads may be under way on this batch."""
+        return _BatchDesc(*self._fields, n_tokens)
 
 
 def paged_attention(ctx: Context, q, cache: PagedCache, batch: PagedBatch, out, *, scale: float = 1.0,

@@ -188,3 +188,14 @@ def test_descriptors_refuse_wrong_tensors():
                       torch.zeros(1, dtype=torch.int32))
     with pytest.raises(ValueError, match="no layers"):
         g4.PagedCaches([])
+
+
+def test_a_batch_gives_each_call_its_own_descriptor(monkeypatch):
+    """Two threads with differently padded q over one batch: neither sees the other's token count."""
+    monkeypatch.setattr(g4.paged, "_cuda", lambda name, t, *_: t)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    batch = g4.PagedBatch(i32(3, 5), i32(4), i32(3))
+    a, b = batch.desc(7), batch.desc(900)
+    assert (a.n_tokens, b.n_tokens) == (7, 900)
+    for d in (a, b):
+        assert (d.max_pages, d.n_seqs, d.table_stride, d.kv_len) == (5, 3, 5, batch.kv_len.data_ptr())

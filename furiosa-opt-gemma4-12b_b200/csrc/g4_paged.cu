@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const __grid
   bool bad = false;
   const int s = seq_of_token(b, t, lane, pos, bad);
   if (s < 0) return;
-  bool live = pos >= 0;
+  bool live = pos >= 0 && !bad;  // (of a sequence that was cut off, the positions are not known)
   if (pos >= a.n_positions) live = false, bad = true;
   int page = 0, row = 0;
   if (live) {  // (pos < kv <= max_pages * page_rows)

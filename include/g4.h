@@ -410,7 +410,8 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
  * take them (sin of the low half negated).  Computed in f32 and rounded to bf16 once, where
  * the single-token entry points round after each step.  q_out may be q.  A token at a
  * negative position is not stored and gets a zero q_out; one at or past n_positions, or whose
- * page is out of range, too, and sets a bit in the device status word. */
+ * page is out of range, or of a sequence whose q_start or kv_len is out of range, too, and sets a
+ * bit in the device status word. */
 g4_status g4_paged_store_qkv(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stride, int64_t q_head_stride,
                              int n_heads, const g4_bf16* k, int64_t k_token_stride, int64_t k_head_stride,
                              const g4_bf16* v, int64_t v_token_stride, int64_t v_head_stride,

@@ -8,7 +8,7 @@ import torch
 
 import g4b200 as g4
 from oracle import paged as op
-from test_paged_gpu import FULL, SLIDING, U, _attend, _check_attention, _setup
+from test_paged_gpu import FULL, SLIDING, U, _attend, _check_attention, _setup, _store_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +161,33 @@ def _prefilled(ctx, q, cache, batch):
     torch.cuda.synchronize()
     assert ctx.poll() == 0
     return out
+
+
+@pytest.mark.parametrize("what", ["kv_long", "kv_negative", "start_high", "start_falls"])
+@pytest.mark.parametrize("heads", [SLIDING, FULL])
+def test_store_leaves_the_rows_of_a_sequence_with_bad_numbers(gpu_ctx, what, heads):
+    """Where a sequence's new tokens belong is not known when its numbers are out of range: none of
+    them is stored over rows that it, or a fork that shares its pages, has already."""
+    lens = [(2, 100), (3, 150)]
+    _, cache, batch, tables = _setup(lens, heads, 16, poison=3.0)
+    q, k, v, qw, kw, cos, sin = _store_inputs(lens, heads, 1)
+    if what == "kv_long":
+        batch.kv_len[1] = batch.tables.shape[1] * 16 + 5
+        batch.tables[1] = batch.tables[1].clamp(min=0)  # every entry a page of the cache
+    elif what == "kv_negative":
+        batch.kv_len[1] = -7
+    elif what == "start_high":
+        batch.q_start[2] = 2 ** 30
+    else:
+        batch.q_start[2] = 1
+    before = cache.k.clone(), cache.v.clone()
+    out = torch.full(q.shape, 9.0, dtype=torch.bfloat16, device="cuda")
+    g4.paged_store_qkv(gpu_ctx, q, k, v, qw, kw, cos, sin, cache, batch, out)
+    with pytest.raises(g4.G4Error):
+        gpu_ctx.poll()
+    assert gpu_ctx.poll() == 0
+    page, row = tables[0][98 // 16], 98 % 16  # the other sequence's two tokens
+    for now, was in zip((cache.k, cache.v), before):
+        changed = (now != was).flatten(2).any(2)
+        assert changed[page, row:row + 2].all() and int(changed.sum()) == 2
+    assert (out[2:] == (9 if what == "start_falls" else 0)).all() and (out[:2] != 9).any()

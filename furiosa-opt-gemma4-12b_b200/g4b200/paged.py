@@ -18,6 +18,7 @@ number of calls while the tensors' contents change.  `PagePool` hands out the pa
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -56,6 +57,14 @@ LIB.g4_page_pool_compact.argtypes = [_vp, _p_i32, _p_i32, _p_i32, _p_i32]
 LIB.g4_page_pool_take_copies.argtypes = [_vp, _p_i32, _p_i32, _p_i32, _i32, _p_i32]
 LIB.g4_page_pool_table.argtypes = [_vp, _i32, _p_i32, _i32, _p_i32]
 LIB.g4_page_pool_free_pages.argtypes = [_vp, _p_i32]
+
+
+def _int32(name: str, value) -> int:
+    """An integer as the library's 32-bit int (ctypes would keep the low bits of a larger one)."""
+    v = operator.index(value)
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise ValueError(f"{name}: {v} does not fit 32 bits")
+    return v
 
 
 def _cuda(name: str, t, dtype, dims: int):
@@ -185,8 +194,9 @@ def paged_attention(ctx: Context, q, cache: PagedCache, batch: PagedBatch, out, 
         raise ValueError(f"q: {heads} heads is not a multiple of the cache's {cache.n_kv_heads}")
     if n == 0:
         return
+    window = max(-1, min(int(window), 2 ** 31 - 1))  # (no position is past that: larger ones mask nothing)
     ctx._check("g4_paged_attention", LIB.g4_paged_attention(
-        ctx.handle, *qa, heads, cache.desc, batch.desc(n), float(scale), int(window), *oa))
+        ctx.handle, *qa, heads, cache.desc, batch.desc(n), float(scale), window, *oa))
 
 
 def paged_store_qkv(ctx: Context, q, k, v, q_rms_weight, k_rms_weight, cos, sin, cache: PagedCache,
@@ -265,6 +275,7 @@ class PagePool:
 
     def __init__(self, n_pages: int, page_rows: int):
         h = _vp()
+        n_pages, page_rows = _int32("n_pages", n_pages), _int32("page_rows", page_rows)
         code = LIB.g4_page_pool_create(n_pages, page_rows, ctypes.byref(h))
         if code != 0:
             raise G4Error("g4_page_pool_create", code, f"n_pages={n_pages}, page_rows={page_rows}")
@@ -280,19 +291,22 @@ class PagePool:
         return s.value
 
     def extend(self, seq: int, n_rows: int) -> None:
-        self._check("g4_page_pool_extend", LIB.g4_page_pool_extend(self.handle, seq, n_rows))
+        self._check("g4_page_pool_extend", LIB.g4_page_pool_extend(
+            self.handle, _int32("seq", seq), _int32("n_rows", n_rows)))
 
     def fork(self, seq: int) -> int:
         s = _i32()
-        self._check("g4_page_pool_fork", LIB.g4_page_pool_fork(self.handle, seq, ctypes.byref(s)))
+        self._check("g4_page_pool_fork", LIB.g4_page_pool_fork(
+            self.handle, _int32("seq", seq), ctypes.byref(s)))
         return s.value
 
     def trim(self, seq: int, first_row: int) -> None:
         """Gives back the pages wholly below row first_row (below a sliding window)."""
-        self._check("g4_page_pool_trim", LIB.g4_page_pool_trim(self.handle, seq, first_row))
+        self._check("g4_page_pool_trim", LIB.g4_page_pool_trim(
+            self.handle, _int32("seq", seq), _int32("first_row", first_row)))
 
     def free(self, seq: int) -> None:
-        self._check("g4_page_pool_free", LIB.g4_page_pool_free(self.handle, seq))
+        self._check("g4_page_pool_free", LIB.g4_page_pool_free(self.handle, _int32("seq", seq)))
 
     @property
     def free_pages(self) -> int:
@@ -302,6 +316,7 @@ class PagePool:
 
     def table(self, seq: int) -> tuple[list[int], int]:
         """(the sequence's pages in order, -1 where given back; its rows)."""
+        seq = _int32("seq", seq)
         room = self.n_pages
         while True:
             out, rows = (_i32 * max(1, room))(*([-2] * max(1, room))), _i32()

@@ -199,3 +199,22 @@ def test_a_batch_gives_each_call_its_own_descriptor(monkeypatch):
     assert (a.n_tokens, b.n_tokens) == (7, 900)
     for d in (a, b):
         assert (d.max_pages, d.n_seqs, d.table_stride, d.kv_len) == (5, 3, 5, batch.kv_len.data_ptr())
+
+
+def test_pool_refuses_numbers_past_32_bits():
+    """Not their low 32 bits in their place."""
+    for args in ((2 ** 32 + 4, 8), (4, 2 ** 32 + 8)):
+        with pytest.raises(ValueError, match="32 bits"):
+            g4.PagePool(*args)
+    pool = g4.PagePool(4, 8)
+    s = pool.add()
+    pool.extend(s, 8)
+    big = 2 ** 32
+    for call in (lambda: pool.extend(s, big + 1), lambda: pool.extend(big + s, 1), lambda: pool.fork(big + s),
+                 lambda: pool.trim(s, big + 8), lambda: pool.trim(big + s, 8), lambda: pool.free(big + s),
+                 lambda: pool.table(big + s), lambda: pool.extend(s, -big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    with pytest.raises(TypeError):
+        pool.extend(s, 1.5)
+    assert pool.table(s) == ([0], 8) and pool.free_pages == 3

@@ -191,3 +191,16 @@ def test_store_leaves_the_rows_of_a_sequence_with_bad_numbers(gpu_ctx, what, hea
         changed = (now != was).flatten(2).any(2)
         assert changed[page, row:row + 2].all() and int(changed.sum()) == 2
     assert (out[2:] == (9 if what == "start_falls" else 0)).all() and (out[:2] != 9).any()
+
+
+def test_attention_numbers_past_32_bits(gpu_ctx):
+    """A window past 32 bits masks nothing (its low bits are not taken), one below them is refused."""
+    lens = [(40, 300), (1, 77)]
+    q, cache, batch, tables = _setup(lens, SLIDING, 16)
+    for window in (2 ** 31, 2 ** 32 + 5, 2 ** 63):
+        _check_attention(_attend(gpu_ctx, q, cache, batch, window=window), q, cache, tables, lens)
+    out = torch.empty_like(q)
+    with pytest.raises(g4.G4Error) as e:
+        g4.paged_attention(gpu_ctx, q, cache, batch, out, window=-2 ** 32)
+    assert e.value.code == 1
+    assert gpu_ctx.poll() == 0

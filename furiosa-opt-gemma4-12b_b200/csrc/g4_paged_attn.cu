@@ -42,6 +42,7 @@
 namespace g4 {
 
 constexpr int kPaThreads = 512;
+constexpr float kPaLog2e = 1.4426950408889634f;  // the softmax's exponentials are powers of two
 constexpr int kPaRows = 256;      // rows per item (both CTAs)
 constexpr int kPaStage = 32768;   // bytes per ring stage: 64 K rows x 256 dims, or 128 V rows x 128 dims
 constexpr uint32_t kPaColS = 256; // tensor memory: O [0, 256), S/P tiles at 256 and 384
@@ -850,7 +851,7 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   if (n_heads < 1 || n_heads > 4096 || n_heads % cache->n_kv_heads != 0)
     return fail(ctx, G4_ERR_BAD_ARG, "n_heads must be a multiple of n_kv_heads, at most 4096");
   if (window < 0) return fail(ctx, G4_ERR_BAD_ARG, "negative window");
-  if (!std::isfinite(scale)) return fail(ctx, G4_ERR_BAD_ARG, "scale is not finite");
+  if (!std::isfinite(scale * kPaLog2e)) return fail(ctx, G4_ERR_BAD_ARG, "scale is not finite, or too large for f32");
   if (batch->n_tokens == 0 || batch->n_seqs == 0) return G4_OK;
   if (static_cast<long long>(batch->n_tokens) * (n_heads / cache->n_kv_heads) > (1 << 30))
     return fail(ctx, G4_ERR_BAD_ARG, "too many tokens times query heads per KV head for one call");
@@ -874,7 +875,7 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   a.by_group = divisor(a.group);
   a.by_page = divisor(cache->page_rows);
   a.window = window;
-  a.scale = scale * 1.4426950408889634f;
+  a.scale = scale * kPaLog2e;
   const PagedBatch b = paged_batch(batch, cache);
   if ((st = paged_scratch(ctx, a)) != G4_OK) return st;
   // Decode steps go to the kernel for few rows: at most 16 rows in all, or as many tokens as

@@ -204,3 +204,12 @@ def test_attention_numbers_past_32_bits(gpu_ctx):
         g4.paged_attention(gpu_ctx, q, cache, batch, out, window=-2 ** 32)
     assert e.value.code == 1
     assert gpu_ctx.poll() == 0
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, math.inf, -math.inf])
+def test_attention_refuses_scales_past_f32(gpu_ctx, scale):
+    """The kernels multiply by scale * log2(e), which has to be finite too."""
+    q, cache, batch, _ = _setup([(2, 20)], SLIDING)
+    with pytest.raises(g4.G4Error) as e:
+        g4.paged_attention(gpu_ctx, q, cache, batch, torch.empty_like(q), scale=scale)
+    assert e.value.code == 1 and gpu_ctx.poll() == 0

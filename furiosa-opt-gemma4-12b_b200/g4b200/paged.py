@@ -280,6 +280,7 @@ class PagePool:
         if code != 0:
             raise G4Error("g4_page_pool_create", code, f"n_pages={n_pages}, page_rows={page_rows}")
         self.handle, self.n_pages, self.page_rows = h, n_pages, page_rows
+        self._copies = []  # groups taken from the library's pool, not launched yet
 
     def _check(self, fn: str, code: int) -> None:
         if code != 0:
@@ -333,23 +334,30 @@ class PagePool:
                 raise ValueError(f"caches: a layer of {c.n_pages} pages of {c.page_rows} rows on cuda:{c.device}, the pool "
                                  f"has {self.n_pages} of {self.page_rows}, the context is on cuda:{ctx.device}")
 
-    def take_copies(self) -> list[tuple[list[int], list[int], list[int]]]:
-        """The waiting page copies as (src, dst, rows) groups, to be run one after another."""
-        groups = []
+    def _collect_copies(self) -> None:
         while True:
             src, dst, rows = ((_i32 * 4096)() for _ in range(3))
             n = _i32()
             self._check("g4_page_pool_take_copies",
                         LIB.g4_page_pool_take_copies(self.handle, src, dst, rows, 4096, ctypes.byref(n)))
             if n.value == 0:
-                return groups
-            groups.append((list(src[:n.value]), list(dst[:n.value]), list(rows[:n.value])))
+                return
+            self._copies.append((list(src[:n.value]), list(dst[:n.value]), list(rows[:n.value])))
+
+    def take_copies(self) -> list[tuple[list[int], list[int], list[int]]]:
+        """The waiting page copies as (src, dst, rows) groups, to be run one after another."""
+        self._collect_copies()
+        groups, self._copies = self._copies, []
+        return groups
 
     def run_copies(self, ctx: Context, caches: PagedCaches) -> None:
-        """Runs the waiting copies on the context's stream."""
+        """Runs the waiting copies on the context's stream.  After an error, those that were not
+        launched still wait."""
         self._check_caches(ctx, caches)
-        for group in self.take_copies():
-            paged_copy(ctx, caches, *[_upload(ctx, x) for x in group])
+        self._collect_copies()
+        while self._copies:
+            paged_copy(ctx, caches, *[_upload(ctx, x) for x in self._copies[0]])
+            del self._copies[0]
 
     def compact(self, ctx: Context, caches: PagedCaches, tables) -> int:
         """Moves the pages in use to the front of every layer's cache and rewrites `tables`
@@ -357,6 +365,8 @@ class PagePool:
         self._check_caches(ctx, caches)  # before the pool forgets where the pages were
         _check_tables(tables)
         _same_device(ctx, tables=tables)
+        if self._copies:
+            raise G4Error("g4_page_pool_compact", 1, "page copies wait to be run")
         src, dst, page_map = ((_i32 * self.n_pages)() for _ in range(3))
         n = _i32()
         self._check("g4_page_pool_compact",

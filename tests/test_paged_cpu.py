@@ -218,3 +218,44 @@ def test_pool_refuses_numbers_past_32_bits():
     with pytest.raises(TypeError):
         pool.extend(s, 1.5)
     assert pool.table(s) == ([0], 8) and pool.free_pages == 3
+
+
+def _no_gpu(monkeypatch):
+    """PagePool's calls of the GPU side, replaced: uploads and checks let everything pass."""
+    monkeypatch.setattr(g4.paged, "_upload", lambda ctx, x: list(x))
+    monkeypatch.setattr(g4.PagePool, "_check_caches", lambda *a: None)
+    monkeypatch.setattr(g4.paged, "_check_tables", lambda *a: None)
+    monkeypatch.setattr(g4.paged, "_same_device", lambda *a, **kw: None)
+
+
+def test_copies_that_were_not_launched_still_wait(monkeypatch):
+    """A launch that fails loses no copy: a forked sequence would attend over a page that was never
+    filled."""
+    _no_gpu(monkeypatch)
+    pool = g4.PagePool(8, 8)
+    a = pool.add()
+    pool.extend(a, 4)
+    b = pool.fork(a)
+    pool.extend(b, 1)
+    c = pool.fork(b)
+    pool.extend(c, 1)  # reads what the first copy fills: a group of its own
+    ran, fail_at = [], 1
+
+    def copy(ctx, caches, *group):
+        if len(ran) == fail_at:
+            raise g4.G4Error("g4_paged_copy", 2, "a launch that fails")
+        ran.append(group)
+
+    monkeypatch.setattr(g4.paged, "paged_copy", copy)
+    with pytest.raises(g4.G4Error, match="fails"):
+        pool.run_copies(None, None)
+    assert ran == [([0], [1], [4])]
+    with pytest.raises(g4.G4Error, match="wait"):
+        pool.compact(None, None, None)
+    d = pool.fork(a)
+    pool.extend(d, 1)
+    fail_at = -1
+    pool.run_copies(None, None)
+    assert ran == [([0], [1], [4]), ([1], [2], [5]), ([0], [3], [4])]
+    pool.run_copies(None, None)
+    assert len(ran) == 3 and pool.take_copies() == []

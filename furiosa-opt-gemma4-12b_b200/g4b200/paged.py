@@ -281,6 +281,7 @@ class PagePool:
             raise G4Error("g4_page_pool_create", code, f"n_pages={n_pages}, page_rows={page_rows}")
         self.handle, self.n_pages, self.page_rows = h, n_pages, page_rows
         self._copies = []  # groups taken from the library's pool, not launched yet
+        self._moves = None  # (src, dst, page_map) of a compaction that is not launched yet
 
     def _check(self, fn: str, code: int) -> None:
         if code != 0:
@@ -317,6 +318,7 @@ class PagePool:
 
     def table(self, seq: int) -> tuple[list[int], int]:
         """(the sequence's pages in order, -1 where given back; its rows)."""
+        self._check_moved()
         seq = _int32("seq", seq)
         room = self.n_pages
         while True:
@@ -335,6 +337,7 @@ class PagePool:
                                  f"has {self.n_pages} of {self.page_rows}, the context is on cuda:{ctx.device}")
 
     def _collect_copies(self) -> None:
+        self._check_moved()
         while True:
             src, dst, rows = ((_i32 * 4096)() for _ in range(3))
             n = _i32()
@@ -361,19 +364,29 @@ class PagePool:
 
     def compact(self, ctx: Context, caches: PagedCaches, tables) -> int:
         """Moves the pages in use to the front of every layer's cache and rewrites `tables`
-        (int32 CUDA [n_seqs, max_pages], as `batch` makes them); returns the pages moved."""
+        (int32 CUDA [n_seqs, max_pages], as `batch` makes them); returns the pages moved.  After
+        an error on the way to the GPU the pool's pages are known by their new numbers, but not
+        moved: until another call with the same tables has moved them, the pool hands out no
+        tables, batches or copies."""
         self._check_caches(ctx, caches)  # before the pool forgets where the pages were
         _check_tables(tables)
         _same_device(ctx, tables=tables)
-        if self._copies:
-            raise G4Error("g4_page_pool_compact", 1, "page copies wait to be run")
-        src, dst, page_map = ((_i32 * self.n_pages)() for _ in range(3))
-        n = _i32()
-        self._check("g4_page_pool_compact",
-                    LIB.g4_page_pool_compact(self.handle, src, dst, page_map, ctypes.byref(n)))
-        paged_compact(ctx, caches, _upload(ctx, src[:n.value]), _upload(ctx, dst[:n.value]), tables,
-                      _upload(ctx, page_map[:]))
-        return n.value
+        if self._moves is None:
+            if self._copies:
+                raise G4Error("g4_page_pool_compact", 1, "page copies wait to be run")
+            src, dst, page_map = ((_i32 * self.n_pages)() for _ in range(3))
+            n = _i32()
+            self._check("g4_page_pool_compact",
+                        LIB.g4_page_pool_compact(self.handle, src, dst, page_map, ctypes.byref(n)))
+            self._moves = src[:n.value], dst[:n.value], page_map[:]
+        src, dst, page_map = self._moves
+        paged_compact(ctx, caches, _upload(ctx, src), _upload(ctx, dst), tables, _upload(ctx, page_map))
+        self._moves = None
+        return len(src)
+
+    def _check_moved(self) -> None:
+        if self._moves is not None:
+            raise G4Error("g4_page_pool_compact", 1, "a compaction did not move its pages: call compact again")
 
     def batch(self, ctx: Context, seqs, new_tokens) -> PagedBatch:
         """The batch of `seqs` with their last `new_tokens[i]` rows as new tokens, in that

@@ -259,3 +259,33 @@ def test_copies_that_were_not_launched_still_wait(monkeypatch):
     assert ran == [([0], [1], [4]), ([1], [2], [5]), ([0], [3], [4])]
     pool.run_copies(None, None)
     assert len(ran) == 3 and pool.take_copies() == []
+
+
+def test_a_compaction_that_was_not_launched_is_taken_up_again(monkeypatch):
+    """The pool has renumbered its pages when the launch fails: nothing goes by the new numbers until
+    the pages are where they say."""
+    _no_gpu(monkeypatch)
+    pool = g4.PagePool(8, 8)
+    a, b = pool.add(), pool.add()
+    pool.extend(a, 16)
+    pool.extend(b, 24)
+    pool.free(a)
+    calls = []
+
+    def compact(ctx, caches, src, dst, tables, page_map):
+        calls.append((src, dst, page_map))
+        if len(calls) == 1:
+            raise g4.G4Error("g4_paged_compact", 2, "a launch that fails")
+
+    monkeypatch.setattr(g4.paged, "paged_compact", compact)
+    with pytest.raises(g4.G4Error, match="fails"):
+        pool.compact(None, None, None)
+    for call in (lambda: pool.table(b), lambda: pool.batch(None, [b], [1]), lambda: pool.run_copies(None, None),
+                 pool.take_copies):
+        with pytest.raises(g4.G4Error, match="compact again"):
+            call()
+    pool.extend(pool.fork(b), 1)
+    assert pool.compact(None, None, None) == 2
+    assert calls[1] == calls[0] == ([3, 4], [0, 1], [0, 1, 2, 0, 1, 5, 6, 7])
+    assert pool.table(b)[0] == [2, 0, 1] and pool.take_copies() == []
+    assert pool.compact(None, None, None) == 0

@@ -242,9 +242,9 @@ g4_status g4_page_pool_table(const g4_page_pool* pool, int32_t seq, int32_t* tab
     if (s == nullptr) return refuse(p, G4_ERR_BAD_ARG, "no such sequence");
     if (out_rows == nullptr || width < 0 || (width > 0 && table == nullptr))
       return refuse(p, G4_ERR_BAD_ARG, "null output or negative width");
+    *out_rows = s->rows;
     if (s->pages.size() > static_cast<size_t>(width)) return refuse(p, G4_ERR_TOO_LARGE, "table wider than its room");
     for (int i = 0; i < width; ++i) table[i] = i < static_cast<int>(s->pages.size()) ? s->pages[i] : -1;
-    *out_rows = s->rows;
     return G4_OK;
   });
 }

@@ -320,15 +320,13 @@ class PagePool:
         """(the sequence's pages in order, -1 where given back; its rows)."""
         self._check_moved()
         seq = _int32("seq", seq)
-        room = self.n_pages
-        while True:
-            out, rows = (_i32 * max(1, room))(*([-2] * max(1, room))), _i32()
-            code = LIB.g4_page_pool_table(self.handle, seq, out, room, ctypes.byref(rows))
-            if code != 6:  # wider than the pool: pages given back still have entries
-                break
-            room *= 2
-        self._check("g4_page_pool_table", code)
-        return list(out[:(rows.value + self.page_rows - 1) // self.page_rows]), rows.value
+        rows = _i32()
+        code = LIB.g4_page_pool_table(self.handle, seq, None, 0, ctypes.byref(rows))
+        if code != 6:  # (no room for its pages: has rows, their number is set)
+            self._check("g4_page_pool_table", code)
+        out = (_i32 * ((rows.value + self.page_rows - 1) // self.page_rows))()
+        self._check("g4_page_pool_table", LIB.g4_page_pool_table(self.handle, seq, out, len(out), ctypes.byref(rows)))
+        return out[:], rows.value
 
     def _check_caches(self, ctx: Context, caches: PagedCaches) -> None:
         for c in caches.layers:

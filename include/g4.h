@@ -461,7 +461,8 @@ g4_status g4_page_pool_compact(g4_page_pool* pool, int32_t* src, int32_t* dst, i
  * starts the next call's group. */
 g4_status g4_page_pool_take_copies(g4_page_pool* pool, int32_t* src, int32_t* dst, int32_t* rows, int cap,
                                    int* out_n);
-/* Sequence seq's table into table[width] (-1 past its pages), its rows so far. */
+/* Sequence seq's table into table[width] (-1 past its pages), its rows so far.  A table wider than
+ * `width` is G4_ERR_TOO_LARGE, with *out_rows set all the same: its width follows from the rows. */
 g4_status g4_page_pool_table(const g4_page_pool* pool, int32_t seq, int32_t* table, int width, int* out_rows);
 g4_status g4_page_pool_free_pages(const g4_page_pool* pool, int* out_n);
 

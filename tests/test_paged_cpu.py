@@ -289,3 +289,23 @@ def test_a_compaction_that_was_not_launched_is_taken_up_again(monkeypatch):
     assert calls[1] == calls[0] == ([3, 4], [0, 1], [0, 1, 2, 0, 1, 5, 6, 7])
     assert pool.table(b)[0] == [2, 0, 1] and pool.take_copies() == []
     assert pool.compact(None, None, None) == 0
+
+
+def test_a_table_takes_the_room_of_its_sequence():
+    """Not of the pool: a server asks for each sequence's table at every step."""
+    import tracemalloc
+
+    pool = g4.PagePool(2 ** 20, 8)
+    seqs = [pool.add() for _ in range(4)]
+    for s in seqs[1:]:
+        pool.extend(s, 8 * 25 - 3)
+    tracemalloc.start()
+    got = [pool.table(s) for s in seqs]
+    peak = tracemalloc.get_traced_memory()[1]
+    tracemalloc.stop()
+    assert got[0] == ([], 0) and all(len(t) == 25 and r == 197 for t, r in got[1:])
+    assert [t[0] for t, _ in got[1:]] == [0, 25, 50]
+    assert peak < 2 ** 16
+    rows = ctypes.c_int32()
+    assert g4.LIB.g4_page_pool_table(pool.handle, seqs[1], None, 0, ctypes.byref(rows)) == 6 and rows.value == 197
+    assert g4.LIB.g4_page_pool_table(pool.handle, 99, None, 0, ctypes.byref(rows)) == 1

@@ -866,10 +866,6 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   a.out = out;
   a.o_ts = out_token_stride;
   a.o_hs = out_head_stride;
-  a.vc = cache->v;
-  a.vp = cache->v_page_stride;
-  a.vr = cache->v_row_stride;
-  a.vh = cache->v_head_stride;
   a.group = n_heads / cache->n_kv_heads;
   a.n_kv = cache->n_kv_heads;
   a.by_group = divisor(a.group);

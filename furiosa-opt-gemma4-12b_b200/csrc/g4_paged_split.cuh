@@ -27,8 +27,6 @@ struct PaArgs {
   long long q_ts, q_hs;
   uint16_t* out;
   long long o_ts, o_hs;
-  const uint16_t* vc;
-  long long vp, vr, vh;
   int group, n_kv, window;  // query heads per KV head, KV heads
   int tile_rows;            // rows of an item
   int item_cost;            // what an item's start and end cost, in units, for the work split
@@ -380,8 +378,8 @@ inline bool tile_map(CUtensorMap* m, const uint16_t* base, const int (&n)[4], co
 }
 
 
-// Scratch of split items for `ranges` tails and `floats` of partial sums, allocated at the first
-// call; both kernels use it, one after the other on the context's stream.
+// Scratch of split items (tails and partial sums), allocated at the first call; both kernels use it,
+// one after the other on the context's stream.
 g4_status paged_scratch(g4_ctx* ctx, PaArgs& a);
 // The kernel of g4_paged_few.cu.
 g4_status launch_paged_few(g4_ctx* ctx, PaArgs a, const PagedBatch& b, const g4_paged_cache* c);

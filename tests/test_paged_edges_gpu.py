@@ -213,3 +213,41 @@ def test_attention_refuses_scales_past_f32(gpu_ctx, scale):
     with pytest.raises(g4.G4Error) as e:
         g4.paged_attention(gpu_ctx, q, cache, batch, torch.empty_like(q), scale=scale)
     assert e.value.code == 1 and gpu_ctx.poll() == 0
+
+
+@pytest.mark.parametrize("heads,lens,layout", [(SLIDING, [(1100, 1500), (1, 77), (0, 9), (199, 199)], "nhd"),
+                                               (SLIDING, [(1300, 1300)], "hnd"),
+                                               (FULL, [(600, 1900), (1, 2000), (600, 601)], "kv_in_page"),
+                                               ((15, 5, 256), [(1, 3), (1700, 1800), (33, 20)], "nhd"),
+                                               ((5, 3, 512), [(1200, 1200), (1300, 1999)], "padded")])
+def test_store_of_many_tokens(gpu_ctx, heads, lens, layout):
+    """Calls so large that a warp takes four heads (or pairs of heads) of a token, also where that leaves
+    a rest; the bounds of test_store."""
+    hq, hkv, d = heads
+    _, cache, batch, tables = _setup(lens, heads, 24, layout=layout, seed=3, poison=3.0)
+    q, k, v, qw, kw, cos, sin = _store_inputs(lens, heads, 5)
+    before = cache.k.clone(), cache.v.clone()
+    out = torch.full(q.shape, 9.0, dtype=torch.bfloat16, device="cuda")
+    g4.paged_store_qkv(gpu_ctx, q, k, v, qw, kw, cos, sin, cache, batch, out)
+    torch.cuda.synchronize()
+    assert gpu_ctx.poll() == 0
+    pos = torch.tensor([kv - n + i for n, kv in lens for i in range(n)], device="cuda")
+    seq = torch.tensor([s for s, (n, _) in enumerate(lens) for _ in range(n)], device="cuda")
+    live = pos >= 0
+    at = pos.clamp(min=0)
+    page = torch.tensor(tables, device="cuda")[seq, at // 24][live]
+    row = (at % 24)[live]
+
+    def close(got, want, size):
+        assert ((got.double() - want).abs() - (U * want.abs() + 2.0 ** -18 * size)).max().item() <= 0
+
+    want, size = op.rotate(op.norm(q, qw), cos[at], sin[at])
+    close(out[live], want[live], size[live])
+    assert (out[~live] == 0).all()
+    want, size = op.rotate(op.norm(k, kw), cos[at], sin[at])
+    close(cache.k[page, row], want[live], size[live])
+    want = op.norm(v)
+    close(cache.v[page, row], want[live], want[live].abs())
+    touched = torch.zeros(cache.n_pages, 24, dtype=torch.bool, device="cuda")
+    touched[page, row] = True
+    assert torch.equal(cache.k[~touched], before[0][~touched]) and torch.equal(cache.v[~touched], before[1][~touched])

@@ -67,8 +67,10 @@ PagedBatch paged_batch(const g4_paged_batch* b, const g4_paged_cache* c) {
 // other meet in one lane, and a warp has two heads of 256 or one of 512 at a time.  A warp takes
 // kIter such steps of one token's q, k or v heads: q, k and v are read once and written once,
 // the token's cos/sin row and the norm weights once per warp.  The heads' loads go out first,
-// ahead of the chain token -> sequence -> page, whose two round trips they hide.  Memory bound by
-// its bytes (4 per element), by instructions before the arithmetic went two f32 at a time.
+// ahead of the chain token -> sequence -> page, whose two round trips they hide (the sequence is
+// found by a scan, 32 a round trip: more than 32 sequences make that chain longer).  4096 sliding
+// tokens keep DRAM 38 % and the SMs' pipes 36 % busy: what bounds them is how much 16 warps an SM (110
+// registers) have in flight.
 struct StoreArgs {
   const uint16_t *q, *k, *v;
   long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;

@@ -876,8 +876,9 @@ g4_status g4_paged_attention(g4_ctx* ctx, const g4_bf16* q, int64_t q_token_stri
   if ((st = paged_scratch(ctx, a)) != G4_OK) return st;
   // Decode steps go to the kernel for few rows: at most 16 rows in all, or as many tokens as
   // sequences, which is taken for one token each (the lengths themselves are on the device; other
-  // lengths are right there too, 16 rows at a time).  32 single tokens of full layers over up to
-  // 8192 rows: 56.5 us there, 80 us here.  With a chunk among them one launch of this kernel beats
+  // lengths are right there too, 16 rows at a time).  A step with an idle sequence or a padded token
+  // is not seen as one and comes here.  32 single tokens of full layers over up to 8192 rows:
+  // 56 us there, 80 us here.  With a chunk among them one launch of this kernel beats
   // one of each (31 tokens beside 509 new ones, sliding: 78 us against 89).
   const bool few = static_cast<long long>(b.n_tokens) * a.group <= kPaFewRows ||
                    (a.group <= kPaFewRows && b.n_tokens == b.n_seqs);

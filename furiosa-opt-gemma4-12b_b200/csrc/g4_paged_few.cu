@@ -502,7 +502,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 // Joins an item's parts as paged_join_kernel does; a block has one row: D / 4 threads a part,
 // kGroups parts at a time, joined in range order within a group and the groups in order.
 // kThreads: 512 where one item may be in all CTAs' hands (one token over 8192 rows of a full layer:
-// 18.0 us in all, 20.1 with 256), 256 where most have two parts (32 tokens: 56.5 us, 58.5 with 512).
+// 18.0 us in all, 20.1 with 256), 256 where most have two parts (32 tokens: 56.5 us, 58.5 with 512;
+// both before P went in as two bf16).
 template <int D, int kThreads>
 __global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const __grid_constant__ PaArgs a,
                                                                          const __grid_constant__ PagedBatch b) {

@@ -388,12 +388,13 @@ typedef struct g4_paged_batch {
  * h / (n_heads / n_kv_heads): out = sum_j softmax_j(scale * q . k_j) v_j.  A token no row is
  * visible to (its position is negative: kv_len counts fewer rows than there are new tokens)
  * gets zeros.  A NaN in a query head's row, or a score that overflows f32 to +inf, makes that
- * head's output NaN (one that overflows to -inf weighs nothing).  Rows outside the visible range of every new token of a sequence are not
- * read, whatever they hold; within it K and V are expected to be finite.  Scores,
- * softmax statistics and sums are f32; the weights of V go to the tensor cores as two bf16
- * (16 bits) in calls of as many tokens as sequences or of at most 16 rows (tokens x query heads
- * per KV head), rounded to one bf16 (8 bits) in others.  q and out are [n_tokens, n_heads, head_dim] with the given strides in elements
- * (multiples of 8).  The new tokens' own K and V rows must be in the cache already
+ * head's output NaN (one that overflows to -inf weighs nothing).  Rows outside the visible
+ * range of every new token of a sequence are not read, whatever they hold; within it K and V
+ * are expected to be finite.  Scores, softmax statistics and sums are f32; the weights of V go
+ * to the tensor cores as two bf16 (16 bits) in calls of as many tokens as sequences or of at
+ * most 16 rows (tokens x query heads per KV head), rounded to one bf16 (8 bits) in others.
+ * scale * log2(e) must be finite.  q and out are [n_tokens, n_heads, head_dim] with the given
+ * strides in elements (multiples of 8).  The new tokens' own K and V rows must be in the cache already
  * (g4_paged_store_qkv).  The first call of a context allocates its scratch (39 MB; make it
  * before a stream capture).  Up to 2^22 new tokens, 2^30 rows (tokens x query heads per KV
  * head: else G4_ERR_BAD_ARG) and 2^30 tiles of 128 cache rows that max_pages and n_tokens

@@ -293,6 +293,7 @@ g4_status g4_ctx_create(int device, g4_ctx** out) {
   if (st == G4_OK) st = check_cuda(ctx, cudaMemset(b.tc_ptag, 0, kTcPartWords * 8), "cudaMemset tc_ptag");
   if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&b.tc_htag, kHFloats * 4), "cudaMalloc tc_htag");
   if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&b.cand, kCandWords * 8), "cudaMalloc cand");
+  if (st == G4_OK) st = check_cuda(ctx, cudaMalloc(&b.beam, kBeamWords * 8), "cudaMalloc beam");
   if (st == G4_OK) st = check_cuda(ctx, cudaMemset(b.tc_htag, 0, kHFloats * 4), "cudaMemset tc_htag");
   if (st == G4_OK) st = check_cuda(ctx, cudaDeviceSynchronize(), "ctx init");
   if (st != G4_OK) {
@@ -319,6 +320,7 @@ g4_status g4_ctx_destroy(g4_ctx* ctx) {
   cudaFree(ctx->buf.tc_ptag);
   cudaFree(ctx->buf.tc_htag);
   cudaFree(ctx->buf.cand);
+  cudaFree(ctx->buf.beam);
   cudaFree(ctx->prefill.xq);
   cudaFree(ctx->prefill.h);
   cudaFree(ctx->prefill.hq);

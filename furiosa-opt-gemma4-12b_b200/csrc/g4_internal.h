@@ -38,6 +38,7 @@ constexpr size_t kAttnFloats = 512 * (2 * 16 + 16 * 512) + 4096;  // 512 chunks 
 constexpr size_t kTcTiles = 15360 / 64 + 3840 / 128;              // gate/up tiles + down tiles
 constexpr size_t kTcSegFloats = 3840;                             // the down projection's H sums
 constexpr size_t kTcPartWords = kTcTiles * 8 * 128;                // tagged segment partials (both phases)
+constexpr size_t kBeamWords = 1 << 19;                             // beam selection: its lists (g4_beam.cu)
 constexpr size_t kCandWords = 16384 + 128 + 8 * 128;              // sampling: candidates, a rank's share, gathered
 
 // Tensor-parallel one-shot all-reduce over peer memory.  Each rank owns one exchange
@@ -71,6 +72,7 @@ struct DeviceBuffers {
   uint64_t* tc_ptag = nullptr;  // [kTcPartWords]
   uint32_t* tc_htag = nullptr;  // [kHFloats]
   uint64_t* cand = nullptr;     // [kCandWords] sampling candidates (g4_sample.cu)
+  uint64_t* beam = nullptr;     // [kBeamWords] beam selection (g4_beam.cu)
 };
 
 // Batched prefill feed-forward scratch, grown to the largest token count seen and kept
@@ -127,6 +129,20 @@ namespace g4 {
 g4_status fail(g4_ctx* ctx, g4_status code, const std::string& msg);
 g4_status check_cuda(g4_ctx* ctx, cudaError_t err, const char* what);
 bool aligned16(const void* p);
+// The context's device as the current one while this lives (the caller's is put back).
+struct DeviceGuard {
+  int before = -1;
+  explicit DeviceGuard(const g4_ctx* ctx) {
+    if (cudaGetDevice(&before) != cudaSuccess || before == ctx->device || cudaSetDevice(ctx->device) != cudaSuccess)
+      before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+// A bf16 matrix argument: 16-byte aligned, its row stride a multiple of 8 of at least `cols` where
+// there are several rows (g4_rows.cu).
+g4_status check_matrix(g4_ctx* ctx, const void* p, int64_t stride, int rows, int cols, const char* what);
 
 // Launchers implemented in the kernel translation units.
 g4_status launch_decoder_feedforward(g4_ctx* ctx, uint16_t* residual, const uint16_t* pre_w,

@@ -156,6 +156,29 @@ g4_status g4_page_pool_fork(g4_page_pool* pool, int32_t seq, int32_t* out_child)
   });
 }
 
+g4_status g4_page_pool_reorder(g4_page_pool* pool, const int32_t* seqs, const int32_t* parents, int n) {
+  return guarded(pool, [&] {
+    if (n < 0 || (n > 0 && (seqs == nullptr || parents == nullptr)))
+      return refuse(pool, G4_ERR_BAD_ARG, "null sequences or a negative count");
+    std::set<int32_t> seen;
+    std::vector<Seq> now;
+    for (int i = 0; i < n; ++i) {
+      if (find(pool, seqs[i]) == nullptr || find(pool, parents[i]) == nullptr)
+        return refuse(pool, G4_ERR_BAD_ARG, "no such sequence");
+      if (!seen.insert(seqs[i]).second) return refuse(pool, G4_ERR_BAD_ARG, "a sequence is listed twice");
+    }
+    for (int i = 0; i < n; ++i) now.push_back(pool->seqs[parents[i]]);
+    for (const Seq& s : now)  // first, so that no page that stays is ever free
+      for (const int32_t p : s.pages)
+        if (p >= 0) ++pool->users[p];
+    for (int i = 0; i < n; ++i) {
+      for (const int32_t p : pool->seqs[seqs[i]].pages) drop(pool, p);
+      pool->seqs[seqs[i]] = std::move(now[i]);
+    }
+    return G4_OK;
+  });
+}
+
 g4_status g4_page_pool_trim(g4_page_pool* pool, int32_t seq, int first_row) {
   return guarded(pool, [&] {
     Seq* s = find(pool, seq);

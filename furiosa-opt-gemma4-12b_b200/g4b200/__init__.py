@@ -652,3 +652,9 @@ from .paged import (PagedBatch, PagedCache, PagedCaches, PagePool, paged_attenti
 
 __all__ += ["PagedBatch", "PagedCache", "PagedCaches", "PagePool", "paged_attention", "paged_compact", "paged_copy",
             "paged_store_qkv"]
+
+from .batch import (Nvfp4Rows, Nvfp4Weight, beam_select, embed_tokens, nvfp4_dequantize, nvfp4_matmul,  # noqa: E402
+                    nvfp4_quantize, residual_norm)
+
+__all__ += ["Nvfp4Rows", "Nvfp4Weight", "beam_select", "embed_tokens", "nvfp4_dequantize", "nvfp4_matmul",
+            "nvfp4_quantize", "residual_norm"]

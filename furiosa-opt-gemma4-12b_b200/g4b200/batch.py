@@ -1,0 +1,223 @@
+"""Host binding of the operators around the attention of a batch (include/g4.h: g4_embed_tokens,
+g4_nvfp4_*, g4_residual_norm, g4_beam_select), for programs that run many sequences or prompt
+chunks where the reference's host runs one position per dispatch (src/host/generate.rs:194-211).
+
+    rows = Nvfp4Rows(ctx, max_tokens, 3840)                  # kept: codes, scales, factors
+    qkv_w = Nvfp4Weight(ctx, codes, block_scales, gscale)    # once per projection
+    embed_tokens(ctx, table, tokens, x)
+    nvfp4_quantize(ctx, x, rows, input_rms_weight)           # per layer
+    nvfp4_matmul(ctx, rows, qkv_w, qkv)
+    ...                                                      # paged_store_qkv, paged_attention
+    nvfp4_quantize(ctx, attended, o_rows)
+    nvfp4_matmul(ctx, o_rows, o_w, y)
+    residual_norm(ctx, y, post_rms_weight, x, x)
+    ...
+    beam_select(ctx, logits, scores, best_scores, beams, next_tokens)
+    pool.reorder(seqs, [seqs[b] for b in beams])             # each group's caches follow
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import LIB, Context, _i32, _i64, _vp
+
+_f32 = ctypes.c_float
+EMBED_SCALE = 62.0  # G4_EMBED_SCALE
+BEAM_MAX = 64  # G4_BEAM_MAX
+
+
+class _RowsDesc(ctypes.Structure):
+    _fields_ = [("codes", _vp), ("scales", _vp), ("factor", _vp), ("max_rows", _i32), ("cols", _i32), ("pieces", _i32)]
+
+
+class _WeightDesc(ctypes.Structure):
+    _fields_ = [("codes", _vp), ("scales", _vp), ("factor", _vp), ("rows", _i32), ("cols", _i32), ("n_factors", _i32)]
+
+
+_rows_p, _weight_p = ctypes.POINTER(_RowsDesc), ctypes.POINTER(_WeightDesc)
+LIB.g4_embed_tokens.argtypes = [_vp, _vp, _i32, _i32, _vp, _i32, _f32, _vp, _i64]
+LIB.g4_residual_norm.argtypes = [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64]
+LIB.g4_nvfp4_scale_bytes.argtypes = [_i32, _i32]
+LIB.g4_nvfp4_scale_bytes.restype = ctypes.c_uint64
+LIB.g4_nvfp4_scale_blocks.argtypes = [_vp, _vp, _i32, _i32, _vp]
+LIB.g4_nvfp4_quantize.argtypes = [_vp, _vp, _i64, _i32, _vp, _rows_p]
+LIB.g4_nvfp4_dequantize.argtypes = [_vp, _rows_p, _i32, _vp, _i64]
+LIB.g4_nvfp4_matmul.argtypes = [_vp, _rows_p, _i32, _weight_p, _vp, _i64, _i32]
+LIB.g4_beam_select.argtypes = [_vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]
+
+_BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+
+
+def _tensor(ctx: Context, name: str, t, dtypes: tuple, dims: int):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch tensor")
+    if t.get_device() != ctx.device:
+        raise ValueError(f"{name}: on {t.device}, the context is on cuda:{ctx.device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtypes[0]}")
+    if t.dim() != dims:
+        raise ValueError(f"{name}: {t.dim()} dimensions, expected {dims}")
+    if t.numel() >= 2 ** 31 and max(t.shape) >= 2 ** 31:  # (ctypes would keep the low 32 bits)
+        raise ValueError(f"{name}: shape {list(t.shape)} does not fit 32 bits")
+    return t
+
+
+def _matrix(ctx: Context, name: str, t, rows, cols, dtypes=(_BF16,)) -> tuple:
+    """A [rows, cols] operand (None: any) with contiguous rows: (pointer, row stride)."""
+    shape = _tensor(ctx, name, t, dtypes, 2).shape
+    if (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
+        raise ValueError(f"{name}: shape {list(shape)}, expected [{'n' if rows is None else rows}, {'any' if cols is None else cols}]")
+    row, col = t.stride()
+    if col != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    return t.data_ptr(), row if shape[0] > 1 else max(row, shape[1])
+
+
+def _whole(ctx: Context, name: str, t, shape: tuple, dtypes) -> int:
+    _tensor(ctx, name, t, dtypes, len(shape))
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: shape {list(t.shape)}, expected {list(shape)}, contiguous")
+    return t.data_ptr()
+
+
+def embed_tokens(ctx: Context, table, tokens, out, scale: float = EMBED_SCALE) -> None:
+    """out[t] = bf16(table[tokens[t]] * scale) (g4_embed_tokens): table bf16 [vocab, dim] contiguous,
+    tokens int32 [n], out bf16 [n, dim].  An id outside the table gives zeros and a device status bit."""
+    vocab, dim = _tensor(ctx, "table", table, (_BF16,), 2).shape
+    n = _tensor(ctx, "tokens", tokens, (_I32,), 1).shape[0]
+    _whole(ctx, "table", table, (vocab, dim), (_BF16,))
+    ids = _whole(ctx, "tokens", tokens, (n,), (_I32,))
+    to = _matrix(ctx, "out", out, n, dim)
+    if n:
+        ctx._check("g4_embed_tokens", LIB.g4_embed_tokens(ctx.handle, table.data_ptr(), vocab, dim, ids, n, scale, *to))
+
+
+def residual_norm(ctx: Context, x, rms_weight, residual, out) -> None:
+    """out = bf16(residual + rmsnorm(x) * rms_weight) by rows (g4_residual_norm); out may be residual."""
+    n, dim = _tensor(ctx, "x", x, (_BF16,), 2).shape
+    xa, ra, oa = _matrix(ctx, "x", x, n, dim), _matrix(ctx, "residual", residual, n, dim), _matrix(ctx, "out", out, n, dim)
+    w = _whole(ctx, "rms_weight", rms_weight, (dim,), (_BF16,))
+    if n:
+        ctx._check("g4_residual_norm", LIB.g4_residual_norm(ctx.handle, *xa, w, *ra, n, dim, *oa))
+
+
+class Nvfp4Rows:
+    """Room for `max_rows` rows of `cols` values as 1 to 3 NVFP4 pieces (g4_nvfp4_rows), on the
+    context's device.  Filled by nvfp4_quantize; calls take the first rows of it."""
+
+    def __init__(self, ctx: Context, max_rows: int, cols: int, pieces: int = 2):
+        if not 1 <= max_rows <= 2 ** 22 or cols % 32 or not 32 <= cols <= 16384 or not 1 <= pieces <= 3:
+            raise ValueError(f"{max_rows} rows of {cols} values in {pieces} pieces: expected 1..2^22 rows of a multiple of "
+                             "32 up to 16384 in 1..3 pieces")
+        self.max_rows, self.cols, self.pieces, self.device = max_rows, cols, pieces, ctx.device
+        blocks = LIB.g4_nvfp4_scale_bytes(max_rows, cols)
+        with torch.cuda.stream(ctx.stream):  # (the memory is used on, and given back to, this stream)
+            dev = f"cuda:{ctx.device}"
+            self.codes = torch.empty((pieces, max_rows, cols // 2), dtype=_U8, device=dev)
+            self.scales = torch.empty((pieces, blocks), dtype=_U8, device=dev)
+            self.factor = torch.empty(max_rows, dtype=_F32, device=dev)
+        self.desc = _RowsDesc(self.codes.data_ptr(), self.scales.data_ptr(), self.factor.data_ptr(), max_rows, cols, pieces)
+
+
+class Nvfp4Weight:
+    """A projection [rows, cols] for nvfp4_matmul (g4_nvfp4_weight): the checkpoint's codes uint8
+    [rows, cols / 2] (kept, not copied), its block scales [rows, cols / 16], which are laid out anew, and
+    the reciprocal global scale f32 [1], or a factor for every row, f32 [rows] (projections stacked
+    along their rows)."""
+
+    def __init__(self, ctx: Context, codes, block_scales, global_scale):
+        n, half = _tensor(ctx, "codes", codes, (_U8,), 2).shape
+        cols = 2 * half
+        if n < 1 or cols % 32 or not 32 <= cols <= 16384:
+            raise ValueError(f"codes: [{n}, {half}] bytes, expected rows of a multiple of 16 up to 8192")
+        _whole(ctx, "codes", codes, (n, half), (_U8,))
+        given = _whole(ctx, "block_scales", block_scales, (n, cols // 16), (_U8, torch.float8_e4m3fn))
+        _tensor(ctx, "global_scale", global_scale, (_F32,), 1)
+        if global_scale.numel() not in (1, n) or not global_scale.is_contiguous():
+            raise ValueError(f"global_scale: {global_scale.numel()} values, expected 1 or {n}, contiguous")
+        with torch.cuda.stream(ctx.stream):
+            scales = torch.empty(LIB.g4_nvfp4_scale_bytes(n, cols), dtype=_U8, device=f"cuda:{ctx.device}")
+        ctx._check("g4_nvfp4_scale_blocks", LIB.g4_nvfp4_scale_blocks(ctx.handle, given, n, cols, scales.data_ptr()))
+        self._set(codes, scales, global_scale, n, cols, ctx.device)
+
+    @classmethod
+    def from_rows(cls, rows: Nvfp4Rows) -> "Nvfp4Weight":
+        """The matrix that nvfp4_quantize wrote into `rows` (one piece, all of its rows), as a weight."""
+        if rows.pieces != 1:
+            raise ValueError(f"rows: {rows.pieces} pieces, a weight has one")
+        w = cls.__new__(cls)
+        w._set(rows.codes, rows.scales, rows.factor, rows.max_rows, rows.cols, rows.device)
+        return w
+
+    def _set(self, codes, scales, factor, n, cols, device):
+        self.codes, self.scales, self.factor, self.rows, self.cols, self.device = codes, scales, factor, n, cols, device
+        self.desc = _WeightDesc(codes.data_ptr(), scales.data_ptr(), factor.data_ptr(), n, cols, factor.numel())
+
+
+def _rows_of(ctx: Context, rows: Nvfp4Rows, n: int) -> None:
+    if rows.device != ctx.device:
+        raise ValueError(f"rows: on cuda:{rows.device}, the context is on cuda:{ctx.device}")
+    if n > rows.max_rows:
+        raise ValueError(f"rows: room for {rows.max_rows}, the call has {n}")
+
+
+def nvfp4_quantize(ctx: Context, x, rows: Nvfp4Rows, rms_weight=None) -> None:
+    """x (bf16 [n, cols]), or rmsnorm(x) * rms_weight rounded to bf16, into the first n rows of `rows`
+    (g4_nvfp4_quantize)."""
+    xa = _matrix(ctx, "x", x, None, rows.cols)
+    n = x.shape[0]
+    _rows_of(ctx, rows, n)
+    w = None if rms_weight is None else _whole(ctx, "rms_weight", rms_weight, (rows.cols,), (_BF16,))
+    if n:
+        ctx._check("g4_nvfp4_quantize", LIB.g4_nvfp4_quantize(ctx.handle, *xa, n, w, rows.desc))
+
+
+def nvfp4_dequantize(ctx: Context, rows: Nvfp4Rows, out) -> None:
+    """The values of the first n rows, rounded to bf16, into out [n, cols] (g4_nvfp4_dequantize)."""
+    oa = _matrix(ctx, "out", out, None, rows.cols)
+    n = out.shape[0]
+    _rows_of(ctx, rows, n)
+    if n:
+        ctx._check("g4_nvfp4_dequantize", LIB.g4_nvfp4_dequantize(ctx.handle, rows.desc, n, *oa))
+
+
+def nvfp4_matmul(ctx: Context, rows: Nvfp4Rows, weight: Nvfp4Weight, out) -> None:
+    """out [n, weight.rows] = the first n rows times the weight's rows (g4_nvfp4_matmul); out bf16, or
+    f32 (a tensor-parallel rank's partial sums)."""
+    oa = _matrix(ctx, "out", out, None, weight.rows, (_BF16, _F32))
+    n = out.shape[0]
+    _rows_of(ctx, rows, n)
+    if weight.device != ctx.device:
+        raise ValueError(f"weight: on cuda:{weight.device}, the context is on cuda:{ctx.device}")
+    if weight.cols != rows.cols:
+        raise ValueError(f"rows of {rows.cols} values, a weight of {weight.cols}")
+    if n:
+        ctx._check("g4_nvfp4_matmul", LIB.g4_nvfp4_matmul(ctx.handle, rows.desc, n, weight.desc, *oa, out.dtype == _F32))
+
+
+def beam_select(ctx: Context, logits, scores, out_scores, out_beams, out_tokens) -> None:
+    """Each group's best continuations (g4_beam_select): logits bf16 [groups, beams, vocab] over any
+    strides with a contiguous last dimension, scores f32 [groups, beams] (-inf: the beam does not
+    count); out_scores f32, out_beams and out_tokens int32 [groups, select], best first, equal scores
+    in the order of (beam, token)."""
+    groups, beams, vocab = _tensor(ctx, "logits", logits, (_BF16,), 3).shape
+    if vocab > 1 and logits.stride(2) != 1:
+        raise ValueError("logits: the last dimension must be contiguous")
+    given = _whole(ctx, "scores", scores, (groups, beams), (_F32,))
+    select = _tensor(ctx, "out_scores", out_scores, (_F32,), 2).shape[1]
+    outs = (_whole(ctx, "out_scores", out_scores, (groups, select), (_F32,)),
+            _whole(ctx, "out_beams", out_beams, (groups, select), (_I32,)),
+            _whole(ctx, "out_tokens", out_tokens, (groups, select), (_I32,)))
+    if not 1 <= beams <= BEAM_MAX or not 1 <= select <= BEAM_MAX or not 1 <= vocab <= 2 ** 20 or select > beams * vocab:
+        raise ValueError(f"{select} of {beams} beams of {vocab} tokens: expected up to {BEAM_MAX} of up to {BEAM_MAX} beams of up "
+                         "to 2^20 tokens, no more than there are")
+    if groups:
+        ctx._check("g4_beam_select", LIB.g4_beam_select(
+            ctx.handle, logits.data_ptr(), logits.stride(0), logits.stride(1), given, groups, beams, vocab, select, *outs))
+
+
+__all__ = ["Nvfp4Rows", "Nvfp4Weight", "embed_tokens", "residual_norm", "nvfp4_quantize", "nvfp4_dequantize",
+           "nvfp4_matmul", "beam_select"]

@@ -51,6 +51,7 @@ LIB.g4_page_pool_last_error.restype = ctypes.c_char_p
 LIB.g4_page_pool_add.argtypes = [_vp, _p_i32]
 LIB.g4_page_pool_extend.argtypes = [_vp, _i32, _i32]
 LIB.g4_page_pool_fork.argtypes = [_vp, _i32, _p_i32]
+LIB.g4_page_pool_reorder.argtypes = [_vp, _p_i32, _p_i32, _i32]
 LIB.g4_page_pool_trim.argtypes = [_vp, _i32, _i32]
 LIB.g4_page_pool_free.argtypes = [_vp, _i32]
 LIB.g4_page_pool_compact.argtypes = [_vp, _p_i32, _p_i32, _p_i32, _p_i32]
@@ -301,6 +302,16 @@ class PagePool:
         self._check("g4_page_pool_fork", LIB.g4_page_pool_fork(
             self.handle, _int32("seq", seq), ctypes.byref(s)))
         return s.value
+
+    def reorder(self, seqs, parents) -> None:
+        """Every seqs[i] becomes a copy of what parents[i] was, all at once and without moving a row:
+        the pages are shared as by a fork (g4_page_pool_reorder).  For beams: parents[i] is the
+        sequence of the beam that beam i continues."""
+        a, b = ([_int32(name, s) for s in x] for name, x in (("seqs", seqs), ("parents", parents)))
+        if len(a) != len(b):
+            raise ValueError("seqs and parents differ in length")
+        self._check("g4_page_pool_reorder", LIB.g4_page_pool_reorder(
+            self.handle, (_i32 * len(a))(*a), (_i32 * len(b))(*b), len(a)))
 
     def trim(self, seq: int, first_row: int) -> None:
         """Gives back the pages wholly below row first_row (below a sliding window)."""

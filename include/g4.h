@@ -454,6 +454,10 @@ g4_status g4_page_pool_fork(g4_page_pool* pool, int32_t seq, int32_t* out_child)
  * table entries become -1. */
 g4_status g4_page_pool_trim(g4_page_pool* pool, int32_t seq, int first_row);
 g4_status g4_page_pool_free(g4_page_pool* pool, int32_t seq);
+/* Beam search's reordering: seqs[i] becomes a copy of what parents[i] was (pages shared as by
+ * a fork), all at once, i < n; the seqs are different ones and keep their numbers.  Pages that no
+ * sequence holds any more are free again. */
+g4_status g4_page_pool_reorder(g4_page_pool* pool, const int32_t* seqs, const int32_t* parents, int n);
 /* Moves the pages in use to 0 .. n_used - 1: n moves src[i] -> dst[i] (arrays of n_pages) and
  * page_map[n_pages] for g4_paged_compact, all in HOST memory.  Refused while copies wait. */
 g4_status g4_page_pool_compact(g4_page_pool* pool, int32_t* src, int32_t* dst, int32_t* page_map, int* out_n);
@@ -466,6 +470,95 @@ g4_status g4_page_pool_take_copies(g4_page_pool* pool, int32_t* src, int32_t* ds
  * `width` is G4_ERR_TOO_LARGE, with *out_rows set all the same: its width follows from the rows. */
 g4_status g4_page_pool_table(const g4_page_pool* pool, int32_t seq, int32_t* table, int width, int* out_rows);
 g4_status g4_page_pool_free_pages(const g4_page_pool* pool, int* out_n);
+
+/* ------------------------------------------------------------------------------ */
+/* Around the attention of a batch: embedding rows, NVFP4 projections of many rows,   */
+/* residual norm, beam selection (no counterpart in the reference: one position per    */
+/* dispatch, src/host/generate.rs:194)                                                  */
+/* ------------------------------------------------------------------------------ */
+
+/* Common to these: bf16 matrices of any row stride (in elements, a multiple of 8, rows not
+ * overlapping where they are written) from 16-byte aligned addresses; calls of no rows do
+ * nothing; sums and statistics in f32 or more, one rounding to bf16 at the end. */
+
+/* ops::embed_token (src/ops.rs:9-36) for n_tokens ids: out[t] = bf16(table[tokens[t]] * scale),
+ * table [vocab, dim] contiguous, dim a multiple of 8, tokens DEVICE int32.  The model's scale is
+ * G4_EMBED_SCALE (bf16(sqrt(H))).  An id outside 0..vocab - 1 gives zeros and sets a bit in the
+ * device status word. */
+#define G4_EMBED_SCALE 62.0f
+g4_status g4_embed_tokens(g4_ctx* ctx, const g4_bf16* table, int vocab, int dim, const int32_t* tokens, int n_tokens,
+                          float scale, g4_bf16* out, int64_t out_stride);
+
+/* out[t] = bf16(residual[t] + x[t] * r * rms_weight), r = 1 / sqrt(mean(x[t]^2) + 1e-6), for n_rows
+ * rows of dim (a multiple of 8 up to 16384): what {sliding,full}_attention_output do after their
+ * product (src/ops.rs:138-158), computed in f32 and rounded once, where the single-token entry
+ * points round after each step.  out may be residual or x. */
+g4_status g4_residual_norm(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, const g4_bf16* rms_weight,
+                           const g4_bf16* residual, int64_t residual_stride, int n_rows, int dim, g4_bf16* out,
+                           int64_t out_stride);
+
+/* Scale blocks: the E4M3 scales of a [rows, cols] NVFP4 matrix in the order the tensor cores read
+ * them.  The scale of row r, columns 16 j .. 16 j + 15, is byte
+ *   ((r / 128) * ceil(cols / 64) + j / 4) * 512 + (r % 32) * 16 + (r % 128 / 32) * 4 + j % 4;
+ * g4_nvfp4_scale_bytes(rows, cols) bytes in all, 16-byte aligned. */
+uint64_t g4_nvfp4_scale_bytes(int rows, int cols);
+/* A checkpoint's block scales [rows, cols / 16] in that order (zeros past the matrix): once per weight. */
+g4_status g4_nvfp4_scale_blocks(g4_ctx* ctx, const g4_f8e4m3* block_scale, int rows, int cols, g4_f8e4m3* out);
+
+/* Rows of activations in NVFP4, as 1 to 3 pieces that add up:
+ *   x[m][k] ~= factor[m] * sum_p e2m1(codes[p][m][k]) * e4m3(scale of piece p, row m, k / 16)
+ * codes [pieces][max_rows][cols / 2], scales [pieces] times scale blocks of [max_rows, cols],
+ * factor [max_rows]; cols a multiple of 32 up to 16384.  Calls take rows 0 .. n_rows - 1 of it. */
+typedef struct g4_nvfp4_rows {
+  g4_f4x2* codes;
+  g4_f8e4m3* scales;
+  float* factor;
+  int32_t max_rows, cols, pieces;
+} g4_nvfp4_rows;
+/* A weight [rows, cols]: codes as the checkpoint has them (the row length of g4_nvfp4_rows, so a
+ * matrix quantised as one piece is one too), scale blocks, and n_factors = 1 (the checkpoint's
+ * reciprocal global scale) or = rows f32 factors (several projections stacked, or quantised rows). */
+typedef struct g4_nvfp4_weight {
+  const g4_f4x2* codes;
+  const g4_f8e4m3* scales;
+  const float* factor;
+  int32_t rows, cols, n_factors;
+} g4_nvfp4_weight;
+
+/* x [n_rows, cols] into `out`.  rms_weight (or NULL): x = bf16(x * r * rms_weight) first, r as in
+ * g4_residual_norm.  Per row, with g the largest power of two up to 2^126 with max|x| * g <= 2688
+ * (6 * 448): y_0 = x * g, and piece p = 0, 1, ..
+ *   s_p = e4m3(max over 16 of |y_p| / 6),  c_p = e2m1(y_p / s_p),  y_{p+1} = y_p - c_p * s_p;
+ * factor = 1 / g.  Roundings are to nearest, ties to even; everything else is exact, so a row's
+ * pieces do not depend on what computes them.  One piece leaves ~10 % of a value, two ~1 %, three
+ * ~0.1 %.  A row of zeros: factor 0; a row with an infinity or a NaN: factor NaN (codes 0), so
+ * that its products are NaN. */
+g4_status g4_nvfp4_quantize(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, int n_rows, const g4_bf16* rms_weight,
+                            const g4_nvfp4_rows* out);
+/* The values `rows` stands for, rounded to bf16: out [n_rows, cols]. */
+g4_status g4_nvfp4_dequantize(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, g4_bf16* out, int64_t out_stride);
+
+/* out[m][n] = rows.factor[m] * weight.factor[n] * sum_k rows[m][k] * weight[n][k] on the
+ * block-scaled FP4 tensor cores, f32 sums: out [n_rows, weight.rows] bf16, or f32 if out_f32 (the
+ * partial sums of a tensor-parallel rank's K-slice, which the ranks add before they round).
+ * n_rows up to 2^22.  Under tensor parallelism a rank passes its rows or its K-slice of the
+ * weight; nothing is exchanged. */
+g4_status g4_nvfp4_matmul(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, const g4_nvfp4_weight* weight, void* out,
+                          int64_t out_stride, int out_f32);
+
+/* Beam search's selection: per group the n_select best continuations of its n_beams beams,
+ *   s(beam, token) = scores[group][beam] + logits[group][beam][token] - log sum_token exp(logits),
+ * best first, equal scores in the order of (beam, token).  logits: row (group, beam) at element
+ * group * group_stride + beam * beam_stride, `vocab` entries, any alignment; scores
+ * [n_groups, n_beams] f32; out_scores f32, out_beams and out_tokens int32 [n_groups, n_select].
+ * Scores are compared before they are rounded (sums in 64 bits).  A beam whose score is not finite,
+ * or whose logits hold a NaN or +inf or nothing but -inf, has only continuations of score -inf (-inf as
+ * a score is how a beam that does not count is passed).  n_beams and n_select up to 64, vocab
+ * up to 2^20, n_select <= n_beams * vocab. */
+#define G4_BEAM_MAX 64
+g4_status g4_beam_select(g4_ctx* ctx, const g4_bf16* logits, int64_t group_stride, int64_t beam_stride,
+                         const float* scores, int n_groups, int n_beams, int vocab, int n_select, float* out_scores,
+                         int32_t* out_beams, int32_t* out_tokens);
 
 /* ------------------------------------------------------------------------------ */
 /* Decode runtime (src/host/load.rs Model, src/host/runtime.rs Workspace / Decode)  */

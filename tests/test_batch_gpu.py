@@ -1,0 +1,490 @@
+"""The operators around a batch's attention on the GPU against the float64 oracle.
+
+Error bounds, from the arithmetic the operators document (u = 2^-8: rounding to bf16 is off by at most
+half a step, 2^-8 of the value; f32 2^-24):
+  quantize, dequantize, embed   roundings of exact values: equal
+  matmul      products of codes and scales are exact; the tensor cores add 64 of them at a time to an f32
+              sum and may cut what they add below the sum's last bit (2^-23 of the sum of magnitudes S
+              for each of pieces * k / 64 additions, which join up to 8 parts), two factors:
+              |error| <= (pieces * k / 64 + 12) 2^-23 S, and u |y| more for bf16
+  norm        f32: x r w to 2^-21 of itself (sum of squares, root, two products), the sum to 2^-24, one
+              rounding to bf16: |error| <= u |y| + 2^-20 (|residual| + |x r w|)
+  beam        scores: f32 exponentials (2^-21 each, ~2^-21 of the sum), 64-bit sums, one rounding
+"""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import g4b200 as g4
+from oracle import batch as ob
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -8
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g, *shape, std=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * std).bfloat16()
+
+
+def _sync(ctx):
+    torch.cuda.synchronize()
+    assert ctx.poll() == 0
+
+
+def _rows(ctx, n, cols, pieces, seed=0, spread=2.0):
+    """Quantised rows from random codes and scales of every size, laid out by the oracle, in a buffer whose
+    other bytes are NaN scales and codes of 6; with the values and factors."""
+    g = _gen(seed)
+    room = n + 3
+    r = g4.Nvfp4Rows(ctx, room, cols, pieces)
+    for t, v in ((r.codes, 0xFF), (r.scales, 0x7F)):
+        t.fill_(v)
+    r.factor.fill_(float("nan"))
+    codes = torch.randint(0, 16, (pieces, n, cols), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.randn((pieces, n, cols // 16), generator=g, device="cuda") * 8 * spread + 56).clamp(0, 126).byte()
+    factor = torch.exp2(torch.randint(-8, 3, (n,), generator=g, device="cuda").float())
+    r.codes[:, :n] = ob.pack(codes)
+    b = torch.arange(cols // 16, device="cuda")[None, :]
+    at = ob.scale_at(torch.arange(n, device="cuda")[:, None], b, cols)
+    for p in range(pieces):
+        r.scales[p][at] = scales[p]
+        if cols % 64:  # columns past the row's end count as zeros
+            r.scales[p][ob.scale_at(torch.arange(n, device="cuda")[:, None], b.new_tensor([[cols // 16, cols // 16 + 1]]), cols)] = 0
+    r.factor[:n] = factor
+    return r, ob.values(codes, scales).sum(0), factor.double()
+
+
+def _weight(ctx, n, cols, factors=1, seed=1):
+    g = _gen(seed)
+    codes = torch.randint(0, 16, (n, cols), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.randn((n, cols // 16), generator=g, device="cuda") * 12 + 56).clamp(0, 126).byte()
+    factor = torch.rand(factors, generator=g, device="cuda") + 0.01
+    return g4.Nvfp4Weight(ctx, ob.pack(codes), scales, factor), ob.values(codes, scales), factor.double()
+
+
+def _product(ctx, m, n, cols, pieces, f32=False, gap=0, factors=1, seed=0):
+    rows, xv, fx = _rows(ctx, m, cols, pieces, seed)
+    weight, wv, fw = _weight(ctx, n, cols, factors, seed + 1)
+    wide = torch.full((m, (n + 7) // 8 * 8 + gap), 7.0, dtype=torch.float32 if f32 else torch.bfloat16, device="cuda")
+    out = wide[:, :n]
+    if (n + 7) // 8 * 8 + gap != n and m == 1:
+        out = wide.as_strided((1, n), (wide.shape[1], 1))
+    g4.nvfp4_matmul(ctx, rows, weight, out)
+    _sync(ctx)
+    want, size = ob.matmul(xv, wv, fx, fw)
+    bound = (pieces * cols / 64 + 12) * 2.0 ** -23 * size + (0 if f32 else U * want.abs())
+    assert torch.isfinite(out).all()
+    worst = ((out.double() - want).abs() - bound).max().item()
+    assert worst <= 0, f"error above its bound by {worst}"
+    assert (wide[:, n:] == 7.0).all()
+    return out
+
+
+SHAPES = [
+    # m, n, cols, pieces
+    (1, 1, 32, 1), (1, 8, 64, 2), (2, 7, 96, 3), (3, 130, 160, 1), (1, 8192, 3840, 2), (5, 515, 3840, 3), (16, 128, 512, 2),
+    (17, 256, 512, 1), (31, 129, 480, 2), (32, 3840, 4096, 2), (33, 257, 1056, 3), (64, 640, 1920, 2), (65, 300, 704, 1),
+    (127, 384, 256, 2), (128, 128, 128, 1), (129, 1000, 992, 2), (255, 511, 3840, 1), (256, 256, 256, 3), (257, 513, 320, 2),
+    (300, 3840, 1024, 2), (509, 1088, 3840, 2), (513, 777, 2080, 3), (1024, 2048, 512, 1), (1111, 512, 3840, 2),
+    (700, 3840, 15360, 1), (2, 3840, 15360, 3), (1300, 4096, 96, 2),
+]
+
+
+@pytest.mark.parametrize("m, n, cols, pieces", SHAPES)
+def test_matmul(gpu_ctx, m, n, cols, pieces):
+    _product(gpu_ctx, m, n, cols, pieces)
+
+
+@pytest.mark.parametrize("m, n, cols, pieces", [(1, 515, 3840, 2), (33, 129, 480, 3), (257, 520, 1056, 1), (640, 300, 3840, 2)])
+def test_matmul_f32_strides_and_factors(gpu_ctx, m, n, cols, pieces):
+    """f32 sums, rows apart (what lies between them is left alone), a factor for every row of the weight."""
+    _product(gpu_ctx, m, n, cols, pieces, f32=True, gap=24, factors=n, seed=5)
+    _product(gpu_ctx, m, n, cols, pieces, f32=False, gap=8, factors=n, seed=6)
+
+
+def test_matmul_is_the_same_for_a_row_alone(gpu_ctx):
+    """A row's sums do not hang on which rows are beside it as long as the same kernel takes them, and
+    repeated calls give the same bits."""
+    rows, _, _ = _rows(gpu_ctx, 600, 1920, 2)
+    weight, _, _ = _weight(gpu_ctx, 1000, 1920)
+    a, b = (torch.empty((600, 1000), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    g4.nvfp4_matmul(gpu_ctx, rows, weight, a)
+    g4.nvfp4_matmul(gpu_ctx, rows, weight, b)
+    _sync(gpu_ctx)
+    assert torch.equal(a, b)
+
+
+def test_matmul_nan_row_stays_in_its_row(gpu_ctx):
+    x = _randn(_gen(3), 140, 512)
+    x[7, 100], x[131, 0], x[20] = float("nan"), float("inf"), 0
+    rows = g4.Nvfp4Rows(gpu_ctx, 140, 512)
+    weight, _, _ = _weight(gpu_ctx, 384, 512)
+    out = torch.empty((140, 384), dtype=torch.bfloat16, device="cuda")
+    g4.nvfp4_quantize(gpu_ctx, x, rows)
+    g4.nvfp4_matmul(gpu_ctx, rows, weight, out)
+    _sync(gpu_ctx)
+    bad = torch.zeros(140, dtype=torch.bool, device="cuda")
+    bad[[7, 131]] = True
+    assert out[bad].isnan().all() and torch.isfinite(out[~bad]).all() and (out[20] == 0).all()
+
+
+def test_quantised_rows_are_a_weight(gpu_ctx):
+    g = _gen(9)
+    a, b = _randn(g, 70, 768), _randn(g, 200, 768, std=0.02)
+    ra, rb = g4.Nvfp4Rows(gpu_ctx, 70, 768, 2), g4.Nvfp4Rows(gpu_ctx, 200, 768, 1)
+    out = torch.empty((70, 200), dtype=torch.float32, device="cuda")
+    g4.nvfp4_quantize(gpu_ctx, a, ra)
+    g4.nvfp4_quantize(gpu_ctx, b, rb)
+    g4.nvfp4_matmul(gpu_ctx, ra, g4.Nvfp4Weight.from_rows(rb), out)
+    _sync(gpu_ctx)
+    ca, sa, fa = ob.quantize(a, 2)
+    cb, sb, fb = ob.quantize(b, 1)
+    want, size = ob.matmul(ob.values(ca, sa).sum(0), ob.values(cb, sb)[0], fa, fb)
+    assert ((out.double() - want).abs() <= (2 * 768 / 64 + 12) * 2.0 ** -23 * size).all()
+
+
+# ------------------------------------------------------------------------------ quantise
+def _check_rows(rows, want, n, cols):
+    codes, scales, factor = want
+    assert torch.equal(rows.codes[:, :n], ob.pack(codes))
+    for p in range(rows.pieces):
+        at = ob.scale_at(torch.arange(n, device="cuda")[:, None], torch.arange(cols // 16, device="cuda")[None, :], cols)
+        assert torch.equal(rows.scales[p][at], scales[p])
+        pad = [b for b in range(cols // 16, -(-cols // 64) * 4)]
+        if pad:
+            at = ob.scale_at(torch.arange(n, device="cuda")[:, None], torch.tensor([pad], device="cuda"), cols)
+            assert (rows.scales[p][at] == 0).all()
+    assert torch.equal(rows.factor[:n].double().nan_to_num(-1.0), factor.nan_to_num(-1.0))
+
+
+@pytest.mark.parametrize("n, cols, pieces", [(1, 32, 1), (1, 3840, 2), (3, 96, 3), (130, 480, 2), (257, 2048, 3), (40, 2080, 1),
+                                             (65, 8192, 2), (9, 15360, 3), (300, 16384, 1)])
+@pytest.mark.parametrize("gap", [0, 8])
+def test_quantize_is_the_oracles(gpu_ctx, n, cols, pieces, gap):
+    x = _randn(_gen(n + cols), n, cols + gap)
+    x *= torch.exp2(torch.randint(-30, 30, (n, 1), generator=_gen(1), device="cuda")).bfloat16()
+    x = x[:, :cols]
+    rows = g4.Nvfp4Rows(gpu_ctx, n + 5, cols, pieces)
+    for t in (rows.codes, rows.scales):
+        t.fill_(0xA5)
+    rows.factor.fill_(-3.0)
+    g4.nvfp4_quantize(gpu_ctx, x, rows)
+    out = torch.full((n, cols + gap), 7.0, dtype=torch.bfloat16, device="cuda")
+    g4.nvfp4_dequantize(gpu_ctx, rows, out[:, :cols])
+    _sync(gpu_ctx)
+    want = ob.quantize(x, pieces)
+    _check_rows(rows, want, n, cols)
+    assert (rows.codes[:, n:] == 0xA5).all() and (rows.factor[n:] == -3.0).all()
+    last = ob.scale_at(torch.arange(n, n + 5, device="cuda")[:, None], torch.arange(cols // 16, device="cuda")[None, :], cols)
+    assert all((rows.scales[p][last] == 0xA5).all() for p in range(pieces))
+    assert torch.equal(out[:, :cols].double(), (ob.values(want[0], want[1]).sum(0) * want[2][:, None]).bfloat16().double())
+    assert (out[:, cols:] == 7.0).all()
+
+
+@pytest.mark.parametrize("n, cols", [(1, 3840), (50, 3840), (7, 96), (20, 8192), (5, 16384)])
+def test_quantize_normed(gpu_ctx, n, cols):
+    """The codes are those of the normed rows rounded to bf16: of the f32 products in their order, with a
+    root from 64-bit sums."""
+    g = _gen(n * cols)
+    x, w = _randn(g, n, cols, std=3.0), (1 + 0.3 * torch.randn(cols, generator=g, device="cuda")).bfloat16()
+    x[0] *= 1e-3
+    rows = g4.Nvfp4Rows(gpu_ctx, n, cols, 2)
+    g4.nvfp4_quantize(gpu_ctx, x, rows, w)
+    _sync(gpu_ctx)
+    r = (1 / (x.double().square().mean(1, keepdim=True) + ob.EPS).sqrt()).float()
+    y = (x.float() * r * w.float()).bfloat16()
+    _check_rows(rows, ob.quantize(y, 2), n, cols)
+    exact = ob.rms(x, w)
+    assert ((y.double() - exact).abs() <= (U + 2.0 ** -20) * exact.abs() + 2.0 ** -130).all()
+
+
+def test_quantize_special_rows(gpu_ctx):
+    """Rows of zeros, of the smallest and the largest numbers, ties of both roundings, infinities and NaN."""
+    x = torch.zeros((14, 64), dtype=torch.bfloat16, device="cuda")
+    x[1, 5] = 2.0 ** -133
+    x[2] = _randn(_gen(1), 64) * 2.0 ** -126
+    x[3, :] = torch.finfo(torch.bfloat16).max
+    x[4, 0], x[4, 17] = torch.finfo(torch.bfloat16).max, 2.0 ** -133
+    x[5, :8] = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    x[5, 8:16] = -x[5, :8]
+    x[6, ::16] = torch.tensor([2688.0, 2688 / 2, 204.0, 6 * 17 / 16])  # scale ties
+    x[7, 0], x[8, 63], x[9, 2] = float("inf"), -float("inf"), float("nan")
+    x[10, 0], x[11, 0] = 42.0, 42.25  # either side of 2688 / 64
+    x[12] = -0.0
+    x[13, 0], x[13, 16:] = 1.0, 2.0 ** -20
+    for pieces in (1, 3):
+        rows = g4.Nvfp4Rows(gpu_ctx, 14, 64, pieces)
+        g4.nvfp4_quantize(gpu_ctx, x, rows)
+        out = torch.empty_like(x)
+        g4.nvfp4_dequantize(gpu_ctx, rows, out)
+        _sync(gpu_ctx)
+        codes, scales, factor = ob.quantize(x, pieces)
+        _check_rows(rows, (codes, scales, factor), 14, 64)
+        assert out[7:10].isnan().all() and (out[12] == 0).all()
+        # one piece of bf16's largest number is past it: max g = 2040, 340 rounds to the scale 352, and 6 of
+        # these are 2112 (read back as inf: there is no bf16 for it)
+        want = (ob.values(codes, scales).sum(0) * factor[:, None]).bfloat16()
+        assert torch.equal(out.nan_to_num(1.0, 2.0, 3.0), want.nan_to_num(1.0, 2.0, 3.0))
+
+
+def test_scale_blocks(gpu_ctx):
+    for n, cols in ((1, 32), (130, 96), (300, 3840)):
+        s = torch.randint(0, 127, (n, cols // 16), generator=_gen(n), device="cuda", dtype=torch.uint8)
+        w = g4.Nvfp4Weight(gpu_ctx, torch.zeros((n, cols // 2), dtype=torch.uint8, device="cuda"), s.view(torch.float8_e4m3fn),
+                           torch.ones(1, device="cuda"))
+        _sync(gpu_ctx)
+        assert torch.equal(w.scales, ob.scale_blocks(s))
+
+
+# ------------------------------------------------------------------------------ rows
+@pytest.mark.parametrize("n, vocab, dim, gap", [(1, 262144, 3840, 0), (1, 1, 8, 0), (300, 1000, 3840, 8), (7, 50, 24, 0),
+                                                (513, 33, 8192, 16), (4096, 262144, 64, 0)])
+def test_embed(gpu_ctx, n, vocab, dim, gap):
+    g = _gen(n + dim)
+    table = _randn(g, vocab, dim)
+    ids = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    ids[0], ids[-1] = vocab - 1, 0
+    wide = torch.full((n, dim + gap), 7.0, dtype=torch.bfloat16, device="cuda")
+    for scale in (62.0, 0.3):
+        g4.embed_tokens(gpu_ctx, table, ids, wide[:, :dim], scale)
+        _sync(gpu_ctx)
+        assert torch.equal(wide[:, :dim], (table[ids.long()].float() * scale).bfloat16())
+        assert (wide[:, dim:] == 7.0).all()
+
+
+def test_embed_ids_outside_the_table(gpu_ctx):
+    table = torch.full((10, 16), float("inf"), dtype=torch.bfloat16, device="cuda")
+    ids = torch.tensor([3, -1, 10, 2 ** 31 - 1, -2 ** 31, 9], dtype=torch.int32, device="cuda")
+    out = torch.full((6, 16), 7.0, dtype=torch.bfloat16, device="cuda")
+    g4.embed_tokens(gpu_ctx, table, ids, out)
+    with pytest.raises(g4.G4Error):
+        gpu_ctx.poll()
+    assert gpu_ctx.poll() == 0
+    assert (out[1:5] == 0).all() and out[[0, 5]].isinf().all()
+
+
+def test_embed_past_32_bits(gpu_ctx):
+    """Rows beyond 2^31 elements of the table."""
+    vocab, dim = 2 ** 18, 8448  # 2^31.04 elements
+    table = torch.zeros((vocab, dim), dtype=torch.bfloat16, device="cuda")
+    table[-1], table[0] = 3.0, 1.0
+    out = torch.empty((2, dim), dtype=torch.bfloat16, device="cuda")
+    g4.embed_tokens(gpu_ctx, table, torch.tensor([vocab - 1, 0], dtype=torch.int32, device="cuda"), out, 2.0)
+    _sync(gpu_ctx)
+    assert (out[0] == 6.0).all() and (out[1] == 2.0).all()
+
+
+@pytest.mark.parametrize("n, dim, gap", [(1, 3840, 0), (1, 8, 0), (33, 3840, 8), (300, 24, 0), (5, 1032, 16), (64, 8192, 0), (9, 16384, 8)])
+def test_residual_norm(gpu_ctx, n, dim, gap):
+    g = _gen(n * dim)
+    x, res = _randn(g, n, dim + gap, std=4.0)[:, :dim], _randn(g, n, dim + gap)[:, :dim]
+    w = (1 + 0.3 * torch.randn(dim, generator=g, device="cuda")).bfloat16()
+    x[0] *= 2.0 ** -20
+    out = torch.full((n, dim + gap), 7.0, dtype=torch.bfloat16, device="cuda")
+    g4.residual_norm(gpu_ctx, x, w, res, out[:, :dim])
+    _sync(gpu_ctx)
+    y = ob.rms(x, w)
+    want = res.double() + y
+    assert ((out[:, :dim].double() - want).abs() <= U * want.abs() + 2.0 ** -20 * (res.double().abs() + y.abs())).all()
+    assert (out[:, dim:] == 7.0).all()
+    for given, into in ((res.clone(), "residual"), (x.clone(), "x")):  # in place of either operand
+        a, b = (x, given) if into == "residual" else (given, res)
+        g4.residual_norm(gpu_ctx, a, w, b, given)
+        _sync(gpu_ctx)
+        assert torch.equal(given, out[:, :dim])
+
+
+def test_residual_norm_zero_and_nan_rows(gpu_ctx):
+    x = torch.zeros((3, 128), dtype=torch.bfloat16, device="cuda")
+    x[1, 5] = float("nan")
+    res = _randn(_gen(2), 3, 128)
+    out = torch.empty_like(res)
+    g4.residual_norm(gpu_ctx, x, torch.ones(128, dtype=torch.bfloat16, device="cuda"), res, out)
+    _sync(gpu_ctx)
+    assert torch.equal(out[[0, 2]], res[[0, 2]]) and out[1].isnan().all()
+
+
+# ------------------------------------------------------------------------------ beams
+def _select(ctx, logits, scores, k):
+    groups = logits.shape[0]
+    out = (torch.full((groups, k), 7.0, device="cuda"), *(torch.full((groups, k), -7, dtype=torch.int32, device="cuda") for _ in range(2)))
+    g4.beam_select(ctx, logits, scores, *out)
+    _sync(ctx)
+    return out
+
+
+def _check_beams(ctx, logits, scores, k):
+    got, beams, tokens = _select(ctx, logits, scores, k)
+    want, wb, wt = ob.beam_select(logits, scores, k)
+    finite = torch.isfinite(want)
+    assert torch.equal(beams.long(), wb) and torch.equal(tokens.long(), wt)
+    assert torch.equal(finite, torch.isfinite(got)) and (got[~finite] == -math.inf).all()
+    err = (got.double() - want)[finite].abs()
+    assert (err <= 2.0 ** -20 + 2.0 ** -24 * want[finite].abs()).all()
+
+
+@pytest.mark.parametrize("groups, beams, vocab, k", [
+    (1, 1, 1, 1), (1, 1, 5, 5), (2, 3, 7, 21), (1, 4, 262144, 8), (32, 4, 262144, 8), (3, 1, 262144, 64), (1, 64, 32003, 64),
+    (5, 8, 4097, 16), (2, 64, 1000, 64), (1, 3, 2 ** 20, 7), (1, 64, 2 ** 20, 64), (700, 2, 333, 4), (9, 5, 65537, 3), (1, 2, 40, 64)])
+def test_beam_select(gpu_ctx, groups, beams, vocab, k):
+    g = _gen(groups + vocab)
+    logits = _randn(g, groups, beams, vocab, std=3.0)
+    scores = -10 * torch.rand((groups, beams), generator=g, device="cuda")
+    _check_beams(gpu_ctx, logits, scores, k)
+
+
+def test_beam_select_strides(gpu_ctx):
+    g = _gen(4)
+    wide = _randn(g, 3, 5, 1100, std=3.0)
+    scores = torch.rand((3, 4), generator=g, device="cuda")
+    for logits in (wide[:, 1:, 3:1004], wide[:, :4, 1:].transpose(0, 1)[:3, :3].contiguous().transpose(0, 1), wide[:, ::2, 5:900]):
+        _check_beams(gpu_ctx, logits, scores[:, :logits.shape[1]].contiguous(), 6)
+
+
+def test_beam_select_a_new_request(gpu_ctx):
+    """All beams hold the prompt, only the first counts; one beam in all, none at all."""
+    logits = _randn(_gen(5), 1, 1, 3000).expand(3, 4, 3000)
+    scores = torch.full((3, 4), -math.inf, device="cuda")
+    scores[0, 0], scores[1, 2] = 0.0, -3.5
+    _check_beams(gpu_ctx, logits, scores, 8)
+    got, beams, tokens = _select(gpu_ctx, logits, scores, 8)
+    assert (beams[0] == 0).all() and (beams[1] == 2).all() and (beams[2] == 0).all()
+    assert (got[2] == -math.inf).all() and tokens[2].tolist() == list(range(8))
+
+
+def test_beam_select_equal_scores(gpu_ctx):
+    """Constant logits, identical beams, few different values: the lowest (beam, token) first."""
+    flat = torch.full((1, 4, 262144), 1.5, dtype=torch.bfloat16, device="cuda")
+    _check_beams(gpu_ctx, flat, torch.zeros((1, 4), device="cuda"), 64)
+    _check_beams(gpu_ctx, flat[..., :77], torch.tensor([[-1.0, 0.0, 0.0, -1.0]], device="cuda"), 64)
+    few = torch.randint(0, 3, (2, 3, 50000), generator=_gen(6), device="cuda").bfloat16()
+    few[:, 1] = few[:, 0]
+    _check_beams(gpu_ctx, few, torch.zeros((2, 3), device="cuda"), 60)
+    # the best ones side by side: all in a few threads' parts
+    peak = _randn(_gen(7), 1, 2, 60000)
+    peak[0, 0, 1024:65536:256] = 20.0
+    peak[0, 1, 512:576] = 25.0
+    _check_beams(gpu_ctx, peak, torch.zeros((1, 2), device="cuda"), 64)
+
+
+def test_beam_select_values_that_are_not_finite(gpu_ctx):
+    """Banned tokens (-inf); beams without any continuation: of +inf, NaN, -inf throughout, scores that are not
+    finite.  They come after every other, in the order of (beam, token)."""
+    logits = _randn(_gen(8), 4, 7, 500)
+    logits[:, 0, ::3] = -math.inf
+    logits[:, 1, 77] = math.nan
+    logits[:, 2, 5] = math.inf
+    logits[:, 3] = -math.inf
+    logits[:, 6, 10:] = -math.inf
+    scores = torch.zeros((4, 7), device="cuda")
+    scores[:, 4], scores[:, 5] = math.nan, math.inf
+    _check_beams(gpu_ctx, logits, scores, 64)
+    scores[1, 0], scores[2, 6], scores[3, [0, 6]] = -math.inf, math.nan, -math.inf
+    _check_beams(gpu_ctx, logits, scores, 64)
+
+
+def test_beam_select_scores_far_apart(gpu_ctx):
+    g = _gen(11)
+    logits = _randn(g, 2, 3, 2000, std=20.0)
+    _check_beams(gpu_ctx, logits, torch.tensor([[-1e4, 0.0, -2e3], [-900.0, -900.25, -899.5]], device="cuda"), 12)
+
+
+# ------------------------------------------------------------------------------ calls
+def test_calls_captured_and_replayed(gpu_ctx):
+    """Embed, quantise, multiply, norm and select in one graph, on a stream of the context's own; replays follow
+    their inputs."""
+    stream = torch.cuda.Stream()
+    ctx = g4.Context(0, stream=stream)
+    g = _gen(12)
+    table, w = _randn(g, 900, 512), torch.ones(512, dtype=torch.bfloat16, device="cuda")
+    x, y, z = (torch.zeros((40, 512), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    logits = torch.zeros((40, 1000), dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros(40, dtype=torch.int32, device="cuda")
+    scores = torch.zeros((10, 4), device="cuda")
+    outs = torch.zeros((10, 6), device="cuda"), *(torch.zeros((10, 6), dtype=torch.int32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    rows = g4.Nvfp4Rows(ctx, 40, 512)
+    square, head = _weight(ctx, 512, 512)[0], _weight(ctx, 1000, 512, seed=3)[0]
+
+    def step():
+        g4.embed_tokens(ctx, table, ids, x)
+        g4.nvfp4_quantize(ctx, x, rows, w)
+        g4.nvfp4_matmul(ctx, rows, square, y)
+        g4.residual_norm(ctx, y, w, x, z)
+        g4.nvfp4_quantize(ctx, z, rows)
+        g4.nvfp4_matmul(ctx, rows, head, logits)
+        g4.beam_select(ctx, logits.view(10, 4, 1000), scores, *outs)
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for i in range(3):
+        ids.copy_(torch.randint(0, 900, (40,), generator=g, device="cuda"))
+        scores.copy_(torch.rand((10, 4), generator=g, device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (logits, *outs)]
+        with torch.cuda.stream(stream):
+            step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (logits, *outs)))
+        assert got[0].float().std() > 0
+    assert ctx.poll() == 0
+    del graph
+    ctx.close()
+
+
+def test_library_refuses(gpu_ctx):
+    """The C entry points' own checks: sizes, alignment, strides, null pointers."""
+    L, h = g4.LIB, gpu_ctx.handle
+    t = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    p = t.data_ptr()
+    rows = lambda codes=p, scales=p, factor=p, m=4, cols=64, pieces=2: g4.batch._RowsDesc(codes, scales, factor, m, cols, pieces)  # noqa: E731
+    weight = lambda codes=p, scales=p, factor=p, n=8, cols=64, f=1: g4.batch._WeightDesc(codes, scales, factor, n, cols, f)  # noqa: E731
+    bad = [
+        L.g4_embed_tokens(h, p, 0, 8, p, 1, 1.0, p, 8), L.g4_embed_tokens(h, p, 4, 12, p, 1, 1.0, p, 16),
+        L.g4_embed_tokens(h, p, 4, 8, p + 2, 1, 1.0, p, 8), L.g4_embed_tokens(h, p + 2, 4, 8, p, 1, 1.0, p, 8),
+        L.g4_embed_tokens(h, p, 4, 8, p, 2, 1.0, p, 4), L.g4_embed_tokens(h, p, 4, 8, p, 2, 1.0, p, 12),
+        L.g4_embed_tokens(h, p, 4, 8, p, -1, 1.0, p, 8), L.g4_embed_tokens(h, p, 4, 8, None, 1, 1.0, p, 8),
+        L.g4_residual_norm(h, p, 8, p, p, 8, 2, 12, p, 16), L.g4_residual_norm(h, p, 4, p, p, 8, 2, 8, p, 8),
+        L.g4_residual_norm(h, p, 8, None, p, 8, 2, 8, p, 8), L.g4_residual_norm(h, p, 8, p, p, 8, -1, 8, p, 8),
+        L.g4_residual_norm(h, p, 32768, p, p, 32768, 1, 32768, p, 32768),
+        L.g4_nvfp4_scale_blocks(h, p, 4, 48, p), L.g4_nvfp4_scale_blocks(h, None, 4, 64, p), L.g4_nvfp4_scale_blocks(h, p, 4, 64, p + 4),
+        L.g4_nvfp4_quantize(h, p, 64, 5, None, rows()), L.g4_nvfp4_quantize(h, p, 64, 4, None, None),
+        L.g4_nvfp4_quantize(h, p, 64, 4, p + 2, rows()), L.g4_nvfp4_quantize(h, p + 2, 64, 4, None, rows()),
+        L.g4_nvfp4_quantize(h, p, 32, 4, None, rows()), L.g4_nvfp4_quantize(h, p, 64, 4, None, rows(pieces=4)),
+        L.g4_nvfp4_quantize(h, p, 64, 4, None, rows(cols=80)), L.g4_nvfp4_quantize(h, p, 64, 4, None, rows(scales=p + 4)),
+        L.g4_nvfp4_quantize(h, p, 64, 4, None, rows(codes=None)), L.g4_nvfp4_quantize(h, p, 64, 0, None, rows(m=0)),
+        L.g4_nvfp4_dequantize(h, rows(), 4, p, 32), L.g4_nvfp4_dequantize(h, rows(), 4, None, 64), L.g4_nvfp4_dequantize(h, rows(), -1, p, 64),
+        L.g4_nvfp4_matmul(h, rows(), 4, weight(cols=96), p, 8, 0), L.g4_nvfp4_matmul(h, rows(), 4, weight(f=2), p, 8, 0),
+        L.g4_nvfp4_matmul(h, rows(), 4, weight(n=0), p, 8, 0), L.g4_nvfp4_matmul(h, rows(), 4, None, p, 8, 0),
+        L.g4_nvfp4_matmul(h, rows(), 4, weight(), p, 4, 0), L.g4_nvfp4_matmul(h, rows(), 4, weight(), p, 12, 0),
+        L.g4_nvfp4_matmul(h, rows(), 4, weight(codes=p + 8), p, 8, 0), L.g4_nvfp4_matmul(h, rows(), 4, weight(factor=None), p, 8, 0),
+        L.g4_nvfp4_matmul(h, rows(), 4, weight(), None, 8, 0), L.g4_nvfp4_matmul(h, rows(), 5, weight(), p, 8, 0),
+        L.g4_beam_select(h, p, 9, 9, p, 1, 0, 9, 1, p, p, p), L.g4_beam_select(h, p, 9, 9, p, 1, 1, 9, 10, p, p, p),
+        L.g4_beam_select(h, p, 9, 9, p, 1, 65, 9, 1, p, p, p), L.g4_beam_select(h, p, 9, 9, p, 1, 2, 0, 1, p, p, p),
+        L.g4_beam_select(h, p, 9, 9, p, 1, 2, 2 ** 20 + 1, 1, p, p, p), L.g4_beam_select(h, p, 9, 9, p, -1, 2, 9, 1, p, p, p),
+        L.g4_beam_select(h, p + 1, 9, 9, p, 1, 2, 9, 1, p, p, p), L.g4_beam_select(h, p, 9, -9, p, 1, 2, 9, 1, p, p, p),
+        L.g4_beam_select(h, p, 9, 9, p + 2, 1, 2, 9, 1, p, p, p), L.g4_beam_select(h, p, 9, 9, p, 1, 2, 9, 1, p, p, None),
+    ]
+    assert bad == [1] * len(bad)
+    assert L.g4_ctx_last_error(h)
+    ok = [L.g4_embed_tokens(h, p, 4, 8, p, 0, 1.0, None, 0), L.g4_nvfp4_quantize(h, None, 0, 0, None, rows()),
+          L.g4_nvfp4_matmul(h, rows(), 0, weight(), None, 0, 0), L.g4_beam_select(h, None, 0, 0, None, 0, 2, 9, 1, None, None, None),
+          L.g4_residual_norm(h, None, 0, None, None, 0, 0, 8, None, 0), L.g4_nvfp4_scale_blocks(h, None, 0, 64, None)]
+    assert ok == [0] * len(ok)
+    _sync(gpu_ctx)
+    assert not t.any()
+    assert ctypes.sizeof(g4.batch._RowsDesc) == 40 and ctypes.sizeof(g4.batch._WeightDesc) == 40

@@ -1,54 +1,301 @@
-// Products of NVFP4 rows and weights:
+// Products of NVFP4 rows and weights on tcgen05 (kind::mxf4nvf4, E4M3 scales per 16):
 //   out[m][n] = fx[m] * fw[n] * sum_k (sum_p cx[p][m][k] sx[p][m][k / 16]) cw[n][k] sw[n][k / 16]
+//
+// Weight rows are the MMA's M, activation rows its N: a single token is a column block of 16 that
+// the tensor cores fill, and the pieces of a row are further MMAs into the same sums that share the
+// weight tile in shared memory.  Products of codes and scales are exact, sums f32.
+//
+// Scales go from shared to tensor memory by tcgen05.cp (32 lanes x 16 bytes, repeated in the four
+// lane quarters), which is why they are kept in blocks of 128 rows x 64 columns: a block is the 512
+// bytes of one such copy, and a stage's four blocks one contiguous copy from global memory.
+#include <string>
+
 #include "g4_nvfp4.cuh"
+#include "g4_paged_split.cuh"
 
 namespace g4 {
 
-// One warp per output: lanes take the 16-column blocks in turn.
-__global__ void __launch_bounds__(256) nv_matmul_kernel(const __grid_constant__ NvMatmulArgs a) {
-  const int lane = threadIdx.x & 31, n = blockIdx.y * 8 + (threadIdx.x >> 5), m = blockIdx.x;
-  pdl_wait();
-  if (n >= a.n) return;
-  const int nb = a.k / 16, kblocks = (a.k + 63) / 64;
-  float sum = 0.f;
-  for (int b = lane; b < nb; b += 32) {
-    const uint2 wc = *reinterpret_cast<const uint2*>(a.w_codes + static_cast<size_t>(n) * (a.k / 2) + 8 * b);
-    uint32_t w[8];
-    cvt_e2m1x8(wc.x, w[0], w[1], w[2], w[3]);
-    cvt_e2m1x8(wc.y, w[4], w[5], w[6], w[7]);
-    const float ws = e4m3_value(a.w_scales[nv_scale_at(n, b, kblocks)]);
-    for (int p = 0; p < a.pieces; ++p) {
-      const uint2 xc = *reinterpret_cast<const uint2*>(
-          a.x_codes + (static_cast<size_t>(p) * a.max_rows + m) * (a.k / 2) + 8 * b);
-      uint32_t x[8];
-      cvt_e2m1x8(xc.x, x[0], x[1], x[2], x[3]);
-      cvt_e2m1x8(xc.y, x[4], x[5], x[6], x[7]);
-      const float xs = e4m3_value(a.x_scales[p * nv_scale_bytes(a.max_rows, a.k) + nv_scale_at(m, b, kblocks)]);
-      float dot = 0.f;  // exact: 16 products of two small numbers
+constexpr int kNvStageK = 256;  // columns per ring stage: 128 bytes of codes, four scale blocks
+
+// ---------------------------------------------------------------------------- PTX
+__device__ __forceinline__ uint64_t nv_scale_desc(uint32_t addr) {  // 8-row groups of 128 bytes, no swizzle
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) |
+         (static_cast<uint64_t>(1u) << 46);
+}
+template <int kCtas>
+__device__ __forceinline__ void nv_cp_scales(uint32_t taddr, uint64_t desc) {
+  if (kCtas == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int kCtas>
+__device__ __forceinline__ void nv_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                       uint32_t acc) {
+  if (kCtas == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.block16 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.block16 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb)
+        : "memory");
+}
+__device__ __forceinline__ void nv_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void nv_tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void nv_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void nv_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  pa_ld_wait();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t q = hmul2_u32(w[e], x[e]);
-        dot += __half2float(__ushort_as_half(static_cast<uint16_t>(q))) +
-               __half2float(__ushort_as_half(static_cast<uint16_t>(q >> 16)));
-      }
-      sum = fmaf(dot, ws * xs, sum);
-    }
-  }
-  sum = warp_sum(sum);
-  if (lane == 0) {
-    const float v = sum * a.x_factor[m] * a.w_factor[a.n_factors > 1 ? n : 0];
-    const size_t at = static_cast<size_t>(m) * a.out_stride + n;
-    if (a.out_f32)
-      static_cast<float*>(a.out)[at] = v;
-    else
-      static_cast<uint16_t*>(a.out)[at] = f32_to_bf16(v);
-  }
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& args) {
-  NvMatmulArgs a = args;
-  void* p[] = {(void*)&a};
-  return launch_kernel(ctx, (const void*)nv_matmul_kernel, dim3(a.m, (a.n + 7) / 8), dim3(256), 0, p, false, "nvfp4 matmul");
+// ---------------------------------------------------------------------------- single CTAs
+// A tile is 128 weight rows x `cols` activation rows; a cluster of `splits` CTAs shares its K range, and
+// each CTA then adds up 128 / splits of the tile's rows, whose parts the others stored into its
+// shared memory (in the cluster's order: no result hangs on timing).
+constexpr int kNvTileThreads = 192;  // warp 0 copies, 1 MMA and tensor memory, 2-5 output
+constexpr uint32_t kNvColSf = 128;   // tensor memory: sums [0, 128), scales behind them
+constexpr int kNvMaxStages = 8;
+
+struct NvTileArgs {
+  NvMatmulArgs a;
+  int cols, splits, stages, stage_bytes, k_stages, kblocks;
+  size_t x_scale_piece;
+};
+struct NvTileBars {
+  uint64_t full[kNvMaxStages], empty[kNvMaxStages], done;
+  uint32_t tmem, abort;
+  float fx[128];
+};
+
+__global__ void __launch_bounds__(kNvTileThreads, 1)
+    nv_tile_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                   const __grid_constant__ NvTileArgs t, Scratch* scr, uint64_t budget) {
+  extern __shared__ uint8_t nv_raw[];
+  __shared__ NvTileBars sm;
+  const NvMatmulArgs& a = t.a;
+  const uint32_t base = (smem_u32(nv_raw) + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x % t.splits, n0 = blockIdx.x / t.splits * 128, m0 = blockIdx.y * t.cols;
+  const int ks0 = t.k_stages * rank / t.splits, ks1 = t.k_stages * (rank + 1) / t.splits;
+  const int P = a.pieces;
+  if (tid == 0) {
+    for (int i = 0; i < t.stages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    mbar_init(&sm.done, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  pa_fence_before();
+  __syncthreads();
+  pa_fence_after();
+  if (t.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (this CTA runs)
+  const uint32_t tbase = sm.tmem;
+  volatile uint32_t* abort = &sm.abort;
+  const uint32_t x_at = 16384, sw_at = x_at + P * t.cols * 128, sx_at = sw_at + 2048;
+  float part[16];
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();
+      const uint8_t* sw = a.w_scales + static_cast<size_t>(n0 >> 7) * t.kblocks * 512;
+      const uint8_t* sx = a.x_scales + static_cast<size_t>(m0 >> 7) * t.kblocks * 512;
+      uint32_t issued = 0;
+      bool ok = true;
+      for (int ks = ks0; ks < ks1; ++ks, ++issued) {
+        const uint32_t st = issued % t.stages, at = base + st * t.stage_bytes;
+        if (issued >= static_cast<uint32_t>(t.stages) && !(ok = pa_wait(&sm.empty[st], (issued / t.stages - 1) & 1, abort, budget)))
+          break;
+        const uint32_t sf = min(4, t.kblocks - 4 * ks) * 512;
+        mbar_arrive_expect_tx(&sm.full[st], 16384 + P * t.cols * 128 + (1 + P) * sf);
+        nv_tma_3d(at, &wmap, ks * 128, n0, 0, &sm.full[st]);
+        nv_bulk(at + sw_at, sw + static_cast<size_t>(ks) * 2048, sf, &sm.full[st]);
+        for (int p = 0; p < P; ++p) {
+          nv_tma_3d(at + x_at + p * t.cols * 128, &xmap, ks * 128, m0, p, &sm.full[st]);
+          nv_bulk(at + sx_at + p * 2048, sx + p * t.x_scale_piece + static_cast<size_t>(ks) * 2048, sf, &sm.full[st]);
+        }
+      }
+      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+      // no copy may be in flight when the CTA exits
+      for (uint32_t j = issued > static_cast<uint32_t>(t.stages) ? issued - t.stages : 0u; j < issued; ++j)
+        mbar_wait_suspend(&sm.full[j % t.stages], (j / t.stages) & 1, global_ns() + budget);
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(t.cols >> 3) << 17) | (8u << 24);
+    const uint32_t slots = (512 - kNvColSf) / (16 * (1 + P));
+    const bool leader = pa_elect();
+    bool ok = true;
+    uint32_t i = 0;
+    for (int ks = ks0; ks < ks1 && ok; ++ks, ++i) {
+      const uint32_t st = i % t.stages, at = base + st * t.stage_bytes;
+      ok = pa_wait_warp(&sm.full[st], (i / t.stages) & 1, abort, budget);
+      if (!ok) break;
+      pa_fence_after();
+      if (leader) {
+        const uint32_t sf = tbase + kNvColSf + (i % slots) * 16 * (1 + P);
+        const int steps = min(4, t.kblocks - 4 * ks);
+        const uint64_t wd = pa_desc(at, 16, 1024), xd = pa_desc(at + x_at, 16, 1024);
+        for (int s = 0; s < steps; ++s) {
+          nv_cp_scales<1>(sf + 4 * s, nv_scale_desc(at + sw_at + 512 * s));
+          for (int p = 0; p < P; ++p)
+            nv_cp_scales<1>(sf + 16 * (1 + p) + 4 * s, nv_scale_desc(at + sx_at + p * 2048 + 512 * s));
+        }
+        for (int s = 0; s < steps; ++s)
+          for (int p = 0; p < P; ++p)
+            nv_mma<1>(tbase, wd + 2 * s, xd + p * t.cols * 8 + 2 * s, idesc, sf + 4 * s,
+                      sf + 16 * (1 + p) + 4 * s + ((m0 & 127) >> 5), (i | s | p) ? 1u : 0u);
+        nv_commit(&sm.empty[st]);
+        if (ks == ks1 - 1) nv_commit(&sm.done);
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+    // (every MMA is done before tensor memory is given back)
+    pa_wait_warp(&sm.done, 0, abort, budget);
+  }
+  __syncwarp();
+  const int q = warp & 3, e = tid - 64;  // output: lane quarter, thread
+  const int valid = min(t.cols, a.m - m0);
+  const int n = n0 + 32 * q + lane;
+  const float fw = warp >= 2 && n < a.n ? a.w_factor[a.n_factors > 1 ? n : 0] : 0.f;
+  bool got = true;
+  if (warp >= 2) {
+    pdl_wait();
+    for (int c = e; c < valid; c += 128) sm.fx[c] = a.x_factor[m0 + c];
+    named_bar_sync(1, 128);
+    got = pa_wait_warp(&sm.done, 0, abort, budget);
+    pa_fence_after();
+  }
+  auto store = [&](int c, int row, float v) {  // (rows past the weight are nobody's)
+    if (row >= a.n) return;
+    const size_t to = static_cast<size_t>(m0 + c) * a.out_stride + row;
+    if (a.out_f32)
+      static_cast<float*>(a.out)[to] = v;
+    else
+      static_cast<uint16_t*>(a.out)[to] = f32_to_bf16(v);
+  };
+  if (t.splits == 1) {
+    if (warp >= 2 && got)
+      for (int c0 = 0; c0 < valid; c0 += 16) {
+        nv_ld16(tbase + c0 + (static_cast<uint32_t>(32 * q) << 16), part);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < valid) store(c0 + j, n, part[j] * sm.fx[c0 + j] * fw);
+      }
+  } else {
+    // row r of the tile is added up by CTA r / per; its parts lie there as [cta][column quad][row][4]
+    const int per = 128 / t.splits, quads = (valid + 3) / 4;
+    const uint32_t red = base + t.stages * t.stage_bytes;
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // (they all run)
+    if (warp >= 2 && got) {
+      const int r = 32 * q + lane;
+      const uint32_t to = pa_map_to(red + (static_cast<uint32_t>(rank * quads * per + r % per) << 4), r / per);
+      for (int c0 = 0; c0 < valid; c0 += 16) {
+        nv_ld16(tbase + c0 + (static_cast<uint32_t>(32 * q) << 16), part);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          if (c0 + j < valid)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((c0 + j) / 4 * per << 4)),
+                         "f"(part[j]), "f"(part[j + 1]), "f"(part[j + 2]), "f"(part[j + 3])
+                         : "memory");
+      }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp >= 2 && got) {
+      for (int x = e; x < quads * per; x += 128) {
+        const int r = x % per, row = n0 + rank * per + r;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < t.splits; ++s) {
+          const uint4 v = lds128(red + (static_cast<uint32_t>(s * quads * per + x) << 4));
+          sum.x += __uint_as_float(v.x), sum.y += __uint_as_float(v.y);
+          sum.z += __uint_as_float(v.z), sum.w += __uint_as_float(v.w);
+        }
+        const float f = row < a.n ? a.w_factor[a.n_factors > 1 ? row : 0] : 0.f;
+        const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (x / per * 4 + j < valid) store(x / per * 4 + j, row, out[j] * sm.fx[x / per * 4 + j] * f);
+      }
+    }
+  }
+  pa_fence_before();
+  __syncthreads();
+  pa_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512u));
+}
+
+// ---------------------------------------------------------------------------- host side
+// Codes [planes][rows][cols bytes] (row stride cols), box of box_rows x 128 bytes, 128-byte swizzle;
+// what lies past the rows and the columns reads as zeros.
+static bool nv_code_map(CUtensorMap* m, const void* p, int cols, int rows, int planes, size_t plane, int box_rows) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(planes > 1 ? plane : cols)};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_rows), 1}, each[3] = {1, 1, 1};
+  const EncodeFn fn = tensor_map_encoder();
+  return fn != nullptr && fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(p), dims, strides, box, each,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
+  NvTileArgs t = {};
+  t.a = a;
+  t.cols = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+  t.kblocks = (a.k + 63) / 64;
+  t.k_stages = (t.kblocks + 3) / 4;
+  t.x_scale_piece = nv_scale_bytes(a.max_rows, a.k);
+  const int row_tiles = (a.n + 127) / 128, col_tiles = (a.m + t.cols - 1) / t.cols;
+  t.splits = 1;
+  while (t.splits < 8 && 2 * t.splits <= t.k_stages && 2ll * t.splits * row_tiles * col_tiles <= ctx->sm_count) t.splits *= 2;
+  t.stage_bytes = 16384 + a.pieces * t.cols * 128 + (1 + a.pieces) * 2048;
+  const int red = t.splits > 1 ? 128 * t.cols * 4 : 0;
+  const int room = 229376 - 1024 - red;
+  t.stages = room / t.stage_bytes < kNvMaxStages ? room / t.stage_bytes : kNvMaxStages;
+  const int most = (t.k_stages + t.splits - 1) / t.splits;
+  if (t.stages > most) t.stages = most;
+  const size_t smem = 1024 + static_cast<size_t>(t.stages) * t.stage_bytes + red;
+  CUtensorMap wmap, xmap;
+  if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
+      !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), t.cols))
+    return fail(ctx, G4_ERR_CUDA, "cuTensorMapEncodeTiled failed (nvfp4 matmul)");
+  const void* fn = (const void*)nv_tile_kernel;
+  const g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "nvfp4 matmul");
+  if (st != G4_OK) return st;
+  Scratch* scr = ctx->buf.scratch;
+  uint64_t budget = ctx->wait_budget_ns;
+  void* args[] = {&wmap, &xmap, &t, &scr, &budget};
+  return launch_kernel(ctx, fn, dim3(row_tiles * t.splits, col_tiles), dim3(kNvTileThreads), smem, args, false, "nvfp4 matmul",
+                       t.splits);
 }
 
 }  // namespace g4

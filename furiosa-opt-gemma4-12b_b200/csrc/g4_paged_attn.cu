@@ -69,23 +69,6 @@ struct __align__(1024) PaSmem {
 };
 
 // ---------------------------------------------------------------------------- PTX
-__device__ __forceinline__ uint32_t pa_map_to(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void pa_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-// Relaxed: what they announce is ordered by the copies themselves (expect) or by the tensor
-// memory fences around them (P).  A release at cluster scope costs about 1000 cycles here.
-__device__ __forceinline__ void pa_expect_cluster(uint32_t addr, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void pa_arrive_relaxed(uint32_t addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
 __device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -98,14 +81,6 @@ __device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t db, u
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(db), "r"(idesc), "r"(acc)
-      : "memory");
-}
-// Arrives on the barrier at this address in both CTAs when the MMAs issued so far are done.
-__device__ __forceinline__ void pa_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
       : "memory");
 }
 __device__ __forceinline__ void pa_tma(uint32_t dst, uint64_t map, int c1, int c2, int c3, int c4, uint32_t bar) {

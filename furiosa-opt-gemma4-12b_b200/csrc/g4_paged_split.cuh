@@ -1,6 +1,6 @@
 // What the two paged attention kernels share (g4_paged_attn.cu: tiles of 256 rows on CTA pairs;
-// g4_paged_few.cu: 16 rows on single CTAs): arguments, bounded waits, tensor-core plumbing and
-// the work split.
+// g4_paged_few.cu: 16 rows on single CTAs): arguments, bounded waits, tensor-core plumbing (the
+// NVFP4 products' too, g4_nvfp4_mm.cu) and the work split.
 #pragma once
 
 #include <cuda.h>
@@ -90,6 +90,31 @@ __device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lbo, uint32_
   return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
          (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (static_cast<uint64_t>(1u) << 46) |
          (static_cast<uint64_t>(2u) << 61);
+}
+__device__ __forceinline__ uint32_t pa_map_to(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void pa_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Relaxed: what they announce is ordered by the copies themselves (expect) or by the tensor
+// memory fences around them (P).  A release at cluster scope costs about 1000 cycles here.
+__device__ __forceinline__ void pa_expect_cluster(uint32_t addr, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void pa_arrive_relaxed(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Arrives on the barrier at this address in both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void pa_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
 }
 __device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -351,10 +376,8 @@ inline PaDiv divisor(int d) {
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// A 5-D tensor of 64-dim rows with the 128-byte swizzle; `stride` in elements.
-inline bool tile_map(CUtensorMap* m, const uint16_t* base, const int (&n)[4], const int64_t (&stride)[4],
-                     const int (&box)[4]) {
-  static EncodeFn fn = [] {
+inline EncodeFn tensor_map_encoder() {
+  static const EncodeFn fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     return (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
@@ -362,6 +385,12 @@ inline bool tile_map(CUtensorMap* m, const uint16_t* base, const int (&n)[4], co
                ? reinterpret_cast<EncodeFn>(p)
                : nullptr;
   }();
+  return fn;
+}
+// A 5-D tensor of 64-dim rows with the 128-byte swizzle; `stride` in elements.
+inline bool tile_map(CUtensorMap* m, const uint16_t* base, const int (&n)[4], const int64_t (&stride)[4],
+                     const int (&box)[4]) {
+  const EncodeFn fn = tensor_map_encoder();
   if (fn == nullptr) return false;
   cuuint64_t dims[5] = {64}, strides[4];
   cuuint32_t boxes[5] = {64};

@@ -8,6 +8,7 @@
 // Scales go from shared to tensor memory by tcgen05.cp (32 lanes x 16 bytes, repeated in the four
 // lane quarters), which is why they are kept in blocks of 128 rows x 64 columns: a block is the 512
 // bytes of one such copy, and a stage's four blocks one contiguous copy from global memory.
+#include <cstdlib>
 #include <string>
 
 #include "g4_nvfp4.cuh"
@@ -254,6 +255,221 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512u));
 }
 
+// ---------------------------------------------------------------------------- CTA pairs
+// Tiles of 256 weight rows x `cols` activation rows for many rows: each CTA of a pair holds 128 of the
+// weight rows and half of the activation rows of a stage (cta_group::2), all of their scales, and
+// gets the sums of its 128 weight rows.  Pairs take tiles in turn.
+//
+// Tensor memory: two sums of `cols` columns and one stage's scales do not fit side by side at 256, so the
+// sums overlap by `overlap` columns: the next tile's products start once these have been read.
+constexpr int kNvPairThreads = 320;  // warp 0 copies, 1 MMA (leader) and tensor memory, 2-9 output
+
+struct NvPairArgs {
+  NvMatmulArgs a;
+  int cols, blocks, stages, stage_bytes, k_stages, kblocks, row_tiles, tiles;
+  int sf_cols, acc_step, first_chunks;  // scale columns; column of the second sums; chunks of 32 columns per warp in the overlap
+};
+struct NvPairBars {
+  uint64_t full[kNvMaxStages], empty[kNvMaxStages], d_full[2], d_free[2];
+  uint32_t tmem, abort;
+};
+
+__device__ __forceinline__ void nv_pair_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+template <bool kF32>
+__global__ void __launch_bounds__(kNvPairThreads, 1)
+    nv_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                   const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap,
+                   const __grid_constant__ NvPairArgs t, Scratch* scr, uint64_t budget) {
+  extern __shared__ uint8_t nv_raw[];
+  __shared__ NvPairBars sm;
+  const NvMatmulArgs& a = t.a;
+  const uint32_t base = (smem_u32(nv_raw) + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int P = a.pieces, half = t.cols / 2;
+  if (tid == 0) {
+    for (int i = 0; i < t.stages; ++i) {
+      mbar_init(&sm.full[i], 2);
+      mbar_init(&sm.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.d_full[i], 1);
+      mbar_init(&sm.d_free[i], 16);
+    }
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  pa_fence_before();
+  __syncthreads();
+  pa_fence_after();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // both CTAs' barriers and tensor memory are ready
+  const uint32_t tbase = sm.tmem;
+  volatile uint32_t* abort = &sm.abort;
+  const uint32_t x_at = 16384, sw_at = x_at + P * half * 128, sx_at = sw_at + 2048;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();
+      const uint32_t full0 = pa_map_to(smem_u32(&sm.full[0]), 0);
+      const uint32_t bytes = 16384 + P * half * 128 + 2048 + P * t.blocks * 2048;
+      uint32_t issued = 0;
+      bool ok = true;
+      for (int tile = pair; tile < t.tiles && ok; tile += pairs) {
+        const int n0 = tile % t.row_tiles * 256 + 128 * cta, m0 = tile / t.row_tiles * t.cols;
+        for (int ks = 0; ks < t.k_stages; ++ks, ++issued) {
+          const uint32_t st = issued % t.stages, at = base + st * t.stage_bytes;
+          if (issued >= static_cast<uint32_t>(t.stages) && !(ok = pa_wait(&sm.empty[st], (issued / t.stages - 1) & 1, abort, budget)))
+            break;
+          const uint32_t bar = full0 + 8 * st;
+          pa_expect_cluster(bar, bytes);
+          nv_pair_tma(at, &wmap, ks * 128, n0, 0, bar);
+          nv_pair_tma(at + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
+          for (int p = 0; p < P; ++p) {
+            nv_pair_tma(at + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
+            nv_pair_tma(at + sx_at + p * t.blocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
+          }
+        }
+      }
+      // Every copy has landed (the leader's products took it) once its stage is empty again; both
+      // CTAs stay until then.
+      for (uint32_t j = issued > static_cast<uint32_t>(t.stages) ? issued - t.stages : 0u; j < issued && ok; ++j)
+        ok = pa_wait(&sm.empty[j % t.stages], (j / t.stages) & 1, abort, budget);
+      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+    }
+  } else if (warp == 1) {
+    if (cta == 0) {
+      const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(t.cols >> 3) << 17) | (16u << 24);
+      const uint32_t sfa = tbase + 512 - t.sf_cols, step_cols = 4 + 4 * t.blocks * P;
+      const bool leader = pa_elect();
+      bool ok = true;
+      uint32_t i = 0, ti = 0;
+      for (int tile = pair; tile < t.tiles && ok; tile += pairs, ++ti) {
+        if (ti >= 1) ok = pa_wait_warp(&sm.d_free[(ti - 1) & 1], ((ti - 1) >> 1) & 1, abort, budget);
+        pa_fence_after();
+        const uint32_t d = tbase + (ti & 1) * t.acc_step;
+        const uint32_t shift = ((tile / t.row_tiles * t.cols) & 127) >> 5;
+        for (int ks = 0; ks < t.k_stages && ok; ++ks, ++i) {
+          const uint32_t st = i % t.stages, at = base + st * t.stage_bytes;
+          ok = pa_wait_warp(&sm.full[st], (i / t.stages) & 1, abort, budget);
+          if (!ok) break;
+          pa_fence_after();
+          if (leader) {
+            const int steps = min(4, t.kblocks - 4 * ks);
+            const uint64_t wd = pa_desc(at, 16, 1024), xd = pa_desc(at + x_at, 16, 1024);
+            for (int s = 0; s < steps; ++s) {
+              const uint32_t sf = sfa + s * step_cols;
+              nv_cp_scales<2>(sf, nv_scale_desc(at + sw_at + 512 * s));
+              for (int p = 0; p < P; ++p)
+                for (int b = 0; b < t.blocks; ++b)
+                  nv_cp_scales<2>(sf + 4 + 4 * (p * t.blocks + b), nv_scale_desc(at + sx_at + (p * t.blocks + b) * 2048 + 512 * s));
+            }
+            for (int s = 0; s < steps; ++s) {
+              const uint32_t sf = sfa + s * step_cols;
+              for (int p = 0; p < P; ++p)
+                nv_mma<2>(d, wd + 2 * s, xd + p * half * 8 + 2 * s, idesc, sf, sf + 4 + 4 * p * t.blocks + shift,
+                          (ks | s | p) ? 1u : 0u);
+            }
+            pa_commit(&sm.empty[st]);
+            if (ks == t.k_stages - 1) pa_commit(&sm.d_full[ti & 1]);
+          }
+          __syncwarp();
+        }
+      }
+      // (the other CTA's last arrivals: nothing of it may be under way when this one ends)
+      if (ok && ti > 0) ok = pa_wait_warp(&sm.d_free[(ti - 1) & 1], ((ti - 1) >> 1) & 1, abort, budget);
+      if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+    }
+  } else {
+    // -------------------------------------------------------------- output
+    pdl_wait();
+    const int q = warp & 3, group = (warp - 2) >> 2, chunks = t.cols / 32;
+    const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
+    const uint32_t free0 = pa_map_to(smem_u32(&sm.d_free[0]), 0);
+    bool ok = true;
+    uint32_t ti = 0;
+    for (int tile = pair; tile < t.tiles; tile += pairs, ++ti) {
+      const int n = tile % t.row_tiles * 256 + 128 * cta + 32 * q + lane, m0 = tile / t.row_tiles * t.cols;
+      const float fw = n < a.n ? a.w_factor[a.n_factors > 1 ? n : 0] : 0.f;
+      if (t.first_chunks == 0) {
+        __syncwarp();
+        if (lane == 0) pa_arrive_relaxed(free0 + 8 * (ti & 1));
+      }
+      ok = pa_wait_warp(&sm.d_full[ti & 1], (ti >> 1) & 1, abort, budget);
+      if (!ok) break;
+      pa_fence_after();
+      const uint32_t d = tbase + (ti & 1) * t.acc_step + lanes;
+      for (int j = group; j < chunks; j += 2) {
+        // the overlap first: the top of the first sums, the bottom of the second
+        const int c0 = 32 * ((ti & 1) ? j : chunks - 1 - j);
+        float v[32];
+        pa_ld32(d + c0, v);
+        pa_ld_wait();
+        if (j >> 1 == t.first_chunks - 1) {
+          pa_fence_before();
+          __syncwarp();
+          if (lane == 0) pa_arrive_relaxed(free0 + 8 * (ti & 1));
+        }
+        const int valid = a.m - (m0 + c0);  // rows of the chunk that there are
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          float f[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) f[x] = c + x < valid ? a.x_factor[m0 + c0 + c + x] : 0.f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[c + x] = v[c + x] * f[x] * fw;
+        }
+        if (kF32) {
+          if (n < a.n) {
+            float* out = static_cast<float*>(a.out) + static_cast<size_t>(m0 + c0) * a.out_stride + n;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (c < valid) out[c * a.out_stride] = v[c];
+          }
+        } else {
+          // two rows' neighbours in 4 bytes: the even lane takes the even activation rows
+          const int n2 = n & ~1, odd = lane & 1;
+          uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<size_t>(m0 + c0 + odd) * a.out_stride + n2;
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const uint32_t mine = pack_bf16x2(v[c], v[c + 1]);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+            const uint32_t two = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+            if (c + odd < valid) {
+              if (n2 + 1 < a.n)
+                *reinterpret_cast<uint32_t*>(out + c * a.out_stride) = two;
+              else if (n2 < a.n)
+                out[c * a.out_stride] = static_cast<uint16_t>(two);
+            }
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+  }
+  __syncthreads();
+  if (sm.abort != 0) {  // gave up somewhere: let the copies in flight land (bounded)
+    const uint64_t end = global_ns() + 1000000;
+    while (global_ns() < end) __nanosleep(1000);
+  }
+  pa_fence_before();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  pa_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512u));
+}
+
 // ---------------------------------------------------------------------------- host side
 // Codes [planes][rows][cols bytes] (row stride cols), box of box_rows x 128 bytes, 128-byte swizzle;
 // what lies past the rows and the columns reads as zeros.
@@ -267,7 +483,55 @@ static bool nv_code_map(CUtensorMap* m, const void* p, int cols, int rows, int p
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Scale blocks [planes][row blocks][column blocks of 512 bytes], box of box_rows row blocks x 4 column blocks.
+static bool nv_scale_map(CUtensorMap* m, const void* p, int kblocks, int rows, int planes, int box_rows) {
+  const cuuint64_t row = static_cast<cuuint64_t>(kblocks) * 512, blocks = (static_cast<cuuint64_t>(rows) + 127) / 128;
+  const cuuint64_t dims[3] = {row / 8, blocks, static_cast<cuuint64_t>(planes)}, strides[2] = {row, row * blocks};
+  const cuuint32_t box[3] = {256, static_cast<cuuint32_t>(box_rows), 1}, each[3] = {1, 1, 1};
+  const EncodeFn fn = tensor_map_encoder();
+  return fn != nullptr && fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT64, 3, const_cast<void*>(p), dims, strides, box, each,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
+  NvPairArgs t = {};
+  t.a = a;
+  t.cols = cols;
+  t.blocks = cols > 128 ? 2 : 1;
+  t.kblocks = (a.k + 63) / 64;
+  t.k_stages = (t.kblocks + 3) / 4;
+  t.row_tiles = (a.n + 255) / 256;
+  t.tiles = t.row_tiles * ((a.m + cols - 1) / cols);
+  t.sf_cols = 4 * (4 + 4 * t.blocks * a.pieces);
+  const int room = 512 - t.sf_cols;
+  t.acc_step = 2 * cols <= room ? cols : room - cols;
+  t.first_chunks = (cols - t.acc_step + 63) / 64;
+  t.stage_bytes = 16384 + a.pieces * (cols / 2) * 128 + 2048 + a.pieces * t.blocks * 2048;
+  t.stages = (229376 - 1024) / t.stage_bytes;
+  if (t.stages > kNvMaxStages) t.stages = kNvMaxStages;
+  const size_t smem = 1024 + static_cast<size_t>(t.stages) * t.stage_bytes;
+  CUtensorMap wmap, xmap, wsmap, xsmap;
+  if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
+      !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), cols / 2) ||
+      !nv_scale_map(&wsmap, a.w_scales, t.kblocks, a.n, 1, 1) ||
+      !nv_scale_map(&xsmap, a.x_scales, t.kblocks, a.max_rows, a.pieces, t.blocks))
+    return fail(ctx, G4_ERR_CUDA, "cuTensorMapEncodeTiled failed (nvfp4 matmul)");
+  const void* fn = a.out_f32 ? (const void*)nv_pair_kernel<true> : (const void*)nv_pair_kernel<false>;
+  const g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "nvfp4 matmul");
+  if (st != G4_OK) return st;
+  Scratch* scr = ctx->buf.scratch;
+  uint64_t budget = ctx->wait_budget_ns;
+  void* args[] = {&wmap, &xmap, &wsmap, &xsmap, &t, &scr, &budget};
+  const int pairs = t.tiles < ctx->sm_count / 2 ? t.tiles : ctx->sm_count / 2;
+  return launch_kernel(ctx, fn, dim3(2 * pairs), dim3(kNvPairThreads), smem, args, false, "nvfp4 matmul", 2);
+}
+
 g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
+  if (a.m > 128) {
+    const char* e = std::getenv("NVCOLS");
+    return launch_pairs(ctx, a, e ? std::atoi(e) : 256);
+  }
   NvTileArgs t = {};
   t.a = a;
   t.cols = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;

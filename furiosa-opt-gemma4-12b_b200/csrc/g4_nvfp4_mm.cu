@@ -282,7 +282,7 @@ __device__ __forceinline__ void nv_pair_tma(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-template <bool kF32>
+template <int P, int kBlocks, bool kF32>
 __global__ void __launch_bounds__(kNvPairThreads, 1)
     nv_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap,
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
   const uint32_t base = (smem_u32(nv_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int P = a.pieces, half = t.cols / 2;
+  const int half = t.cols / 2;
   if (tid == 0) {
     for (int i = 0; i < t.stages; ++i) {
       mbar_init(&sm.full[i], 2);
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
     if (lane == 0) {
       pdl_wait();
       const uint32_t full0 = pa_map_to(smem_u32(&sm.full[0]), 0);
-      const uint32_t bytes = 16384 + P * half * 128 + 2048 + P * t.blocks * 2048;
+      const uint32_t bytes = 16384 + P * half * 128 + 2048 + P * kBlocks * 2048;
       uint32_t issued = 0;
       bool ok = true;
       for (int tile = pair; tile < t.tiles && ok; tile += pairs) {
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
           nv_pair_tma(at + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
           for (int p = 0; p < P; ++p) {
             nv_pair_tma(at + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
-            nv_pair_tma(at + sx_at + p * t.blocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
+            nv_pair_tma(at + sx_at + p * kBlocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
           }
         }
       }
@@ -351,40 +351,51 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
   } else if (warp == 1) {
     if (cta == 0) {
       const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(t.cols >> 3) << 17) | (16u << 24);
-      const uint32_t sfa = tbase + 512 - t.sf_cols, step_cols = 4 + 4 * t.blocks * P;
+      constexpr uint32_t kStep = 4 + 4 * kBlocks * P;  // scale columns of 64 columns' products
+      const uint32_t sfa = tbase + 512 - 4 * kStep;
       const bool leader = pa_elect();
+      const uint64_t wd0 = pa_desc(base, 16, 1024), xd0 = pa_desc(base + x_at, 16, 1024);
+      const uint64_t swd0 = nv_scale_desc(base + sw_at), sxd0 = nv_scale_desc(base + sx_at);
+      const uint32_t stage16 = t.stage_bytes / 16, piece16 = half * 8;
       bool ok = true;
-      uint32_t i = 0, ti = 0;
+      PaRing at(0, t.stages);
+      uint32_t ti = 0;
       for (int tile = pair; tile < t.tiles && ok; tile += pairs, ++ti) {
         if (ti >= 1) ok = pa_wait_warp(&sm.d_free[(ti - 1) & 1], ((ti - 1) >> 1) & 1, abort, budget);
         pa_fence_after();
         const uint32_t d = tbase + (ti & 1) * t.acc_step;
         const uint32_t shift = ((tile / t.row_tiles * t.cols) & 127) >> 5;
-        for (int ks = 0; ks < t.k_stages && ok; ++ks, ++i) {
-          const uint32_t st = i % t.stages, at = base + st * t.stage_bytes;
-          ok = pa_wait_warp(&sm.full[st], (i / t.stages) & 1, abort, budget);
+        for (int ks = 0; ks < t.k_stages && ok; ++ks) {
+          ok = pa_wait_warp(&sm.full[at.stage], at.parity, abort, budget);
           if (!ok) break;
           pa_fence_after();
+          const uint64_t off = at.stage * stage16;
+          const int steps = t.kblocks - 4 * ks;
           if (leader) {
-            const int steps = min(4, t.kblocks - 4 * ks);
-            const uint64_t wd = pa_desc(at, 16, 1024), xd = pa_desc(at + x_at, 16, 1024);
-            for (int s = 0; s < steps; ++s) {
-              const uint32_t sf = sfa + s * step_cols;
-              nv_cp_scales<2>(sf, nv_scale_desc(at + sw_at + 512 * s));
-              for (int p = 0; p < P; ++p)
-                for (int b = 0; b < t.blocks; ++b)
-                  nv_cp_scales<2>(sf + 4 + 4 * (p * t.blocks + b), nv_scale_desc(at + sx_at + (p * t.blocks + b) * 2048 + 512 * s));
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              if (s < steps) {
+                const uint32_t sf = sfa + s * kStep;
+                nv_cp_scales<2>(sf, swd0 + off + 32 * s);
+#pragma unroll
+                for (int b = 0; b < P * kBlocks; ++b) nv_cp_scales<2>(sf + 4 + 4 * b, sxd0 + off + 128 * b + 32 * s);
+              }
             }
-            for (int s = 0; s < steps; ++s) {
-              const uint32_t sf = sfa + s * step_cols;
-              for (int p = 0; p < P; ++p)
-                nv_mma<2>(d, wd + 2 * s, xd + p * half * 8 + 2 * s, idesc, sf, sf + 4 + 4 * p * t.blocks + shift,
-                          (ks | s | p) ? 1u : 0u);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              if (s < steps) {
+                const uint32_t sf = sfa + s * kStep;
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                  nv_mma<2>(d, wd0 + off + 2 * s, xd0 + off + p * piece16 + 2 * s, idesc, sf, sf + 4 + 4 * p * kBlocks + shift,
+                            (s | p) ? 1u : static_cast<uint32_t>(ks));
+              }
             }
-            pa_commit(&sm.empty[st]);
+            pa_commit(&sm.empty[at.stage]);
             if (ks == t.k_stages - 1) pa_commit(&sm.d_full[ti & 1]);
           }
           __syncwarp();
+          at.next();
         }
       }
       // (the other CTA's last arrivals: nothing of it may be under way when this one ends)
@@ -494,6 +505,17 @@ static bool nv_scale_map(CUtensorMap* m, const void* p, int kblocks, int rows, i
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <bool kF32>
+static const void* pair_kernel(int pieces, int blocks) {
+  if (blocks == 1)
+    return pieces == 1   ? (const void*)nv_pair_kernel<1, 1, kF32>
+           : pieces == 2 ? (const void*)nv_pair_kernel<2, 1, kF32>
+                         : (const void*)nv_pair_kernel<3, 1, kF32>;
+  return pieces == 1   ? (const void*)nv_pair_kernel<1, 2, kF32>
+         : pieces == 2 ? (const void*)nv_pair_kernel<2, 2, kF32>
+                       : (const void*)nv_pair_kernel<3, 2, kF32>;
+}
+
 static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   NvPairArgs t = {};
   t.a = a;
@@ -517,7 +539,7 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
       !nv_scale_map(&wsmap, a.w_scales, t.kblocks, a.n, 1, 1) ||
       !nv_scale_map(&xsmap, a.x_scales, t.kblocks, a.max_rows, a.pieces, t.blocks))
     return fail(ctx, G4_ERR_CUDA, "cuTensorMapEncodeTiled failed (nvfp4 matmul)");
-  const void* fn = a.out_f32 ? (const void*)nv_pair_kernel<true> : (const void*)nv_pair_kernel<false>;
+  const void* fn = a.out_f32 ? pair_kernel<true>(a.pieces, t.blocks) : pair_kernel<false>(a.pieces, t.blocks);
   const g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "nvfp4 matmul");
   if (st != G4_OK) return st;
   Scratch* scr = ctx->buf.scratch;

@@ -272,7 +272,20 @@ struct NvPairArgs {
 struct NvPairBars {
   uint64_t full[kNvMaxStages], empty[kNvMaxStages], d_full[2], d_free[2];
   uint32_t tmem, abort;
+  __align__(16) float fx[2][256];
 };
+constexpr int kNvOutBytes = 32 * 128 * 2;  // a chunk on its way out; two for each group of output warps
+// The output warps agree on whether all of their waits held (they meet at barriers of their own).
+__device__ __forceinline__ bool nv_agree(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
+}
 
 __device__ __forceinline__ void nv_pair_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
@@ -286,7 +299,7 @@ template <int P, int kBlocks, bool kF32>
 __global__ void __launch_bounds__(kNvPairThreads, 1)
     nv_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap,
-                   const __grid_constant__ NvPairArgs t, Scratch* scr, uint64_t budget) {
+                   const __grid_constant__ CUtensorMap omap, const __grid_constant__ NvPairArgs t, Scratch* scr, uint64_t budget) {
   extern __shared__ uint8_t nv_raw[];
   __shared__ NvPairBars sm;
   const NvMatmulArgs& a = t.a;
@@ -324,28 +337,28 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
       pdl_wait();
       const uint32_t full0 = pa_map_to(smem_u32(&sm.full[0]), 0);
       const uint32_t bytes = 16384 + P * half * 128 + 2048 + P * kBlocks * 2048;
-      uint32_t issued = 0;
       bool ok = true;
+      PaRing at(0, t.stages);
+      auto free = [&]() {  // the stage's last products are done
+        return at.passed < static_cast<uint32_t>(t.stages) || pa_wait(&sm.empty[at.stage], at.parity ^ 1, abort, budget);
+      };
       for (int tile = pair; tile < t.tiles && ok; tile += pairs) {
         const int n0 = tile % t.row_tiles * 256 + 128 * cta, m0 = tile / t.row_tiles * t.cols;
-        for (int ks = 0; ks < t.k_stages; ++ks, ++issued) {
-          const uint32_t st = issued % t.stages, at = base + st * t.stage_bytes;
-          if (issued >= static_cast<uint32_t>(t.stages) && !(ok = pa_wait(&sm.empty[st], (issued / t.stages - 1) & 1, abort, budget)))
-            break;
-          const uint32_t bar = full0 + 8 * st;
+        for (int ks = 0; ks < t.k_stages && (ok = free()); ++ks) {
+          const uint32_t to = base + at.stage * t.stage_bytes, bar = full0 + 8 * at.stage;
           pa_expect_cluster(bar, bytes);
-          nv_pair_tma(at, &wmap, ks * 128, n0, 0, bar);
-          nv_pair_tma(at + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
-          for (int p = 0; p < P; ++p) {
-            nv_pair_tma(at + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
-            nv_pair_tma(at + sx_at + p * kBlocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
-          }
+          nv_pair_tma(to, &wmap, ks * 128, n0, 0, bar);
+#pragma unroll
+          for (int p = 0; p < P; ++p) nv_pair_tma(to + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
+          nv_pair_tma(to + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
+#pragma unroll
+          for (int p = 0; p < P; ++p) nv_pair_tma(to + sx_at + p * kBlocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
+          at.next();
         }
       }
-      // Every copy has landed (the leader's products took it) once its stage is empty again; both
+      // Every copy has landed (the leader's products took it) once its stage is free again; both
       // CTAs stay until then.
-      for (uint32_t j = issued > static_cast<uint32_t>(t.stages) ? issued - t.stages : 0u; j < issued && ok; ++j)
-        ok = pa_wait(&sm.empty[j % t.stages], (j / t.stages) & 1, abort, budget);
+      for (int i = 0; i < t.stages && ok; ++i, at.next()) ok = free();
       if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     }
   } else if (warp == 1) {
@@ -405,19 +418,24 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
   } else {
     // -------------------------------------------------------------- output
     pdl_wait();
-    const int q = warp & 3, group = (warp - 2) >> 2, chunks = t.cols / 32;
+    const int e = tid - 64, q = warp & 3, group = e >> 7, chunks = t.cols / 32;
     const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
     const uint32_t free0 = pa_map_to(smem_u32(&sm.d_free[0]), 0);
+    const uint32_t stage = base + t.stages * t.stage_bytes + group * 2 * kNvOutBytes;
+    const bool sender = (e & 127) == 0;
     bool ok = true;
-    uint32_t ti = 0;
+    uint32_t ti = 0, sent = 0;
     for (int tile = pair; tile < t.tiles; tile += pairs, ++ti) {
-      const int n = tile % t.row_tiles * 256 + 128 * cta + 32 * q + lane, m0 = tile / t.row_tiles * t.cols;
+      const int n0 = tile % t.row_tiles * 256 + 128 * cta, m0 = tile / t.row_tiles * t.cols;
+      const int n = n0 + 32 * q + lane;
       const float fw = n < a.n ? a.w_factor[a.n_factors > 1 ? n : 0] : 0.f;
+      float* fx = sm.fx[ti & 1];
+      if (e < t.cols) fx[e] = m0 + e < a.m ? a.x_factor[m0 + e] : 0.f;
       if (t.first_chunks == 0) {
         __syncwarp();
         if (lane == 0) pa_arrive_relaxed(free0 + 8 * (ti & 1));
       }
-      ok = pa_wait_warp(&sm.d_full[ti & 1], (ti >> 1) & 1, abort, budget);
+      ok = nv_agree(pa_wait_warp(&sm.d_full[ti & 1], (ti >> 1) & 1, abort, budget));
       if (!ok) break;
       pa_fence_after();
       const uint32_t d = tbase + (ti & 1) * t.acc_step + lanes;
@@ -433,40 +451,54 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
           if (lane == 0) pa_arrive_relaxed(free0 + 8 * (ti & 1));
         }
         const int valid = a.m - (m0 + c0);  // rows of the chunk that there are
+        if (valid <= 0 || n0 >= a.n) continue;
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          float f[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) f[x] = c + x < valid ? a.x_factor[m0 + c0 + c + x] : 0.f;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) v[c + x] = v[c + x] * f[x] * fw;
+          const float4 f = *reinterpret_cast<const float4*>(fx + c0 + c);
+          v[c] *= f.x * fw, v[c + 1] *= f.y * fw, v[c + 2] *= f.z * fw, v[c + 3] *= f.w * fw;
         }
-        if (kF32) {
+        if (kF32 || (a.n % 8 != 0 && n0 + 128 > a.n)) {
+          // (a copy out of shared memory writes whole 16 bytes, past an end that is not on such a border)
           if (n < a.n) {
-            float* out = static_cast<float*>(a.out) + static_cast<size_t>(m0 + c0) * a.out_stride + n;
+            const size_t to = static_cast<size_t>(m0 + c0) * a.out_stride + n;
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (c < valid) out[c * a.out_stride] = v[c];
-          }
-        } else {
-          // two rows' neighbours in 4 bytes: the even lane takes the even activation rows
-          const int n2 = n & ~1, odd = lane & 1;
-          uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<size_t>(m0 + c0 + odd) * a.out_stride + n2;
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const uint32_t mine = pack_bf16x2(v[c], v[c + 1]);
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-            const uint32_t two = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-            if (c + odd < valid) {
-              if (n2 + 1 < a.n)
-                *reinterpret_cast<uint32_t*>(out + c * a.out_stride) = two;
-              else if (n2 < a.n)
-                out[c * a.out_stride] = static_cast<uint16_t>(two);
+            for (int c = 0; c < 32; ++c) {
+              if (c >= valid) continue;
+              if (kF32)
+                static_cast<float*>(a.out)[to + c * a.out_stride] = v[c];
+              else
+                static_cast<uint16_t*>(a.out)[to + c * a.out_stride] = f32_to_bf16(v[c]);
             }
           }
+        } else {
+          // [32 activation rows][128 weight rows] leave as one copy: 256 bytes a row, clipped to what there is
+          const uint32_t buf = stage + (sent & 1) * kNvOutBytes;
+          if (sent >= 2) {
+            if (sender) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            named_bar_sync(2 + group, 128);
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const uint32_t two = pack_bf16x2(v[c], v[c + 1]);
+            const uint32_t to = buf + c * 256 + 2 * (32 * q + lane);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(static_cast<uint16_t>(two)) : "memory");
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + 256), "h"(static_cast<uint16_t>(two >> 16)) : "memory");
+          }
+          fence_proxy_async();
+          named_bar_sync(2 + group, 128);
+          if (sender) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                             reinterpret_cast<uint64_t>(&omap)),
+                         "r"(n0), "r"(m0 + c0), "r"(buf)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          ++sent;
         }
       }
     }
+    if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   }
   __syncthreads();
@@ -505,6 +537,17 @@ static bool nv_scale_map(CUtensorMap* m, const void* p, int kblocks, int rows, i
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The bf16 output [rows][cols], box of 32 rows x 128 columns.
+static bool nv_out_map(CUtensorMap* m, const void* p, int cols, int rows, long long stride) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+  const cuuint32_t box[2] = {128, 32}, each[2] = {1, 1};
+  const EncodeFn fn = tensor_map_encoder();
+  return fn != nullptr && fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, box, each,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <bool kF32>
 static const void* pair_kernel(int pieces, int blocks) {
   if (blocks == 1)
@@ -530,21 +573,23 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   t.acc_step = 2 * cols <= room ? cols : room - cols;
   t.first_chunks = (cols - t.acc_step + 63) / 64;
   t.stage_bytes = 16384 + a.pieces * (cols / 2) * 128 + 2048 + a.pieces * t.blocks * 2048;
-  t.stages = (229376 - 1024) / t.stage_bytes;
+  const int out_bytes = a.out_f32 ? 0 : 4 * kNvOutBytes;
+  t.stages = (229376 - 1024 - out_bytes) / t.stage_bytes;
   if (t.stages > kNvMaxStages) t.stages = kNvMaxStages;
-  const size_t smem = 1024 + static_cast<size_t>(t.stages) * t.stage_bytes;
-  CUtensorMap wmap, xmap, wsmap, xsmap;
+  const size_t smem = 1024 + static_cast<size_t>(t.stages) * t.stage_bytes + out_bytes;
+  CUtensorMap wmap, xmap, wsmap, xsmap, omap;
   if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
       !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), cols / 2) ||
       !nv_scale_map(&wsmap, a.w_scales, t.kblocks, a.n, 1, 1) ||
-      !nv_scale_map(&xsmap, a.x_scales, t.kblocks, a.max_rows, a.pieces, t.blocks))
+      !nv_scale_map(&xsmap, a.x_scales, t.kblocks, a.max_rows, a.pieces, t.blocks) ||
+      (!a.out_f32 && !nv_out_map(&omap, a.out, a.n, a.m, a.out_stride)))
     return fail(ctx, G4_ERR_CUDA, "cuTensorMapEncodeTiled failed (nvfp4 matmul)");
   const void* fn = a.out_f32 ? pair_kernel<true>(a.pieces, t.blocks) : pair_kernel<false>(a.pieces, t.blocks);
   const g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "nvfp4 matmul");
   if (st != G4_OK) return st;
   Scratch* scr = ctx->buf.scratch;
   uint64_t budget = ctx->wait_budget_ns;
-  void* args[] = {&wmap, &xmap, &wsmap, &xsmap, &t, &scr, &budget};
+  void* args[] = {&wmap, &xmap, &wsmap, &xsmap, a.out_f32 ? &wmap : &omap, &t, &scr, &budget};
   const int pairs = t.tiles < ctx->sm_count / 2 ? t.tiles : ctx->sm_count / 2;
   return launch_kernel(ctx, fn, dim3(2 * pairs), dim3(kNvPairThreads), smem, args, false, "nvfp4 matmul", 2);
 }

@@ -48,6 +48,7 @@ g4_status launch_kernel(g4_ctx* ctx, const void* fn, dim3 grid, dim3 block, size
                         bool cooperative, const char* what, unsigned cluster_x) {
   cudaLaunchAttribute attrs[3];
   unsigned n = 0;
+  ctx->weights_ahead = false;
   if (cooperative) {
     attrs[n].id = cudaLaunchAttributeCooperative;
     attrs[n].val.cooperative = 1;

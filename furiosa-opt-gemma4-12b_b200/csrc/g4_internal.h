@@ -122,6 +122,9 @@ struct g4_ctx {
   g4::PrefillBuffers prefill;
   g4::PagedBuffers paged;
   int prefill_pieces = 2;  // NVFP4 pieces per prefill activation (1..3)
+  // The last launch quantised activations of several pieces (which are nobody's weight) and lets its
+  // successor start once its own predecessors are done: weights may be read ahead of it.
+  bool weights_ahead = false;
 };
 
 namespace g4 {

@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(T) nv_quant_kernel(const __grid_constant__ Qua
   __shared__ double redd[T / 32];
   const int row = blockIdx.x, tid = threadIdx.x;
   pdl_wait();
+  if (P > 1) pdl_launch_dependents();  // (one piece may be a weight, which a product reads ahead of its wait)
   const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.x_stride);
   uint32_t w[NB][8];
 #pragma unroll
@@ -286,7 +287,9 @@ g4_status g4_nvfp4_quantize(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, int
                    : out->pieces == 2 ? quant_kernel<2>(4 * a.kblocks, threads)
                                       : quant_kernel<3>(4 * a.kblocks, threads);
   void* args[] = {(void*)&a};
-  return launch_kernel(ctx, fn, dim3(n_rows), dim3(threads), 0, args, false, "nvfp4 quantize");
+  st = launch_kernel(ctx, fn, dim3(n_rows), dim3(threads), 0, args, false, "nvfp4 quantize");
+  ctx->weights_ahead = st == G4_OK && ctx->pdl_ok && out->pieces > 1;
+  return st;
 }
 
 g4_status g4_nvfp4_dequantize(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, g4_bf16* out, int64_t out_stride) {

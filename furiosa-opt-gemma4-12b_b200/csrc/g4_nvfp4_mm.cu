@@ -78,12 +78,12 @@ __device__ __forceinline__ void nv_ld16(uint32_t taddr, float (&v)[16]) {
 // each CTA then adds up 128 / splits of the tile's rows, whose parts the others stored into its
 // shared memory (in the cluster's order: no result hangs on timing).
 constexpr int kNvTileThreads = 192;  // warp 0 copies, 1 MMA and tensor memory, 2-5 output
-constexpr uint32_t kNvColSf = 128;   // tensor memory: sums [0, 128), scales behind them
 constexpr int kNvMaxStages = 8;
 
 struct NvTileArgs {
   NvMatmulArgs a;
-  int cols, splits, stages, stage_bytes, k_stages, kblocks;
+  int cols, splits, stages, stage_bytes, k_stages, kblocks, tmem_cols;
+  int early;  // the weights may be fetched before the previous kernel is done
   size_t x_scale_piece;
 };
 struct NvTileBars {
@@ -92,6 +92,7 @@ struct NvTileBars {
   float fx[128];
 };
 
+template <int P>
 __global__ void __launch_bounds__(kNvTileThreads, 1)
     nv_tile_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const __grid_constant__ NvTileArgs t, Scratch* scr, uint64_t budget) {
@@ -102,7 +103,6 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x % t.splits, n0 = blockIdx.x / t.splits * 128, m0 = blockIdx.y * t.cols;
   const int ks0 = t.k_stages * rank / t.splits, ks1 = t.k_stages * (rank + 1) / t.splits;
-  const int P = a.pieces;
   if (tid == 0) {
     for (int i = 0; i < t.stages; ++i) {
       mbar_init(&sm.full[i], 1);
@@ -113,7 +113,8 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u));
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
+                 "r"(static_cast<uint32_t>(t.tmem_cols)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   pa_fence_before();
@@ -122,62 +123,86 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   if (t.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (this CTA runs)
   const uint32_t tbase = sm.tmem;
   volatile uint32_t* abort = &sm.abort;
-  const uint32_t x_at = 16384, sw_at = x_at + P * t.cols * 128, sx_at = sw_at + 2048;
-  float part[16];
+  const uint32_t x_bytes = t.cols * 128;
+  const uint32_t x_at = 16384, sw_at = x_at + P * x_bytes, sx_at = sw_at + 2048;
 
   if (warp == 0) {
     if (lane == 0) {
-      pdl_wait();
       const uint8_t* sw = a.w_scales + static_cast<size_t>(n0 >> 7) * t.kblocks * 512;
       const uint8_t* sx = a.x_scales + static_cast<size_t>(m0 >> 7) * t.kblocks * 512;
-      uint32_t issued = 0;
-      bool ok = true;
-      for (int ks = ks0; ks < ks1; ++ks, ++issued) {
-        const uint32_t st = issued % t.stages, at = base + st * t.stage_bytes;
-        if (issued >= static_cast<uint32_t>(t.stages) && !(ok = pa_wait(&sm.empty[st], (issued / t.stages - 1) & 1, abort, budget)))
-          break;
-        const uint32_t sf = min(4, t.kblocks - 4 * ks) * 512;
-        mbar_arrive_expect_tx(&sm.full[st], 16384 + P * t.cols * 128 + (1 + P) * sf);
-        nv_tma_3d(at, &wmap, ks * 128, n0, 0, &sm.full[st]);
-        nv_bulk(at + sw_at, sw + static_cast<size_t>(ks) * 2048, sf, &sm.full[st]);
+      auto weights = [&](int ks, int st) {
+        const uint32_t to = base + st * t.stage_bytes, sf = min(4, t.kblocks - 4 * ks) * 512;
+        mbar_arrive_expect_tx(&sm.full[st], 16384 + P * x_bytes + (1 + P) * sf);
+        nv_tma_3d(to, &wmap, ks * 128, n0, 0, &sm.full[st]);
+        nv_bulk(to + sw_at, sw + static_cast<size_t>(ks) * 2048, sf, &sm.full[st]);
+      };
+      auto rows = [&](int ks, int st) {
+        const uint32_t to = base + st * t.stage_bytes, sf = min(4, t.kblocks - 4 * ks) * 512;
+#pragma unroll
         for (int p = 0; p < P; ++p) {
-          nv_tma_3d(at + x_at + p * t.cols * 128, &xmap, ks * 128, m0, p, &sm.full[st]);
-          nv_bulk(at + sx_at + p * 2048, sx + p * t.x_scale_piece + static_cast<size_t>(ks) * 2048, sf, &sm.full[st]);
+          nv_tma_3d(to + x_at + p * x_bytes, &xmap, ks * 128, m0, p, &sm.full[st]);
+          nv_bulk(to + sx_at + p * 2048, sx + p * t.x_scale_piece + static_cast<size_t>(ks) * 2048, sf, &sm.full[st]);
         }
+      };
+      const int ahead = min(t.stages, ks1 - ks0);
+      if (t.early)
+        for (int i = 0; i < ahead; ++i) weights(ks0 + i, i);
+      pdl_wait();
+      pdl_launch_dependents();
+      PaRing at(0, t.stages);
+      bool ok = true;
+      for (int ks = ks0; ks < ks1; ++ks, at.next()) {
+        if (ks - ks0 >= ahead && !(ok = pa_wait(&sm.empty[at.stage], at.parity ^ 1, abort, budget))) break;
+        if (!t.early || ks - ks0 >= ahead) weights(ks, at.stage);
+        rows(ks, at.stage);
       }
-      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
-      // no copy may be in flight when the CTA exits
-      for (uint32_t j = issued > static_cast<uint32_t>(t.stages) ? issued - t.stages : 0u; j < issued; ++j)
-        mbar_wait_suspend(&sm.full[j % t.stages], (j / t.stages) & 1, global_ns() + budget);
+      if (!ok) {
+        atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
+        // no copy may be in flight when the CTA exits (otherwise the products have taken them all)
+        const uint64_t end = global_ns() + 1000000;
+        while (global_ns() < end) __nanosleep(1000);
+      }
     }
   } else if (warp == 1) {
+    constexpr uint32_t kStep = 4 * (1 + P);
     const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(t.cols >> 3) << 17) | (8u << 24);
-    const uint32_t slots = (512 - kNvColSf) / (16 * (1 + P));
+    const uint32_t sfa = tbase + t.cols;
     const bool leader = pa_elect();
+    const uint64_t wd0 = pa_desc(base, 16, 1024), xd0 = pa_desc(base + x_at, 16, 1024);
+    const uint64_t swd0 = nv_scale_desc(base + sw_at), sxd0 = nv_scale_desc(base + sx_at);
+    const uint32_t stage16 = t.stage_bytes / 16, piece16 = x_bytes / 16;
+    const uint32_t shift = (m0 & 127) >> 5;
     bool ok = true;
-    uint32_t i = 0;
-    for (int ks = ks0; ks < ks1 && ok; ++ks, ++i) {
-      const uint32_t st = i % t.stages, at = base + st * t.stage_bytes;
-      ok = pa_wait_warp(&sm.full[st], (i / t.stages) & 1, abort, budget);
+    PaRing at(0, t.stages);
+    for (int ks = ks0; ks < ks1; ++ks) {
+      ok = pa_wait_warp(&sm.full[at.stage], at.parity, abort, budget);
       if (!ok) break;
       pa_fence_after();
+      const uint64_t off = at.stage * stage16;
+      const int steps = t.kblocks - 4 * ks;
       if (leader) {
-        const uint32_t sf = tbase + kNvColSf + (i % slots) * 16 * (1 + P);
-        const int steps = min(4, t.kblocks - 4 * ks);
-        const uint64_t wd = pa_desc(at, 16, 1024), xd = pa_desc(at + x_at, 16, 1024);
-        for (int s = 0; s < steps; ++s) {
-          nv_cp_scales<1>(sf + 4 * s, nv_scale_desc(at + sw_at + 512 * s));
-          for (int p = 0; p < P; ++p)
-            nv_cp_scales<1>(sf + 16 * (1 + p) + 4 * s, nv_scale_desc(at + sx_at + p * 2048 + 512 * s));
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (s < steps) {
+            nv_cp_scales<1>(sfa + s * kStep, swd0 + off + 32 * s);
+#pragma unroll
+            for (int p = 0; p < P; ++p) nv_cp_scales<1>(sfa + s * kStep + 4 + 4 * p, sxd0 + off + 128 * p + 32 * s);
+          }
         }
-        for (int s = 0; s < steps; ++s)
-          for (int p = 0; p < P; ++p)
-            nv_mma<1>(tbase, wd + 2 * s, xd + p * t.cols * 8 + 2 * s, idesc, sf + 4 * s,
-                      sf + 16 * (1 + p) + 4 * s + ((m0 & 127) >> 5), (i | s | p) ? 1u : 0u);
-        nv_commit(&sm.empty[st]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (s < steps) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+              nv_mma<1>(tbase, wd0 + off + 2 * s, xd0 + off + p * piece16 + 2 * s, idesc, sfa + s * kStep,
+                        sfa + s * kStep + 4 + 4 * p + shift, (s | p) ? 1u : static_cast<uint32_t>(ks - ks0));
+          }
+        }
+        nv_commit(&sm.empty[at.stage]);
         if (ks == ks1 - 1) nv_commit(&sm.done);
       }
       __syncwarp();
+      at.next();
     }
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     // (every MMA is done before tensor memory is given back)
@@ -196,6 +221,7 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
     got = pa_wait_warp(&sm.done, 0, abort, budget);
     pa_fence_after();
   }
+  float part[16];
   auto store = [&](int c, int row, float v) {  // (rows past the weight are nobody's)
     if (row >= a.n) return;
     const size_t to = static_cast<size_t>(m0 + c) * a.out_stride + row;
@@ -252,7 +278,8 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   pa_fence_before();
   __syncthreads();
   pa_fence_after();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512u));
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase),
+                 "r"(static_cast<uint32_t>(t.tmem_cols)));
 }
 
 // ---------------------------------------------------------------------------- CTA pairs
@@ -594,20 +621,19 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   return launch_kernel(ctx, fn, dim3(2 * pairs), dim3(kNvPairThreads), smem, args, false, "nvfp4 matmul", 2);
 }
 
-g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
-  if (a.m > 128) {
-    const char* e = std::getenv("NVCOLS");
-    return launch_pairs(ctx, a, e ? std::atoi(e) : 256);
-  }
+static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a) {
   NvTileArgs t = {};
   t.a = a;
   t.cols = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
   t.kblocks = (a.k + 63) / 64;
   t.k_stages = (t.kblocks + 3) / 4;
   t.x_scale_piece = nv_scale_bytes(a.max_rows, a.k);
+  t.early = ctx->weights_ahead;
   const int row_tiles = (a.n + 127) / 128, col_tiles = (a.m + t.cols - 1) / t.cols;
   t.splits = 1;
   while (t.splits < 8 && 2 * t.splits <= t.k_stages && 2ll * t.splits * row_tiles * col_tiles <= ctx->sm_count) t.splits *= 2;
+  t.tmem_cols = 32;
+  while (t.tmem_cols < t.cols + 16 * (1 + a.pieces)) t.tmem_cols *= 2;
   t.stage_bytes = 16384 + a.pieces * t.cols * 128 + (1 + a.pieces) * 2048;
   const int red = t.splits > 1 ? 128 * t.cols * 4 : 0;
   const int room = 229376 - 1024 - red;
@@ -619,7 +645,9 @@ g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
   if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
       !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), t.cols))
     return fail(ctx, G4_ERR_CUDA, "cuTensorMapEncodeTiled failed (nvfp4 matmul)");
-  const void* fn = (const void*)nv_tile_kernel;
+  const void* fn = a.pieces == 1   ? (const void*)nv_tile_kernel<1>
+                   : a.pieces == 2 ? (const void*)nv_tile_kernel<2>
+                                   : (const void*)nv_tile_kernel<3>;
   const g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "nvfp4 matmul");
   if (st != G4_OK) return st;
   Scratch* scr = ctx->buf.scratch;
@@ -627,6 +655,13 @@ g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
   void* args[] = {&wmap, &xmap, &t, &scr, &budget};
   return launch_kernel(ctx, fn, dim3(row_tiles * t.splits, col_tiles), dim3(kNvTileThreads), smem, args, false, "nvfp4 matmul",
                        t.splits);
+}
+
+g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
+  const char* e = std::getenv("NVCOLS");
+  int c = e ? std::atoi(e) : 0;
+  if (c == 0 ? a.m > 128 : c > 0) return launch_pairs(ctx, a, c > 0 ? c : 256);
+  return launch_tiles(ctx, a);
 }
 
 }  // namespace g4

@@ -7,16 +7,14 @@
 //
 // Scales go from shared to tensor memory by tcgen05.cp (32 lanes x 16 bytes, repeated in the four
 // lane quarters), which is why they are kept in blocks of 128 rows x 64 columns: a block is the 512
-// bytes of one such copy, and a stage's four blocks one contiguous copy from global memory.
-#include <cstdlib>
+// bytes of one such copy, and a stage's four blocks one contiguous copy from global memory.  A ring
+// stage is 256 columns: 128 bytes of codes a row.
 #include <string>
 
 #include "g4_nvfp4.cuh"
 #include "g4_paged_split.cuh"
 
 namespace g4 {
-
-constexpr int kNvStageK = 256;  // columns per ring stage: 128 bytes of codes, four scale blocks
 
 // ---------------------------------------------------------------------------- PTX
 __device__ __forceinline__ uint64_t nv_scale_desc(uint32_t addr) {  // 8-row groups of 128 bytes, no swizzle
@@ -77,7 +75,7 @@ __device__ __forceinline__ void nv_ld16(uint32_t taddr, float (&v)[16]) {
 // A tile is 128 weight rows x `cols` activation rows; a cluster of `splits` CTAs shares its K range, and
 // each CTA then adds up 128 / splits of the tile's rows, whose parts the others stored into its
 // shared memory (in the cluster's order: no result hangs on timing).
-constexpr int kNvTileThreads = 192;  // warp 0 copies, 1 MMA and tensor memory, 2-5 output
+constexpr int kNvTileThreads = 320;  // warp 0 copies, 1 MMA and tensor memory, 2-9 output
 constexpr int kNvMaxStages = 8;
 
 struct NvTileArgs {
@@ -89,7 +87,7 @@ struct NvTileArgs {
 struct NvTileBars {
   uint64_t full[kNvMaxStages], empty[kNvMaxStages], done;
   uint32_t tmem, abort;
-  float fx[128];
+  float fx[128], fw[128];
 };
 
 template <int P>
@@ -209,15 +207,16 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
     pa_wait_warp(&sm.done, 0, abort, budget);
   }
   __syncwarp();
-  const int q = warp & 3, e = tid - 64;  // output: lane quarter, thread
+  // output: two warps a lane quarter, every other 16 columns each
+  const int q = warp & 3, e = tid - 64, r = 32 * q + lane;
   const int valid = min(t.cols, a.m - m0);
-  const int n = n0 + 32 * q + lane;
-  const float fw = warp >= 2 && n < a.n ? a.w_factor[a.n_factors > 1 ? n : 0] : 0.f;
+  const uint32_t from = tbase + (static_cast<uint32_t>(32 * q) << 16);
   bool got = true;
   if (warp >= 2) {
     pdl_wait();
-    for (int c = e; c < valid; c += 128) sm.fx[c] = a.x_factor[m0 + c];
-    named_bar_sync(1, 128);
+    if (e < valid) sm.fx[e] = a.x_factor[m0 + e];
+    if (e >= 128) sm.fw[e - 128] = n0 + e - 128 < a.n ? a.w_factor[a.n_factors > 1 ? n0 + e - 128 : 0] : 0.f;
+    named_bar_sync(1, 256);
     got = pa_wait_warp(&sm.done, 0, abort, budget);
     pa_fence_after();
   }
@@ -231,27 +230,28 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
       static_cast<uint16_t*>(a.out)[to] = f32_to_bf16(v);
   };
   if (t.splits == 1) {
-    if (warp >= 2 && got)
-      for (int c0 = 0; c0 < valid; c0 += 16) {
-        nv_ld16(tbase + c0 + (static_cast<uint32_t>(32 * q) << 16), part);
+    if (warp >= 2 && got) {
+      const float fw = sm.fw[r];
+      for (int c0 = 16 * (e >> 7); c0 < valid; c0 += 32) {
+        nv_ld16(from + c0, part);
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (c0 + j < valid) store(c0 + j, n, part[j] * sm.fx[c0 + j] * fw);
+          if (c0 + j < valid) store(c0 + j, n0 + r, part[j] * sm.fx[c0 + j] * fw);
       }
+    }
   } else {
     // row r of the tile is added up by CTA r / per; its parts lie there as [cta][column quad][row][4]
-    const int per = 128 / t.splits, quads = (valid + 3) / 4;
+    const int shift = __ffs(128 / t.splits) - 1, per = 1 << shift, quads = (valid + 3) / 4;
     const uint32_t red = base + t.stages * t.stage_bytes;
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // (they all run)
     if (warp >= 2 && got) {
-      const int r = 32 * q + lane;
-      const uint32_t to = pa_map_to(red + (static_cast<uint32_t>(rank * quads * per + r % per) << 4), r / per);
-      for (int c0 = 0; c0 < valid; c0 += 16) {
-        nv_ld16(tbase + c0 + (static_cast<uint32_t>(32 * q) << 16), part);
+      const uint32_t to = pa_map_to(red + (static_cast<uint32_t>((rank * quads << shift) + (r & (per - 1))) << 4), r >> shift);
+      for (int c0 = 16 * (e >> 7); c0 < valid; c0 += 32) {
+        nv_ld16(from + c0, part);
 #pragma unroll
         for (int j = 0; j < 16; j += 4)
           if (c0 + j < valid)
-            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((c0 + j) / 4 * per << 4)),
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((c0 + j) / 4 << shift) << 4)),
                          "f"(part[j]), "f"(part[j + 1]), "f"(part[j + 2]), "f"(part[j + 3])
                          : "memory");
       }
@@ -259,19 +259,20 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp >= 2 && got) {
-      for (int x = e; x < quads * per; x += 128) {
-        const int r = x % per, row = n0 + rank * per + r;
+      const int all = quads << shift;
+      for (int x = e; x < all; x += 256) {
+        const int own = rank * per + (x & (per - 1)), c = (x >> shift) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int s = 0; s < t.splits; ++s) {
-          const uint4 v = lds128(red + (static_cast<uint32_t>(s * quads * per + x) << 4));
+          const uint4 v = lds128(red + (static_cast<uint32_t>(s * all + x) << 4));
           sum.x += __uint_as_float(v.x), sum.y += __uint_as_float(v.y);
           sum.z += __uint_as_float(v.z), sum.w += __uint_as_float(v.w);
         }
-        const float f = row < a.n ? a.w_factor[a.n_factors > 1 ? row : 0] : 0.f;
+        const float f = sm.fw[own];
         const float out[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (x / per * 4 + j < valid) store(x / per * 4 + j, row, out[j] * sm.fx[x / per * 4 + j] * f);
+          if (c + j < valid) store(c + j, n0 + own, out[j] * sm.fx[c + j] * f);
       }
     }
   }
@@ -419,12 +420,6 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
                 nv_cp_scales<2>(sf, swd0 + off + 32 * s);
 #pragma unroll
                 for (int b = 0; b < P * kBlocks; ++b) nv_cp_scales<2>(sf + 4 + 4 * b, sxd0 + off + 128 * b + 32 * s);
-              }
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              if (s < steps) {
-                const uint32_t sf = sfa + s * kStep;
 #pragma unroll
                 for (int p = 0; p < P; ++p)
                   nv_mma<2>(d, wd0 + off + 2 * s, xd0 + off + p * piece16 + 2 * s, idesc, sf, sf + 4 + 4 * p * kBlocks + shift,
@@ -621,17 +616,16 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   return launch_kernel(ctx, fn, dim3(2 * pairs), dim3(kNvPairThreads), smem, args, false, "nvfp4 matmul", 2);
 }
 
-static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a) {
+static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a, int cols, int splits) {
   NvTileArgs t = {};
   t.a = a;
-  t.cols = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+  t.cols = cols;
+  t.splits = splits;
   t.kblocks = (a.k + 63) / 64;
   t.k_stages = (t.kblocks + 3) / 4;
   t.x_scale_piece = nv_scale_bytes(a.max_rows, a.k);
   t.early = ctx->weights_ahead;
   const int row_tiles = (a.n + 127) / 128, col_tiles = (a.m + t.cols - 1) / t.cols;
-  t.splits = 1;
-  while (t.splits < 8 && 2 * t.splits <= t.k_stages && 2ll * t.splits * row_tiles * col_tiles <= ctx->sm_count) t.splits *= 2;
   t.tmem_cols = 32;
   while (t.tmem_cols < t.cols + 16 * (1 + a.pieces)) t.tmem_cols *= 2;
   t.stage_bytes = 16384 + a.pieces * t.cols * 128 + (1 + a.pieces) * 2048;
@@ -657,11 +651,44 @@ static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a) {
                        t.splits);
 }
 
+// Which kernel, how wide a tile, how many CTAs to a K range: the least of what each would take, by a model of
+// start + rounds x (K stages x a stage + a tile's end), in microseconds, fitted to sweeps of 1 to 4096
+// activation rows over the decoder's projections and their tensor-parallel shares (1 to 3 pieces; it names
+// the fastest or one within 6 % of it).  What it weighs, two pieces:
+//   one token, 8192 x 3840       single CTAs 6.7, pairs 9.2    (more of them, K split: all SMs at work)
+//   32 rows, 3840 x 4096         single CTAs 5.7, pairs 10.1
+//   64 rows, 30720 x 3840        single CTAs 22.4, pairs of 64 columns 17.0
+//   256 rows, 8192 x 3840        single CTAs 14.6, pairs of 128 columns 11.1, of 256 columns 15.8
+//   509 rows, 8704 x 3840        pairs of 128 columns 17.6, of 256 columns 16.7
+//   4096 rows, 8192 x 3840       pairs of 128 columns 103, of 256 columns 89
+// Tiles start at multiples of 64 activation rows, or there is one: the MMA wants its scales at an even
+// column of tensor memory.
 g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
-  const char* e = std::getenv("NVCOLS");
-  int c = e ? std::atoi(e) : 0;
-  if (c == 0 ? a.m > 128 : c > 0) return launch_pairs(ctx, a, c > 0 ? c : 256);
-  return launch_tiles(ctx, a);
+  const int stages = (a.k + 255) / 256, P = a.pieces;
+  auto ceil = [](int x, int y) { return (x + y - 1) / y; };
+  float best = 1e30f;
+  int best_cols = 0, best_splits = 0;  // 0 splits: pairs
+  auto offer = [&](float us, int cols, int splits) {
+    if (us < best) best = us, best_cols = cols, best_splits = splits;
+  };
+  for (int cols = a.m <= 16 ? 16 : a.m <= 32 ? 32 : 64; cols <= 128; cols *= 2) {
+    const int tiles = ceil(a.n, 128) * ceil(a.m, cols);
+    int splits = 1;
+    while (splits < 8 && 2 * splits <= stages && 2ll * splits * tiles <= ctx->sm_count) splits *= 2;
+    const float stage = cols <= 64 ? 0.3f + 0.075f * P : 0.2f + 0.27f * P, end = 0.5f + 0.03f * (a.m < cols ? a.m : cols);
+    offer(2.6f + ceil(tiles * splits, ctx->sm_count) * (ceil(stages, splits) * stage + end), cols, splits);
+    if (a.m <= 32) break;
+  }
+  for (int cols = 64; cols <= 256; cols *= 2) {
+    const int rounds = ceil(ceil(a.n, 256) * ceil(a.m, cols), ctx->sm_count / 2);
+    if (cols == 64)
+      offer(2.9f + rounds * (stages * (0.25f + 0.07f * P) + 0.55f), cols, 0);
+    else if (cols == 128)
+      offer(3.1f + rounds * (stages * (0.21f + 0.11f * P) + 0.8f), cols, 0);
+    else
+      offer(5.1f + rounds * (stages * (P == 1 ? 0.4f : P == 2 ? 0.62f : 1.1f) + 1.f), cols, 0);
+  }
+  return best_splits == 0 ? launch_pairs(ctx, a, best_cols) : launch_tiles(ctx, a, best_cols, best_splits);
 }
 
 }  // namespace g4

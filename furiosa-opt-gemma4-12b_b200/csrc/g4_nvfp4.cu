@@ -13,24 +13,69 @@
 
 namespace g4 {
 
-__device__ __forceinline__ uint32_t nv_e2m1x2(float lo, float hi) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\t.reg .b16 h;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tmov.b16 h, {t, 0};\n\t"
-      "cvt.u32.u16 %0, h;\n\t}"
-      : "=r"(r)
-      : "f"(hi), "f"(lo));
+// Two f32 side by side: Blackwell's FMA units take them in one instruction.
+__device__ __forceinline__ float2 nv_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 nv_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 nv_mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 nv_halves(uint32_t h) {
+  return make_float2(__half2float(__ushort_as_half(static_cast<uint16_t>(h))),
+                     __half2float(__ushort_as_half(static_cast<uint16_t>(h >> 16))));
+}
+// Values as E2M1 codes, the first in the low nibble.  (Four bytes packed by one mov.b32 came out right in
+// the word but not where the same word was taken apart again: pairs of bytes do.)
+__device__ __forceinline__ uint32_t nv_e2m1x4(float2 a, float2 b) {
+  uint16_t r;
+  asm("{\n\t.reg .b8 t0, t1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 t0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 t1, %4, %3;\n\t"
+      "mov.b16 %0, {t0, t1};\n\t}"
+      : "=h"(r)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
+}
+__device__ __forceinline__ uint32_t nv_e2m1x8(float2 a, float2 b, float2 c, float2 d) {
+  return __byte_perm(nv_e2m1x4(a, b), nv_e2m1x4(c, d), 0x5410);
 }
 __device__ __forceinline__ uint32_t nv_e4m3(float v) {
   uint16_t s;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s) : "f"(v), "f"(v));
   return s & 0xFFu;
 }
-// y / s correctly rounded, rcp = 1 / s rounded: the quotient's first guess is within an ulp, its
-// remainder is exact in one FMA, and one correction rounds right (Markstein's theorem).
-__device__ __forceinline__ float nv_div(float y, float s, float rcp) {
-  const float q = __fmul_rn(y, rcp);
-  return __fmaf_rn(__fmaf_rn(-q, s, y), rcp, q);
+// Quotients by multiplication, right in every tie.  What is divided has at most 11 significant bits (x g has 8,
+// y - c s at most 11: it is a multiple of 2^-9 of the scale's power of two and no larger than the scale), the
+// borders of both formats have few (3 bits of E2M1's by 4 of the scale; 6 by 5 bits of E4M3's).  So a quotient
+// that is not on a border is at least 2^-11 of itself away from it, and one that is has come out within
+// 2^-22 of it: rounding the approximate quotient to 2^-16 (E2M1: by adding 192 and taking it off again) or to
+// 16 significant bits (E4M3) puts the second on the border and leaves the first on its side.
+__device__ __forceinline__ uint32_t nv_scale_of(float top) {
+  const uint32_t q = __float_as_uint(top * (1.0f / 6.0f));
+  return nv_e4m3(__uint_as_float((q + 0x80u) & ~0xFFu));
+}
+__device__ __forceinline__ float nv_rcp(float s) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return r;
 }
 __device__ __forceinline__ float lo_f32(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_f32(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
@@ -100,12 +145,16 @@ __global__ void __launch_bounds__(T) nv_quant_kernel(const __grid_constant__ Qua
     }
   }
   // |x| orders like its low 15 bits
-  uint32_t top = 0u;
+  uint32_t own[NB], top = 0u;
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < NB; ++i) {
+    uint32_t m = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = __vmaxu2(top, w[i][e] & 0x7FFF7FFFu);
-  top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+    for (int e = 0; e < 8; ++e) m = __vmaxu2(m, w[i][e] & 0x7FFF7FFFu);
+    own[i] = max(m & 0xFFFFu, m >> 16);
+    top = max(top, own[i]);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
   if ((tid & 31) == 0) redu[tid >> 5] = top;
   __syncthreads();
   top = 0u;
@@ -116,38 +165,40 @@ __global__ void __launch_bounds__(T) nv_quant_kernel(const __grid_constant__ Qua
   const uint32_t ge = min(253u, ((top & 0x7Fu) <= 40u ? 265u : 264u) - (live ? top >> 7 : 0u));
   const float g = live ? __uint_as_float(ge << 23) : 0.f;
   if (tid == 0) a.factor[row] = live ? __uint_as_float((254u - ge) << 23) : (finite ? 0.f : CUDART_NAN_F);
+  const float2 g2 = make_float2(g, g), snap = make_float2(192.f, 192.f), unsnap = make_float2(-192.f, -192.f);
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     const int b = tid + i * T;
-    float y[16];
+    if (i > 0 && i * T >= 4 * a.kblocks) break;  // (of all threads)
+    float2 y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      y[2 * e] = live ? __fmul_rn(lo_f32(w[i][e]), g) : 0.f;
-      y[2 * e + 1] = live ? __fmul_rn(hi_f32(w[i][e]), g) : 0.f;
+      const uint32_t v = live ? w[i][e] : 0u;  // (an infinity times 0 is NaN)
+      y[e] = nv_mul2(make_float2(lo_f32(v), hi_f32(v)), g2);
     }
+    float m = live ? lo_f32(own[i]) * g : 0.f;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      float smax = 0.f;
+      const uint32_t sc = nv_scale_of(m);
+      const float sf = e4m3_value(sc), rcp = sc != 0u ? nv_rcp(sf) : 0.f;
+      const float2 r2 = make_float2(rcp, rcp);
+      float2 q[8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) smax = fmaxf(smax, fabsf(y[e]));
-      const uint32_t sc = nv_e4m3(__fdiv_rn(smax, 6.0f));
-      const float sf = e4m3_value(sc);
-      uint32_t packed[2] = {0u, 0u};
-      if (sf > 0.f) {
-        const float rcp = __frcp_rn(sf);
+      for (int e = 0; e < 8; ++e) q[e] = nv_add2(nv_fma2(y[e], r2, snap), unsnap);
+      const uint2 c = make_uint2(nv_e2m1x8(q[0], q[1], q[2], q[3]), nv_e2m1x8(q[4], q[5], q[6], q[7]));
+      if (p + 1 < P) {  // what the piece leaves, and its largest
+        uint32_t h[8];
+        cvt_e2m1x8(c.x, h[0], h[1], h[2], h[3]);
+        cvt_e2m1x8(c.y, h[4], h[5], h[6], h[7]);
+        const float2 s2 = make_float2(-sf, -sf);
+        m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const uint32_t two = nv_e2m1x2(nv_div(y[e], sf, rcp), nv_div(y[e + 1], sf, rcp));
-          packed[e >> 3] |= two << (8 * ((e >> 1) & 3));
-          if (p + 1 < P) {
-            const uint32_t hv = cvt_e2m1x2(two);
-            y[e] = __fmaf_rn(-__half2float(__ushort_as_half(static_cast<uint16_t>(hv))), sf, y[e]);
-            y[e + 1] = __fmaf_rn(-__half2float(__ushort_as_half(static_cast<uint16_t>(hv >> 16))), sf, y[e + 1]);
-          }
+        for (int e = 0; e < 8; ++e) {
+          y[e] = nv_fma2(nv_halves(h[e]), s2, y[e]);
+          m = fmaxf(m, fmaxf(fabsf(y[e].x), fabsf(y[e].y)));
         }
       }
-      if (b < a.nb)
-        *reinterpret_cast<uint2*>(a.codes + p * a.code_piece + row * a.code_row + 8 * b) = make_uint2(packed[0], packed[1]);
+      if (b < a.nb) *reinterpret_cast<uint2*>(a.codes + p * a.code_piece + row * a.code_row + 8 * b) = c;
       // four lanes' scales are neighbours in a scale block (zeros past the row's end)
       uint32_t four = sc | __shfl_down_sync(0xffffffffu, sc, 1) << 8;
       four |= __shfl_down_sync(0xffffffffu, four, 2) << 16;

@@ -532,7 +532,7 @@ typedef struct g4_nvfp4_weight {
  * factor = 1 / g.  Roundings are to nearest, ties to even; everything else is exact, so a row's
  * pieces do not depend on what computes them.  One piece leaves ~10 % of a value, two ~1 %, three
  * ~0.1 %.  A row of zeros: factor 0; a row with an infinity or a NaN: factor NaN (codes 0), so
- * that its products are NaN. */
+ * that its products are NaN.  What rounds to zero has code 0 or 8. */
 g4_status g4_nvfp4_quantize(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, int n_rows, const g4_bf16* rms_weight,
                             const g4_nvfp4_rows* out);
 /* The values `rows` stands for, rounded to bf16: out [n_rows, cols]. */

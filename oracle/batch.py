@@ -43,7 +43,7 @@ def quantize(x, pieces):
         s = torch.tensor(E4M3, dtype=torch.float64, device=x.device)[at][..., None]
         c = torch.where(s > 0, _nearest((y / s.clamp(min=2.0 ** -9)).abs(), E2M1), 0)
         value = torch.tensor(E2M1, dtype=torch.float64, device=x.device)[c] * torch.sign(y)
-        codes.append((c + 8 * ((y < 0) | ((y == 0) & torch.signbit(y))) * (s > 0)).view(m, k).byte())
+        codes.append((c + 8 * ((y < 0) & (c > 0))).view(m, k).byte())
         scales.append(at.byte())
         y = y - value * s
     factor = torch.where(live, 1 / g, torch.where(torch.isfinite(x).all(1), 0.0, torch.nan))

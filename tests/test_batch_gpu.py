@@ -153,7 +153,8 @@ def test_quantised_rows_are_a_weight(gpu_ctx):
 # ------------------------------------------------------------------------------ quantise
 def _check_rows(rows, want, n, cols):
     codes, scales, factor = want
-    assert torch.equal(rows.codes[:, :n], ob.pack(codes))
+    got = ob.unpack(rows.codes[:, :n])
+    assert torch.equal(torch.where(got == 8, 0, got), codes)  # (zero has either sign)
     for p in range(rows.pieces):
         at = ob.scale_at(torch.arange(n, device="cuda")[:, None], torch.arange(cols // 16, device="cuda")[None, :], cols)
         assert torch.equal(rows.scales[p][at], scales[p])

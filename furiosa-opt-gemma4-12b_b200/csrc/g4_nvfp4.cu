@@ -10,6 +10,7 @@
 #include <string>
 
 #include "g4_nvfp4.cuh"
+#include "g4_paged_split.cuh"
 
 namespace g4 {
 
@@ -92,9 +93,13 @@ struct QuantArgs {
   float* factor;
 };
 
-// One block of T threads per row; thread t holds the row's 16-element blocks t, t + T, ... (at most NB).
+// What bounds it: the conversion unit.  Two values to E2M1 are two of its operations, back to values one: a
+// block of 16 takes it 25 a piece and 8 more between pieces (100 % busy at 4096 x 15360 in two pieces, 48 us;
+// the bytes alone are 30 us; decoding by byte tables instead took 53 us, the issue slots being short then).
+//
+// One block of T threads per row; thread t holds the row's 16-element blocks t and t + T (at most NB).
 template <int T, int NB, int P>
-__global__ void __launch_bounds__(T) nv_quant_kernel(const __grid_constant__ QuantArgs a) {
+__global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_constant__ QuantArgs a) {
   __shared__ uint32_t redu[T / 32];
   __shared__ double redd[T / 32];
   const int row = blockIdx.x, tid = threadIdx.x;
@@ -165,6 +170,14 @@ __global__ void __launch_bounds__(T) nv_quant_kernel(const __grid_constant__ Qua
   const uint32_t ge = min(253u, ((top & 0x7Fu) <= 40u ? 265u : 264u) - (live ? top >> 7 : 0u));
   const float g = live ? __uint_as_float(ge << 23) : 0.f;
   if (tid == 0) a.factor[row] = live ? __uint_as_float((254u - ge) << 23) : (finite ? 0.f : CUDART_NAN_F);
+  if (!live) {  // nothing to divide by (and an infinity times 0 would be NaN)
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      own[i] = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[i][e] = 0u;
+    }
+  }
   const float2 g2 = make_float2(g, g), snap = make_float2(192.f, 192.f), unsnap = make_float2(-192.f, -192.f);
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
@@ -172,11 +185,8 @@ __global__ void __launch_bounds__(T) nv_quant_kernel(const __grid_constant__ Qua
     if (i > 0 && i * T >= 4 * a.kblocks) break;  // (of all threads)
     float2 y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t v = live ? w[i][e] : 0u;  // (an infinity times 0 is NaN)
-      y[e] = nv_mul2(make_float2(lo_f32(v), hi_f32(v)), g2);
-    }
-    float m = live ? lo_f32(own[i]) * g : 0.f;
+    for (int e = 0; e < 8; ++e) y[e] = nv_mul2(make_float2(lo_f32(w[i][e]), hi_f32(w[i][e])), g2);
+    float m = lo_f32(own[i]) * g;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const uint32_t sc = nv_scale_of(m);
@@ -187,15 +197,15 @@ __global__ void __launch_bounds__(T) nv_quant_kernel(const __grid_constant__ Qua
       for (int e = 0; e < 8; ++e) q[e] = nv_add2(nv_fma2(y[e], r2, snap), unsnap);
       const uint2 c = make_uint2(nv_e2m1x8(q[0], q[1], q[2], q[3]), nv_e2m1x8(q[4], q[5], q[6], q[7]));
       if (p + 1 < P) {  // what the piece leaves, and its largest
+        const float2 s2 = make_float2(-sf, -sf);
         uint32_t h[8];
         cvt_e2m1x8(c.x, h[0], h[1], h[2], h[3]);
         cvt_e2m1x8(c.y, h[4], h[5], h[6], h[7]);
-        const float2 s2 = make_float2(-sf, -sf);
         m = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           y[e] = nv_fma2(nv_halves(h[e]), s2, y[e]);
-          m = fmaxf(m, fmaxf(fabsf(y[e].x), fabsf(y[e].y)));
+          m = pa_max3(m, fabsf(y[e].x), fabsf(y[e].y));
         }
       }
       if (b < a.nb) *reinterpret_cast<uint2*>(a.codes + p * a.code_piece + row * a.code_row + 8 * b) = c;
@@ -288,12 +298,11 @@ static QuantArgs quant_args(const g4_nvfp4_rows* r) {
 }
 template <int P>
 static const void* quant_kernel(int nb4, int& threads) {
-  threads = 128;
+  threads = nb4 <= 256 ? 128 : nb4 <= 512 ? 256 : 512;
   if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P>;
   if (nb4 <= 256) return (const void*)nv_quant_kernel<128, 2, P>;
-  if (nb4 <= 512) return (const void*)nv_quant_kernel<128, 4, P>;
-  threads = 256;
-  return (const void*)nv_quant_kernel<256, 4, P>;
+  if (nb4 <= 512) return (const void*)nv_quant_kernel<256, 2, P>;
+  return (const void*)nv_quant_kernel<512, 2, P>;
 }
 
 }  // namespace g4

@@ -38,59 +38,141 @@ struct BeamArgs {
   int32_t* out_tokens;
 };
 
-// Order-preserving 16 bits of a bf16 (never 0 but for the lowest NaN).
+// Order-preserving 16 bits of a bf16 (-0 as 0, and none is 0).
 __device__ __forceinline__ uint32_t bm_order(uint32_t bits) {
-  return (bits & 0x8000u) ? (~bits & 0xFFFFu) : (bits | 0x8000u);
+  return (bits & 0x8000u) ? 0x8000u - (bits & 0x7FFFu) : (bits | 0x8000u);
 }
 __device__ __forceinline__ float bm_logit(uint32_t order) {
-  return bf16_to_f32(static_cast<uint16_t>((order & 0x8000u) ? (order & 0x7FFFu) : (~order & 0xFFFFu)));
+  return bf16_to_f32(static_cast<uint16_t>((order & 0x8000u) ? (order & 0x7FFFu) : 0x8000u | (0x8000u - order)));
+}
+__device__ __forceinline__ uint32_t bm_key(uint32_t bits, int i) { return bm_order(bits) << 16 | (0xFFFFu - i); }
+__device__ __forceinline__ uint32_t bm_max2(uint32_t a, uint32_t b) {  // of two bf16 each; a NaN loses
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
-// The threads' best keys are met by a bisection that counts how many are at or above the middle.
+// A thread takes every 256th 16-byte piece of the stretch; what lies before the first 16-byte border and
+// behind the last is one element each of the first threads.
+//
+// What bounds it at many rows: the exponentials (one of the conversion unit's operations a logit) beside the
+// bytes; at few, the chain of load, maximum, ranks and the pieces looked at again.
 __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_constant__ BeamArgs a) {
   extern __shared__ uint32_t found[];  // [k * the logits of a thread]
+  __shared__ __align__(16) uint32_t keys[kBmThreads];
   __shared__ float red_top[kBmThreads / 32];
   __shared__ double red_sum[kBmThreads / 32];
-  __shared__ uint32_t n_found;
-  const int tid = threadIdx.x, part = blockIdx.x, beam = blockIdx.y;
+  __shared__ uint32_t n_found, bound;
+  const int tid = threadIdx.x, lane = tid & 31, part = blockIdx.x, beam = blockIdx.y;
   const long long row = static_cast<long long>(blockIdx.z) * a.n_beams + beam;
   const int first = part * a.stretch, n = min(a.stretch, a.vocab - first);
-  if (tid == 0) n_found = 0;
+  if (tid == 0) n_found = 0, bound = 1;
   pdl_wait();
   const uint16_t* x = a.logits + blockIdx.z * a.group_stride + beam * a.beam_stride + first;
+  const int head = min(n, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / 2);
+  const int pieces = (n - head) / 8, tail = head + 8 * pieces;
+  const uint4* body = reinterpret_cast<const uint4*>(x + head);
+  // a thread's element outside the body, or none
+  auto single = [&](int t) { return t < 8 ? (t < head ? t : -1) : (t < 16 && tail + t - 8 < n ? tail + t - 8 : -1); };
+
   float m = -CUDART_INF_F, sum = 0.f;
-  uint32_t best = 0;
-  for (int i = tid; i < n; i += kBmThreads) {
-    const uint32_t bits = x[i];
-    const float l = bf16_to_f32(static_cast<uint16_t>(bits));
-    if (l > m) {
-      sum *= exp2f((m - l) * kBmLog2e);
-      m = l;
+  int at = -1;  // where the first m is: an element, or a piece's first element
+  bool whole = false;
+  auto raise = [&](float v, int i, bool piece) {
+    if (v > m) {
+      sum *= exp2f((m - v) * kBmLog2e);  // (-inf - v: 0; never -inf - -inf)
+      m = v;
+      at = i;
+      whole = piece;
     }
-    sum += l == -CUDART_INF_F ? 0.f : exp2f((l - m) * kBmLog2e);
-    best = max(best, bm_order(bits) << 16 | (0xFFFFu - i));
+  };
+  auto take = [&](const uint4& v, int j) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t two = bm_max2(bm_max2(w[0], w[1]), bm_max2(w[2], w[3]));
+    const float top = fmaxf(__uint_as_float(two << 16), __uint_as_float(two & 0xFFFF0000u));
+    raise(top, head + 8 * j, true);
+    if (m == -CUDART_INF_F) {
+      if (top != top) sum = top;  // nothing but NaN
+      if (at < 0) at = head + 8 * j, whole = true;
+      return;
+    }
+    float more = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      more += exp2f((__uint_as_float(w[e] << 16) - m) * kBmLog2e);
+      more += exp2f((__uint_as_float(w[e] & 0xFFFF0000u) - m) * kBmLog2e);
+    }
+    sum += more;
+  };
+  const int mine = single(tid);
+  if (mine >= 0) {
+    const float v = bf16_to_f32(x[mine]);
+    raise(v, mine, false);
+    if (at < 0) at = mine;
+    if (v != -CUDART_INF_F) sum += exp2f((v - m) * kBmLog2e);
   }
+  int j = tid;
+  for (; j + 3 * kBmThreads < pieces; j += 4 * kBmThreads) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = __ldg(body + j + u * kBmThreads);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) take(v[u], j + u * kBmThreads);
+  }
+  for (; j < pieces; j += kBmThreads) take(__ldg(body + j), j);
+  uint32_t best = 0;
+  if (at >= 0) {
+    if (whole) {  // which of the piece's elements
+      int e = 7;
+#pragma unroll
+      for (int i = 7; i >= 0; --i)
+        if (bf16_to_f32(x[at + i]) == m) e = i;
+      at += e;
+    }
+    best = bm_key(__float_as_uint(m) >> 16, at);
+  }
+  keys[tid] = best;
   // (a NaN has to stay one: nothing here compares sums)
   const float wm = warp_max(m);
   double wide = sum == 0.f ? 0.0 : static_cast<double>(sum) * exp2f((m - wm) * kBmLog2e);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
-  if ((tid & 31) == 0) red_top[tid >> 5] = wm, red_sum[tid >> 5] = wide;
-  uint32_t bound = 0;
-  for (int bit = 31; bit >= 0; --bit)  // the k-th best of the threads' best (0: fewer than k)
-    if (__syncthreads_count(best >= (bound | 1u << bit)) >= a.k) bound |= 1u << bit;
-  if (best >= max(bound, 1u))
-    for (int i = tid; i < n; i += kBmThreads) {
-      const uint32_t key = bm_order(x[i]) << 16 | (0xFFFFu - i);
-      if (key >= max(bound, 1u)) found[atomicAdd(&n_found, 1u)] = key;
+  if (lane == 0) red_top[tid >> 5] = wm, red_sum[tid >> 5] = wide;
+  __syncthreads();
+  int rank = 0;
+#pragma unroll 8
+  for (int i = 0; i < kBmThreads; i += 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(keys + i);
+    rank += (v.x > best) + (v.y > best) + (v.z > best) + (v.w > best);
+  }
+  if (rank == a.k - 1 && best != 0u) bound = best;
+  __syncthreads();
+  const uint32_t least = bound;
+  // the pieces of the threads whose best is in, each looked at by its whole warp
+  for (uint32_t in = __ballot_sync(0xffffffffu, best >= least); in != 0u; in &= in - 1) {
+    const int t = (tid & ~31) + __ffs(in) - 1;
+    for (int p = t + lane * kBmThreads; p < pieces; p += 32 * kBmThreads) {
+      const uint4 v = __ldg(body + p);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t key = bm_key((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, head + 8 * p + e);
+        if (key >= least) found[atomicAdd(&n_found, 1u)] = key;
+      }
     }
+    const int one = single(t);
+    if (lane == 0 && one >= 0) {
+      const uint32_t key = bm_key(x[one], one);
+      if (key >= least) found[atomicAdd(&n_found, 1u)] = key;
+    }
+  }
   __syncthreads();
   const int have = n_found;
   const long long list = row * a.stretches + part;
   for (int i = tid; i < have; i += kBmThreads) {
-    int rank = 0;
-    for (int j = 0; j < have && rank < a.k; ++j) rank += found[j] > found[i];
-    if (rank < a.k) a.keys[list * a.k + rank] = found[i];
+    int above = 0;
+    for (int o = 0; o < have && above < a.k; ++o) above += found[o] > found[i];
+    if (above < a.k) a.keys[list * a.k + above] = found[i];
   }
   if (tid >= have && tid < a.k) a.keys[list * a.k + tid] = 0u;
   if (tid == 0) {
@@ -229,7 +311,7 @@ extern "C" g4_status g4_beam_select(g4_ctx* ctx, const g4_bf16* logits, int64_t 
   a.stretches = (vocab + a.stretch - 1) / a.stretch;
   const size_t lists = static_cast<size_t>(n_beams) * a.stretches;
   const size_t bytes = lists * (sizeof(BeamSum) + 4 * n_select);
-  const size_t list_smem = 4 * static_cast<size_t>(n_select) * ((a.stretch + kBmThreads - 1) / kBmThreads);
+  const size_t list_smem = 4 * static_cast<size_t>(n_select) * (8 * ((a.stretch / 8 + kBmThreads - 1) / kBmThreads) + 1);
   const size_t join_smem = sizeof(BeamItem) * (kBmMaxLists + static_cast<size_t>(n_select) * n_select);
   g4_status st = allow_max_dynamic_smem(ctx, (const void*)beam_lists_kernel, list_smem, "beam lists");
   if (st == G4_OK) st = allow_max_dynamic_smem(ctx, (const void*)beam_join_kernel, join_smem, "beam join");

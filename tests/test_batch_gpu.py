@@ -489,3 +489,20 @@ def test_library_refuses(gpu_ctx):
     _sync(gpu_ctx)
     assert not t.any()
     assert ctypes.sizeof(g4.batch._RowsDesc) == 40 and ctypes.sizeof(g4.batch._WeightDesc) == 40
+
+
+def test_beam_select_zero_of_either_sign(gpu_ctx):
+    """-0 and 0 are equal scores: the lower token first, whichever sign it has."""
+    logits = torch.full((1, 2, 3000), -5.0, dtype=torch.bfloat16, device="cuda")
+    logits[0, 0, 100:140:2], logits[0, 0, 101:140:2] = -0.0, 0.0
+    logits[0, 1, 2900:] = -0.0
+    _check_beams(gpu_ctx, logits, torch.tensor([[0.0, -0.5]], device="cuda"), 64)
+
+
+@pytest.mark.parametrize("offset", range(8))
+def test_beam_select_alignments(gpu_ctx, offset):
+    """Rows that start and end anywhere between 16-byte borders."""
+    g = _gen(offset)
+    for vocab in (1, 6, 9, 15, 16, 17, 23, 300, 4100):
+        wide = _randn(g, 2, 3, vocab + 16 + offset, std=3.0)
+        _check_beams(gpu_ctx, wide[:, :, offset:offset + vocab], torch.rand((2, 3), generator=g, device="cuda"), min(5, 3 * vocab))

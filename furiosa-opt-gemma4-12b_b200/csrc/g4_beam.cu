@@ -19,6 +19,8 @@ namespace g4 {
 
 constexpr int kBmThreads = 256, kBmJoinThreads = 512;
 constexpr int kBmStretch = 65536;  // logits a block may take: 16 bits of index in a key
+constexpr int kBmQuads = 16;       // up to as many selected, four threads are a part
+constexpr int kBmNear = 8192;      // keys of a group that are copied to shared memory
 constexpr int kBmMaxLists = 1024;  // lists of a group (64 beams of 2^20 logits)
 constexpr float kBmLog2e = 1.4426950408889634f;
 
@@ -46,9 +48,15 @@ __device__ __forceinline__ float bm_logit(uint32_t order) {
   return bf16_to_f32(static_cast<uint16_t>((order & 0x8000u) ? (order & 0x7FFFu) : 0x8000u | (0x8000u - order)));
 }
 __device__ __forceinline__ uint32_t bm_key(uint32_t bits, int i) { return bm_order(bits) << 16 | (0xFFFFu - i); }
-__device__ __forceinline__ uint32_t bm_max2(uint32_t a, uint32_t b) {  // of two bf16 each; a NaN loses
+__device__ __forceinline__ float bm_exp2(float x) {  // x <= 0 (or next to it): what underflows counts for nothing
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float bm_exp(float x) { return bm_exp2(x * kBmLog2e); }
+__device__ __forceinline__ uint32_t bm_max2(uint32_t a, uint32_t b) {  // of two bf16 each; a NaN stays one
   uint32_t d;
-  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 
@@ -76,76 +84,115 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   auto single = [&](int t) { return t < 8 ? (t < head ? t : -1) : (t < 16 && tail + t - 8 < n ? tail + t - 8 : -1); };
 
   float m = -CUDART_INF_F, sum = 0.f;
-  int at = -1;  // where the first m is: an element, or a piece's first element
+  int at = -1;  // where the first m is: an element, or the first of four pieces
   bool whole = false;
-  auto raise = [&](float v, int i, bool piece) {
+  // The sum is of 2^(l log2 e - ref), one FMA a logit, where ref is m log2 e rounded to f32: what the rounding
+  // took is put back (in 64 bits) when the sum leaves the thread.
+  float ref = 0.f;
+  auto raise = [&](float v, int i, bool pieces_of_it) {
     if (v > m) {
-      sum *= exp2f((m - v) * kBmLog2e);  // (-inf - v: 0; never -inf - -inf)
+      const float to = v * kBmLog2e;
+      sum = m == -CUDART_INF_F ? sum : sum * bm_exp2(ref - to);
+      ref = to;
       m = v;
       at = i;
-      whole = piece;
+      whole = pieces_of_it;
+    } else if (at < 0) {  // (nothing but -inf so far)
+      at = i;
+      whole = pieces_of_it;
     }
-  };
-  auto take = [&](const uint4& v, int j) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    const uint32_t two = bm_max2(bm_max2(w[0], w[1]), bm_max2(w[2], w[3]));
-    const float top = fmaxf(__uint_as_float(two << 16), __uint_as_float(two & 0xFFFF0000u));
-    raise(top, head + 8 * j, true);
-    if (m == -CUDART_INF_F) {
-      if (top != top) sum = top;  // nothing but NaN
-      if (at < 0) at = head + 8 * j, whole = true;
-      return;
-    }
-    float more = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      more += exp2f((__uint_as_float(w[e] << 16) - m) * kBmLog2e);
-      more += exp2f((__uint_as_float(w[e] & 0xFFFF0000u) - m) * kBmLog2e);
-    }
-    sum += more;
+    if (v != v) sum = v;
   };
   const int mine = single(tid);
   if (mine >= 0) {
     const float v = bf16_to_f32(x[mine]);
     raise(v, mine, false);
-    if (at < 0) at = mine;
-    if (v != -CUDART_INF_F) sum += exp2f((v - m) * kBmLog2e);
+    if (m != -CUDART_INF_F) sum += bm_exp2(fmaf(v, kBmLog2e, -ref));
   }
-  int j = tid;
-  for (; j + 3 * kBmThreads < pieces; j += 4 * kBmThreads) {
-    uint4 v[4];
+  // four pieces are on their way while four are looked at; what is not there counts as -inf
+  uint4 now[4], next[4];
+  auto fetch = [&](uint4 (&v)[4], int j) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = __ldg(body + j + u * kBmThreads);
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t none = 0xFF80FF80u;
+      v[u] = j + u * kBmThreads < pieces ? __ldg(body + j + u * kBmThreads) : make_uint4(none, none, none, none);
+    }
+  };
+  fetch(now, tid);
+  for (int j = tid; j < pieces; j += 4 * kBmThreads) {
+    fetch(next, j + 4 * kBmThreads);
+    uint32_t two = bm_max2(bm_max2(now[0].x, now[0].y), bm_max2(now[0].z, now[0].w));
 #pragma unroll
-    for (int u = 0; u < 4; ++u) take(v[u], j + u * kBmThreads);
+    for (int u = 1; u < 4; ++u)
+      two = bm_max2(two, bm_max2(bm_max2(now[u].x, now[u].y), bm_max2(now[u].z, now[u].w)));
+    const uint32_t both = bm_max2(two, __byte_perm(two, 0, 0x1032));
+    raise(__uint_as_float(both << 16), j, true);
+    if (m != -CUDART_INF_F) {
+      const float2 scale = make_float2(kBmLog2e, kBmLog2e), off = make_float2(-ref, -ref);
+      float2 more[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x2 =
+              fma_f32x2(make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u)), scale, off);
+          more[e & 1] = add_f32x2(more[e & 1], make_float2(bm_exp2(x2.x), bm_exp2(x2.y)));
+        }
+      }
+      more[0] = add_f32x2(more[0], more[1]);
+      sum += more[0].x + more[0].y;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) now[u] = next[u];
   }
-  for (; j < pieces; j += kBmThreads) take(__ldg(body + j), j);
+  pdl_launch_dependents();  // (the join waits for all of this kernel)
   uint32_t best = 0;
   if (at >= 0) {
-    if (whole) {  // which of the piece's elements
-      int e = 7;
+    if (whole) {  // which of the four pieces' elements
+      const int j = at;
+      at = -1;
 #pragma unroll
-      for (int i = 7; i >= 0; --i)
-        if (bf16_to_f32(x[at + i]) == m) e = i;
-      at += e;
+      for (int u = 3; u >= 0; --u) {
+        const int p = j + u * kBmThreads;
+        if (p >= pieces) continue;
+        const uint4 v = __ldg(body + p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 7; e >= 0; --e)
+          if (__uint_as_float((w[e >> 1] >> (16 * (e & 1))) << 16) == m) at = head + 8 * p + e;
+      }
     }
-    best = bm_key(__float_as_uint(m) >> 16, at);
+    if (at >= 0) best = bm_key(__float_as_uint(m) >> 16, at);  // (none: all are NaN)
   }
-  keys[tid] = best;
+  // parts of a thread each, or of four where so few are wanted that ranking a quarter of the parts does
+  const int parts = a.k <= kBmQuads ? kBmThreads / 4 : kBmThreads;
+  uint32_t part_best = best;
+  if (a.k <= kBmQuads) {
+    part_best = max(part_best, __shfl_xor_sync(0xffffffffu, part_best, 1));
+    part_best = max(part_best, __shfl_xor_sync(0xffffffffu, part_best, 2));
+    if ((tid & 3) == 0) keys[tid >> 2] = part_best;
+  } else {
+    keys[tid] = part_best;
+  }
   // (a NaN has to stay one: nothing here compares sums)
   const float wm = warp_max(m);
-  double wide = sum == 0.f ? 0.0 : static_cast<double>(sum) * exp2f((m - wm) * kBmLog2e);
+  const double lost = (static_cast<double>(ref) - static_cast<double>(m) * kBmLog2e) * 0.6931471805599453;
+  double wide = sum == 0.f ? 0.0 : static_cast<double>(sum) * (1.0 + lost) * bm_exp(m - wm);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
   if (lane == 0) red_top[tid >> 5] = wm, red_sum[tid >> 5] = wide;
   __syncthreads();
-  int rank = 0;
-#pragma unroll 8
-  for (int i = 0; i < kBmThreads; i += 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(keys + i);
-    rank += (v.x > best) + (v.y > best) + (v.z > best) + (v.w > best);
+  if (tid < parts) {
+    const uint32_t key = keys[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < parts; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(keys + i);
+      rank += (v.x > key) + (v.y > key) + (v.z > key) + (v.w > key);
+    }
+    if (rank == a.k - 1 && key != 0u) bound = key;
   }
-  if (rank == a.k - 1 && best != 0u) bound = best;
   __syncthreads();
   const uint32_t least = bound;
   // the pieces of the threads whose best is in, each looked at by its whole warp
@@ -180,7 +227,7 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
     double total = 0.0;
     for (int w = 0; w < kBmThreads / 32; ++w) top = fmaxf(top, red_top[w]);
     for (int w = 0; w < kBmThreads / 32; ++w)
-      if (!(red_sum[w] == 0.0)) total += red_sum[w] * exp2f((red_top[w] - top) * kBmLog2e);
+      if (!(red_sum[w] == 0.0)) total += red_sum[w] * bm_exp(red_top[w] - top);
     a.sums[list] = {total, top};
   }
 }
@@ -188,38 +235,50 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
 // What is compared: the score, then the lower beam, the higher logit (scores that 64 bits cannot tell
 // apart), the lower token.
 struct BeamItem {
-  double score;
-  uint64_t rest;  // beam inverted : 16 | logit order : 16 | token inverted : 32
+  uint64_t score;  // order-preserving bits of the f64
+  uint64_t rest;   // beam inverted : 16 | logit order : 16 | token inverted : 32 (never 0)
 };
+__device__ __forceinline__ uint64_t bm_bits(double s) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(s + 0.0));  // (-0 as 0)
+  return (u >> 63) ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ double bm_score(uint64_t bits) {
+  return __longlong_as_double(static_cast<long long>((bits >> 63) ? bits & ~(1ull << 63) : ~bits));
+}
 __device__ __forceinline__ bool bm_above(const BeamItem& a, const BeamItem& b) {
   return a.score > b.score || (a.score == b.score && a.rest > b.rest);
 }
 __device__ __forceinline__ BeamItem bm_item(const BeamArgs& a, double base, int beam, int part, uint32_t key) {
   const uint32_t token = part * a.stretch + (0xFFFFu - (key & 0xFFFFu));
   const bool none = base == -CUDART_INF;  // no order of logits among the continuations of such a beam
-  return {none ? base : base + static_cast<double>(bm_logit(key >> 16)),
+  return {bm_bits(none ? base : base + static_cast<double>(bm_logit(key >> 16))),
           static_cast<uint64_t>(0xFFFFu - beam) << 48 | static_cast<uint64_t>(none ? 0u : key >> 16) << 32 |
               (0xFFFFFFFFu - token)};
 }
 
 __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
-  BeamItem* heads = reinterpret_cast<BeamItem*>(raw);            // [lists]
-  BeamItem* found = heads + kBmMaxLists;                         // [k * k]
+  BeamItem* heads = reinterpret_cast<BeamItem*>(raw);              // [kBmMaxLists]
+  BeamItem* found = heads + kBmMaxLists;                           // [k * k]
+  uint32_t* near = reinterpret_cast<uint32_t*>(found + a.k * a.k);  // the lists' keys where they have room
   __shared__ double base[G4_BEAM_MAX];
-  __shared__ BeamItem bound;
+  __shared__ int in[G4_BEAM_MAX];  // the lists whose heads are among the k best
   __shared__ uint32_t n_found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row0 = static_cast<long long>(blockIdx.x) * a.n_beams;
   const int lists = a.n_beams * a.stretches;
-  if (tid == 0) {
-    n_found = 0;
-    bound = {-CUDART_INF, 0ull};
-  }
+  if (tid == 0) n_found = 0;
+  if (tid < a.k) in[tid] = -1;
   pdl_wait();
+  const uint32_t* keys = a.keys + row0 * a.stretches * a.k;
+  if (lists * a.k <= kBmNear) {
+    for (int i = tid; i < lists * a.k; i += kBmJoinThreads) near[i] = keys[i];
+    keys = near;
+  }
   // base = scores[beam] - logsumexp, -inf for a beam that does not count
   for (int b = warp; b < a.n_beams; b += kBmJoinThreads / 32) {
     const BeamSum* st = a.sums + (row0 + b) * a.stretches;
+    const float score = a.scores[row0 + b];
     float top = -CUDART_INF_F;
     for (int i = lane; i < a.stretches; i += 32) top = fmaxf(top, st[i].top);
     top = warp_max(top);
@@ -229,49 +288,60 @@ __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) {
-      const double v = static_cast<double>(a.scores[row0 + b]) - (static_cast<double>(top) + log(total));
+      const double v = static_cast<double>(score) - (static_cast<double>(top) + log(total));
       base[b] = isfinite(v) ? v : -CUDART_INF;
     }
   }
   __syncthreads();
   // (a beam that does not count has one list, its first k tokens)
-  auto list_key = [&](int list, int i) -> uint32_t {
-    const int beam = list / a.stretches, part = list % a.stretches;
-    if (base[beam] != -CUDART_INF) return a.keys[(row0 * a.stretches + list) * a.k + i];
-    return part == 0 && i < min(a.vocab, a.k) ? 0x10000u | (0xFFFFu - i) : 0u;
+  auto key_of = [&](int beam, int part, int i, uint32_t key) -> uint32_t {
+    if (base[beam] != -CUDART_INF) return key;
+    return part == 0 && i < a.vocab ? 0x10000u | (0xFFFFu - i) : 0u;
   };
   for (int i = tid; i < lists; i += kBmJoinThreads) {
-    const uint32_t key = list_key(i, 0);
-    const int beam = i / a.stretches;
-    heads[i] = key ? bm_item(a, base[beam], beam, i % a.stretches, key) : BeamItem{-CUDART_INF, 0ull};
+    const int beam = i / a.stretches, part = i - beam * a.stretches;
+    const uint32_t key = key_of(beam, part, 0, keys[i * a.k]);
+    heads[i] = key ? bm_item(a, base[beam], beam, part, key) : BeamItem{0ull, 0ull};
   }
   __syncthreads();
-  for (int i = tid; i < lists; i += kBmJoinThreads) {
-    if (heads[i].rest == 0ull) continue;
+  // `each` threads, neighbours of one warp, rank a head
+  int each = 32;
+  while (each > 1 && each * lists > kBmJoinThreads) each >>= 1;
+  for (int i0 = 0; i0 < lists; i0 += kBmJoinThreads / each) {
+    const int i = i0 + tid / each;
+    const BeamItem mine = i < lists ? heads[i] : BeamItem{0ull, 0ull};
     int rank = 0;
-    for (int j = 0; j < lists; ++j) rank += bm_above(heads[j], heads[i]);
-    if (rank == a.k - 1) bound = heads[i];
+    if (mine.rest != 0ull) {
+#pragma unroll 4
+      for (int j = tid & (each - 1); j < lists; j += each) rank += bm_above(heads[j], mine);
+    }
+    for (int o = 1; o < each; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if ((tid & (each - 1)) == 0 && mine.rest != 0ull && rank < a.k) in[rank] = i;
   }
   __syncthreads();
-  for (int c = tid; c < lists * a.k; c += kBmJoinThreads) {
-    const int list = c / a.k;
-    if (heads[list].rest == 0ull || bm_above(bound, heads[list])) continue;
-    const uint32_t key = list_key(list, c % a.k);
+  // nothing below the last head that is in can be (with fewer lists than that, everything can)
+  const int last = in[a.k - 1];
+  const BeamItem bound = last >= 0 ? heads[last] : BeamItem{0ull, 0ull};
+  for (int c = tid; c < a.k * a.k; c += kBmJoinThreads) {
+    const int list = in[c / a.k], i = c % a.k;
+    if (list < 0) continue;
+    const int beam = list / a.stretches, part = list - beam * a.stretches;
+    const uint32_t key = key_of(beam, part, i, keys[list * a.k + i]);
     if (key == 0u) continue;
-    const int beam = list / a.stretches;
-    const BeamItem item = bm_item(a, base[beam], beam, list % a.stretches, key);
+    const BeamItem item = bm_item(a, base[beam], beam, part, key);
     if (!bm_above(bound, item)) found[atomicAdd(&n_found, 1u)] = item;
   }
   __syncthreads();
   const int have = n_found;
   for (int i = tid; i < have; i += kBmJoinThreads) {
+    const BeamItem mine = found[i];
     int rank = 0;
-    for (int j = 0; j < have && rank < a.k; ++j) rank += bm_above(found[j], found[i]);
+    for (int j = 0; j < have && rank < a.k; ++j) rank += bm_above(found[j], mine);
     if (rank < a.k) {
       const long long at = static_cast<long long>(blockIdx.x) * a.k + rank;
-      a.out_scores[at] = static_cast<float>(found[i].score);
-      a.out_beams[at] = 0xFFFF - static_cast<int>(found[i].rest >> 48);
-      a.out_tokens[at] = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(found[i].rest));
+      a.out_scores[at] = static_cast<float>(bm_score(mine.score));
+      a.out_beams[at] = 0xFFFF - static_cast<int>(mine.rest >> 48);
+      a.out_tokens[at] = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine.rest));
     }
   }
 }
@@ -301,18 +371,22 @@ extern "C" g4_status g4_beam_select(g4_ctx* ctx, const g4_bf16* logits, int64_t 
   const long long rows = static_cast<long long>(n_groups) * n_beams;
   BeamArgs a = {logits, n_groups > 1 ? group_stride : 0, n_beams > 1 ? beam_stride : 0, scores, n_beams, vocab, n_select,
                 0, 0, nullptr, nullptr, out_scores, out_beams, out_tokens};
-  // stretches of a row: enough blocks to fill the device, none of few logits, within both limits
-  const int least = (vocab + kBmStretch - 1) / kBmStretch, useful = (vocab + 4095) / 4096;
-  const long long fill = (4ll * ctx->sm_count + rows - 1) / rows;
-  int parts = fill < useful ? static_cast<int>(fill) : useful;
+  // Stretches of a row.  More of them keep the SMs busier, fewer leave the join less: of 262144 logits, 4 rows
+  // take 10.8 us in 16 stretches (12.1 in 32, 11.8 in 8), one row 8.1 in 32 (8.4 in 16), 128 rows 27.2 in 4
+  // (30.4 in 8).
+  const int least = (vocab + kBmStretch - 1) / kBmStretch;
+  const int logits_each = rows <= 2 ? 8192 : rows < 96 ? 16384 : kBmStretch;
+  int parts = (vocab + logits_each - 1) / logits_each;
   if (parts > kBmMaxLists / n_beams) parts = kBmMaxLists / n_beams;
   if (parts < least) parts = least;  // (at most 16: kBmMaxLists / 64)
   a.stretch = ((vocab + parts - 1) / parts + 7) / 8 * 8;
   a.stretches = (vocab + a.stretch - 1) / a.stretch;
   const size_t lists = static_cast<size_t>(n_beams) * a.stretches;
   const size_t bytes = lists * (sizeof(BeamSum) + 4 * n_select);
-  const size_t list_smem = 4 * static_cast<size_t>(n_select) * (8 * ((a.stretch / 8 + kBmThreads - 1) / kBmThreads) + 1);
-  const size_t join_smem = sizeof(BeamItem) * (kBmMaxLists + static_cast<size_t>(n_select) * n_select);
+  const size_t list_smem = 4 * static_cast<size_t>(n_select) * (8 * ((a.stretch / 8 + kBmThreads - 1) / kBmThreads) + 1) *
+                            (n_select <= kBmQuads ? 4 : 1);
+  const size_t join_smem = sizeof(BeamItem) * (kBmMaxLists + static_cast<size_t>(n_select) * n_select) +
+                           (lists * n_select <= kBmNear ? 4 * lists * n_select : 0);
   g4_status st = allow_max_dynamic_smem(ctx, (const void*)beam_lists_kernel, list_smem, "beam lists");
   if (st == G4_OK) st = allow_max_dynamic_smem(ctx, (const void*)beam_join_kernel, join_smem, "beam join");
   // as many groups at a time as the context's lists have room for

@@ -14,31 +14,6 @@
 
 namespace g4 {
 
-// Two f32 side by side: Blackwell's FMA units take them in one instruction.
-__device__ __forceinline__ float2 nv_fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 nv_add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 nv_mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
 __device__ __forceinline__ float2 nv_halves(uint32_t h) {
   return make_float2(__half2float(__ushort_as_half(static_cast<uint16_t>(h))),
                      __half2float(__ushort_as_half(static_cast<uint16_t>(h >> 16))));
@@ -185,7 +160,7 @@ __global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_cons
     if (i > 0 && i * T >= 4 * a.kblocks) break;  // (of all threads)
     float2 y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = nv_mul2(make_float2(lo_f32(w[i][e]), hi_f32(w[i][e])), g2);
+    for (int e = 0; e < 8; ++e) y[e] = mul_f32x2(make_float2(lo_f32(w[i][e]), hi_f32(w[i][e])), g2);
     float m = lo_f32(own[i]) * g;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -194,7 +169,7 @@ __global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_cons
       const float2 r2 = make_float2(rcp, rcp);
       float2 q[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = nv_add2(nv_fma2(y[e], r2, snap), unsnap);
+      for (int e = 0; e < 8; ++e) q[e] = add_f32x2(fma_f32x2(y[e], r2, snap), unsnap);
       const uint2 c = make_uint2(nv_e2m1x8(q[0], q[1], q[2], q[3]), nv_e2m1x8(q[4], q[5], q[6], q[7]));
       if (p + 1 < P) {  // what the piece leaves, and its largest
         const float2 s2 = make_float2(-sf, -sf);
@@ -204,7 +179,7 @@ __global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_cons
         m = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          y[e] = nv_fma2(nv_halves(h[e]), s2, y[e]);
+          y[e] = fma_f32x2(nv_halves(h[e]), s2, y[e]);
           m = pa_max3(m, fabsf(y[e].x), fabsf(y[e].y));
         }
       }

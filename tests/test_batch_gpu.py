@@ -387,6 +387,9 @@ def test_beam_select_values_that_are_not_finite(gpu_ctx):
     scores = torch.zeros((4, 7), device="cuda")
     scores[:, 4], scores[:, 5] = math.nan, math.inf
     _check_beams(gpu_ctx, logits, scores, 64)
+    wide = torch.full((1, 3, 40000), -math.inf, dtype=torch.bfloat16, device="cuda")
+    wide[0, :, 7], wide[0, 0, 39000], wide[0, 1, 8:4000:9] = 1.0, math.nan, math.nan  # NaN with nothing but -inf about it
+    _check_beams(gpu_ctx, wide, torch.zeros((1, 3), device="cuda"), 9)
     scores[1, 0], scores[2, 6], scores[3, [0, 6]] = -math.inf, math.nan, -math.inf
     _check_beams(gpu_ctx, logits, scores, 64)
 

@@ -76,6 +76,30 @@ def _matrix(ctx: Context, name: str, t, rows, cols, dtypes=(_BF16,)) -> tuple:
     return t.data_ptr(), row if shape[0] > 1 else max(row, shape[1])
 
 
+def _operand(ctx: Context, name: str, t, rows, cols, dtype=_BF16) -> tuple:
+    """_matrix, and its rows and columns: (rows, columns, pointer, row stride), in few steps where all is well
+    (a call of few rows takes the GPU less than its checks take the host)."""
+    try:
+        if t.get_device() == ctx.device and t.dtype is dtype:
+            (r, c), (stride, one) = t.shape, t.stride()
+            if one == 1 and (rows is None or r == rows) and (cols is None or c == cols) and r < 2 ** 31 > c:
+                return r, c, t.data_ptr(), stride if r > 1 else c
+    except (AttributeError, ValueError):
+        pass
+    at = _matrix(ctx, name, t, rows, cols, (dtype,))
+    return *t.shape, *at
+
+
+def _vector(ctx: Context, name: str, t, n, dtype) -> int:
+    """A contiguous [n] operand's pointer."""
+    try:
+        if t.get_device() == ctx.device and t.dtype is dtype and t.shape == (n,) and t.stride(0) == 1:
+            return t.data_ptr()
+    except (AttributeError, IndexError):
+        pass
+    return _whole(ctx, name, t, (n,), (dtype,))
+
+
 def _whole(ctx: Context, name: str, t, shape: tuple, dtypes) -> int:
     _tensor(ctx, name, t, dtypes, len(shape))
     if t.shape != shape or not t.is_contiguous():
@@ -86,22 +110,23 @@ def _whole(ctx: Context, name: str, t, shape: tuple, dtypes) -> int:
 def embed_tokens(ctx: Context, table, tokens, out, scale: float = EMBED_SCALE) -> None:
     """out[t] = bf16(table[tokens[t]] * scale) (g4_embed_tokens): table bf16 [vocab, dim] contiguous,
     tokens int32 [n], out bf16 [n, dim].  An id outside the table gives zeros and a device status bit."""
-    vocab, dim = _tensor(ctx, "table", table, (_BF16,), 2).shape
-    n = _tensor(ctx, "tokens", tokens, (_I32,), 1).shape[0]
-    _whole(ctx, "table", table, (vocab, dim), (_BF16,))
-    ids = _whole(ctx, "tokens", tokens, (n,), (_I32,))
-    to = _matrix(ctx, "out", out, n, dim)
+    vocab, dim, rows, stride = _operand(ctx, "table", table, None, None)
+    n, _, to, out_stride = _operand(ctx, "out", out, None, dim)
+    ids = _vector(ctx, "tokens", tokens, n, _I32)
+    if stride != dim:
+        raise ValueError("table: must be contiguous")
     if n:
-        ctx._check("g4_embed_tokens", LIB.g4_embed_tokens(ctx.handle, table.data_ptr(), vocab, dim, ids, n, scale, *to))
+        ctx._check("g4_embed_tokens", LIB.g4_embed_tokens(ctx.handle, rows, vocab, dim, ids, n, scale, to, out_stride))
 
 
 def residual_norm(ctx: Context, x, rms_weight, residual, out) -> None:
     """out = bf16(residual + rmsnorm(x) * rms_weight) by rows (g4_residual_norm); out may be residual."""
-    n, dim = _tensor(ctx, "x", x, (_BF16,), 2).shape
-    xa, ra, oa = _matrix(ctx, "x", x, n, dim), _matrix(ctx, "residual", residual, n, dim), _matrix(ctx, "out", out, n, dim)
-    w = _whole(ctx, "rms_weight", rms_weight, (dim,), (_BF16,))
+    n, dim, xp, xs = _operand(ctx, "x", x, None, None)
+    _, _, rp, rs = _operand(ctx, "residual", residual, n, dim)
+    _, _, op, os = _operand(ctx, "out", out, n, dim)
+    w = _vector(ctx, "rms_weight", rms_weight, dim, _BF16)
     if n:
-        ctx._check("g4_residual_norm", LIB.g4_residual_norm(ctx.handle, *xa, w, *ra, n, dim, *oa))
+        ctx._check("g4_residual_norm", LIB.g4_residual_norm(ctx.handle, xp, xs, w, rp, rs, n, dim, op, os))
 
 
 class Nvfp4Rows:
@@ -167,35 +192,33 @@ def _rows_of(ctx: Context, rows: Nvfp4Rows, n: int) -> None:
 def nvfp4_quantize(ctx: Context, x, rows: Nvfp4Rows, rms_weight=None) -> None:
     """x (bf16 [n, cols]), or rmsnorm(x) * rms_weight rounded to bf16, into the first n rows of `rows`
     (g4_nvfp4_quantize)."""
-    xa = _matrix(ctx, "x", x, None, rows.cols)
-    n = x.shape[0]
+    n, _, xp, xs = _operand(ctx, "x", x, None, rows.cols)
     _rows_of(ctx, rows, n)
-    w = None if rms_weight is None else _whole(ctx, "rms_weight", rms_weight, (rows.cols,), (_BF16,))
+    w = None if rms_weight is None else _vector(ctx, "rms_weight", rms_weight, rows.cols, _BF16)
     if n:
-        ctx._check("g4_nvfp4_quantize", LIB.g4_nvfp4_quantize(ctx.handle, *xa, n, w, rows.desc))
+        ctx._check("g4_nvfp4_quantize", LIB.g4_nvfp4_quantize(ctx.handle, xp, xs, n, w, rows.desc))
 
 
 def nvfp4_dequantize(ctx: Context, rows: Nvfp4Rows, out) -> None:
     """The values of the first n rows, rounded to bf16, into out [n, cols] (g4_nvfp4_dequantize)."""
-    oa = _matrix(ctx, "out", out, None, rows.cols)
-    n = out.shape[0]
+    n, _, op, os = _operand(ctx, "out", out, None, rows.cols)
     _rows_of(ctx, rows, n)
     if n:
-        ctx._check("g4_nvfp4_dequantize", LIB.g4_nvfp4_dequantize(ctx.handle, rows.desc, n, *oa))
+        ctx._check("g4_nvfp4_dequantize", LIB.g4_nvfp4_dequantize(ctx.handle, rows.desc, n, op, os))
 
 
 def nvfp4_matmul(ctx: Context, rows: Nvfp4Rows, weight: Nvfp4Weight, out) -> None:
     """out [n, weight.rows] = the first n rows times the weight's rows (g4_nvfp4_matmul); out bf16, or
     f32 (a tensor-parallel rank's partial sums)."""
-    oa = _matrix(ctx, "out", out, None, weight.rows, (_BF16, _F32))
-    n = out.shape[0]
+    f32 = isinstance(out, torch.Tensor) and out.dtype is _F32
+    n, _, op, os = _operand(ctx, "out", out, None, weight.rows, _F32 if f32 else _BF16)
     _rows_of(ctx, rows, n)
     if weight.device != ctx.device:
         raise ValueError(f"weight: on cuda:{weight.device}, the context is on cuda:{ctx.device}")
     if weight.cols != rows.cols:
         raise ValueError(f"rows of {rows.cols} values, a weight of {weight.cols}")
     if n:
-        ctx._check("g4_nvfp4_matmul", LIB.g4_nvfp4_matmul(ctx.handle, rows.desc, n, weight.desc, *oa, out.dtype == _F32))
+        ctx._check("g4_nvfp4_matmul", LIB.g4_nvfp4_matmul(ctx.handle, rows.desc, n, weight.desc, op, os, f32))
 
 
 def beam_select(ctx: Context, logits, scores, out_scores, out_beams, out_tokens) -> None:
@@ -204,19 +227,21 @@ def beam_select(ctx: Context, logits, scores, out_scores, out_beams, out_tokens)
     count); out_scores f32, out_beams and out_tokens int32 [groups, select], best first, equal scores
     in the order of (beam, token)."""
     groups, beams, vocab = _tensor(ctx, "logits", logits, (_BF16,), 3).shape
-    if vocab > 1 and logits.stride(2) != 1:
+    group_stride, beam_stride, one = logits.stride()
+    if vocab > 1 and one != 1:
         raise ValueError("logits: the last dimension must be contiguous")
-    given = _whole(ctx, "scores", scores, (groups, beams), (_F32,))
-    select = _tensor(ctx, "out_scores", out_scores, (_F32,), 2).shape[1]
-    outs = (_whole(ctx, "out_scores", out_scores, (groups, select), (_F32,)),
-            _whole(ctx, "out_beams", out_beams, (groups, select), (_I32,)),
-            _whole(ctx, "out_tokens", out_tokens, (groups, select), (_I32,)))
+    _, select, best, stride = _operand(ctx, "out_scores", out_scores, groups, None, _F32)
+    given, given_stride = _operand(ctx, "scores", scores, groups, beams, _F32)[2:]
+    of, of_stride = _operand(ctx, "out_beams", out_beams, groups, select, _I32)[2:]
+    to, to_stride = _operand(ctx, "out_tokens", out_tokens, groups, select, _I32)[2:]
+    if given_stride != beams or (stride, of_stride, to_stride) != (select,) * 3:
+        raise ValueError("scores and outputs must be contiguous")
     if not 1 <= beams <= BEAM_MAX or not 1 <= select <= BEAM_MAX or not 1 <= vocab <= 2 ** 20 or select > beams * vocab:
         raise ValueError(f"{select} of {beams} beams of {vocab} tokens: expected up to {BEAM_MAX} of up to {BEAM_MAX} beams of up "
                          "to 2^20 tokens, no more than there are")
     if groups:
         ctx._check("g4_beam_select", LIB.g4_beam_select(
-            ctx.handle, logits.data_ptr(), logits.stride(0), logits.stride(1), given, groups, beams, vocab, select, *outs))
+            ctx.handle, logits.data_ptr(), group_stride, beam_stride, given, groups, beams, vocab, select, best, of, to))
 
 
 __all__ = ["Nvfp4Rows", "Nvfp4Weight", "embed_tokens", "residual_norm", "nvfp4_quantize", "nvfp4_dequantize",

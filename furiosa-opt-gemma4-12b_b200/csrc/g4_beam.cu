@@ -70,11 +70,12 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   __shared__ __align__(16) uint32_t keys[kBmThreads];
   __shared__ float red_top[kBmThreads / 32];
   __shared__ double red_sum[kBmThreads / 32];
-  __shared__ uint32_t n_found, bound;
+  __shared__ uint32_t n_found, n_who, bound;
+  __shared__ uint8_t who[kBmThreads];
   const int tid = threadIdx.x, lane = tid & 31, part = blockIdx.x, beam = blockIdx.y;
   const long long row = static_cast<long long>(blockIdx.z) * a.n_beams + beam;
   const int first = part * a.stretch, n = min(a.stretch, a.vocab - first);
-  if (tid == 0) n_found = 0, bound = 1;
+  if (tid == 0) n_found = 0, n_who = 0, bound = 1;
   pdl_wait();
   const uint16_t* x = a.logits + blockIdx.z * a.group_stride + beam * a.beam_stride + first;
   const int head = min(n, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / 2);
@@ -87,12 +88,14 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   int at = -1;  // where the first m is: an element, or the first of four pieces
   bool whole = false;
   // The sum is of 2^(l log2 e - ref), one FMA a logit, where ref is m log2 e rounded to f32: what the rounding
-  // took is put back (in 64 bits) when the sum leaves the thread.
+  // took is put back (in 64 bits) when the sum leaves the thread.  Where m is beyond 2^100 (rows masked with
+  // the lowest number there is) ref might not be finite: the difference to m comes first there.
   float ref = 0.f;
+  auto far = [](float v) { return fabsf(v) > 0x1p100f; };
   auto raise = [&](float v, int i, bool pieces_of_it) {
     if (v > m) {
       const float to = v * kBmLog2e;
-      sum = m == -CUDART_INF_F ? sum : sum * bm_exp2(ref - to);
+      if (m != -CUDART_INF_F) sum *= far(m) || far(v) ? bm_exp(m - v) : bm_exp2(ref - to);
       ref = to;
       m = v;
       at = i;
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   if (mine >= 0) {
     const float v = bf16_to_f32(x[mine]);
     raise(v, mine, false);
-    if (m != -CUDART_INF_F) sum += bm_exp2(fmaf(v, kBmLog2e, -ref));
+    if (m != -CUDART_INF_F) sum += bm_exp(v - m);
   }
   // four pieces are on their way while four are looked at; what is not there counts as -inf
   uint4 now[4], next[4];
@@ -127,7 +130,13 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
       two = bm_max2(two, bm_max2(bm_max2(now[u].x, now[u].y), bm_max2(now[u].z, now[u].w)));
     const uint32_t both = bm_max2(two, __byte_perm(two, 0, 0x1032));
     raise(__uint_as_float(both << 16), j, true);
-    if (m != -CUDART_INF_F) {
+    if (far(m) && m != -CUDART_INF_F) {
+      for (int u = 0; u < 4; ++u)
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t w = e == 0 ? now[u].x : e == 1 ? now[u].y : e == 2 ? now[u].z : now[u].w;
+          sum += bm_exp(__uint_as_float(w << 16) - m) + bm_exp(__uint_as_float(w & 0xFFFF0000u) - m);
+        }
+    } else if (m != -CUDART_INF_F) {
       const float2 scale = make_float2(kBmLog2e, kBmLog2e), off = make_float2(-ref, -ref);
       float2 more[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -177,7 +186,7 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   }
   // (a NaN has to stay one: nothing here compares sums)
   const float wm = warp_max(m);
-  const double lost = (static_cast<double>(ref) - static_cast<double>(m) * kBmLog2e) * 0.6931471805599453;
+  const double lost = far(m) ? 0.0 : (static_cast<double>(ref) - static_cast<double>(m) * kBmLog2e) * 0.6931471805599453;
   double wide = sum == 0.f ? 0.0 : static_cast<double>(sum) * (1.0 + lost) * bm_exp(m - wm);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
@@ -195,22 +204,28 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   }
   __syncthreads();
   const uint32_t least = bound;
-  // the pieces of the threads whose best is in, each looked at by its whole warp
-  for (uint32_t in = __ballot_sync(0xffffffffu, best >= least); in != 0u; in &= in - 1) {
-    const int t = (tid & ~31) + __ffs(in) - 1;
-    for (int p = t + lane * kBmThreads; p < pieces; p += 32 * kBmThreads) {
+  // the threads whose best is in, and then all of their pieces by all threads
+  if (best >= least) who[atomicAdd(&n_who, 1u)] = static_cast<uint8_t>(tid);
+  __syncthreads();
+  const int turns = (pieces + kBmThreads - 1) / kBmThreads + 1;  // pieces of a thread, and the element outside
+  for (int c = tid; c < static_cast<int>(n_who) * turns; c += kBmThreads) {
+    const int q = c / turns, turn = c - q * turns, t = who[q], p = t + turn * kBmThreads;
+    if (turn == turns - 1) {
+      const int one = single(t);
+      if (one < 0) continue;
+      const uint32_t key = bm_key(x[one], one);
+      if (key >= least) found[atomicAdd(&n_found, 1u)] = key;
+    } else if (p < pieces) {
       const uint4 v = __ldg(body + p);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      // (most pieces have nothing: their largest says so)
+      const uint32_t two = bm_max2(bm_max2(w[0], w[1]), bm_max2(w[2], w[3]));
+      if (max(bm_order(two & 0xFFFFu), bm_order(two >> 16)) < least >> 16) continue;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t key = bm_key((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, head + 8 * p + e);
         if (key >= least) found[atomicAdd(&n_found, 1u)] = key;
       }
-    }
-    const int one = single(t);
-    if (lane == 0 && one >= 0) {
-      const uint32_t key = bm_key(x[one], one);
-      if (key >= least) found[atomicAdd(&n_found, 1u)] = key;
     }
   }
   __syncthreads();
@@ -218,17 +233,22 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   const long long list = row * a.stretches + part;
   for (int i = tid; i < have; i += kBmThreads) {
     int above = 0;
-    for (int o = 0; o < have && above < a.k; ++o) above += found[o] > found[i];
+#pragma unroll 4
+    for (int o = 0; o < have; ++o) above += found[o] > found[i];
     if (above < a.k) a.keys[list * a.k + above] = found[i];
   }
   if (tid >= have && tid < a.k) a.keys[list * a.k + tid] = 0u;
-  if (tid == 0) {
-    float top = -CUDART_INF_F;
-    double total = 0.0;
-    for (int w = 0; w < kBmThreads / 32; ++w) top = fmaxf(top, red_top[w]);
-    for (int w = 0; w < kBmThreads / 32; ++w)
-      if (!(red_sum[w] == 0.0)) total += red_sum[w] * bm_exp(red_top[w] - top);
-    a.sums[list] = {total, top};
+  if (tid < kBmThreads / 32) {
+    constexpr uint32_t kAll = (1u << (kBmThreads / 32)) - 1;
+    const float mine_top = red_top[tid];
+    float top = mine_top;
+#pragma unroll
+    for (int o = kBmThreads / 64; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+    double total = red_sum[tid];
+    if (!(total == 0.0)) total *= bm_exp(mine_top - top);
+#pragma unroll
+    for (int o = kBmThreads / 64; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
+    if (tid == 0) a.sums[list] = {total, top};
   }
 }
 
@@ -248,10 +268,13 @@ __device__ __forceinline__ double bm_score(uint64_t bits) {
 __device__ __forceinline__ bool bm_above(const BeamItem& a, const BeamItem& b) {
   return a.score > b.score || (a.score == b.score && a.rest > b.rest);
 }
-__device__ __forceinline__ BeamItem bm_item(const BeamArgs& a, double base, int beam, int part, uint32_t key) {
+struct BeamBase {  // of a beam: its largest logit, and scores[beam] - log sum exp(l - largest), -inf if it does not count
+  double top, rest;
+};
+__device__ __forceinline__ BeamItem bm_item(const BeamArgs& a, const BeamBase& base, int beam, int part, uint32_t key) {
   const uint32_t token = part * a.stretch + (0xFFFFu - (key & 0xFFFFu));
-  const bool none = base == -CUDART_INF;  // no order of logits among the continuations of such a beam
-  return {bm_bits(none ? base : base + static_cast<double>(bm_logit(key >> 16))),
+  const bool none = base.rest == -CUDART_INF;  // no order of logits among the continuations of such a beam
+  return {bm_bits(none ? base.rest : base.rest + (static_cast<double>(bm_logit(key >> 16)) - base.top)),
           static_cast<uint64_t>(0xFFFFu - beam) << 48 | static_cast<uint64_t>(none ? 0u : key >> 16) << 32 |
               (0xFFFFFFFFu - token)};
 }
@@ -261,7 +284,7 @@ __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_
   BeamItem* heads = reinterpret_cast<BeamItem*>(raw);              // [kBmMaxLists]
   BeamItem* found = heads + kBmMaxLists;                           // [k * k]
   uint32_t* near = reinterpret_cast<uint32_t*>(found + a.k * a.k);  // the lists' keys where they have room
-  __shared__ double base[G4_BEAM_MAX];
+  __shared__ BeamBase base[G4_BEAM_MAX];
   __shared__ int in[G4_BEAM_MAX];  // the lists whose heads are among the k best
   __shared__ uint32_t n_found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -275,7 +298,6 @@ __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_
     for (int i = tid; i < lists * a.k; i += kBmJoinThreads) near[i] = keys[i];
     keys = near;
   }
-  // base = scores[beam] - logsumexp, -inf for a beam that does not count
   for (int b = warp; b < a.n_beams; b += kBmJoinThreads / 32) {
     const BeamSum* st = a.sums + (row0 + b) * a.stretches;
     const float score = a.scores[row0 + b];
@@ -288,14 +310,14 @@ __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) {
-      const double v = static_cast<double>(score) - (static_cast<double>(top) + log(total));
-      base[b] = isfinite(v) ? v : -CUDART_INF;
+      const double v = static_cast<double>(score) - log(total);
+      base[b] = {static_cast<double>(top), isfinite(v) && isfinite(top) ? v : -CUDART_INF};
     }
   }
   __syncthreads();
   // (a beam that does not count has one list, its first k tokens)
   auto key_of = [&](int beam, int part, int i, uint32_t key) -> uint32_t {
-    if (base[beam] != -CUDART_INF) return key;
+    if (base[beam].rest != -CUDART_INF) return key;
     return part == 0 && i < a.vocab ? 0x10000u | (0xFFFFu - i) : 0u;
   };
   for (int i = tid; i < lists; i += kBmJoinThreads) {

@@ -87,7 +87,9 @@ def matmul(x, w, fx, fw):
 def beam_select(logits, scores, k):
     """(scores, beams, tokens) of each group's k best, equal scores in the order of (beam, token)."""
     logits, scores = logits.double(), scores.double()
-    base = scores - torch.logsumexp(logits, -1)
-    s = torch.where(torch.isfinite(base)[..., None], base[..., None] + logits, -torch.inf).flatten(1)
+    top = logits.amax(-1, keepdim=True)
+    base = scores - torch.log(torch.exp(logits - top).sum(-1))
+    counts = torch.isfinite(base) & torch.isfinite(top[..., 0])
+    s = torch.where(counts[..., None], base[..., None] + (logits - top), -torch.inf).flatten(1)
     best, at = torch.sort(s, dim=1, descending=True, stable=True)
     return best[:, :k], at[:, :k] // logits.shape[-1], at[:, :k] % logits.shape[-1]

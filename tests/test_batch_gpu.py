@@ -394,6 +394,19 @@ def test_beam_select_values_that_are_not_finite(gpu_ctx):
     _check_beams(gpu_ctx, logits, scores, 64)
 
 
+def test_beam_select_lowest_and_largest_numbers(gpu_ctx):
+    """Masks of the type's lowest value, rows of nothing else, logits as large as the type's."""
+    low, high = torch.finfo(torch.bfloat16).min, torch.finfo(torch.bfloat16).max
+    logits = _randn(_gen(13), 5, 3, 9000)
+    logits[0, 0, 5:] = low
+    logits[1] = low
+    logits[2, 1, ::2], logits[2, 2, 77] = low, high
+    logits[3, :, 100:200] = high
+    logits[4, 0] = low
+    logits[4, 0, 8000] = 2.0 ** 101
+    _check_beams(gpu_ctx, logits, torch.tensor([[0.0, -1.0, -2.0]] * 5, device="cuda"), 16)
+
+
 def test_beam_select_scores_far_apart(gpu_ctx):
     g = _gen(11)
     logits = _randn(g, 2, 3, 2000, std=20.0)

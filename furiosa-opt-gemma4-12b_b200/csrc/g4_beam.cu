@@ -393,12 +393,12 @@ extern "C" g4_status g4_beam_select(g4_ctx* ctx, const g4_bf16* logits, int64_t 
   const long long rows = static_cast<long long>(n_groups) * n_beams;
   BeamArgs a = {logits, n_groups > 1 ? group_stride : 0, n_beams > 1 ? beam_stride : 0, scores, n_beams, vocab, n_select,
                 0, 0, nullptr, nullptr, out_scores, out_beams, out_tokens};
-  // Stretches of a row.  More of them keep the SMs busier, fewer leave the join less: of 262144 logits, 4 rows
-  // take 10.8 us in 16 stretches (12.1 in 32, 11.8 in 8), one row 8.1 in 32 (8.4 in 16), 128 rows 27.2 in 4
-  // (30.4 in 8).
-  const int least = (vocab + kBmStretch - 1) / kBmStretch;
-  const int logits_each = rows <= 2 ? 8192 : rows < 96 ? 16384 : kBmStretch;
-  int parts = (vocab + logits_each - 1) / logits_each;
+  // Stretches of a row: more of them keep the SMs busier, fewer leave the join less.  Of 262144 logits, one row
+  // takes 7.6 us in 32 stretches (8.2 in 16), 4 rows 9.3 in 16 (10.6 in 8 and in 32), 64 rows 18.4 in 8 (20.6 in
+  // 16), 128 rows 26.4 in 4 (27.9 in 8); 4 rows of 32000 8.5 in 16 (10.2 in 4).
+  const int least = (vocab + kBmStretch - 1) / kBmStretch, useful = (vocab + 2047) / 2048;
+  int parts = rows <= 2 ? 32 : rows <= 32 ? 16 : rows < 96 ? 8 : 4;
+  if (parts > useful) parts = useful;
   if (parts > kBmMaxLists / n_beams) parts = kBmMaxLists / n_beams;
   if (parts < least) parts = least;  // (at most 16: kBmMaxLists / 64)
   a.stretch = ((vocab + parts - 1) / parts + 7) / 8 * 8;

@@ -295,6 +295,7 @@ constexpr int kNvPairThreads = 320;  // warp 0 copies, 1 MMA (leader) and tensor
 struct NvPairArgs {
   NvMatmulArgs a;
   int cols, blocks, stages, stage_bytes, k_stages, kblocks, row_tiles, tiles;
+  int early;                            // the weights may be fetched before the previous kernel is done
   int sf_cols, acc_step, first_chunks;  // scale columns; column of the second sums; chunks of 32 columns per warp in the overlap
 };
 struct NvPairBars {
@@ -362,7 +363,6 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      pdl_wait();
       const uint32_t full0 = pa_map_to(smem_u32(&sm.full[0]), 0);
       const uint32_t bytes = 16384 + P * half * 128 + 2048 + P * kBlocks * 2048;
       bool ok = true;
@@ -370,17 +370,27 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
       auto free = [&]() {  // the stage's last products are done
         return at.passed < static_cast<uint32_t>(t.stages) || pa_wait(&sm.empty[at.stage], at.parity ^ 1, abort, budget);
       };
+      auto weights = [&](int n0, int ks, int st) {
+        const uint32_t to = base + st * t.stage_bytes, bar = full0 + 8 * st;
+        pa_expect_cluster(bar, bytes);
+        nv_pair_tma(to, &wmap, ks * 128, n0, 0, bar);
+        nv_pair_tma(to + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
+      };
+      // the first tile's weights, as far as the ring goes, while the activations are still being quantised
+      const int ahead = t.early ? min(t.stages, t.k_stages) : 0;
+      for (int ks = 0; ks < ahead; ++ks) weights(pair % t.row_tiles * 256 + 128 * cta, ks, ks);
+      pdl_wait();
+      pdl_launch_dependents();
       for (int tile = pair; tile < t.tiles && ok; tile += pairs) {
         const int n0 = tile % t.row_tiles * 256 + 128 * cta, m0 = tile / t.row_tiles * t.cols;
         for (int ks = 0; ks < t.k_stages && (ok = free()); ++ks) {
           const uint32_t to = base + at.stage * t.stage_bytes, bar = full0 + 8 * at.stage;
-          pa_expect_cluster(bar, bytes);
-          nv_pair_tma(to, &wmap, ks * 128, n0, 0, bar);
+          if (at.passed >= static_cast<uint32_t>(ahead)) weights(n0, ks, at.stage);
 #pragma unroll
-          for (int p = 0; p < P; ++p) nv_pair_tma(to + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
-          nv_pair_tma(to + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
-#pragma unroll
-          for (int p = 0; p < P; ++p) nv_pair_tma(to + sx_at + p * kBlocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
+          for (int p = 0; p < P; ++p) {
+            nv_pair_tma(to + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
+            nv_pair_tma(to + sx_at + p * kBlocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
+          }
           at.next();
         }
       }
@@ -519,7 +529,7 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
         }
       }
     }
-    if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // (shared memory is still there for them)
     __syncwarp();
     if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   }
@@ -585,6 +595,7 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   NvPairArgs t = {};
   t.a = a;
   t.cols = cols;
+  t.early = ctx->weights_ahead;
   t.blocks = cols > 128 ? 2 : 1;
   t.kblocks = (a.k + 63) / 64;
   t.k_stages = (t.kblocks + 3) / 4;

@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   pa_fence_before();
   __syncthreads();
   pa_fence_after();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase),
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase),
                  "r"(static_cast<uint32_t>(t.tmem_cols)));
 }
 
@@ -289,13 +290,12 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
 // gets the sums of its 128 weight rows.  Pairs take tiles in turn.
 //
 // Tensor memory: two sums of `cols` columns and one stage's scales do not fit side by side at 256, so the
-// sums overlap by `overlap` columns: the next tile's products start once these have been read.
+// sums overlap (columns acc_step to cols): the next tile's products start once these have been read.
 constexpr int kNvPairThreads = 320;  // warp 0 copies, 1 MMA (leader) and tensor memory, 2-9 output
 
 struct NvPairArgs {
   NvMatmulArgs a;
   int cols, blocks, stages, stage_bytes, k_stages, kblocks, row_tiles, tiles;
-  int early;                            // the weights may be fetched before the previous kernel is done
   int sf_cols, acc_step, first_chunks;  // scale columns; column of the second sums; chunks of 32 columns per warp in the overlap
 };
 struct NvPairBars {
@@ -370,27 +370,19 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
       auto free = [&]() {  // the stage's last products are done
         return at.passed < static_cast<uint32_t>(t.stages) || pa_wait(&sm.empty[at.stage], at.parity ^ 1, abort, budget);
       };
-      auto weights = [&](int n0, int ks, int st) {
-        const uint32_t to = base + st * t.stage_bytes, bar = full0 + 8 * st;
-        pa_expect_cluster(bar, bytes);
-        nv_pair_tma(to, &wmap, ks * 128, n0, 0, bar);
-        nv_pair_tma(to + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
-      };
-      // the first tile's weights, as far as the ring goes, while the activations are still being quantised
-      const int ahead = t.early ? min(t.stages, t.k_stages) : 0;
-      for (int ks = 0; ks < ahead; ++ks) weights(pair % t.row_tiles * 256 + 128 * cta, ks, ks);
       pdl_wait();
       pdl_launch_dependents();
       for (int tile = pair; tile < t.tiles && ok; tile += pairs) {
         const int n0 = tile % t.row_tiles * 256 + 128 * cta, m0 = tile / t.row_tiles * t.cols;
         for (int ks = 0; ks < t.k_stages && (ok = free()); ++ks) {
           const uint32_t to = base + at.stage * t.stage_bytes, bar = full0 + 8 * at.stage;
-          if (at.passed >= static_cast<uint32_t>(ahead)) weights(n0, ks, at.stage);
+          pa_expect_cluster(bar, bytes);
+          nv_pair_tma(to, &wmap, ks * 128, n0, 0, bar);
 #pragma unroll
-          for (int p = 0; p < P; ++p) {
-            nv_pair_tma(to + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
-            nv_pair_tma(to + sx_at + p * kBlocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
-          }
+          for (int p = 0; p < P; ++p) nv_pair_tma(to + x_at + p * half * 128, &xmap, ks * 128, m0 + half * cta, p, bar);
+          nv_pair_tma(to + sw_at, &wsmap, ks * 256, n0 >> 7, 0, bar);
+#pragma unroll
+          for (int p = 0; p < P; ++p) nv_pair_tma(to + sx_at + p * kBlocks * 2048, &xsmap, ks * 256, m0 >> 7, p, bar);
           at.next();
         }
       }
@@ -546,6 +538,14 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
 }
 
 // ---------------------------------------------------------------------------- host side
+// Shared memory of a CTA that takes `tmem_cols` columns of tensor memory: at least its share of an SM's, so that
+// CTAs which fit an SM's shared memory together fit its tensor memory too.  (A CTA that waits for columns while
+// its cluster waits for it, beside another cluster's in the same position, would wait for good.)
+constexpr size_t kNvSmem = 229376;
+static size_t nv_smem(size_t need, int tmem_cols) {
+  const size_t share = kNvSmem * tmem_cols / 512;
+  return need > share ? need : share;
+}
 // Codes [planes][rows][cols bytes] (row stride cols), box of box_rows x 128 bytes, 128-byte swizzle;
 // what lies past the rows and the columns reads as zeros.
 static bool nv_code_map(CUtensorMap* m, const void* p, int cols, int rows, int planes, size_t plane, int box_rows) {
@@ -595,7 +595,6 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   NvPairArgs t = {};
   t.a = a;
   t.cols = cols;
-  t.early = ctx->weights_ahead;
   t.blocks = cols > 128 ? 2 : 1;
   t.kblocks = (a.k + 63) / 64;
   t.k_stages = (t.kblocks + 3) / 4;
@@ -607,9 +606,9 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   t.first_chunks = (cols - t.acc_step + 63) / 64;
   t.stage_bytes = 16384 + a.pieces * (cols / 2) * 128 + 2048 + a.pieces * t.blocks * 2048;
   const int out_bytes = a.out_f32 ? 0 : 4 * kNvOutBytes;
-  t.stages = (229376 - 1024 - out_bytes) / t.stage_bytes;
+  t.stages = (static_cast<int>(kNvSmem) - 1024 - out_bytes) / t.stage_bytes;
   if (t.stages > kNvMaxStages) t.stages = kNvMaxStages;
-  const size_t smem = 1024 + static_cast<size_t>(t.stages) * t.stage_bytes + out_bytes;
+  const size_t smem = nv_smem(1024 + static_cast<size_t>(t.stages) * t.stage_bytes + out_bytes, 512);
   CUtensorMap wmap, xmap, wsmap, xsmap, omap;
   if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
       !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), cols / 2) ||
@@ -641,11 +640,11 @@ static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a, int cols, int 
   while (t.tmem_cols < t.cols + 16 * (1 + a.pieces)) t.tmem_cols *= 2;
   t.stage_bytes = 16384 + a.pieces * t.cols * 128 + (1 + a.pieces) * 2048;
   const int red = t.splits > 1 ? 128 * t.cols * 4 : 0;
-  const int room = 229376 - 1024 - red;
+  const int room = static_cast<int>(kNvSmem) - 1024 - red;
   t.stages = room / t.stage_bytes < kNvMaxStages ? room / t.stage_bytes : kNvMaxStages;
   const int most = (t.k_stages + t.splits - 1) / t.splits;
   if (t.stages > most) t.stages = most;
-  const size_t smem = 1024 + static_cast<size_t>(t.stages) * t.stage_bytes + red;
+  const size_t smem = nv_smem(1024 + static_cast<size_t>(t.stages) * t.stage_bytes + red, t.tmem_cols);
   CUtensorMap wmap, xmap;
   if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
       !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), t.cols))

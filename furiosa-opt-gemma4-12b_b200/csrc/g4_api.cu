@@ -337,6 +337,7 @@ g4_status g4_ctx_destroy(g4_ctx* ctx) {
 g4_status g4_ctx_set_stream(g4_ctx* ctx, g4_stream_t stream) {
   G4_CHECK_CTX(ctx);
   ctx->stream = reinterpret_cast<cudaStream_t>(stream);
+  ctx->weights_ahead = false;  // (what precedes the next launch is another one now)
   return G4_OK;
 }
 

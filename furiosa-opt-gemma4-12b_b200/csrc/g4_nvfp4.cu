@@ -91,16 +91,16 @@ __global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_cons
     w[i][4] = v.x, w[i][5] = v.y, w[i][6] = v.z, w[i][7] = v.w;
   }
   if (a.norm_w != nullptr) {
-    // 64-bit sums: bf16 squares are exact in f32, and a factor that is the same however it is added up
-    // leaves no element on the other side of a rounding border
+    // 64-bit sums: a factor that is the same however it is added up leaves no element on the other side of
+    // a rounding border
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float p = lo_f32(w[i][e]), q = hi_f32(w[i][e]);
-        ss += static_cast<double>(__fmul_rn(p, p));
-        ss += static_cast<double>(__fmul_rn(q, q));
+        const double p = lo_f32(w[i][e]), q = hi_f32(w[i][e]);
+        ss = fma(p, p, ss);
+        ss = fma(q, q, ss);
       }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);

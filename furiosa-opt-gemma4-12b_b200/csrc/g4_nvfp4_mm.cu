@@ -80,7 +80,7 @@ constexpr int kNvMaxStages = 8;
 
 struct NvTileArgs {
   NvMatmulArgs a;
-  int cols, splits, stages, stage_bytes, k_stages, kblocks, tmem_cols;
+  int cols, splits, stages, stage_bytes, k_stages, kblocks, tmem_cols, row_tiles;
   int early;  // the weights may be fetched before the previous kernel is done
   size_t x_scale_piece;
 };
@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   const NvMatmulArgs& a = t.a;
   const uint32_t base = (smem_u32(nv_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = blockIdx.x % t.splits, n0 = blockIdx.x / t.splits * 128, m0 = blockIdx.y * t.cols;
+  const int rank = blockIdx.x % t.splits, tile = blockIdx.x / t.splits;
+  const int n0 = tile % t.row_tiles * 128, m0 = tile / t.row_tiles * t.cols;
   const int ks0 = t.k_stages * rank / t.splits, ks1 = t.k_stages * (rank + 1) / t.splits;
   if (tid == 0) {
     for (int i = 0; i < t.stages; ++i) {
@@ -538,14 +539,10 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
 }
 
 // ---------------------------------------------------------------------------- host side
-// Shared memory of a CTA that takes `tmem_cols` columns of tensor memory: at least its share of an SM's, so that
-// CTAs which fit an SM's shared memory together fit its tensor memory too.  (A CTA that waits for columns while
-// its cluster waits for it, beside another cluster's in the same position, would wait for good.)
+// CTAs of clusters ask for all of an SM's shared memory, so that an SM has one of them at a time: tensor memory is
+// not among what a cluster is given before it starts, and a CTA that waits for columns while its cluster waits
+// for it, beside another cluster's in the same position, would wait for good.
 constexpr size_t kNvSmem = 229376;
-static size_t nv_smem(size_t need, int tmem_cols) {
-  const size_t share = kNvSmem * tmem_cols / 512;
-  return need > share ? need : share;
-}
 // Codes [planes][rows][cols bytes] (row stride cols), box of box_rows x 128 bytes, 128-byte swizzle;
 // what lies past the rows and the columns reads as zeros.
 static bool nv_code_map(CUtensorMap* m, const void* p, int cols, int rows, int planes, size_t plane, int box_rows) {
@@ -608,7 +605,7 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   const int out_bytes = a.out_f32 ? 0 : 4 * kNvOutBytes;
   t.stages = (static_cast<int>(kNvSmem) - 1024 - out_bytes) / t.stage_bytes;
   if (t.stages > kNvMaxStages) t.stages = kNvMaxStages;
-  const size_t smem = nv_smem(1024 + static_cast<size_t>(t.stages) * t.stage_bytes + out_bytes, 512);
+  const size_t smem = kNvSmem;
   CUtensorMap wmap, xmap, wsmap, xsmap, omap;
   if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
       !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), cols / 2) ||
@@ -635,7 +632,8 @@ static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a, int cols, int 
   t.k_stages = (t.kblocks + 3) / 4;
   t.x_scale_piece = nv_scale_bytes(a.max_rows, a.k);
   t.early = ctx->weights_ahead;
-  const int row_tiles = (a.n + 127) / 128, col_tiles = (a.m + t.cols - 1) / t.cols;
+  t.row_tiles = (a.n + 127) / 128;
+  const int col_tiles = (a.m + t.cols - 1) / t.cols;
   t.tmem_cols = 32;
   while (t.tmem_cols < t.cols + 16 * (1 + a.pieces)) t.tmem_cols *= 2;
   t.stage_bytes = 16384 + a.pieces * t.cols * 128 + (1 + a.pieces) * 2048;
@@ -644,7 +642,7 @@ static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a, int cols, int 
   t.stages = room / t.stage_bytes < kNvMaxStages ? room / t.stage_bytes : kNvMaxStages;
   const int most = (t.k_stages + t.splits - 1) / t.splits;
   if (t.stages > most) t.stages = most;
-  const size_t smem = nv_smem(1024 + static_cast<size_t>(t.stages) * t.stage_bytes + red, t.tmem_cols);
+  const size_t smem = t.splits > 1 ? kNvSmem : 1024 + static_cast<size_t>(t.stages) * t.stage_bytes;
   CUtensorMap wmap, xmap;
   if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
       !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), t.cols))
@@ -657,8 +655,8 @@ static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a, int cols, int 
   Scratch* scr = ctx->buf.scratch;
   uint64_t budget = ctx->wait_budget_ns;
   void* args[] = {&wmap, &xmap, &t, &scr, &budget};
-  return launch_kernel(ctx, fn, dim3(row_tiles * t.splits, col_tiles), dim3(kNvTileThreads), smem, args, false, "nvfp4 matmul",
-                       t.splits);
+  return launch_kernel(ctx, fn, dim3(static_cast<unsigned>(t.row_tiles) * col_tiles * t.splits), dim3(kNvTileThreads), smem,
+                       args, false, "nvfp4 matmul", t.splits);
 }
 
 // Which kernel, how wide a tile, how many CTAs to a K range: the least of what each would take, by a model of
@@ -675,22 +673,22 @@ static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a, int cols, int 
 // column of tensor memory.
 g4_status launch_nvfp4_matmul(g4_ctx* ctx, const NvMatmulArgs& a) {
   const int stages = (a.k + 255) / 256, P = a.pieces;
-  auto ceil = [](int x, int y) { return (x + y - 1) / y; };
+  auto ceil = [](long long x, long long y) { return (x + y - 1) / y; };
   float best = 1e30f;
   int best_cols = 0, best_splits = 0;  // 0 splits: pairs
   auto offer = [&](float us, int cols, int splits) {
     if (us < best) best = us, best_cols = cols, best_splits = splits;
   };
   for (int cols = a.m <= 16 ? 16 : a.m <= 32 ? 32 : 64; cols <= 128; cols *= 2) {
-    const int tiles = ceil(a.n, 128) * ceil(a.m, cols);
+    const long long tiles = ceil(a.n, 128) * ceil(a.m, cols);
     int splits = 1;
-    while (splits < 8 && 2 * splits <= stages && 2ll * splits * tiles <= ctx->sm_count) splits *= 2;
+    while (splits < 8 && 2 * splits <= stages && 2 * splits * tiles <= ctx->sm_count) splits *= 2;
     const float stage = cols <= 64 ? 0.3f + 0.075f * P : 0.2f + 0.27f * P, end = 0.5f + 0.03f * (a.m < cols ? a.m : cols);
     offer(2.6f + ceil(tiles * splits, ctx->sm_count) * (ceil(stages, splits) * stage + end), cols, splits);
     if (a.m <= 32) break;
   }
   for (int cols = 64; cols <= 256; cols *= 2) {
-    const int rounds = ceil(ceil(a.n, 256) * ceil(a.m, cols), ctx->sm_count / 2);
+    const float rounds = static_cast<float>(ceil(ceil(a.n, 256) * ceil(a.m, cols), ctx->sm_count / 2));
     if (cols == 64)
       offer(2.9f + rounds * (stages * (0.25f + 0.07f * P) + 0.55f), cols, 0);
     else if (cols == 128)

@@ -74,24 +74,32 @@ __global__ void __launch_bounds__(T) residual_norm_kernel(const uint16_t* x, lon
     rv[j] = i < vecs ? rr[i] : none;
     wv[j] = i < vecs ? __ldg(reinterpret_cast<const uint4*>(w) + i) : none;
   }
-  float ss = 0.f;
+  auto squares = [&](float scale) {  // of x times scale, added up over the block
+    float ss = 0.f;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const uint32_t v[4] = {xv[j].x, xv[j].y, xv[j].z, xv[j].w};
+    for (int j = 0; j < NB; ++j) {
+      const uint32_t v[4] = {xv[j].x, xv[j].y, xv[j].z, xv[j].w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = __uint_as_float(v[e] << 16), b = __uint_as_float(v[e] & 0xFFFF0000u);
-      ss = fmaf(a, a, ss);
-      ss = fmaf(b, b, ss);
+      for (int e = 0; e < 4; ++e) {
+        const float a = __uint_as_float(v[e] << 16) * scale, b = __uint_as_float(v[e] & 0xFFFF0000u) * scale;
+        ss = fmaf(a, a, ss);
+        ss = fmaf(b, b, ss);
+      }
     }
-  }
-  ss = warp_sum(ss);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  float total = 0.f;
+    ss = warp_sum(ss);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
+    __syncthreads();
+    float total = 0.f;
 #pragma unroll
-  for (int i = 0; i < T / 32; ++i) total += red[i];
-  const float r = rms_factor(total, 8 * vecs);
+    for (int i = 0; i < T / 32; ++i) total += red[i];
+    return total;
+  };
+  float total = squares(1.f), r = rms_factor(total, 8 * vecs);
+  if (!(total <= 3e38f)) {  // (beyond f32, where 1e-6 counts for nothing; what is not finite stays so)
+    total = squares(0x1p-80f);
+    r = 0x1p-80f / sqrtf(total / static_cast<float>(8 * vecs));
+  }
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int i = threadIdx.x + j * T;

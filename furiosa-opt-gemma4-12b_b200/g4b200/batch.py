@@ -48,6 +48,9 @@ LIB.g4_nvfp4_dequantize.argtypes = [_vp, _rows_p, _i32, _vp, _i64]
 LIB.g4_nvfp4_matmul.argtypes = [_vp, _rows_p, _i32, _weight_p, _vp, _i64, _i32]
 LIB.g4_beam_select.argtypes = [_vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]
 
+_g4_embed_tokens, _g4_residual_norm, _g4_beam_select = LIB.g4_embed_tokens, LIB.g4_residual_norm, LIB.g4_beam_select
+_g4_nvfp4_quantize, _g4_nvfp4_dequantize, _g4_nvfp4_matmul = LIB.g4_nvfp4_quantize, LIB.g4_nvfp4_dequantize, LIB.g4_nvfp4_matmul
+
 _BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
 
@@ -115,8 +118,8 @@ def embed_tokens(ctx: Context, table, tokens, out, scale: float = EMBED_SCALE) -
     ids = _vector(ctx, "tokens", tokens, n, _I32)
     if stride != dim:
         raise ValueError("table: must be contiguous")
-    if n:
-        ctx._check("g4_embed_tokens", LIB.g4_embed_tokens(ctx.handle, rows, vocab, dim, ids, n, scale, to, out_stride))
+    if n and (code := _g4_embed_tokens(ctx.handle, rows, vocab, dim, ids, n, scale, to, out_stride)):
+        ctx._check("g4_embed_tokens", code)
 
 
 def residual_norm(ctx: Context, x, rms_weight, residual, out) -> None:
@@ -125,8 +128,8 @@ def residual_norm(ctx: Context, x, rms_weight, residual, out) -> None:
     _, _, rp, rs = _operand(ctx, "residual", residual, n, dim)
     _, _, op, os = _operand(ctx, "out", out, n, dim)
     w = _vector(ctx, "rms_weight", rms_weight, dim, _BF16)
-    if n:
-        ctx._check("g4_residual_norm", LIB.g4_residual_norm(ctx.handle, xp, xs, w, rp, rs, n, dim, op, os))
+    if n and (code := _g4_residual_norm(ctx.handle, xp, xs, w, rp, rs, n, dim, op, os)):
+        ctx._check("g4_residual_norm", code)
 
 
 class Nvfp4Rows:
@@ -195,16 +198,16 @@ def nvfp4_quantize(ctx: Context, x, rows: Nvfp4Rows, rms_weight=None) -> None:
     n, _, xp, xs = _operand(ctx, "x", x, None, rows.cols)
     _rows_of(ctx, rows, n)
     w = None if rms_weight is None else _vector(ctx, "rms_weight", rms_weight, rows.cols, _BF16)
-    if n:
-        ctx._check("g4_nvfp4_quantize", LIB.g4_nvfp4_quantize(ctx.handle, xp, xs, n, w, rows.desc))
+    if n and (code := _g4_nvfp4_quantize(ctx.handle, xp, xs, n, w, rows.desc)):
+        ctx._check("g4_nvfp4_quantize", code)
 
 
 def nvfp4_dequantize(ctx: Context, rows: Nvfp4Rows, out) -> None:
     """The values of the first n rows, rounded to bf16, into out [n, cols] (g4_nvfp4_dequantize)."""
     n, _, op, os = _operand(ctx, "out", out, None, rows.cols)
     _rows_of(ctx, rows, n)
-    if n:
-        ctx._check("g4_nvfp4_dequantize", LIB.g4_nvfp4_dequantize(ctx.handle, rows.desc, n, op, os))
+    if n and (code := _g4_nvfp4_dequantize(ctx.handle, rows.desc, n, op, os)):
+        ctx._check("g4_nvfp4_dequantize", code)
 
 
 def nvfp4_matmul(ctx: Context, rows: Nvfp4Rows, weight: Nvfp4Weight, out) -> None:
@@ -217,8 +220,8 @@ def nvfp4_matmul(ctx: Context, rows: Nvfp4Rows, weight: Nvfp4Weight, out) -> Non
         raise ValueError(f"weight: on cuda:{weight.device}, the context is on cuda:{ctx.device}")
     if weight.cols != rows.cols:
         raise ValueError(f"rows of {rows.cols} values, a weight of {weight.cols}")
-    if n:
-        ctx._check("g4_nvfp4_matmul", LIB.g4_nvfp4_matmul(ctx.handle, rows.desc, n, weight.desc, op, os, f32))
+    if n and (code := _g4_nvfp4_matmul(ctx.handle, rows.desc, n, weight.desc, op, os, f32)):
+        ctx._check("g4_nvfp4_matmul", code)
 
 
 def beam_select(ctx: Context, logits, scores, out_scores, out_beams, out_tokens) -> None:
@@ -239,9 +242,9 @@ def beam_select(ctx: Context, logits, scores, out_scores, out_beams, out_tokens)
     if not 1 <= beams <= BEAM_MAX or not 1 <= select <= BEAM_MAX or not 1 <= vocab <= 2 ** 20 or select > beams * vocab:
         raise ValueError(f"{select} of {beams} beams of {vocab} tokens: expected up to {BEAM_MAX} of up to {BEAM_MAX} beams of up "
                          "to 2^20 tokens, no more than there are")
-    if groups:
-        ctx._check("g4_beam_select", LIB.g4_beam_select(
-            ctx.handle, logits.data_ptr(), group_stride, beam_stride, given, groups, beams, vocab, select, best, of, to))
+    if groups and (code := _g4_beam_select(ctx.handle, logits.data_ptr(), group_stride, beam_stride, given, groups, beams,
+                                           vocab, select, best, of, to)):
+        ctx._check("g4_beam_select", code)
 
 
 __all__ = ["Nvfp4Rows", "Nvfp4Weight", "embed_tokens", "residual_norm", "nvfp4_quantize", "nvfp4_dequantize",

@@ -124,6 +124,22 @@ def test_matmul_repeats_itself(gpu_ctx):
     assert torch.equal(a, b)
 
 
+def test_matmul_of_the_most_rows(gpu_ctx):
+    """2^22 rows of 32 values: more tiles than a grid's second dimension has room for."""
+    m = 2 ** 22
+    rows = g4.Nvfp4Rows(gpu_ctx, m, 32, 1)
+    x = _randn(_gen(21), m, 32)
+    weight, wv, fw = _weight(gpu_ctx, 8, 32)
+    out = torch.empty((m, 8), dtype=torch.float32, device="cuda")
+    g4.nvfp4_quantize(gpu_ctx, x, rows)
+    g4.nvfp4_matmul(gpu_ctx, rows, weight, out)
+    _sync(gpu_ctx)
+    for at in (slice(0, 3000), slice(m // 2 - 5, m // 2 + 3000), slice(m - 3000, m)):
+        codes, scales, factor = ob.quantize(x[at], 1)
+        want, size = ob.matmul(ob.values(codes, scales)[0], wv, factor, fw)
+        assert ((out[at].double() - want).abs() <= 13 * 2.0 ** -23 * size).all()
+
+
 def test_matmul_nan_row_stays_in_its_row(gpu_ctx):
     x = _randn(_gen(3), 140, 512)
     x[7, 100], x[131, 0], x[20] = float("nan"), float("inf"), 0
@@ -199,6 +215,7 @@ def test_quantize_normed(gpu_ctx, n, cols):
     g = _gen(n * cols)
     x, w = _randn(g, n, cols, std=3.0), (1 + 0.3 * torch.randn(cols, generator=g, device="cuda")).bfloat16()
     x[0] *= 1e-3
+    x[n // 2:] *= 2.0 ** 100  # squares beyond f32
     rows = g4.Nvfp4Rows(gpu_ctx, n, cols, 2)
     g4.nvfp4_quantize(gpu_ctx, x, rows, w)
     _sync(gpu_ctx)
@@ -291,6 +308,7 @@ def test_residual_norm(gpu_ctx, n, dim, gap):
     x, res = _randn(g, n, dim + gap, std=4.0)[:, :dim], _randn(g, n, dim + gap)[:, :dim]
     w = (1 + 0.3 * torch.randn(dim, generator=g, device="cuda")).bfloat16()
     x[0] *= 2.0 ** -20
+    x[n // 2 + 1:] *= 2.0 ** 90  # squares beyond f32
     out = torch.full((n, dim + gap), 7.0, dtype=torch.bfloat16, device="cuda")
     g4.residual_norm(gpu_ctx, x, w, res, out[:, :dim])
     _sync(gpu_ctx)
@@ -464,6 +482,46 @@ def test_calls_captured_and_replayed(gpu_ctx):
     assert ctx.poll() == 0
     del graph
     ctx.close()
+
+
+def test_two_contexts_at_once(gpu_ctx):
+    """Products (clusters, pairs, single CTAs) and selections of two contexts on two streams, side by side: the same
+    bits as one after another."""
+    g = _gen(30)
+    logits, scores = _randn(g, 3, 4, 20000, std=3.0), torch.rand((3, 4), generator=g, device="cuda")
+    shapes = [(1, 3840, 4096, 2), (40, 1024, 3840, 2), (600, 2048, 992, 1), (7, 30720, 512, 2), (300, 3840, 1024, 3)]
+    ctxs = [g4.Context(0, stream=torch.cuda.Stream()) for _ in range(2)]
+    sets = []
+    for ctx in ctxs:
+        ops = []
+        for m, n, k, p in shapes:
+            rows, weight = _rows(ctx, m, k, p)[0], _weight(ctx, n, k)[0]
+            ops.append((rows, weight, torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")))
+        outs = torch.zeros((3, 9), device="cuda"), *(torch.zeros((3, 9), dtype=torch.int32, device="cuda") for _ in range(2))
+        sets.append((ops, outs))
+
+    def run(ctx, ops, outs):
+        for rows, weight, out in ops:
+            g4.nvfp4_matmul(ctx, rows, weight, out)
+        g4.beam_select(ctx, logits, scores, *outs)
+
+    torch.cuda.synchronize()
+    want = []
+    for ctx, s in zip(ctxs, sets):
+        run(ctx, *s)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in [o[2] for o in s[0]] + list(s[1])])
+        for t in [o[2] for o in s[0]] + list(s[1]):
+            t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for ctx, s in zip(ctxs, sets):
+            run(ctx, *s)
+    torch.cuda.synchronize()
+    for ctx, s, w in zip(ctxs, sets, want):
+        assert all(torch.equal(a, b) for a, b in zip([o[2] for o in s[0]] + list(s[1]), w))
+        assert ctx.poll() == 0
+        ctx.close()
 
 
 def test_library_refuses(gpu_ctx):

@@ -18,6 +18,11 @@ __device__ __forceinline__ float2 nv_halves(uint32_t h) {
   return make_float2(__half2float(__ushort_as_half(static_cast<uint16_t>(h))),
                      __half2float(__ushort_as_half(static_cast<uint16_t>(h >> 16))));
 }
+__device__ __forceinline__ uint32_t nv_abs_max2(uint32_t a, uint32_t b) {  // of two bf16 each, its sign of no meaning
+  uint32_t d;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 // Values as E2M1 codes, the first in the low nibble.  (Four bytes packed by one mov.b32 came out right in
 // the word but not where the same word was taken apart again: pairs of bytes do.)
 __device__ __forceinline__ uint32_t nv_e2m1x4(float2 a, float2 b) {
@@ -33,21 +38,20 @@ __device__ __forceinline__ uint32_t nv_e2m1x4(float2 a, float2 b) {
 __device__ __forceinline__ uint32_t nv_e2m1x8(float2 a, float2 b, float2 c, float2 d) {
   return __byte_perm(nv_e2m1x4(a, b), nv_e2m1x4(c, d), 0x5410);
 }
-__device__ __forceinline__ uint32_t nv_e4m3(float v) {
-  uint16_t s;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s) : "f"(v), "f"(v));
-  return s & 0xFFu;
-}
 // Quotients by multiplication, right in every tie.  What is divided has at most 11 significant bits (x g has 8,
 // y - c s at most 11: it is a multiple of 2^-9 of the scale's power of two and no larger than the scale), the
 // borders of both formats have few (3 bits of E2M1's by 4 of the scale; 6 by 5 bits of E4M3's).  So a quotient
 // that is not on a border is at least 2^-11 of itself away from it, and one that is has come out within
 // 2^-22 of it: rounding the approximate quotient to 2^-16 (E2M1: by adding 192 and taking it off again) or to
 // 16 significant bits (E4M3) puts the second on the border and leaves the first on its side.
+// E4M3 with integers: at 2^-120 of its value an f32 has the format's exponents, subnormal ones among them, and
+// its leading bits are the code.  (By conversions, with the borders between the codes, 51 us at the size below.)
 __device__ __forceinline__ uint32_t nv_scale_of(float top) {
   const uint32_t q = __float_as_uint(top * (1.0f / 6.0f));
-  return nv_e4m3(__uint_as_float((q + 0x80u) & ~0xFFu));
+  const uint32_t b = __float_as_uint(__uint_as_float((q + 0x80u) & ~0xFFu) * 0x1p-120f);
+  return (b + 0x7FFFFu + ((b >> 20) & 1u)) >> 20;  // (at most 448: max|y| is at most 2688)
 }
+__device__ __forceinline__ float nv_scale_value(uint32_t code) { return __uint_as_float(code << 20) * 0x1p120f; }
 __device__ __forceinline__ float nv_rcp(float s) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
@@ -68,9 +72,9 @@ struct QuantArgs {
   float* factor;
 };
 
-// What bounds it: the conversion unit.  Two values to E2M1 are two of its operations, back to values one: a
-// block of 16 takes it 25 a piece and 8 more between pieces (100 % busy at 4096 x 15360 in two pieces, 48 us;
-// the bytes alone are 30 us; decoding by byte tables instead took 53 us, the issue slots being short then).
+// What bounds it: instructions, and among them the integer pipe's (62 % busy at 4096 x 15360 in two pieces, 49 us
+// where the bytes alone are 30 us): unpacking, maxima, codes and their bytes.  Rows through shared memory, the
+// next one on its way, took 54 us; one f32 an instruction 58 us; back from codes by byte tables 53 us.
 //
 // One block of T threads per row; thread t holds the row's 16-element blocks t and t + T (at most NB).
 template <int T, int NB, int P>
@@ -130,16 +134,15 @@ __global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_cons
   for (int i = 0; i < NB; ++i) {
     uint32_t m = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = __vmaxu2(m, w[i][e] & 0x7FFF7FFFu);
+    for (int e = 0; e < 8; ++e) m = nv_abs_max2(m, w[i][e]);
+    m &= 0x7FFF7FFFu;
     own[i] = max(m & 0xFFFFu, m >> 16);
     top = max(top, own[i]);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((tid & 31) == 0) redu[tid >> 5] = top;
   __syncthreads();
-  top = 0u;
-#pragma unroll
-  for (int i = 0; i < T / 32; ++i) top = max(top, redu[i]);
+  top = __reduce_max_sync(0xffffffffu, redu[tid & (T / 32 - 1)]);
   const bool finite = top < 0x7F80u, live = finite && top != 0u;
   // g's biased exponent: 2688 = 1.3125 * 2^11, and 1.3125 is 40 of the 128 steps of a bf16 mantissa
   const uint32_t ge = min(253u, ((top & 0x7Fu) <= 40u ? 265u : 264u) - (live ? top >> 7 : 0u));
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_cons
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const uint32_t sc = nv_scale_of(m);
-      const float sf = e4m3_value(sc), rcp = sc != 0u ? nv_rcp(sf) : 0.f;
+      const float sf = nv_scale_value(sc), rcp = sc != 0u ? nv_rcp(sf) : 0.f;
       const float2 r2 = make_float2(rcp, rcp);
       float2 q[8];
 #pragma unroll

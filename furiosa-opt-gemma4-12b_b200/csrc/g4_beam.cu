@@ -9,7 +9,7 @@
 // part per thread, or the lists' heads), the n_select-th bounds the answer from below, and every value
 // above that bound lies in one of the n_select parts whose best is.  What is left is ranked by
 // counting, so results hang on no order of arrival.  Keys (order-preserving logit bits, then
-// the inverted index) are all different: equal logits rank by lower token, and the bound is sharp.
+// the inverted index) are all different: equal logits rank by lower token.
 #include <string>
 
 #include "g4_internal.h"
@@ -33,6 +33,7 @@ struct BeamArgs {
   long long group_stride, beam_stride;
   const float* scores;
   int n_beams, vocab, k, stretch, stretches;
+  uint32_t room, room_groups;  // of a stretch's candidates, and of its groups that may have some
   BeamSum* sums;   // [group][beam][stretch]
   uint32_t* keys;  // [group][beam][stretch][k], best first, 0 past a short list's end
   float* out_scores;
@@ -60,58 +61,135 @@ __device__ __forceinline__ uint32_t bm_max2(uint32_t a, uint32_t b) {  // of two
   return d;
 }
 
-// A thread takes every 256th 16-byte piece of the stretch; what lies before the first 16-byte border and
-// behind the last is one element each of the first threads.
+// A stretch as its block's threads take it: every kBmThreads-th 16-byte piece, four of them (a group) at a time;
+// what lies before the first 16-byte border and behind the last is one element each of the first threads.
+struct BmStretch {
+  const uint16_t* x;
+  int n, head, pieces, groups, tail;
+  __device__ __forceinline__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head); }
+  // a thread's element before the body or behind it, or none
+  __device__ __forceinline__ int before(int t) const { return t < head ? t : -1; }
+  __device__ __forceinline__ int behind(int t) const { return tail + t < n ? tail + t : -1; }
+};
+constexpr int kBmGroups = kBmStretch / (32 * kBmThreads);
+constexpr uint32_t kBmOf = 31u;  // a group's place in a key: earlier groups hold lower tokens
+struct BmShared {
+  __align__(16) uint32_t keys[kBmThreads];
+  uint16_t most[kBmGroups][kBmThreads];  // the largest of each thread's groups
+  uint32_t n_groups, n_found, bound;
+};
+// Value and place, comparable.
+__device__ __forceinline__ uint32_t bm_place(uint32_t bits, int group) { return bm_order(bits) << 8 | (kBmOf - group); }
+
+// The k-th of the parts' best keys (all different; 0: none), 1 if there are fewer.  Parts are a thread each, or
+// four where so few are wanted that ranking a quarter of the parts does.
+__device__ __forceinline__ uint32_t bm_bound(BmShared& s, int k, uint32_t best) {
+  const int tid = threadIdx.x;
+  int parts = kBmThreads;
+  if (k <= kBmQuads) {
+    parts = kBmThreads / 4;
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
+    if ((tid & 3) == 0) s.keys[tid >> 2] = best;
+  } else {
+    s.keys[tid] = best;
+  }
+  __syncthreads();
+  if (tid < parts) {
+    const uint32_t key = s.keys[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < parts; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(s.keys + i);
+      rank += (v.x > key) + (v.y > key) + (v.z > key) + (v.w > key);
+    }
+    if (rank == k - 1 && key != 0u) s.bound = key;
+  }
+  __syncthreads();
+  return s.bound;
+}
+
+__device__ __forceinline__ uint32_t bm_max8(const uint4& v) { return bm_max2(bm_max2(v.x, v.y), bm_max2(v.z, v.w)); }
+
+// Calls f(bits, index) for each element of a piece.
+template <class F>
+__device__ __forceinline__ void bm_each(const uint4& v, int i, F f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, i + e);
+}
+
+// The candidates where too many groups reach the bound `least` (a place, of values that are all alike): the best
+// key of each thread's groups that do, the bound of those, and what reaches that one.
+__device__ __noinline__ void bm_again(BmShared& s, const BmStretch& r, int k, uint32_t least, uint32_t* found) {
+  const int tid = threadIdx.x;
+  auto each = [&](auto f) {
+    const int one[2] = {r.before(tid), r.behind(tid)};
+    for (int o = 0; o < 2; ++o)
+      if (one[o] >= 0 && bm_place(r.x[one[o]], o == 0 ? 0 : static_cast<int>(kBmOf)) >= least) f(r.x[one[o]], one[o]);
+    for (int g = 0; g < r.groups; ++g) {
+      if (bm_place(s.most[g][tid], g) < least) continue;
+      for (int p = tid + 4 * g * kBmThreads; p < min(r.pieces, 4 * (g + 1) * kBmThreads); p += kBmThreads)
+        bm_each(__ldg(r.body() + p), r.head + 8 * p, f);
+    }
+  };
+  uint32_t best = 0;
+  each([&](uint32_t bits, int i) { best = max(best, bm_key(bits, i)); });
+  __syncthreads();
+  if (tid == 0) s.n_found = 0, s.bound = 1;
+  const uint32_t sharp = bm_bound(s, k, best);
+  if (best >= sharp)
+    each([&](uint32_t bits, int i) {
+      if (bm_key(bits, i) >= sharp) found[atomicAdd(&s.n_found, 1u)] = bm_key(bits, i);
+    });
+  __syncthreads();
+}
+
+// One pass: sums, and the largest value of each thread's groups.  Of the threads' largest (with the group where
+// they first come) the k-th is the bound, and the few groups that reach it are looked at again.
 //
-// What bounds it at many rows: the exponentials (one of the conversion unit's operations a logit) beside the
-// bytes; at few, the chain of load, maximum, ranks and the pieces looked at again.
+// What bounds it at many rows (18 us of 128 x 262144, 3.7 TB/s): the bytes and the exponentials, 16 us with the first
+// loads' latency and SMs that have four blocks where others have three; bounds, second look and ranks are 2 us behind
+// them.  (Collecting candidates as they pass, above the bound of the first group, takes 21 us; finding each thread's
+// best exactly first, and then looking through all of the best threads' pieces, 21 us.)  At few rows: the
+// chain of latencies, 4.6 us of 4 x 262144.
 __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_constant__ BeamArgs a) {
-  extern __shared__ uint32_t found[];  // [k * the logits of a thread]
-  __shared__ __align__(16) uint32_t keys[kBmThreads];
+  extern __shared__ uint32_t shared[];
+  __shared__ BmShared s;
   __shared__ float red_top[kBmThreads / 32];
   __shared__ double red_sum[kBmThreads / 32];
-  __shared__ uint32_t n_found, n_who, bound;
-  __shared__ uint8_t who[kBmThreads];
   const int tid = threadIdx.x, lane = tid & 31, part = blockIdx.x, beam = blockIdx.y;
   const long long row = static_cast<long long>(blockIdx.z) * a.n_beams + beam;
-  const int first = part * a.stretch, n = min(a.stretch, a.vocab - first);
-  if (tid == 0) n_found = 0, n_who = 0, bound = 1;
+  const int first = part * a.stretch;
+  if (tid == 0) s.n_groups = 0, s.n_found = 0, s.bound = 1;
   pdl_wait();
-  const uint16_t* x = a.logits + blockIdx.z * a.group_stride + beam * a.beam_stride + first;
-  const int head = min(n, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / 2);
-  const int pieces = (n - head) / 8, tail = head + 8 * pieces;
-  const uint4* body = reinterpret_cast<const uint4*>(x + head);
-  // a thread's element outside the body, or none
-  auto single = [&](int t) { return t < 8 ? (t < head ? t : -1) : (t < 16 && tail + t - 8 < n ? tail + t - 8 : -1); };
+  BmStretch r;
+  r.x = a.logits + blockIdx.z * a.group_stride + beam * a.beam_stride + first;
+  r.n = min(a.stretch, a.vocab - first);
+  r.head = min(r.n, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(r.x) & 15u)) & 15u) / 2);
+  r.pieces = (r.n - r.head) / 8;
+  r.groups = (r.pieces + 4 * kBmThreads - 1) / (4 * kBmThreads);
+  r.tail = r.head + 8 * r.pieces;
+  const uint4* body = r.body();
+  const int pieces = r.pieces;
 
   float m = -CUDART_INF_F, sum = 0.f;
-  int at = -1;  // where the first m is: an element, or the first of four pieces
-  bool whole = false;
+  int in = 0;  // the group where m first is
   // The sum is of 2^(l log2 e - ref), one FMA a logit, where ref is m log2 e rounded to f32: what the rounding
   // took is put back (in 64 bits) when the sum leaves the thread.  Where m is beyond 2^100 (rows masked with
   // the lowest number there is) ref might not be finite: the difference to m comes first there.
   float ref = 0.f;
   auto far = [](float v) { return fabsf(v) > 0x1p100f; };
-  auto raise = [&](float v, int i, bool pieces_of_it) {
+  auto raise = [&](float v, int group) {
     if (v > m) {
       const float to = v * kBmLog2e;
       if (m != -CUDART_INF_F) sum *= far(m) || far(v) ? bm_exp(m - v) : bm_exp2(ref - to);
       ref = to;
       m = v;
-      at = i;
-      whole = pieces_of_it;
-    } else if (at < 0) {  // (nothing but -inf so far)
-      at = i;
-      whole = pieces_of_it;
+      in = group;
     }
     if (v != v) sum = v;
   };
-  const int mine = single(tid);
-  if (mine >= 0) {
-    const float v = bf16_to_f32(x[mine]);
-    raise(v, mine, false);
-    if (m != -CUDART_INF_F) sum += bm_exp(v - m);
-  }
   // four pieces are on their way while four are looked at; what is not there counts as -inf
   uint4 now[4], next[4];
   auto fetch = [&](uint4 (&v)[4], int j) {
@@ -122,14 +200,21 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
     }
   };
   fetch(now, tid);
-  for (int j = tid; j < pieces; j += 4 * kBmThreads) {
+  const int lo = r.before(tid), hi = r.behind(tid);
+  const uint32_t lo_bits = lo >= 0 ? r.x[lo] : 0xFF80u, hi_bits = hi >= 0 ? r.x[hi] : 0xFF80u;
+  if (lo >= 0) {
+    const float v = __uint_as_float(lo_bits << 16);
+    raise(v, 0);
+    if (m != -CUDART_INF_F) sum += bm_exp(v - m);
+  }
+  for (int g = 0, j = tid; j < pieces; ++g, j += 4 * kBmThreads) {
     fetch(next, j + 4 * kBmThreads);
-    uint32_t two = bm_max2(bm_max2(now[0].x, now[0].y), bm_max2(now[0].z, now[0].w));
+    uint32_t two = bm_max8(now[0]);
 #pragma unroll
-    for (int u = 1; u < 4; ++u)
-      two = bm_max2(two, bm_max2(bm_max2(now[u].x, now[u].y), bm_max2(now[u].z, now[u].w)));
+    for (int u = 1; u < 4; ++u) two = bm_max2(two, bm_max8(now[u]));
     const uint32_t both = bm_max2(two, __byte_perm(two, 0, 0x1032));
-    raise(__uint_as_float(both << 16), j, true);
+    s.most[g][tid] = static_cast<uint16_t>(both);
+    raise(__uint_as_float(both << 16), g);
     if (far(m) && m != -CUDART_INF_F) {
       for (int u = 0; u < 4; ++u)
         for (int e = 0; e < 4; ++e) {
@@ -152,38 +237,56 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
       more[0] = add_f32x2(more[0], more[1]);
       sum += more[0].x + more[0].y;
     }
+    if (j + 4 * kBmThreads >= pieces) break;  // (the last group stays)
 #pragma unroll
     for (int u = 0; u < 4; ++u) now[u] = next[u];
   }
   pdl_launch_dependents();  // (the join waits for all of this kernel)
-  uint32_t best = 0;
-  if (at >= 0) {
-    if (whole) {  // which of the four pieces' elements
-      const int j = at;
-      at = -1;
-#pragma unroll
-      for (int u = 3; u >= 0; --u) {
-        const int p = j + u * kBmThreads;
-        if (p >= pieces) continue;
-        const uint4 v = __ldg(body + p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 7; e >= 0; --e)
-          if (__uint_as_float((w[e >> 1] >> (16 * (e & 1))) << 16) == m) at = head + 8 * p + e;
-      }
-    }
-    if (at >= 0) best = bm_key(__float_as_uint(m) >> 16, at);  // (none: all are NaN)
+  if (hi >= 0) {
+    const float v = __uint_as_float(hi_bits << 16);
+    raise(v, static_cast<int>(kBmOf));
+    if (m != -CUDART_INF_F) sum += bm_exp(v - m);
   }
-  // parts of a thread each, or of four where so few are wanted that ranking a quarter of the parts does
-  const int parts = a.k <= kBmQuads ? kBmThreads / 4 : kBmThreads;
-  uint32_t part_best = best;
-  if (a.k <= kBmQuads) {
-    part_best = max(part_best, __shfl_xor_sync(0xffffffffu, part_best, 1));
-    part_best = max(part_best, __shfl_xor_sync(0xffffffffu, part_best, 2));
-    if ((tid & 3) == 0) keys[tid >> 2] = part_best;
-  } else {
-    keys[tid] = part_best;
+  const bool any = tid < pieces || lo >= 0 || hi >= 0;
+  const uint32_t best = any ? bm_place(__float_as_uint(m) >> 16, in) << 8 | (0xFFu - tid) : 0u;
+  const uint32_t least = bm_bound(s, a.k, best) >> 8;
+  uint32_t* found = shared;
+  uint16_t* which = reinterpret_cast<uint16_t*>(found + a.room);  // groups: place in the stretch : 8 | thread : 8
+  auto take = [&](uint32_t bits, int i) {
+    const uint32_t at = atomicAdd(&s.n_found, 1u);
+    if (at < a.room) found[at] = bm_key(bits, i);
+  };
+  if (lo >= 0 && bm_place(lo_bits, 0) >= least) take(lo_bits, lo);
+  if (hi >= 0 && bm_place(hi_bits, static_cast<int>(kBmOf)) >= least) take(hi_bits, hi);
+  auto look = [&](const uint4& v, int p, int g) {
+    const uint32_t two = bm_max8(v);  // (most pieces have nothing: their largest says so)
+    if (max(bm_place(two & 0xFFFFu, g), bm_place(two >> 16, g)) < least) return;
+    bm_each(v, r.head + 8 * p, [&](uint32_t bits, int at) {
+      if (bm_place(bits, g) >= least) take(bits, at);
+    });
+  };
+  const bool mine = best >> 8 >= least;  // (no group of a thread's is above its best)
+  if (r.groups > 1) {
+    if (mine)
+      for (int g = 0, j = tid; j < pieces; ++g, j += 4 * kBmThreads)
+        if (bm_place(s.most[g][tid], g) >= least) {
+          const uint32_t at = atomicAdd(&s.n_groups, 1u);
+          if (at < a.room_groups) which[at] = static_cast<uint16_t>(g << 8 | tid);
+        }
+    __syncthreads();
+  } else if (mine) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (tid + u * kBmThreads < pieces) look(now[u], tid + u * kBmThreads, 0);
   }
+  // (the sums are joined while the first of the pieces comes back)
+  const int again = s.n_groups <= a.room_groups ? 4 * s.n_groups : 0;
+  auto piece = [&](int i, int& g) {
+    g = which[i >> 2] >> 8;
+    return (which[i >> 2] & 0xFF) + (4 * g + (i & 3)) * kBmThreads;
+  };
+  int g0 = 0, p0 = tid < again ? piece(tid, g0) : pieces;
+  if (p0 < pieces) now[0] = __ldg(body + p0);
   // (a NaN has to stay one: nothing here compares sums)
   const float wm = warp_max(m);
   const double lost = far(m) ? 0.0 : (static_cast<double>(ref) - static_cast<double>(m) * kBmLog2e) * 0.6931471805599453;
@@ -191,45 +294,15 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
   if (lane == 0) red_top[tid >> 5] = wm, red_sum[tid >> 5] = wide;
-  __syncthreads();
-  if (tid < parts) {
-    const uint32_t key = keys[tid];
-    int rank = 0;
-#pragma unroll 4
-    for (int i = 0; i < parts; i += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(keys + i);
-      rank += (v.x > key) + (v.y > key) + (v.z > key) + (v.w > key);
-    }
-    if (rank == a.k - 1 && key != 0u) bound = key;
+  if (p0 < pieces) look(now[0], p0, g0);
+  for (int i = tid + kBmThreads; i < again; i += kBmThreads) {
+    int g;
+    const int p = piece(i, g);
+    if (p < pieces) look(__ldg(body + p), p, g);
   }
   __syncthreads();
-  const uint32_t least = bound;
-  // the threads whose best is in, and then all of their pieces by all threads
-  if (best >= least) who[atomicAdd(&n_who, 1u)] = static_cast<uint8_t>(tid);
-  __syncthreads();
-  const int turns = (pieces + kBmThreads - 1) / kBmThreads + 1;  // pieces of a thread, and the element outside
-  for (int c = tid; c < static_cast<int>(n_who) * turns; c += kBmThreads) {
-    const int q = c / turns, turn = c - q * turns, t = who[q], p = t + turn * kBmThreads;
-    if (turn == turns - 1) {
-      const int one = single(t);
-      if (one < 0) continue;
-      const uint32_t key = bm_key(x[one], one);
-      if (key >= least) found[atomicAdd(&n_found, 1u)] = key;
-    } else if (p < pieces) {
-      const uint4 v = __ldg(body + p);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      // (most pieces have nothing: their largest says so)
-      const uint32_t two = bm_max2(bm_max2(w[0], w[1]), bm_max2(w[2], w[3]));
-      if (max(bm_order(two & 0xFFFFu), bm_order(two >> 16)) < least >> 16) continue;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t key = bm_key((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, head + 8 * p + e);
-        if (key >= least) found[atomicAdd(&n_found, 1u)] = key;
-      }
-    }
-  }
-  __syncthreads();
-  const int have = n_found;
+  if (s.n_groups > a.room_groups || s.n_found > a.room) bm_again(s, r, a.k, least, found);
+  const int have = s.n_found;
   const long long list = row * a.stretches + part;
   for (int i = tid; i < have; i += kBmThreads) {
     int above = 0;
@@ -238,17 +311,17 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
     if (above < a.k) a.keys[list * a.k + above] = found[i];
   }
   if (tid >= have && tid < a.k) a.keys[list * a.k + tid] = 0u;
-  if (tid < kBmThreads / 32) {
-    constexpr uint32_t kAll = (1u << (kBmThreads / 32)) - 1;
-    const float mine_top = red_top[tid];
+  if (tid >= kBmThreads - kBmThreads / 32) {  // (not the warp that ranks)
+    constexpr uint32_t kAll = ~((1u << (32 - kBmThreads / 32)) - 1);
+    const float mine_top = red_top[tid - (kBmThreads - kBmThreads / 32)];
     float top = mine_top;
 #pragma unroll
     for (int o = kBmThreads / 64; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-    double total = red_sum[tid];
+    double total = red_sum[tid - (kBmThreads - kBmThreads / 32)];
     if (!(total == 0.0)) total *= bm_exp(mine_top - top);
 #pragma unroll
     for (int o = kBmThreads / 64; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
-    if (tid == 0) a.sums[list] = {total, top};
+    if (tid == kBmThreads - 1) a.sums[list] = {total, top};
   }
 }
 
@@ -285,6 +358,7 @@ __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_
   BeamItem* found = heads + kBmMaxLists;                           // [k * k]
   uint32_t* near = reinterpret_cast<uint32_t*>(found + a.k * a.k);  // the lists' keys where they have room
   __shared__ BeamBase base[G4_BEAM_MAX];
+  __shared__ BeamItem deep[8];
   __shared__ int in[G4_BEAM_MAX];  // the lists whose heads are among the k best
   __shared__ uint32_t n_found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -294,18 +368,25 @@ __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_
   if (tid < a.k) in[tid] = -1;
   pdl_wait();
   const uint32_t* keys = a.keys + row0 * a.stretches * a.k;
+  // (all that comes from memory is asked for at once)
+  auto sum_of = [&](int b) {
+    return b < a.n_beams && lane < a.stretches ? a.sums[(row0 + b) * a.stretches + lane] : BeamSum{0.0, -CUDART_INF_F};
+  };
+  const BeamSum own0 = sum_of(warp);
+  const float score0 = warp < a.n_beams ? a.scores[row0 + warp] : 0.f;
   if (lists * a.k <= kBmNear) {
     for (int i = tid; i < lists * a.k; i += kBmJoinThreads) near[i] = keys[i];
     keys = near;
   }
   for (int b = warp; b < a.n_beams; b += kBmJoinThreads / 32) {
     const BeamSum* st = a.sums + (row0 + b) * a.stretches;
-    const float score = a.scores[row0 + b];
-    float top = -CUDART_INF_F;
-    for (int i = lane; i < a.stretches; i += 32) top = fmaxf(top, st[i].top);
+    const BeamSum own = b == warp ? own0 : sum_of(b);
+    const float score = b == warp ? score0 : a.scores[row0 + b];
+    float top = own.top;
+    for (int i = lane + 32; i < a.stretches; i += 32) top = fmaxf(top, st[i].top);
     top = warp_max(top);
-    double total = 0.0;
-    for (int i = lane; i < a.stretches; i += 32)
+    double total = own.sum == 0.0 ? 0.0 : own.sum * exp(static_cast<double>(own.top) - top);
+    for (int i = lane + 32; i < a.stretches; i += 32)
       if (!(st[i].sum == 0.0)) total += st[i].sum * exp(static_cast<double>(st[i].top) - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -326,40 +407,67 @@ __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_
     heads[i] = key ? bm_item(a, base[beam], beam, part, key) : BeamItem{0ull, 0ull};
   }
   __syncthreads();
-  // `each` threads, neighbours of one warp, rank a head
-  int each = 32;
-  while (each > 1 && each * lists > kBmJoinThreads) each >>= 1;
-  for (int i0 = 0; i0 < lists; i0 += kBmJoinThreads / each) {
-    const int i = i0 + tid / each;
+  // so many threads, neighbours of one warp, rank one of n
+  auto sharing = [](int n) {
+    int each = 32;
+    while (each > 1 && each * n > kBmJoinThreads) each >>= 1;
+    return each;
+  };
+  int share = sharing(lists);
+  for (int i0 = 0; i0 < lists; i0 += kBmJoinThreads / share) {
+    const int i = i0 + tid / share;
     const BeamItem mine = i < lists ? heads[i] : BeamItem{0ull, 0ull};
     int rank = 0;
     if (mine.rest != 0ull) {
 #pragma unroll 4
-      for (int j = tid & (each - 1); j < lists; j += each) rank += bm_above(heads[j], mine);
+      for (int j = tid & (share - 1); j < lists; j += share) rank += bm_above(heads[j], mine);
     }
-    for (int o = 1; o < each; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-    if ((tid & (each - 1)) == 0 && mine.rest != 0ull && rank < a.k) in[rank] = i;
+    for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if ((tid & (share - 1)) == 0 && mine.rest != 0ull && rank < a.k) in[rank] = i;
   }
   __syncthreads();
   // nothing below the last head that is in can be (with fewer lists than that, everything can)
   const int last = in[a.k - 1];
-  const BeamItem bound = last >= 0 ? heads[last] : BeamItem{0ull, 0ull};
-  for (int c = tid; c < a.k * a.k; c += kBmJoinThreads) {
-    const int list = in[c / a.k], i = c % a.k;
-    if (list < 0) continue;
+  BeamItem bound = last >= 0 ? heads[last] : BeamItem{0ull, 0ull};
+  auto item_of = [&](int list, int i) {
+    if (list < 0) return BeamItem{0ull, 0ull};
     const int beam = list / a.stretches, part = list - beam * a.stretches;
     const uint32_t key = key_of(beam, part, i, keys[list * a.k + i]);
-    if (key == 0u) continue;
-    const BeamItem item = bm_item(a, base[beam], beam, part, key);
-    if (!bm_above(bound, item)) found[atomicAdd(&n_found, 1u)] = item;
+    return key ? bm_item(a, base[beam], beam, part, key) : BeamItem{0ull, 0ull};
+  };
+  // nor can what is below the (k/d)-th best of those lists' d-th: where many are selected and one beam leads, the
+  // heads alone leave thousands to rank (64 of 32 beams of 262144: 420 us, and 37 us so)
+  if (a.k > kBmQuads) {
+    int depths = 0;
+    while ((2 << depths) <= a.k) ++depths;
+    for (int c = tid; c < depths * a.k; c += kBmJoinThreads) found[c] = item_of(in[c % a.k], (2 << c / a.k) - 1);
+    if (tid < 8) deep[tid] = BeamItem{0ull, 0ull};
+    __syncthreads();
+    for (int c = tid; c < depths * a.k; c += kBmJoinThreads) {
+      const int t = c / a.k, d = 2 << t;
+      const BeamItem mine = found[c];
+      int rank = 0;
+      for (int j = 0; j < a.k; ++j) rank += bm_above(found[t * a.k + j], mine);
+      if (mine.rest != 0ull && rank == (a.k + d - 1) / d - 1) deep[t] = mine;
+    }
+    __syncthreads();
+    for (int t = 0; t < depths; ++t)
+      if (bm_above(deep[t], bound)) bound = deep[t];
+  }
+  for (int c = tid; c < a.k * a.k; c += kBmJoinThreads) {
+    const BeamItem item = item_of(in[c / a.k], c % a.k);
+    if (item.rest != 0ull && !bm_above(bound, item)) found[atomicAdd(&n_found, 1u)] = item;
   }
   __syncthreads();
   const int have = n_found;
-  for (int i = tid; i < have; i += kBmJoinThreads) {
-    const BeamItem mine = found[i];
+  share = sharing(have);
+  for (int i0 = 0; i0 < have; i0 += kBmJoinThreads / share) {
+    const int i = i0 + tid / share;
+    const BeamItem mine = i < have ? found[i] : BeamItem{0ull, 0ull};
     int rank = 0;
-    for (int j = 0; j < have && rank < a.k; ++j) rank += bm_above(found[j], mine);
-    if (rank < a.k) {
+    for (int j = tid & (share - 1); j < have && rank < a.k; j += share) rank += bm_above(found[j], mine);
+    for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if ((tid & (share - 1)) == 0 && i < have && rank < a.k) {
       const long long at = static_cast<long long>(blockIdx.x) * a.k + rank;
       a.out_scores[at] = static_cast<float>(bm_score(mine.score));
       a.out_beams[at] = 0xFFFF - static_cast<int>(mine.rest >> 48);
@@ -392,21 +500,28 @@ extern "C" g4_status g4_beam_select(g4_ctx* ctx, const g4_bf16* logits, int64_t 
   DeviceGuard on(ctx);
   const long long rows = static_cast<long long>(n_groups) * n_beams;
   BeamArgs a = {logits, n_groups > 1 ? group_stride : 0, n_beams > 1 ? beam_stride : 0, scores, n_beams, vocab, n_select,
-                0, 0, nullptr, nullptr, out_scores, out_beams, out_tokens};
+                0, 0, 0, 0, nullptr, nullptr, out_scores, out_beams, out_tokens};
   // Stretches of a row: more of them keep the SMs busier, fewer leave the join less.  Of 262144 logits, one row
-  // takes 7.6 us in 32 stretches (8.2 in 16), 4 rows 9.3 in 16 (10.6 in 8 and in 32), 64 rows 18.4 in 8 (20.6 in
-  // 16), 128 rows 26.4 in 4 (27.9 in 8); 4 rows of 32000 8.5 in 16 (10.2 in 4).
+  // takes 7.4 us in 32 stretches (7.9 in 16), 4 rows 8.8 in 16 (9.5 in 8, 9.8 in 32), 64 rows 16.0 in 8 (16.3 in
+  // 4, 18.6 in 16), 80 rows 19.1 in 4 (20.4 in 8), 128 rows 22.7 in 4 (24.9 in 8).  And of a group no more lists
+  // than 128, or 64 where they are long: 32 selected of 8 beams in 4 groups take 20.0 us in 8 (29.6 in 16).
   const int least = (vocab + kBmStretch - 1) / kBmStretch, useful = (vocab + 2047) / 2048;
-  int parts = rows <= 2 ? 32 : rows <= 32 ? 16 : rows < 96 ? 8 : 4;
+  const int few = (n_select <= kBmQuads ? 128 : 64) / n_beams;
+  int parts = rows <= 2 ? 32 : rows <= 32 ? 16 : rows < 72 ? 8 : 4;
   if (parts > useful) parts = useful;
-  if (parts > kBmMaxLists / n_beams) parts = kBmMaxLists / n_beams;
-  if (parts < least) parts = least;  // (at most 16: kBmMaxLists / 64)
+  if (parts > few) parts = few;
+  if (parts < least) parts = least;  // (at most 16, which is kBmMaxLists / 64)
   a.stretch = ((vocab + parts - 1) / parts + 7) / 8 * 8;
   a.stretches = (vocab + a.stretch - 1) / a.stretch;
   const size_t lists = static_cast<size_t>(n_beams) * a.stretches;
   const size_t bytes = lists * (sizeof(BeamSum) + 4 * n_select);
-  const size_t list_smem = 4 * static_cast<size_t>(n_select) * (8 * ((a.stretch / 8 + kBmThreads - 1) / kBmThreads) + 1) *
-                            (n_select <= kBmQuads ? 4 : 1);
+  // the candidates of a stretch: as many as there are in the groups of n_select parts, should it come to that
+  const int threads = n_select * (n_select <= kBmQuads ? 4 : 1), turns = (a.stretch / 8 + kBmThreads - 1) / kBmThreads;
+  const int worst = threads * (8 * turns + 2);
+  a.room = 16 * n_select + 384;
+  a.room_groups = 8 * n_select + 64;
+  const size_t once = 4 * static_cast<size_t>(a.room) + 2 * a.room_groups;
+  const size_t list_smem = 4 * static_cast<size_t>(worst) > once ? 4 * static_cast<size_t>(worst) : once;
   const size_t join_smem = sizeof(BeamItem) * (kBmMaxLists + static_cast<size_t>(n_select) * n_select) +
                            (lists * n_select <= kBmNear ? 4 * lists * n_select : 0);
   g4_status st = allow_max_dynamic_smem(ctx, (const void*)beam_lists_kernel, list_smem, "beam lists");

@@ -428,6 +428,34 @@ def test_beam_select_lowest_and_largest_numbers(gpu_ctx):
     _check_beams(gpu_ctx, logits, torch.tensor([[0.0, -1.0, -2.0]] * 5, device="cuda"), 16)
 
 
+@pytest.mark.parametrize("k", [1, 8, 16, 17, 64])
+def test_beam_select_orders(gpu_ctx, k):
+    """Rows in order of value and against it, masked but for a few tokens, masked up to a place or from it, of two
+    values: where the best lie together, or a great many are as good as the last one that is in."""
+    g = _gen(40 + k)
+    logits = _randn(g, 9, 2, 140003, std=3.0)
+    logits[0], logits[1] = logits[0].sort(-1).values, logits[1].sort(-1, descending=True).values
+    keep = torch.randint(0, 140003, (2, 40), generator=g, device="cuda")
+    few = torch.full((2, 140003), -math.inf, dtype=torch.bfloat16, device="cuda")
+    logits[2] = few.scatter(1, keep, logits[2].gather(1, keep))
+    logits[3] = few.scatter(1, keep[:, :5], 1.0)
+    logits[4, :, :70000], logits[5, :, 9000:] = -math.inf, torch.finfo(torch.bfloat16).min
+    logits[6] = (torch.arange(140003, device="cuda") % 8192 > 8000).bfloat16()
+    logits[7] = (torch.rand((2, 140003), generator=g, device="cuda") < 1e-3).bfloat16()
+    logits[8, :, 1:140000] = 0.0  # both ends alone in what no 16-byte piece holds
+    _check_beams(gpu_ctx, logits, -torch.rand((9, 2), generator=g, device="cuda"), k)
+    _check_beams(gpu_ctx, logits[..., 3:131076], -torch.rand((9, 2), generator=g, device="cuda"), k)
+
+
+def test_beam_select_one_beam_leads(gpu_ctx):
+    """All of the best are one beam's, and a second's between them."""
+    logits = _randn(_gen(41), 2, 32, 70001, std=3.0)
+    scores = torch.full((2, 32), -300.0, device="cuda")
+    scores[0, 7], scores[1, 0], scores[1, 31] = 0.0, 0.0, -0.125
+    for k in (64, 33, 17):
+        _check_beams(gpu_ctx, logits, scores, k)
+
+
 def test_beam_select_scores_far_apart(gpu_ctx):
     g = _gen(11)
     logits = _randn(g, 2, 3, 2000, std=20.0)

@@ -352,6 +352,8 @@ __device__ __forceinline__ BeamItem bm_item(const BeamArgs& a, const BeamBase& b
               (0xFFFFFFFFu - token)};
 }
 
+// One block per group.  What bounds it: latencies in a chain (the lists and sums come back, sums joined in 64 bits,
+// heads ranked, what is left ranked), 4 to 5 us behind the lists of 4 beams of 262144, 16 lists or 64 of them.
 __global__ void __launch_bounds__(kBmJoinThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   BeamItem* heads = reinterpret_cast<BeamItem*>(raw);              // [kBmMaxLists]

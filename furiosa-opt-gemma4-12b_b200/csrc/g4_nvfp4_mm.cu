@@ -75,6 +75,11 @@ __device__ __forceinline__ void nv_ld16(uint32_t taddr, float (&v)[16]) {
 // A tile is 128 weight rows x `cols` activation rows; a cluster of `splits` CTAs shares its K range, and
 // each CTA then adds up 128 / splits of the tile's rows, whose parts the others stored into its
 // shared memory (in the cluster's order: no result hangs on timing).
+//
+// What bounds it: few rows are a read of the weights, 2.7 us of the 17.7 MB of 8192 x 3840, and the chain around it:
+// launch, a CTA's first stage, its 4 to 15 stages, the exchange in the cluster and the end, 4 us more.  One token
+// takes 6.7 us, 32 rows of 3840 x 8192 7.5 us.  Scales by tcgen05.st instead of the copy took longer, and so did a
+// warp of their own for the copies, or copying a stage ahead.
 constexpr int kNvTileThreads = 320;  // warp 0 copies, 1 MMA and tensor memory, 2-9 output
 constexpr int kNvMaxStages = 8;
 
@@ -292,6 +297,12 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
 //
 // Tensor memory: two sums of `cols` columns and one stage's scales do not fit side by side at 256, so the
 // sums overlap (columns acc_step to cols): the next tile's products start once these have been read.
+//
+// What bounds it: 4096 rows of 8192 x 3840 take 52.6 us in one piece (4.9 PFLOP/s, 75 % of four times the measured
+// bf16 rate) and 88.6 us in two (5.8 PFLOP/s, 89 %).  In one piece it is the way from L2 to the SMs: a stage's 39 KB
+// for 128 x 256 x 256 products of an SM are 54 bytes a clock at the full rate, and copies alone ran at 58.  A
+// second piece uses each weight tile twice.  Other orders of the tiles, and weights fetched while the
+// activations are quantised (509 rows 22.0 us instead of 20.2), did not help.
 constexpr int kNvPairThreads = 320;  // warp 0 copies, 1 MMA (leader) and tensor memory, 2-9 output
 
 struct NvPairArgs {

@@ -122,9 +122,10 @@ struct g4_ctx {
   g4::PrefillBuffers prefill;
   g4::PagedBuffers paged;
   int prefill_pieces = 2;  // NVFP4 pieces per prefill activation (1..3)
-  // The last launch quantised activations of several pieces (which are nobody's weight) and lets its
-  // successor start once its own predecessors are done: weights may be read ahead of it.
+  // The last launch quantised rows of several pieces and lets its successor start once its own predecessors
+  // are done: weights that are not among what it writes may be read ahead of it.
   bool weights_ahead = false;
+  g4_nvfp4_rows quantised = {};  // what it writes
 };
 
 namespace g4 {

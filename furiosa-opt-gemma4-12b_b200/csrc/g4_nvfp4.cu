@@ -327,6 +327,7 @@ g4_status g4_nvfp4_quantize(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, int
   void* args[] = {(void*)&a};
   st = launch_kernel(ctx, fn, dim3(n_rows), dim3(threads), 0, args, false, "nvfp4 quantize");
   ctx->weights_ahead = st == G4_OK && ctx->pdl_ok && out->pieces > 1;
+  ctx->quantised = *out;
   return st;
 }
 
@@ -362,6 +363,14 @@ g4_status g4_nvfp4_matmul(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, co
   if (n_rows == 0) return G4_OK;
   if ((st = check_matrix(ctx, out, out_stride, n_rows, weight->rows, "out")) != G4_OK) return st;
   DeviceGuard on(ctx);
+  if (ctx->weights_ahead) {  // (a weight made of one of the rows' pieces is not there yet)
+    const QuantArgs q = quant_args(&ctx->quantised);
+    auto meet = [](const uint8_t* a, size_t na, const uint8_t* b, size_t nb) { return a < b + nb && b < a + na; };
+    const size_t codes = static_cast<size_t>(weight->rows) * (weight->cols / 2);
+    if (meet(weight->codes, codes, q.codes, q.code_piece * ctx->quantised.pieces) ||
+        meet(weight->scales, nv_scale_bytes(weight->rows, weight->cols), q.scales, q.scale_piece * ctx->quantised.pieces))
+      ctx->weights_ahead = false;
+  }
   return launch_nvfp4_matmul(ctx, {rows->codes, rows->scales, rows->factor, weight->codes, weight->scales, weight->factor,
                                    n_rows, weight->rows, rows->cols, rows->pieces, rows->max_rows, weight->n_factors,
                                    out_f32 != 0, out, out_stride});

@@ -462,6 +462,24 @@ def test_beam_select_scores_far_apart(gpu_ctx):
     _check_beams(gpu_ctx, logits, torch.tensor([[-1e4, 0.0, -2e3], [-900.0, -900.25, -899.5]], device="cuda"), 12)
 
 
+def test_matmul_by_a_piece_of_the_rows_before(gpu_ctx):
+    """The C descriptors let a weight be one piece of rows of several, quantised by the call before."""
+    g = _gen(60)
+    x, w = _randn(g, 3, 4096), _randn(g, 2048, 4096)
+    rows, made, first = g4.Nvfp4Rows(gpu_ctx, 3, 4096), g4.Nvfp4Rows(gpu_ctx, 2048, 4096, 2), g4.Nvfp4Rows(gpu_ctx, 2048, 4096, 1)
+    out, want = (torch.empty((3, 2048), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    g4.nvfp4_quantize(gpu_ctx, x, rows)
+    g4.nvfp4_quantize(gpu_ctx, w, first)
+    g4.nvfp4_matmul(gpu_ctx, rows, g4.Nvfp4Weight.from_rows(first), want)
+    piece = g4.Nvfp4Weight.from_rows(first)
+    piece._set(made.codes, made.scales, made.factor, 2048, 4096, made.device)
+    for _ in range(20):
+        made.codes.fill_(0x77), made.scales.fill_(0x38)
+        g4.nvfp4_quantize(gpu_ctx, w, made)
+        g4.nvfp4_matmul(gpu_ctx, rows, piece, out)
+        assert torch.equal(out, want)
+
+
 # ------------------------------------------------------------------------------ calls
 def test_calls_captured_and_replayed(gpu_ctx):
     """Embed, quantise, multiply, norm and select in one graph, on a stream of the context's own; replays follow

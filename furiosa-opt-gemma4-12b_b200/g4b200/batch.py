@@ -96,11 +96,21 @@ def _operand(ctx: Context, name: str, t, rows, cols, dtype=_BF16) -> tuple:
 def _vector(ctx: Context, name: str, t, n, dtype) -> int:
     """A contiguous [n] operand's pointer."""
     try:
-        if t.get_device() == ctx.device and t.dtype is dtype and t.shape == (n,) and t.stride(0) == 1:
+        if t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.get_device() == ctx.device and t.is_contiguous():
             return t.data_ptr()
-    except (AttributeError, IndexError):
+    except AttributeError:
         pass
     return _whole(ctx, name, t, (n,), (dtype,))
+
+
+def _exact(ctx: Context, name: str, t, shape: tuple, dtype) -> int:
+    """A contiguous operand's pointer."""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == ctx.device and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    return _whole(ctx, name, t, shape, (dtype,))
 
 
 def _whole(ctx: Context, name: str, t, shape: tuple, dtypes) -> int:
@@ -126,7 +136,7 @@ def residual_norm(ctx: Context, x, rms_weight, residual, out) -> None:
     """out = bf16(residual + rmsnorm(x) * rms_weight) by rows (g4_residual_norm); out may be residual."""
     n, dim, xp, xs = _operand(ctx, "x", x, None, None)
     _, _, rp, rs = _operand(ctx, "residual", residual, n, dim)
-    _, _, op, os = _operand(ctx, "out", out, n, dim)
+    _, _, op, os = (n, dim, rp, rs) if out is residual else _operand(ctx, "out", out, n, dim)
     w = _vector(ctx, "rms_weight", rms_weight, dim, _BF16)
     if n and (code := _g4_residual_norm(ctx.handle, xp, xs, w, rp, rs, n, dim, op, os)):
         ctx._check("g4_residual_norm", code)
@@ -229,16 +239,23 @@ def beam_select(ctx: Context, logits, scores, out_scores, out_beams, out_tokens)
     strides with a contiguous last dimension, scores f32 [groups, beams] (-inf: the beam does not
     count); out_scores f32, out_beams and out_tokens int32 [groups, select], best first, equal scores
     in the order of (beam, token)."""
-    groups, beams, vocab = _tensor(ctx, "logits", logits, (_BF16,), 3).shape
-    group_stride, beam_stride, one = logits.stride()
+    try:
+        fits = logits.dtype is _BF16 and logits.get_device() == ctx.device
+        (groups, beams, vocab), (group_stride, beam_stride, one) = logits.shape, logits.stride()
+        fits = fits and groups < 2 ** 31
+    except (AttributeError, ValueError):
+        fits = False
+    if not fits:
+        groups, beams, vocab = _tensor(ctx, "logits", logits, (_BF16,), 3).shape
+        group_stride, beam_stride, one = logits.stride()
     if vocab > 1 and one != 1:
         raise ValueError("logits: the last dimension must be contiguous")
-    _, select, best, stride = _operand(ctx, "out_scores", out_scores, groups, None, _F32)
-    given, given_stride = _operand(ctx, "scores", scores, groups, beams, _F32)[2:]
-    of, of_stride = _operand(ctx, "out_beams", out_beams, groups, select, _I32)[2:]
-    to, to_stride = _operand(ctx, "out_tokens", out_tokens, groups, select, _I32)[2:]
-    if given_stride != beams or (stride, of_stride, to_stride) != (select,) * 3:
-        raise ValueError("scores and outputs must be contiguous")
+    given = _exact(ctx, "scores", scores, (groups, beams), _F32)
+    two = isinstance(out_scores, torch.Tensor) and out_scores.dim() == 2
+    select = (out_scores if two else _tensor(ctx, "out_scores", out_scores, (_F32,), 2)).shape[1]
+    best = _exact(ctx, "out_scores", out_scores, (groups, select), _F32)
+    of = _exact(ctx, "out_beams", out_beams, (groups, select), _I32)
+    to = _exact(ctx, "out_tokens", out_tokens, (groups, select), _I32)
     if not 1 <= beams <= BEAM_MAX or not 1 <= select <= BEAM_MAX or not 1 <= vocab <= 2 ** 20 or select > beams * vocab:
         raise ValueError(f"{select} of {beams} beams of {vocab} tokens: expected up to {BEAM_MAX} of up to {BEAM_MAX} beams of up "
                          "to 2^20 tokens, no more than there are")

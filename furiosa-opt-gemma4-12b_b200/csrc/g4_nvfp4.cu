@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t nv_e2m1x8(float2 a, float2 b, float2 c, floa
 // 2^-22 of it: rounding the approximate quotient to 2^-16 (E2M1: by adding 192 and taking it off again) or to
 // 16 significant bits (E4M3) puts the second on the border and leaves the first on its side.
 // E4M3 with integers: at 2^-120 of its value an f32 has the format's exponents, subnormal ones among them, and
-// its leading bits are the code.  (By conversions, with the borders between the codes, 51 us at the size below.)
+// its leading bits are the code.  (By conversions, with the borders between the codes, 51 us where this took 49.)
 __device__ __forceinline__ uint32_t nv_scale_of(float top) {
   const uint32_t q = __float_as_uint(top * (1.0f / 6.0f));
   const uint32_t b = __float_as_uint(__uint_as_float((q + 0x80u) & ~0xFFu) * 0x1p-120f);
@@ -72,13 +72,14 @@ struct QuantArgs {
   float* factor;
 };
 
-// What bounds it: instructions, and among them the integer pipe's (62 % busy at 4096 x 15360 in two pieces, 49 us
-// where the bytes alone are 30 us): unpacking, maxima, codes and their bytes.  Rows through shared memory, the
-// next one on its way, took 54 us; one f32 an instruction 58 us; back from codes by byte tables 53 us.
+// What bounds it: instructions, and among them the integer pipe's (62 % busy when 4096 x 15360 in two pieces took 49
+// us, now 41 us, with more of its rows on an SM; the bytes alone are 30 us): unpacking, maxima, codes and their
+// bytes.  Beside the 49 us, rows through shared memory, the next one on its way, took 54 us; one f32 an
+// instruction 58 us; back from codes by byte tables 53 us.
 //
 // One block of T threads per row; thread t holds the row's 16-element blocks t and t + T (at most NB).
-template <int T, int NB, int P>
-__global__ void __launch_bounds__(T, 1024 / T) nv_quant_kernel(const __grid_constant__ QuantArgs a) {
+template <int T, int NB, int P, int kPerSm>
+__global__ void __launch_bounds__(T, kPerSm) nv_quant_kernel(const __grid_constant__ QuantArgs a) {
   __shared__ uint32_t redu[T / 32];
   __shared__ double redd[T / 32];
   const int row = blockIdx.x, tid = threadIdx.x;
@@ -274,13 +275,26 @@ static QuantArgs quant_args(const g4_nvfp4_rows* r) {
   a.factor = r->factor;
   return a;
 }
+// Threads to a row, blocks to a thread and rows to an SM (which is registers to a thread).  Many rows want several
+// on an SM, each at another point of its way from load to codes; no more rows than SMs want all threads that
+// have work for each.  Two pieces: 1024 rows of 3840 take 5.2 us as 128 x 2, 8 to an SM (5.8 with 10 to an SM; 4096 of
+// them 12.5 and 12.4, 16.2 as 256 x 2); 2048 rows of 8192 12.7 as 256 x 2 (12.8 as 128 x 4, 18.7 as 512 x 2); 4096
+// rows of 15360 41 as 256 x 4 (42 as 128 x 8, 49 as 512 x 2).  One row of 15360 takes 2.8 as 512 x 2 (3.2 as
+// 256 x 4), one of 3840 with its norm 2.7 as 256 x 1 (2.9 as 128 x 2).
 template <int P>
-static const void* quant_kernel(int nb4, int& threads) {
-  threads = nb4 <= 256 ? 128 : nb4 <= 512 ? 256 : 512;
-  if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P>;
-  if (nb4 <= 256) return (const void*)nv_quant_kernel<128, 2, P>;
-  if (nb4 <= 512) return (const void*)nv_quant_kernel<256, 2, P>;
-  return (const void*)nv_quant_kernel<512, 2, P>;
+static const void* quant_kernel(int nb4, int rows, int sm_count, int& threads) {
+  if (rows <= sm_count) {
+    threads = nb4 <= 128 ? 128 : nb4 <= 256 ? 256 : 512;
+    if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P, 8>;
+    if (nb4 <= 256) return (const void*)nv_quant_kernel<256, 1, P, 4>;
+    if (nb4 <= 512) return (const void*)nv_quant_kernel<512, 1, P, 2>;
+    return (const void*)nv_quant_kernel<512, 2, P, 2>;
+  }
+  threads = nb4 <= 256 ? 128 : 256;
+  if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P, 8>;
+  if (nb4 <= 256) return (const void*)nv_quant_kernel<128, 2, P, 8>;
+  if (nb4 <= 512) return (const void*)nv_quant_kernel<256, 2, P, 5>;
+  return (const void*)nv_quant_kernel<256, 4, P, 4>;
 }
 
 }  // namespace g4
@@ -321,9 +335,9 @@ g4_status g4_nvfp4_quantize(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, int
   a.x_stride = x_stride;
   a.norm_w = rms_weight;
   int threads = 0;
-  const void* fn = out->pieces == 1   ? quant_kernel<1>(4 * a.kblocks, threads)
-                   : out->pieces == 2 ? quant_kernel<2>(4 * a.kblocks, threads)
-                                      : quant_kernel<3>(4 * a.kblocks, threads);
+  const void* fn = out->pieces == 1   ? quant_kernel<1>(4 * a.kblocks, n_rows, ctx->sm_count, threads)
+                   : out->pieces == 2 ? quant_kernel<2>(4 * a.kblocks, n_rows, ctx->sm_count, threads)
+                                      : quant_kernel<3>(4 * a.kblocks, n_rows, ctx->sm_count, threads);
   void* args[] = {(void*)&a};
   st = launch_kernel(ctx, fn, dim3(n_rows), dim3(threads), 0, args, false, "nvfp4 quantize");
   ctx->weights_ahead = st == G4_OK && ctx->pdl_ok && out->pieces > 1;

@@ -226,6 +226,27 @@ def test_quantize_normed(gpu_ctx, n, cols):
     assert ((y.double() - exact).abs() <= (U + 2.0 ** -20) * exact.abs() + 2.0 ** -130).all()
 
 
+@pytest.mark.parametrize("cols", [2048, 2080, 4096, 4128, 8192, 8224, 16384])
+@pytest.mark.parametrize("pieces, normed", [(1, False), (2, True), (3, False)])
+def test_quantize_many_rows_as_few(gpu_ctx, cols, pieces, normed):
+    """A call of more rows than the GPU has SMs and calls of fewer give the same bits, the oracle's."""
+    g = _gen(cols + pieces)
+    x, w = _randn(g, 301, cols, std=2.0), (1 + 0.3 * torch.randn(cols, generator=g, device="cuda")).bfloat16() if normed else None
+    x[5] = 0
+    many, few = g4.Nvfp4Rows(gpu_ctx, 301, cols, pieces), [g4.Nvfp4Rows(gpu_ctx, 128, cols, pieces) for _ in range(3)]
+    for r in (many, *few):
+        r.scales.fill_(0)
+    g4.nvfp4_quantize(gpu_ctx, x, many, w)
+    for i, r in enumerate(few):
+        g4.nvfp4_quantize(gpu_ctx, x[128 * i:128 * i + 128], r, w)
+    _sync(gpu_ctx)
+    assert torch.equal(many.codes, torch.cat([r.codes for r in few], 1)[:, :301])
+    assert torch.equal(many.factor, torch.cat([r.factor for r in few])[:301])
+    assert torch.equal(many.scales.view(pieces, -1), torch.cat([r.scales.view(pieces, -1) for r in few], 1))
+    if not normed:
+        _check_rows(many, ob.quantize(x, pieces), 301, cols)
+
+
 def test_quantize_special_rows(gpu_ctx):
     """Rows of zeros, of the smallest and the largest numbers, ties of both roundings, infinities and NaN."""
     x = torch.zeros((14, 64), dtype=torch.bfloat16, device="cuda")

@@ -376,6 +376,7 @@ g4_status g4_nvfp4_matmul(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, co
     return fail(ctx, G4_ERR_BAD_ARG, "nvfp4 weight: factor is null or misaligned");
   if (n_rows == 0) return G4_OK;
   if ((st = check_matrix(ctx, out, out_stride, n_rows, weight->rows, "out")) != G4_OK) return st;
+  if (n_rows == 1) out_stride = (static_cast<int64_t>(weight->rows) + 7) / 8 * 8;  // (of no meaning, but tensor maps want one)
   DeviceGuard on(ctx);
   if (ctx->weights_ahead) {  // (a weight made of one of the rows' pieces is not there yet)
     const QuantArgs q = quant_args(&ctx->quantised);

@@ -154,6 +154,12 @@ def test_matmul_nan_row_stays_in_its_row(gpu_ctx):
     assert out[bad].isnan().all() and torch.isfinite(out[~bad]).all() and (out[20] == 0).all()
 
 
+def test_matmul_one_row_of_any_width(gpu_ctx):
+    """One row's output has no row stride to speak of: wide, odd, by the kernel of many tiles."""
+    for m, n in ((1, 160001), (1, 160008), (2, 160008)):
+        _product(gpu_ctx, m, n, 32, 2)
+
+
 def test_quantised_rows_are_a_weight(gpu_ctx):
     g = _gen(9)
     a, b = _randn(g, 70, 768), _randn(g, 200, 768, std=0.02)

@@ -175,16 +175,16 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
 
   float m = -CUDART_INF_F, sum = 0.f;
   int in = 0;  // the group where m first is
-  // The sum is of 2^(l log2 e - ref), one FMA a logit, where ref is m log2 e rounded to f32: what the rounding
-  // took is put back (in 64 bits) when the sum leaves the thread.  Where m is beyond 2^100 (rows masked with
-  // the lowest number there is) ref might not be finite: the difference to m comes first there.
-  float ref = 0.f;
+  // The sum is of 2^((l - m) log2 e) as 2^(fma(l, log2 e, -ref) - rest), where ref is m log2 e rounded to f32 and rest
+  // what the rounding took: m itself counts as 1 exactly.  Where m is beyond 2^100 (rows masked with the lowest
+  // number there is) ref might not be finite: the difference to m comes first there.
+  float ref = 0.f, rest = 0.f;
   auto far = [](float v) { return fabsf(v) > 0x1p100f; };
   auto raise = [&](float v, int group) {
     if (v > m) {
-      const float to = v * kBmLog2e;
-      if (m != -CUDART_INF_F) sum *= far(m) || far(v) ? bm_exp(m - v) : bm_exp2(ref - to);
-      ref = to;
+      if (m != -CUDART_INF_F) sum *= bm_exp(m - v);
+      ref = v * kBmLog2e;
+      rest = fmaf(v, kBmLog2e, -ref);
       m = v;
       in = group;
     }
@@ -222,15 +222,16 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
           sum += bm_exp(__uint_as_float(w << 16) - m) + bm_exp(__uint_as_float(w & 0xFFFF0000u) - m);
         }
     } else if (m != -CUDART_INF_F) {
-      const float2 scale = make_float2(kBmLog2e, kBmLog2e), off = make_float2(-ref, -ref);
+      const float2 scale = make_float2(kBmLog2e, kBmLog2e), off = make_float2(-ref, -ref),
+                   less = make_float2(-rest, -rest);
       float2 more[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 x2 =
-              fma_f32x2(make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u)), scale, off);
+          const float2 l2 = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u));
+          const float2 x2 = add_f32x2(fma_f32x2(l2, scale, off), less);
           more[e & 1] = add_f32x2(more[e & 1], make_float2(bm_exp2(x2.x), bm_exp2(x2.y)));
         }
       }
@@ -289,8 +290,7 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   if (p0 < pieces) now[0] = __ldg(body + p0);
   // (a NaN has to stay one: nothing here compares sums)
   const float wm = warp_max(m);
-  const double lost = far(m) ? 0.0 : (static_cast<double>(ref) - static_cast<double>(m) * kBmLog2e) * 0.6931471805599453;
-  double wide = sum == 0.f ? 0.0 : static_cast<double>(sum) * (1.0 + lost) * bm_exp(m - wm);
+  double wide = sum == 0.f ? 0.0 : static_cast<double>(sum) * bm_exp(m - wm);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
   if (lane == 0) red_top[tid >> 5] = wm, red_sum[tid >> 5] = wide;

@@ -551,7 +551,8 @@ g4_status g4_nvfp4_matmul(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, co
  * best first, equal scores in the order of (beam, token).  logits: row (group, beam) at element
  * group * group_stride + beam * beam_stride, `vocab` entries, any alignment; scores
  * [n_groups, n_beams] f32; out_scores f32, out_beams and out_tokens int32 [n_groups, n_select].
- * Scores are compared before they are rounded (sums in 64 bits).  A beam whose score is not finite,
+ * Scores are compared before they are rounded; exponentials are f32 (joined in 64 bits), so tokens of
+ * different beams whose scores are within 1e-6 of one another may come in either order.  A beam whose score is not finite,
  * or whose logits hold a NaN or +inf or nothing but -inf, has only continuations of score -inf (-inf as
  * a score is how a beam that does not count is passed).  n_beams and n_select up to 64, vocab
  * up to 2^20, n_select <= n_beams * vocab.  The lists between its two kernels are the context's: calls,

@@ -507,6 +507,15 @@ def test_matmul_by_a_piece_of_the_rows_before(gpu_ctx):
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("vocab, offset", [(46, 7), (15, 1), (30, 5), (3000, 3)])
+def test_beam_select_large_logits(gpu_ctx, vocab, offset):
+    """Logits some hundreds in size, where a difference of exponents rounded to 32 bits shows in a score, of rows that
+    are hardly more than what lies outside 16-byte pieces."""
+    g = _gen(vocab)
+    logits = _randn(g, 5, 17, vocab + offset, std=60.0)[..., offset:]
+    _check_beams(gpu_ctx, logits, -torch.rand((5, 17), generator=g, device="cuda"), min(60, 17 * vocab))
+
+
 # ------------------------------------------------------------------------------ calls
 def test_calls_captured_and_replayed(gpu_ctx):
     """Embed, quantise, multiply, norm and select in one graph, on a stream of the context's own; replays follow

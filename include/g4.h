@@ -552,11 +552,11 @@ g4_status g4_nvfp4_matmul(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, co
  * group * group_stride + beam * beam_stride, `vocab` entries, any alignment; scores
  * [n_groups, n_beams] f32; out_scores f32, out_beams and out_tokens int32 [n_groups, n_select].
  * Scores are compared before they are rounded; exponentials are f32 (joined in 64 bits), so tokens of
- * different beams whose scores are within 1e-6 of one another may come in either order.  A beam whose score is not finite,
- * or whose logits hold a NaN or +inf or nothing but -inf, has only continuations of score -inf (-inf as
- * a score is how a beam that does not count is passed).  n_beams and n_select up to 64, vocab
- * up to 2^20, n_select <= n_beams * vocab.  The lists between its two kernels are the context's: calls,
- * and replays of graphs captured from them, run one after another. */
+ * different beams whose scores are within 1e-6 of one another may come in either order.  A beam whose
+ * score is not finite, or whose logits hold a NaN or +inf or nothing but -inf, has only continuations
+ * of score -inf (-inf as a score is how a beam that does not count is passed).  n_beams and n_select up
+ * to 64, vocab up to 2^20, n_select <= n_beams * vocab.  The lists between its two kernels are the
+ * context's: calls, and replays of graphs captured from them, run one after another. */
 #define G4_BEAM_MAX 64
 g4_status g4_beam_select(g4_ctx* ctx, const g4_bf16* logits, int64_t group_stride, int64_t beam_stride,
                          const float* scores, int n_groups, int n_beams, int vocab, int n_select, float* out_scores,

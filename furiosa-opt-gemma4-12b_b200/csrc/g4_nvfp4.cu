@@ -8,6 +8,7 @@
 // activations meet ties of both formats all the time (0.4 % of the blocks of a prompt's rows changed
 // their scale between 32- and 64-bit arithmetic with the recipe of the weights).
 #include <string>
+#include <type_traits>
 
 #include "g4_nvfp4.cuh"
 #include "g4_paged_split.cuh"
@@ -73,12 +74,12 @@ struct QuantArgs {
 };
 
 // What bounds it: instructions, and among them the integer pipe's (62 % busy when 4096 x 15360 in two pieces took 49
-// us, now 41 us, with more of its rows on an SM; the bytes alone are 30 us): unpacking, maxima, codes and their
+// us, now 40 us, with more of its rows on an SM; the bytes alone are 30 us): unpacking, maxima, codes and their
 // bytes.  Beside the 49 us, rows through shared memory, the next one on its way, took 54 us; one f32 an
 // instruction 58 us; back from codes by byte tables 53 us.
 //
 // One block of T threads per row; thread t holds the row's 16-element blocks t and t + T (at most NB).
-template <int T, int NB, int P, int kPerSm>
+template <int T, int NB, int P, int kPerSm, bool kNorm>
 __global__ void __launch_bounds__(T, kPerSm) nv_quant_kernel(const __grid_constant__ QuantArgs a) {
   __shared__ uint32_t redu[T / 32];
   __shared__ double redd[T / 32];
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(T, kPerSm) nv_quant_kernel(const __grid_consta
     w[i][0] = u.x, w[i][1] = u.y, w[i][2] = u.z, w[i][3] = u.w;
     w[i][4] = v.x, w[i][5] = v.y, w[i][6] = v.z, w[i][7] = v.w;
   }
-  if (a.norm_w != nullptr) {
+  if (kNorm) {
     // 64-bit sums: a factor that is the same however it is added up leaves no element on the other side of
     // a rounding border
     double ss = 0.0;
@@ -277,24 +278,24 @@ static QuantArgs quant_args(const g4_nvfp4_rows* r) {
 }
 // Threads to a row, blocks to a thread and rows to an SM (which is registers to a thread).  Many rows want several
 // on an SM, each at another point of its way from load to codes; no more rows than SMs want all threads that
-// have work for each.  Two pieces: 1024 rows of 3840 take 5.2 us as 128 x 2, 8 to an SM (5.8 with 10 to an SM; 4096 of
-// them 12.5 and 12.4, 16.2 as 256 x 2); 2048 rows of 8192 12.7 as 256 x 2 (12.8 as 128 x 4, 18.7 as 512 x 2); 4096
-// rows of 15360 41 as 256 x 4 (42 as 128 x 8, 49 as 512 x 2).  One row of 15360 takes 2.8 as 512 x 2 (3.2 as
+// have work for each.  Two pieces: 1024 rows of 3840 take 4.1 us as 128 x 2, 8 to an SM (5.5 with 12 to an SM; 4096 of
+// them 12.4 and 12.6, 16.2 as 256 x 2); 2048 rows of 8192 12.7 as 256 x 2 (12.8 as 128 x 4, 18.7 as 512 x 2); 4096
+// rows of 15360 40 as 256 x 4 (44 with 5 to an SM, 42 as 128 x 8, 49 as 512 x 2).  One row of 15360 takes 2.8 as 512 x 2 (3.2 as
 // 256 x 4), one of 3840 with its norm 2.7 as 256 x 1 (2.9 as 128 x 2).
-template <int P>
+template <int P, bool kNorm>
 static const void* quant_kernel(int nb4, int rows, int sm_count, int& threads) {
   if (rows <= sm_count) {
     threads = nb4 <= 128 ? 128 : nb4 <= 256 ? 256 : 512;
-    if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P, 8>;
-    if (nb4 <= 256) return (const void*)nv_quant_kernel<256, 1, P, 4>;
-    if (nb4 <= 512) return (const void*)nv_quant_kernel<512, 1, P, 2>;
-    return (const void*)nv_quant_kernel<512, 2, P, 2>;
+    if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P, 8, kNorm>;
+    if (nb4 <= 256) return (const void*)nv_quant_kernel<256, 1, P, 4, kNorm>;
+    if (nb4 <= 512) return (const void*)nv_quant_kernel<512, 1, P, 2, kNorm>;
+    return (const void*)nv_quant_kernel<512, 2, P, 2, kNorm>;
   }
   threads = nb4 <= 256 ? 128 : 256;
-  if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P, 8>;
-  if (nb4 <= 256) return (const void*)nv_quant_kernel<128, 2, P, 8>;
-  if (nb4 <= 512) return (const void*)nv_quant_kernel<256, 2, P, 5>;
-  return (const void*)nv_quant_kernel<256, 4, P, 4>;
+  if (nb4 <= 128) return (const void*)nv_quant_kernel<128, 1, P, 8, kNorm>;
+  if (nb4 <= 256) return (const void*)nv_quant_kernel<128, 2, P, 8, kNorm>;
+  if (nb4 <= 512) return (const void*)nv_quant_kernel<256, 2, P, 5, kNorm>;
+  return (const void*)nv_quant_kernel<256, 4, P, 4, kNorm>;
 }
 
 }  // namespace g4
@@ -335,9 +336,13 @@ g4_status g4_nvfp4_quantize(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, int
   a.x_stride = x_stride;
   a.norm_w = rms_weight;
   int threads = 0;
-  const void* fn = out->pieces == 1   ? quant_kernel<1>(4 * a.kblocks, n_rows, ctx->sm_count, threads)
-                   : out->pieces == 2 ? quant_kernel<2>(4 * a.kblocks, n_rows, ctx->sm_count, threads)
-                                      : quant_kernel<3>(4 * a.kblocks, n_rows, ctx->sm_count, threads);
+  auto kernel = [&](auto norm) {
+    const int nb4 = 4 * a.kblocks;
+    return out->pieces == 1   ? quant_kernel<1, decltype(norm)::value>(nb4, n_rows, ctx->sm_count, threads)
+           : out->pieces == 2 ? quant_kernel<2, decltype(norm)::value>(nb4, n_rows, ctx->sm_count, threads)
+                              : quant_kernel<3, decltype(norm)::value>(nb4, n_rows, ctx->sm_count, threads);
+  };
+  const void* fn = rms_weight != nullptr ? kernel(std::true_type()) : kernel(std::false_type());
   void* args[] = {(void*)&a};
   st = launch_kernel(ctx, fn, dim3(n_rows), dim3(threads), 0, args, false, "nvfp4 quantize");
   ctx->weights_ahead = st == G4_OK && ctx->pdl_ok && out->pieces > 1;

@@ -173,8 +173,11 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
   const uint4* body = r.body();
   const int pieces = r.pieces;
 
+  const int lo = r.before(tid), hi = r.behind(tid);
   float m = -CUDART_INF_F, sum = 0.f;
-  int in = 0;  // the group where m first is
+  // The group where m first is.  What raises it is above -inf: a thread of nothing else has its first element's, so
+  // that what the thread stands for in the bound is an element that reaches it.
+  int in = tid < pieces || lo >= 0 ? 0 : static_cast<int>(kBmOf);
   // The sum is of 2^((l - m) log2 e) as 2^(fma(l, log2 e, -ref) - rest), where ref is m log2 e rounded to f32 and rest
   // what the rounding took: m itself counts as 1 exactly.  Where m is beyond 2^100 (rows masked with the lowest
   // number there is) ref might not be finite: the difference to m comes first there.
@@ -200,7 +203,6 @@ __global__ void __launch_bounds__(kBmThreads) beam_lists_kernel(const __grid_con
     }
   };
   fetch(now, tid);
-  const int lo = r.before(tid), hi = r.behind(tid);
   const uint32_t lo_bits = lo >= 0 ? r.x[lo] : 0xFF80u, hi_bits = hi >= 0 ? r.x[hi] : 0xFF80u;
   if (lo >= 0) {
     const float v = __uint_as_float(lo_bits << 16);

@@ -667,6 +667,25 @@ def test_beam_select_alignments(gpu_ctx, offset):
         _check_beams(gpu_ctx, wide[:, :, offset:offset + vocab], torch.rand((2, 3), generator=g, device="cuda"), min(5, 3 * vocab))
 
 
+@pytest.mark.parametrize("offset", range(8))
+def test_beam_select_short_rows_of_few_tokens(gpu_ctx, offset):
+    """Rows that are hardly more than what lies outside 16-byte pieces, -inf but for none to three tokens, beside a beam
+    that counts and one that does not: as many as were asked for come out, whatever their score."""
+    g = _gen(70 + offset)
+    groups = 24
+    for vocab in range(1, 41):
+        keep = torch.rand((groups, 2, vocab), generator=g, device="cuda").argsort(-1) < torch.arange(groups, device="cuda")[:, None, None] % 4
+        wide = torch.zeros((groups, 2, vocab + 8), dtype=torch.bfloat16, device="cuda")
+        logits = wide[..., offset:offset + vocab]
+        logits.copy_(torch.where(keep, _randn(g, groups, 2, vocab, std=2.0), -math.inf))
+        scores = torch.zeros((groups, 2), device="cuda")
+        scores[::2, 1], scores[1::4, 0] = -math.inf, -0.5
+        for beams in (1, 2):
+            for k in (1, 2, 3, 7, 16, 17, 64):
+                if k <= beams * vocab:
+                    _check_beams(gpu_ctx, logits[:, :beams], scores[:, :beams].contiguous(), k)
+
+
 def test_beam_example():
     """Three requests' beams through six layers, their caches reordered at every step: the score that the search kept
     is the one that the best beam's text has when it is run alone.  (24 logits and their sums, each off by what

@@ -467,7 +467,8 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
       const float fw = n < a.n ? a.w_factor[a.n_factors > 1 ? n : 0] : 0.f;
       float* fx = sm.fx[ti & 1];
       if (e < t.cols) fx[e] = m0 + e < a.m ? a.x_factor[m0 + e] : 0.f;
-      if (t.first_chunks == 0) {
+      if (t.first_chunks == 0) {  // (this tile's sums lie beside the previous tile's, which have been read)
+        pa_fence_before();
         __syncwarp();
         if (lane == 0) pa_arrive_relaxed(free0 + 8 * (ti & 1));
       }

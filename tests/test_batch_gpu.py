@@ -124,6 +124,23 @@ def test_matmul_repeats_itself(gpu_ctx):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("m, n, cols, pieces", [(60, 30720, 256, 2), (200, 30720, 256, 1), (1000, 8192, 96, 2), (2500, 8192, 96, 3)])
+def test_matmul_sums_side_by_side(gpu_ctx, m, n, cols, pieces):
+    """Several short tiles a pair, whose sums alternate between two places of tensor memory, one read while the next
+    tile's are formed in the other: the oracle's, and the same bits again and again."""
+    rows, xv, fx = _rows(gpu_ctx, m, cols, pieces, 41)
+    weight, wv, fw = _weight(gpu_ctx, n, cols, 1, 42)
+    want, size = ob.matmul(xv, wv, fx, fw)
+    out, first = torch.empty((m, n), dtype=torch.bfloat16, device="cuda"), None
+    for _ in range(30):
+        out.fill_(7.0)
+        g4.nvfp4_matmul(gpu_ctx, rows, weight, out)
+        first = out.clone() if first is None else first
+        assert torch.equal(out, first)
+    _sync(gpu_ctx)
+    assert ((first.double() - want).abs() <= (pieces * cols / 64 + 12) * 2.0 ** -23 * size + U * want.abs()).all()
+
+
 def test_matmul_of_the_most_rows(gpu_ctx):
     """2^22 rows of 32 values: more tiles than a grid's second dimension has room for."""
     m = 2 ** 22

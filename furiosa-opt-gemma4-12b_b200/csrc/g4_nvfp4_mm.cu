@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
       }
     }
   } else if (warp == 1) {
+    pdl_wait();  // (the budget of a wait is for this kernel's copies, not for what the kernel before has left to do)
     constexpr uint32_t kStep = 4 * (1 + P);
     const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(t.cols >> 3) << 17) | (8u << 24);
     const uint32_t sfa = tbase + t.cols;
@@ -405,6 +406,7 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
     }
   } else if (warp == 1) {
     if (cta == 0) {
+      pdl_wait();  // (as in the kernel above: no budget runs before it)
       const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(t.cols >> 3) << 17) | (16u << 24);
       constexpr uint32_t kStep = 4 + 4 * kBlocks * P;  // scale columns of 64 columns' products
       const uint32_t sfa = tbase + 512 - 4 * kStep;

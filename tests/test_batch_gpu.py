@@ -583,6 +583,41 @@ def test_calls_captured_and_replayed(gpu_ctx):
     ctx.close()
 
 
+WORK_ON = """
+extern "C" __global__ void work_on(int microseconds, unsigned* out) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  unsigned long long now, end;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+  end = now + 1000ull * microseconds;
+  unsigned turns = 0;
+  while (now < end && ++turns < 100000000u) asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+  out[0] = turns;
+}
+"""
+
+
+@pytest.mark.parametrize("m, n, cols, pieces", [(1, 3840, 4096, 2), (33, 129, 480, 3), (100, 2049, 8192, 1), (600, 2048, 992, 1)])
+def test_matmul_behind_a_kernel_that_works_on(gpu_ctx, m, n, cols, pieces):
+    """The kernel before lets its dependents start and then takes ten times the context's wait budget: that is no time
+    of the product's own waits, which hold and give the oracle's values."""
+    ctx = g4.Context(0, stream=torch.cuda.Stream())
+    ctx.set_wait_budget(2000)
+    work_on = torch.cuda._compile_kernel(WORK_ON, "work_on")
+    turns = torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows, xv, fx = _rows(gpu_ctx, m, cols, pieces, 51)
+    weight, wv, fw = _weight(gpu_ctx, n, cols, 1, 52)
+    out = torch.full((m, (n + 7) // 8 * 8), 7.0, dtype=torch.bfloat16, device="cuda")[:, :n]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(ctx.stream):
+        work_on(grid=(1, 1, 1), block=(32, 1, 1), args=[20000, turns])
+        g4.nvfp4_matmul(ctx, rows, weight, out)
+    torch.cuda.synchronize()
+    assert turns.item() > 0 and ctx.poll() == 0
+    want, size = ob.matmul(xv, wv, fx, fw)
+    assert ((out.double() - want).abs() <= (pieces * cols / 64 + 12) * 2.0 ** -23 * size + U * want.abs()).all()
+    ctx.close()
+
+
 def test_two_contexts_at_once(gpu_ctx):
     """Products (clusters, pairs, single CTAs) and selections of two contexts on two streams, side by side: the same
     bits as one after another."""

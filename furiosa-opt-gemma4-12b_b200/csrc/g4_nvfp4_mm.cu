@@ -160,12 +160,7 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
         if (!t.early || ks - ks0 >= ahead) weights(ks, at.stage);
         rows(ks, at.stage);
       }
-      if (!ok) {
-        atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
-        // no copy may be in flight when the CTA exits (otherwise the products have taken them all)
-        const uint64_t end = global_ns() + 1000000;
-        while (global_ns() < end) __nanosleep(1000);
-      }
+      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     }
   } else if (warp == 1) {
     pdl_wait();  // (the budget of a wait is for this kernel's copies, not for what the kernel before has left to do)
@@ -286,6 +281,12 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   pa_fence_before();
   __syncthreads();
   pa_fence_after();
+  if (sm.abort != 0) {
+    // Gave up somewhere: copies that no product will take and products issued before may be under way (the copying
+    // lane may have had no wait of its own left).  Let them land (bounded) before memory is given back.
+    const uint64_t end = global_ns() + 1000000;
+    while (global_ns() < end) __nanosleep(1000);
+  }
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase),
                  "r"(static_cast<uint32_t>(t.tmem_cols)));

@@ -154,13 +154,11 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
       pdl_wait();
       pdl_launch_dependents();
       PaRing at(0, t.stages);
-      bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, at.next()) {
-        if (ks - ks0 >= ahead && !(ok = pa_wait(&sm.empty[at.stage], at.parity ^ 1, abort, budget))) break;
+        if (ks - ks0 >= ahead && !pa_wait(&sm.empty[at.stage], at.parity ^ 1, abort, budget)) break;
         if (!t.early || ks - ks0 >= ahead) weights(ks, at.stage);
         rows(ks, at.stage);
       }
-      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     }
   } else if (warp == 1) {
     pdl_wait();  // (the budget of a wait is for this kernel's copies, not for what the kernel before has left to do)
@@ -172,11 +170,9 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
     const uint64_t swd0 = nv_scale_desc(base + sw_at), sxd0 = nv_scale_desc(base + sx_at);
     const uint32_t stage16 = t.stage_bytes / 16, piece16 = x_bytes / 16;
     const uint32_t shift = (m0 & 127) >> 5;
-    bool ok = true;
     PaRing at(0, t.stages);
     for (int ks = ks0; ks < ks1; ++ks) {
-      ok = pa_wait_warp(&sm.full[at.stage], at.parity, abort, budget);
-      if (!ok) break;
+      if (!pa_wait_warp(&sm.full[at.stage], at.parity, abort, budget)) break;
       pa_fence_after();
       const uint64_t off = at.stage * stage16;
       const int steps = t.kblocks - 4 * ks;
@@ -204,7 +200,6 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
       __syncwarp();
       at.next();
     }
-    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     // (every MMA is done before tensor memory is given back)
     pa_wait_warp(&sm.done, 0, abort, budget);
   }
@@ -282,8 +277,10 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   __syncthreads();
   pa_fence_after();
   if (sm.abort != 0) {
-    // Gave up somewhere: copies that no product will take and products issued before may be under way (the copying
-    // lane may have had no wait of its own left).  Let them land (bounded) before memory is given back.
+    // Gave up somewhere, whichever warp it was: say so.  Copies that no product will take and products issued before may
+    // be under way (the copying lane may have had no wait of its own left): let them land (bounded) before memory is
+    // given back.
+    if (tid == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     const uint64_t end = global_ns() + 1000000;
     while (global_ns() < end) __nanosleep(1000);
   }
@@ -403,7 +400,6 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
       // Every copy has landed (the leader's products took it) once its stage is free again; both
       // CTAs stay until then.
       for (int i = 0; i < t.stages && ok; ++i, at.next()) ok = free();
-      if (!ok) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     }
   } else if (warp == 1) {
     if (cta == 0) {
@@ -452,7 +448,6 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
       }
       // (the other CTA's last arrivals: nothing of it may be under way when this one ends)
       if (ok && ti > 0) ok = pa_wait_warp(&sm.d_free[(ti - 1) & 1], ((ti - 1) >> 1) & 1, abort, budget);
-      if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     }
   } else {
     // -------------------------------------------------------------- output
@@ -539,10 +534,10 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
     }
     if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // (shared memory is still there for them)
     __syncwarp();
-    if (!ok && lane == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
   }
   __syncthreads();
-  if (sm.abort != 0) {  // gave up somewhere: let the copies in flight land (bounded)
+  if (sm.abort != 0) {  // gave up somewhere: say so, and let the copies in flight land (bounded)
+    if (tid == 0) atomicOr(&scr->status, DEV_ERR_TIMEOUT_MBAR);
     const uint64_t end = global_ns() + 1000000;
     while (global_ns() < end) __nanosleep(1000);
   }

@@ -44,11 +44,19 @@ g4_status allow_max_dynamic_smem(g4_ctx* ctx, const void* fn, size_t need, const
   return st;
 }
 
+std::atomic<uint64_t>& launches_on(const g4_ctx* ctx) {
+  static std::atomic<uint64_t> counts[256];
+  uint64_t key = reinterpret_cast<uintptr_t>(ctx->stream);
+  if (ctx->stream == cudaStreamLegacy) key = 0;  // (two names of one stream)
+  key = (key + static_cast<uint64_t>(ctx->device)) * 0x9E3779B97F4A7C15ull;
+  return counts[key >> 56];
+}
+
 g4_status launch_kernel(g4_ctx* ctx, const void* fn, dim3 grid, dim3 block, size_t smem, void** args,
                         bool cooperative, const char* what, unsigned cluster_x) {
   cudaLaunchAttribute attrs[3];
   unsigned n = 0;
-  ctx->weights_ahead = false;
+  ++launches_on(ctx);
   if (cooperative) {
     attrs[n].id = cudaLaunchAttributeCooperative;
     attrs[n].val.cooperative = 1;
@@ -337,7 +345,7 @@ g4_status g4_ctx_destroy(g4_ctx* ctx) {
 g4_status g4_ctx_set_stream(g4_ctx* ctx, g4_stream_t stream) {
   G4_CHECK_CTX(ctx);
   ctx->stream = reinterpret_cast<cudaStream_t>(stream);
-  ctx->weights_ahead = false;  // (what precedes the next launch is another one now)
+  ctx->quantised = 0;  // (what precedes the next launch is another one now)
   return G4_OK;
 }
 

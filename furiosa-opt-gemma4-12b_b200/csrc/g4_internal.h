@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -122,10 +123,9 @@ struct g4_ctx {
   g4::PrefillBuffers prefill;
   g4::PagedBuffers paged;
   int prefill_pieces = 2;  // NVFP4 pieces per prefill activation (1..3)
-  // The last launch quantised rows of several pieces and lets its successor start once its own predecessors
-  // are done: weights that are not among what it writes may be read ahead of it.
-  bool weights_ahead = false;
-  g4_nvfp4_rows quantised = {};  // what it writes
+  // The number, among the launches on this stream (launches_on), of a quantisation that lets its successor start once
+  // its own predecessors are done: a constant weight may be read ahead of it.  0: none.
+  uint64_t quantised = 0;
 };
 
 namespace g4 {
@@ -144,6 +144,9 @@ struct DeviceGuard {
     if (before >= 0) cudaSetDevice(before);
   }
 };
+// How many launches all contexts of the process have made on this one's stream so far.  (Streams may share a counter:
+// one that has not moved says that nothing was launched, one that has moved says nothing.)
+std::atomic<uint64_t>& launches_on(const g4_ctx* ctx);
 // A bf16 matrix argument: 16-byte aligned, its row stride a multiple of 8 of at least `cols` where
 // there are several rows (g4_rows.cu).
 g4_status check_matrix(g4_ctx* ctx, const void* p, int64_t stride, int rows, int cols, const char* what);

@@ -345,8 +345,7 @@ g4_status g4_nvfp4_quantize(g4_ctx* ctx, const g4_bf16* x, int64_t x_stride, int
   const void* fn = rms_weight != nullptr ? kernel(std::true_type()) : kernel(std::false_type());
   void* args[] = {(void*)&a};
   st = launch_kernel(ctx, fn, dim3(n_rows), dim3(threads), 0, args, false, "nvfp4 quantize");
-  ctx->weights_ahead = st == G4_OK && ctx->pdl_ok && out->pieces > 1;
-  ctx->quantised = *out;
+  ctx->quantised = st == G4_OK && ctx->pdl_ok && out->pieces > 1 ? launches_on(ctx).load() : 0;
   return st;
 }
 
@@ -373,6 +372,8 @@ g4_status g4_nvfp4_matmul(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, co
   if (weight == nullptr) return fail(ctx, G4_ERR_BAD_ARG, "nvfp4 weight: null descriptor");
   if (weight->rows < 1 || weight->rows > kNvMaxRows || weight->cols != rows->cols)
     return fail(ctx, G4_ERR_BAD_ARG, "nvfp4 weight: rows out of range, or cols other than the activations'");
+  if (weight->constant != 0 && weight->constant != 1)
+    return fail(ctx, G4_ERR_BAD_ARG, "nvfp4 weight: constant is 0 or 1");
   if (weight->n_factors != 1 && weight->n_factors != weight->rows)
     return fail(ctx, G4_ERR_BAD_ARG, "nvfp4 weight: one factor, or one for each row");
   if (!aligned16(weight->codes) || !aligned16(weight->scales))
@@ -383,17 +384,12 @@ g4_status g4_nvfp4_matmul(g4_ctx* ctx, const g4_nvfp4_rows* rows, int n_rows, co
   if ((st = check_matrix(ctx, out, out_stride, n_rows, weight->rows, "out")) != G4_OK) return st;
   if (n_rows == 1) out_stride = (static_cast<int64_t>(weight->rows) + 7) / 8 * 8;  // (of no meaning, but tensor maps want one)
   DeviceGuard on(ctx);
-  if (ctx->weights_ahead) {  // (a weight made of one of the rows' pieces is not there yet)
-    const QuantArgs q = quant_args(&ctx->quantised);
-    auto meet = [](const uint8_t* a, size_t na, const uint8_t* b, size_t nb) { return a < b + nb && b < a + na; };
-    const size_t codes = static_cast<size_t>(weight->rows) * (weight->cols / 2);
-    if (meet(weight->codes, codes, q.codes, q.code_piece * ctx->quantised.pieces) ||
-        meet(weight->scales, nv_scale_bytes(weight->rows, weight->cols), q.scales, q.scale_piece * ctx->quantised.pieces))
-      ctx->weights_ahead = false;
-  }
+  // Nothing behind that quantisation on the stream: no launch of any context (one may have laid this weight out, or be
+  // about to overwrite it as one of its rows' pieces), and no kernel of the caller's that could write a constant weight.
+  const bool early = weight->constant != 0 && ctx->quantised != 0 && ctx->quantised == launches_on(ctx).load();
   return launch_nvfp4_matmul(ctx, {rows->codes, rows->scales, rows->factor, weight->codes, weight->scales, weight->factor,
                                    n_rows, weight->rows, rows->cols, rows->pieces, rows->max_rows, weight->n_factors,
-                                   out_f32 != 0, out, out_stride});
+                                   out_f32 != 0, early, out, out_stride});
 }
 
 }  // extern "C"

@@ -25,6 +25,7 @@ struct NvMatmulArgs {
   const uint8_t* w_scales;
   const float* w_factor;
   int m, n, k, pieces, max_rows, n_factors, out_f32;
+  int early;  // the weights may be fetched before the previous kernel is done
   void* out;
   long long out_stride;
 };

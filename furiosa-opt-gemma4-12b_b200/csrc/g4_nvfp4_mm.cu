@@ -86,7 +86,6 @@ constexpr int kNvMaxStages = 8;
 struct NvTileArgs {
   NvMatmulArgs a;
   int cols, splits, stages, stage_bytes, k_stages, kblocks, tmem_cols, row_tiles;
-  int early;  // the weights may be fetched before the previous kernel is done
   size_t x_scale_piece;
 };
 struct NvTileBars {
@@ -149,14 +148,14 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
         }
       };
       const int ahead = min(t.stages, ks1 - ks0);
-      if (t.early)
+      if (a.early)
         for (int i = 0; i < ahead; ++i) weights(ks0 + i, i);
       pdl_wait();
       pdl_launch_dependents();
       PaRing at(0, t.stages);
       for (int ks = ks0; ks < ks1; ++ks, at.next()) {
         if (ks - ks0 >= ahead && !pa_wait(&sm.empty[at.stage], at.parity ^ 1, abort, budget)) break;
-        if (!t.early || ks - ks0 >= ahead) weights(ks, at.stage);
+        if (!a.early || ks - ks0 >= ahead) weights(ks, at.stage);
         rows(ks, at.stage);
       }
     }
@@ -641,7 +640,6 @@ static g4_status launch_tiles(g4_ctx* ctx, const NvMatmulArgs& a, int cols, int 
   t.kblocks = (a.k + 63) / 64;
   t.k_stages = (t.kblocks + 3) / 4;
   t.x_scale_piece = nv_scale_bytes(a.max_rows, a.k);
-  t.early = ctx->weights_ahead;
   t.row_tiles = (a.n + 127) / 128;
   const int col_tiles = (a.m + t.cols - 1) / t.cols;
   t.tmem_cols = 32;

@@ -34,7 +34,8 @@ class _RowsDesc(ctypes.Structure):
 
 
 class _WeightDesc(ctypes.Structure):
-    _fields_ = [("codes", _vp), ("scales", _vp), ("factor", _vp), ("rows", _i32), ("cols", _i32), ("n_factors", _i32)]
+    _fields_ = [("codes", _vp), ("scales", _vp), ("factor", _vp), ("rows", _i32), ("cols", _i32), ("n_factors", _i32),
+                ("constant", _i32)]
 
 
 _rows_p, _weight_p = ctypes.POINTER(_RowsDesc), ctypes.POINTER(_WeightDesc)
@@ -164,7 +165,8 @@ class Nvfp4Weight:
     """A projection [rows, cols] for nvfp4_matmul (g4_nvfp4_weight): the checkpoint's codes uint8
     [rows, cols / 2] (kept, not copied), its block scales [rows, cols / 16], which are laid out anew, and
     the reciprocal global scale f32 [1], or a factor for every row, f32 [rows] (projections stacked
-    along their rows)."""
+    along their rows).  Codes and scales are constant (g4.h): nothing may write them between the nvfp4_quantize
+    and the nvfp4_matmul of a product, which reads them ahead; a weight that changes is one of `from_rows`."""
 
     def __init__(self, ctx: Context, codes, block_scales, global_scale):
         n, half = _tensor(ctx, "codes", codes, (_U8,), 2).shape
@@ -179,7 +181,7 @@ class Nvfp4Weight:
         with torch.cuda.stream(ctx.stream):
             scales = torch.empty(LIB.g4_nvfp4_scale_bytes(n, cols), dtype=_U8, device=f"cuda:{ctx.device}")
         ctx._check("g4_nvfp4_scale_blocks", LIB.g4_nvfp4_scale_blocks(ctx.handle, given, n, cols, scales.data_ptr()))
-        self._set(codes, scales, global_scale, n, cols, ctx.device)
+        self._set(codes, scales, global_scale, n, cols, ctx.device, 1)
 
     @classmethod
     def from_rows(cls, rows: Nvfp4Rows) -> "Nvfp4Weight":
@@ -190,9 +192,9 @@ class Nvfp4Weight:
         w._set(rows.codes, rows.scales, rows.factor, rows.max_rows, rows.cols, rows.device)
         return w
 
-    def _set(self, codes, scales, factor, n, cols, device):
+    def _set(self, codes, scales, factor, n, cols, device, constant=0):
         self.codes, self.scales, self.factor, self.rows, self.cols, self.device = codes, scales, factor, n, cols, device
-        self.desc = _WeightDesc(codes.data_ptr(), scales.data_ptr(), factor.data_ptr(), n, cols, factor.numel())
+        self.desc = _WeightDesc(codes.data_ptr(), scales.data_ptr(), factor.data_ptr(), n, cols, factor.numel(), constant)
 
 
 def _rows_of(ctx: Context, rows: Nvfp4Rows, n: int) -> None:

@@ -517,12 +517,15 @@ typedef struct g4_nvfp4_rows {
 } g4_nvfp4_rows;
 /* A weight [rows, cols]: codes as the checkpoint has them (the row length of g4_nvfp4_rows, so a
  * matrix quantised as one piece is one too), scale blocks, and n_factors = 1 (the checkpoint's
- * reciprocal global scale) or = rows f32 factors (several projections stacked, or quantised rows). */
+ * reciprocal global scale) or = rows f32 factors (several projections stacked, or quantised rows).
+ * constant = 1 says that codes and scales are written by nothing that is still to run, on any stream, when rows are
+ * quantised for a product by them: then the product may read them while that g4_nvfp4_quantize, the launch in front
+ * of it, still runs.  With 0 it reads them in stream order, like everything else. */
 typedef struct g4_nvfp4_weight {
   const g4_f4x2* codes;
   const g4_f8e4m3* scales;
   const float* factor;
-  int32_t rows, cols, n_factors;
+  int32_t rows, cols, n_factors, constant;
 } g4_nvfp4_weight;
 
 /* x [n_rows, cols] into `out`.  rms_weight (or NULL): x = bf16(x * r * rms_weight) first, r as in

@@ -115,6 +115,12 @@ def test_c_entry_points_refuse_a_null_context():
     assert L.g4_beam_select(None, None, 0, 0, None, 1, 1, 9, 1, None, None, None) == 1
 
 
+def test_weight_descriptors_in_place():
+    """The field behind n_factors fills what was padding: descriptors keep their size."""
+    assert ctypes.sizeof(g4.batch._WeightDesc) == 40 and g4.batch._WeightDesc.constant.offset == 36
+    assert g4.batch._WeightDesc(1, 2, 3, 4, 5, 6).constant == 0
+
+
 def test_scale_bytes():
     assert g4.LIB.g4_nvfp4_scale_bytes(1, 32) == 512
     assert g4.LIB.g4_nvfp4_scale_bytes(129, 3840) == 2 * 60 * 512

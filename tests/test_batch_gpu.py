@@ -157,6 +157,72 @@ def test_matmul_of_the_most_rows(gpu_ctx):
         assert ((out[at].double() - want).abs() <= 13 * 2.0 ** -23 * size).all()
 
 
+@pytest.mark.parametrize("m, n, cols", [(1, 3840, 15360), (32, 3840, 8192), (17, 300, 2080), (100, 2049, 8192), (1, 8192, 3840)])
+@pytest.mark.parametrize("pieces", [2, 3])
+def test_matmul_ahead_of_the_quantisation(gpu_ctx, m, n, cols, pieces):
+    """A constant weight's first stages are read while the rows are still being quantised, the rest behind that: the
+    oracle's values, and the bits of products that read nothing ahead."""
+    x = _randn(_gen(m + n), m, cols)
+    rows = g4.Nvfp4Rows(gpu_ctx, m, cols, pieces)
+    weight, wv, fw = _weight(gpu_ctx, n, cols, 1, 71)
+    changing = g4.Nvfp4Weight.__new__(g4.Nvfp4Weight)
+    changing._set(weight.codes, weight.scales, weight.factor, n, cols, 0)
+    assert weight.desc.constant == 1 and changing.desc.constant == 0
+    ahead, after, ordered = (torch.full((m, (n + 7) // 8 * 8), 7.0, dtype=torch.bfloat16, device="cuda")[:, :n] for _ in range(3))
+    for _ in range(5):
+        g4.nvfp4_quantize(gpu_ctx, x, rows)
+        g4.nvfp4_matmul(gpu_ctx, rows, weight, ahead)
+        g4.nvfp4_matmul(gpu_ctx, rows, weight, after)  # (a launch lies between)
+        g4.nvfp4_quantize(gpu_ctx, x, rows)
+        g4.nvfp4_matmul(gpu_ctx, rows, changing, ordered)
+        _sync(gpu_ctx)
+        assert torch.equal(ahead, after) and torch.equal(ahead, ordered)
+    codes, scales, factor = ob.quantize(x, pieces)
+    want, size = ob.matmul(ob.values(codes, scales).sum(0), wv, factor, fw)
+    assert ((ahead.double() - want).abs() <= (pieces * cols / 64 + 12) * 2.0 ** -23 * size + U * want.abs()).all()
+
+
+def test_matmul_by_what_another_context_makes(gpu_ctx):
+    """Two contexts on one stream: one quantises rows, the other then makes the weight (a piece of rows, scale blocks of
+    a checkpoint's), and the first multiplies by it."""
+    stream = torch.cuda.Stream()
+    a, b = g4.Context(0, stream=stream), g4.Context(0, stream=stream)
+    g = _gen(72)
+    x, w = _randn(g, 3, 4096), _randn(g, 2048, 4096)
+    codes = torch.randint(0, 256, (2048, 2048), generator=g, device="cuda", dtype=torch.uint8)
+    given = [torch.randint(40, 70, (2048, 256), generator=g, device="cuda", dtype=torch.uint8) for _ in range(2)]
+    one = torch.ones(1, device="cuda")
+    torch.cuda.synchronize()
+    rows, made, first = g4.Nvfp4Rows(a, 3, 4096), g4.Nvfp4Rows(b, 2048, 4096, 2), g4.Nvfp4Rows(b, 2048, 4096, 1)
+    piece = g4.Nvfp4Weight.from_rows(first)
+    piece._set(made.codes, made.scales, made.factor, 2048, 4096, made.device)
+    out, want = (torch.empty((3, 2048), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        g4.nvfp4_quantize(b, w, first)
+        g4.nvfp4_quantize(a, x, rows)
+        torch.cuda.synchronize()
+        g4.nvfp4_matmul(a, rows, g4.Nvfp4Weight.from_rows(first), want)
+        for _ in range(20):
+            made.codes.fill_(0x77), made.scales.fill_(0x38)
+            g4.nvfp4_quantize(a, x, rows)
+            g4.nvfp4_quantize(b, w, made)
+            g4.nvfp4_matmul(a, rows, piece, out)
+            assert torch.equal(out, want)
+        cx, sx, fx = ob.quantize(x, 2)
+        for i in range(20):
+            scales = given[i % 2]
+            g4.nvfp4_quantize(a, x, rows)
+            weight = g4.Nvfp4Weight(b, codes, scales, one)
+            g4.nvfp4_matmul(a, rows, weight, out)
+            y, size = ob.matmul(ob.values(cx, sx).sum(0), ob.values(ob.unpack(codes), scales), fx, one.double())
+            assert ((out.double() - y).abs() <= (2 * 4096 / 64 + 12) * 2.0 ** -23 * size + U * y.abs()).all()
+    torch.cuda.synchronize()
+    for ctx in (a, b):
+        assert ctx.poll() == 0
+        ctx.close()
+
+
 def test_matmul_nan_row_stays_in_its_row(gpu_ctx):
     x = _randn(_gen(3), 140, 512)
     x[7, 100], x[131, 0], x[20] = float("nan"), float("inf"), 0
@@ -743,6 +809,16 @@ def test_library_refuses(gpu_ctx):
     _sync(gpu_ctx)
     assert not t.any()
     assert ctypes.sizeof(g4.batch._RowsDesc) == 40 and ctypes.sizeof(g4.batch._WeightDesc) == 40
+
+
+def test_library_refuses_other_constants(gpu_ctx):
+    t = torch.zeros(1 << 14, dtype=torch.uint8, device="cuda")
+    p = t.data_ptr()
+    rows, weight = g4.batch._RowsDesc(p, p, p, 4, 64, 2), g4.batch._WeightDesc(p, p, p, 8, 64, 1, 2)
+    assert g4.LIB.g4_nvfp4_matmul(gpu_ctx.handle, rows, 4, weight, p, 8, 0) == 1
+    weight.constant = -1
+    assert g4.LIB.g4_nvfp4_matmul(gpu_ctx.handle, rows, 4, weight, p, 8, 0) == 1
+    _sync(gpu_ctx)
 
 
 def test_beam_select_zero_of_either_sign(gpu_ctx):

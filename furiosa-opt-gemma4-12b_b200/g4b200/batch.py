@@ -181,6 +181,7 @@ class Nvfp4Weight:
         with torch.cuda.stream(ctx.stream):
             scales = torch.empty(LIB.g4_nvfp4_scale_bytes(n, cols), dtype=_U8, device=f"cuda:{ctx.device}")
         ctx._check("g4_nvfp4_scale_blocks", LIB.g4_nvfp4_scale_blocks(ctx.handle, given, n, cols, scales.data_ptr()))
+        block_scales.record_stream(ctx.stream)  # (not kept: their memory is nobody else's until that has read them)
         self._set(codes, scales, global_scale, n, cols, ctx.device, 1)
 
     @classmethod

@@ -374,6 +374,31 @@ def test_scale_blocks(gpu_ctx):
         assert torch.equal(w.scales, ob.scale_blocks(s))
 
 
+def test_weights_made_in_a_loop_on_another_stream(gpu_ctx):
+    """Block scales that are dropped as soon as the constructor is back, on a stream other than the context's, which is
+    busy: each weight is laid out from its own, and multiplies as the oracle says."""
+    ctx = g4.Context(0, stream=torch.cuda.Stream())
+    n, cols = 700, 1024
+    g = _gen(81)
+    codes = torch.randint(0, 256, (n, cols // 2), generator=g, device="cuda", dtype=torch.uint8)
+    kept = [torch.randint(30, 70, (n, cols // 16), generator=g, device="cuda", dtype=torch.uint8) for _ in range(6)]
+    rows, xv, fx = _rows(gpu_ctx, 5, cols, 2, 82)
+    one, outs = torch.ones(1, device="cuda"), torch.zeros((6, 5, 704), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(ctx.stream):
+        torch.cuda._sleep(100_000_000)  # (some 50 ms)
+    weights = [g4.Nvfp4Weight(ctx, codes, k.clone().view(torch.float8_e4m3fn), one) for k in kept]
+    for w, out in zip(weights, outs):
+        g4.nvfp4_matmul(ctx, rows, w, out[:, :n])
+    torch.cuda.synchronize()
+    assert ctx.poll() == 0
+    for w, k, out in zip(weights, kept, outs):
+        assert torch.equal(w.scales, ob.scale_blocks(k))
+        want, size = ob.matmul(xv, ob.values(ob.unpack(codes), k), fx, one.double())
+        assert ((out[:, :n].double() - want).abs() <= (2 * cols / 64 + 12) * 2.0 ** -23 * size + U * want.abs()).all()
+    ctx.close()
+
+
 # ------------------------------------------------------------------------------ rows
 @pytest.mark.parametrize("n, vocab, dim, gap", [(1, 262144, 3840, 0), (1, 1, 8, 0), (300, 1000, 3840, 8), (7, 50, 24, 0),
                                                 (513, 33, 8192, 16), (4096, 262144, 64, 0)])

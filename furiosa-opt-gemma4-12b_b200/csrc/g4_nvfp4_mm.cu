@@ -71,6 +71,27 @@ __device__ __forceinline__ void nv_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// Whether it holds for all of the 256 threads of the output warps, which meet here.
+__device__ __forceinline__ bool nv_agree(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
+}
+
+// A sum (2^-20 to 2^45, or 0) times the factors of its row and its weight row.  The factors' product comes first: where
+// both are within 2^-60 to 2^60 it is a normal number, and the result leaves f32's range only if it has to.  Other
+// factors (rows next to an end of bf16's range) may have a product beyond f32 that the sum brings back, and so may
+// the sum and either of them: 64 bits.
+__device__ __forceinline__ bool nv_plain(float f) { return !(fabsf(f) > 0x1p60f) && !(fabsf(f) < 0x1p-60f && f != 0.f); }
+__device__ __noinline__ float nv_wide(float v, float fx, float fw) {
+  return static_cast<float>(static_cast<double>(v) * fx * fw);
+}
+
 // ---------------------------------------------------------------------------- single CTAs
 // A tile is 128 weight rows x `cols` activation rows; a cluster of `splits` CTAs shares its K range, and
 // each CTA then adds up 128 / splits of the tile's rows, whose parts the others stored into its
@@ -207,12 +228,17 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
   const int q = warp & 3, e = tid - 64, r = 32 * q + lane;
   const int valid = min(t.cols, a.m - m0);
   const uint32_t from = tbase + (static_cast<uint32_t>(32 * q) << 16);
-  bool got = true;
+  bool got = true, plain = true;
   if (warp >= 2) {
     pdl_wait();
-    if (e < valid) sm.fx[e] = a.x_factor[m0 + e];
-    if (e >= 128) sm.fw[e - 128] = n0 + e - 128 < a.n ? a.w_factor[a.n_factors > 1 ? n0 + e - 128 : 0] : 0.f;
-    named_bar_sync(1, 256);
+    if (e < valid) {
+      sm.fx[e] = a.x_factor[m0 + e];
+      plain = nv_plain(sm.fx[e]);
+    } else if (e >= 128) {
+      sm.fw[e - 128] = n0 + e - 128 < a.n ? a.w_factor[a.n_factors > 1 ? n0 + e - 128 : 0] : 0.f;
+      plain = nv_plain(sm.fw[e - 128]);
+    }
+    plain = nv_agree(plain);
     got = pa_wait_warp(&sm.done, 0, abort, budget);
     pa_fence_after();
   }
@@ -232,7 +258,7 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
         nv_ld16(from + c0, part);
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (c0 + j < valid) store(c0 + j, n0 + r, part[j] * sm.fx[c0 + j] * fw);
+          if (c0 + j < valid) store(c0 + j, n0 + r, plain ? part[j] * (sm.fx[c0 + j] * fw) : nv_wide(part[j], sm.fx[c0 + j], fw));
       }
     }
   } else {
@@ -265,10 +291,16 @@ __global__ void __launch_bounds__(kNvTileThreads, 1)
           sum.z += __uint_as_float(v.z), sum.w += __uint_as_float(v.w);
         }
         const float f = sm.fw[own];
-        const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+        float out[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (plain) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out[j] *= sm.fx[c + j] * f;
+        } else {
+          for (int j = 0; j < 4; ++j) out[j] = nv_wide(out[j], sm.fx[c + j], f);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (c + j < valid) store(c + j, n0 + own, out[j] * sm.fx[c + j] * f);
+          if (c + j < valid) store(c + j, n0 + own, out[j]);
       }
     }
   }
@@ -314,18 +346,6 @@ struct NvPairBars {
   __align__(16) float fx[2][256];
 };
 constexpr int kNvOutBytes = 32 * 128 * 2;  // a chunk on its way out; two for each group of output warps
-// The output warps agree on whether all of their waits held (they meet at barriers of their own).
-__device__ __forceinline__ bool nv_agree(bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(static_cast<uint32_t>(ok))
-      : "memory");
-  return r != 0;
-}
-
 __device__ __forceinline__ void nv_pair_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
@@ -464,6 +484,7 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
       const float fw = n < a.n ? a.w_factor[a.n_factors > 1 ? n : 0] : 0.f;
       float* fx = sm.fx[ti & 1];
       if (e < t.cols) fx[e] = m0 + e < a.m ? a.x_factor[m0 + e] : 0.f;
+      const bool plain = nv_agree(nv_plain(fw) && (e >= t.cols || nv_plain(fx[e])));
       if (t.first_chunks == 0) {  // (this tile's sums lie beside the previous tile's, which have been read)
         pa_fence_before();
         __syncwarp();
@@ -486,10 +507,15 @@ __global__ void __launch_bounds__(kNvPairThreads, 1)
         }
         const int valid = a.m - (m0 + c0);  // rows of the chunk that there are
         if (valid <= 0 || n0 >= a.n) continue;
+        if (plain) {
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(fx + c0 + c);
-          v[c] *= f.x * fw, v[c + 1] *= f.y * fw, v[c + 2] *= f.z * fw, v[c + 3] *= f.w * fw;
+          for (int c = 0; c < 32; c += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(fx + c0 + c);
+            v[c] *= f.x * fw, v[c + 1] *= f.y * fw, v[c + 2] *= f.z * fw, v[c + 3] *= f.w * fw;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = nv_wide(v[c], fx[c0 + c], fw);
         }
         if (kF32 || (a.n % 8 != 0 && n0 + 128 > a.n)) {
           // (a copy out of shared memory writes whole 16 bytes, past an end that is not on such a border)

@@ -114,6 +114,34 @@ def test_matmul_f32_strides_and_factors(gpu_ctx, m, n, cols, pieces):
     _product(gpu_ctx, m, n, cols, pieces, f32=False, gap=8, factors=n, seed=6)
 
 
+@pytest.mark.parametrize("m, n, cols, pieces", [(1, 515, 3840, 2), (20, 301, 992, 1), (40, 6001, 2080, 1), (33, 129, 480, 3),
+                                                (257, 520, 1056, 1), (509, 8704, 96, 2), (2050, 8192, 96, 3)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_matmul_factors_far_apart(gpu_ctx, m, n, cols, pieces, f32):
+    """Factors of rows and weights whose product, or the sum's with either, leaves f32's range while the result is in it.
+    Bounds as above, with half a step of subnormal results more (f32 2^-150, bf16 2^-134); what is twice f32's
+    largest number is infinite."""
+    rows, xv, fx = _rows(gpu_ctx, m, cols, pieces, 31)
+    weight, wv, fw = _weight(gpu_ctx, n, cols, n, 32)
+    g = _gen(33)
+    pick = lambda exponents, count: torch.exp2(torch.tensor(exponents, device="cuda")[  # noqa: E731
+        torch.randint(0, len(exponents), (count,), generator=g, device="cuda")].double()).float()
+    rows.factor[:m] = pick([-126.0, -100.0, -60.0, 0.0, 60.0, 100.0, 117.0], m)
+    if m == 1:
+        rows.factor[0] = 2.0 ** 117
+    weight.factor.copy_(pick([-140.0, -126.0, -90.0, -17.0, 0.0, 90.0, 125.0], n) * (1 + torch.rand(n, generator=g, device="cuda")))
+    out = torch.empty((m, (n + 7) // 8 * 8), dtype=torch.float32 if f32 else torch.bfloat16, device="cuda")[:, :n]
+    g4.nvfp4_matmul(gpu_ctx, rows, weight, out)
+    _sync(gpu_ctx)
+    want, size = ob.matmul(xv, wv, rows.factor[:m].double(), weight.factor.double())
+    bound = (pieces * cols / 64 + 12) * 2.0 ** -23 * size + (2.0 ** -150 if f32 else U * want.abs() + 2.0 ** -134)
+    inside, beyond = (want.abs() + bound) < 2.0 ** 127, (want.abs() - bound) > 2.0 ** 129
+    assert inside.any() and (m == 1 or beyond.any())
+    worst = ((out.double() - want).abs() - bound)[inside].max().item()
+    assert worst <= 0, f"error above its bound by {worst}"
+    assert torch.isinf(out[beyond]).all()
+
+
 def test_matmul_repeats_itself(gpu_ctx):
     rows, _, _ = _rows(gpu_ctx, 600, 1920, 2)
     weight, _, _ = _weight(gpu_ctx, 1000, 1920)

@@ -337,8 +337,8 @@ constexpr int kNvPairThreads = 320;  // warp 0 copies, 1 MMA (leader) and tensor
 
 struct NvPairArgs {
   NvMatmulArgs a;
-  int cols, blocks, stages, stage_bytes, k_stages, kblocks, row_tiles, tiles;
-  int sf_cols, acc_step, first_chunks;  // scale columns; column of the second sums; chunks of 32 columns per warp in the overlap
+  int cols, stages, stage_bytes, k_stages, kblocks, row_tiles, tiles;
+  int acc_step, first_chunks;  // column of the second sums; chunks of 32 columns per warp in the overlap
 };
 struct NvPairBars {
   uint64_t full[kNvMaxStages], empty[kNvMaxStages], d_full[2], d_free[2];
@@ -627,16 +627,15 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   NvPairArgs t = {};
   t.a = a;
   t.cols = cols;
-  t.blocks = cols > 128 ? 2 : 1;
+  const int blocks = cols > 128 ? 2 : 1;  // of scales, across a tile's activation rows
   t.kblocks = (a.k + 63) / 64;
   t.k_stages = (t.kblocks + 3) / 4;
   t.row_tiles = (a.n + 255) / 256;
   t.tiles = t.row_tiles * ((a.m + cols - 1) / cols);
-  t.sf_cols = 4 * (4 + 4 * t.blocks * a.pieces);
-  const int room = 512 - t.sf_cols;
+  const int room = 512 - 4 * (4 + 4 * blocks * a.pieces);  // beside a stage's scales
   t.acc_step = 2 * cols <= room ? cols : room - cols;
   t.first_chunks = (cols - t.acc_step + 63) / 64;
-  t.stage_bytes = 16384 + a.pieces * (cols / 2) * 128 + 2048 + a.pieces * t.blocks * 2048;
+  t.stage_bytes = 16384 + a.pieces * (cols / 2) * 128 + 2048 + a.pieces * blocks * 2048;
   const int out_bytes = a.out_f32 ? 0 : 4 * kNvOutBytes;
   t.stages = (static_cast<int>(kNvSmem) - 1024 - out_bytes) / t.stage_bytes;
   if (t.stages > kNvMaxStages) t.stages = kNvMaxStages;
@@ -645,10 +644,10 @@ static g4_status launch_pairs(g4_ctx* ctx, const NvMatmulArgs& a, int cols) {
   if (!nv_code_map(&wmap, a.w_codes, a.k / 2, a.n, 1, 0, 128) ||
       !nv_code_map(&xmap, a.x_codes, a.k / 2, a.m, a.pieces, static_cast<size_t>(a.max_rows) * (a.k / 2), cols / 2) ||
       !nv_scale_map(&wsmap, a.w_scales, t.kblocks, a.n, 1, 1) ||
-      !nv_scale_map(&xsmap, a.x_scales, t.kblocks, a.max_rows, a.pieces, t.blocks) ||
+      !nv_scale_map(&xsmap, a.x_scales, t.kblocks, a.max_rows, a.pieces, blocks) ||
       (!a.out_f32 && !nv_out_map(&omap, a.out, a.n, a.m, a.out_stride)))
     return fail(ctx, G4_ERR_CUDA, "cuTensorMapEncodeTiled failed (nvfp4 matmul)");
-  const void* fn = a.out_f32 ? pair_kernel<true>(a.pieces, t.blocks) : pair_kernel<false>(a.pieces, t.blocks);
+  const void* fn = a.out_f32 ? pair_kernel<true>(a.pieces, blocks) : pair_kernel<false>(a.pieces, blocks);
   const g4_status st = allow_max_dynamic_smem(ctx, fn, smem, "nvfp4 matmul");
   if (st != G4_OK) return st;
   Scratch* scr = ctx->buf.scratch;

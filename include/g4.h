@@ -515,9 +515,11 @@ typedef struct g4_nvfp4_rows {
   float* factor;
   int32_t max_rows, cols, pieces;
 } g4_nvfp4_rows;
-/* A weight [rows, cols]: codes as the checkpoint has them (the row length of g4_nvfp4_rows, so a
+/* A weight [rows, cols]: codes as an NVFP4 checkpoint has them, in the row length of g4_nvfp4_rows (so a
  * matrix quantised as one piece is one too), scale blocks, and n_factors = 1 (the checkpoint's
  * reciprocal global scale) or = rows f32 factors (several projections stacked, or quantised rows).
+ * The reference's checkpoint has the MLP like this, but the attention's projections in FP8
+ * (src/host/load.rs:89-386): those become weights by being dequantised and quantised as one piece.
  * constant = 1 says that codes and scales are written by nothing that is still to run, on any stream, when rows are
  * quantised for a product by them: then the product may read them while that g4_nvfp4_quantize, the launch in front
  * of it, still runs.  With 0 it reads them in stream order, like everything else. */

@@ -34,7 +34,7 @@ def weight(ctx, g, n, k):
     """A random projection, quantised on the GPU."""
     rows = g4.Nvfp4Rows(ctx, n, k, 1)
     g4.nvfp4_quantize(ctx, (torch.randn((n, k), generator=g, device="cuda") * k ** -0.5).bfloat16(), rows)
-    return g4.Nvfp4Weight.from_rows(rows)
+    return g4.Nvfp4Weight.from_rows(rows, constant=True)
 
 
 def stored(g, n, k):

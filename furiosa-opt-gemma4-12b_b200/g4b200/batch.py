@@ -166,7 +166,7 @@ class Nvfp4Weight:
     [rows, cols / 2] (kept, not copied), its block scales [rows, cols / 16], which are laid out anew, and
     the reciprocal global scale f32 [1], or a factor for every row, f32 [rows] (projections stacked
     along their rows).  Codes and scales are constant (g4.h): nothing may write them between the nvfp4_quantize
-    and the nvfp4_matmul of a product, which reads them ahead; a weight that changes is one of `from_rows`."""
+    and the nvfp4_matmul of a product, which reads them ahead; a weight that changes is one of from_rows."""
 
     def __init__(self, ctx: Context, codes, block_scales, global_scale):
         n, half = _tensor(ctx, "codes", codes, (_U8,), 2).shape
@@ -185,12 +185,13 @@ class Nvfp4Weight:
         self._set(codes, scales, global_scale, n, cols, ctx.device, 1)
 
     @classmethod
-    def from_rows(cls, rows: Nvfp4Rows) -> "Nvfp4Weight":
-        """The matrix that nvfp4_quantize wrote into `rows` (one piece, all of its rows), as a weight."""
+    def from_rows(cls, rows: Nvfp4Rows, constant: bool = False) -> "Nvfp4Weight":
+        """The matrix that nvfp4_quantize wrote into `rows` (one piece, all of its rows), as a weight; constant: the
+        rows stay what they are (a projection quantised once), and products may read them ahead."""
         if rows.pieces != 1:
             raise ValueError(f"rows: {rows.pieces} pieces, a weight has one")
         w = cls.__new__(cls)
-        w._set(rows.codes, rows.scales, rows.factor, rows.max_rows, rows.cols, rows.device)
+        w._set(rows.codes, rows.scales, rows.factor, rows.max_rows, rows.cols, rows.device, int(constant))
         return w
 
     def _set(self, codes, scales, factor, n, cols, device, constant=0):

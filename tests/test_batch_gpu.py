@@ -210,6 +210,26 @@ def test_matmul_ahead_of_the_quantisation(gpu_ctx, m, n, cols, pieces):
     assert ((ahead.double() - want).abs() <= (pieces * cols / 64 + 12) * 2.0 ** -23 * size + U * want.abs()).all()
 
 
+@pytest.mark.parametrize("m, n, cols", [(1, 3840, 4096), (40, 520, 992)])
+def test_matmul_ahead_by_quantised_rows(gpu_ctx, m, n, cols):
+    """A projection quantised once, just in front of the rows, and used as a constant weight: the same bits as in stream
+    order, a new one each time."""
+    g = _gen(73)
+    rows, made = g4.Nvfp4Rows(gpu_ctx, m, cols), [g4.Nvfp4Rows(gpu_ctx, n, cols, 1) for _ in range(8)]
+    x, ws = _randn(g, m, cols), [_randn(g, n, cols, std=0.02) for _ in made]
+    ahead, ordered = torch.empty((8, m, n), dtype=torch.bfloat16, device="cuda"), torch.empty((8, m, n), dtype=torch.bfloat16, device="cuda")
+    assert g4.Nvfp4Weight.from_rows(made[0], constant=True).desc.constant == 1
+    assert g4.Nvfp4Weight.from_rows(made[0]).desc.constant == 0
+    for constant, outs in ((True, ahead), (False, ordered)):
+        for w, r, out in zip(ws, made, outs):
+            r.codes.fill_(0x77), r.scales.fill_(0x38)
+            g4.nvfp4_quantize(gpu_ctx, w, r)
+            g4.nvfp4_quantize(gpu_ctx, x, rows)
+            g4.nvfp4_matmul(gpu_ctx, rows, g4.Nvfp4Weight.from_rows(r, constant=constant), out)
+    _sync(gpu_ctx)
+    assert torch.equal(ahead, ordered) and torch.isfinite(ahead).all() and ahead.float().std() > 0
+
+
 def test_matmul_by_what_another_context_makes(gpu_ctx):
     """Two contexts on one stream: one quantises rows, the other then makes the weight (a piece of rows, scale blocks of
     a checkpoint's), and the first multiplies by it."""
